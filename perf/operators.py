@@ -1,0 +1,407 @@
+"""The 8-bit K/V cache's operators and the windowed read: the work whose speed is measured.
+
+The kinds:
+
+  write    rows appended to a cache held in 8 bits (`quantize_append`) and read back (`dequantize_rows`).
+  quant    attention over an 8-bit cache: one query of every request, or a causal prompt chunk (`quant_attention`).
+  rows     one query's read of a listed set of rows of an 8-bit cache (`quant_gather_attention`).
+  window   attention over a bfloat16 cache with a sliding window and a few first tokens that stay visible
+           (`window_attention`), one query or a chunk.
+
+The cache: codes in e4m3 [B, G, C, 128], a power-of-two scale for each block of 16, 32 or 64 positions, KV head and
+tensor. Shapes: 8 KV groups, head_dim 128, as in the Qwen3 shapes of bench.py; contexts from 1K to 128K, one request to
+32, 1 to 8 query heads per KV group. Synthetic data: K, V and queries ~ N(0, 1), with a few loud channels in K, as
+rotated keys have them.
+
+`own` False: every operator in elementary torch operations. True: the framework's calls.
+"""
+from __future__ import annotations
+
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+DEV = "cuda"
+G, D = 8, 128
+LOWEST = -110      # a block's scale is at least 2^-110
+LARGEST = 1.875 * 2.0 ** 127
+SRC = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def listed():
+    return [
+        # one token of 16 requests of different lengths, every layer's write of a decode step
+        dict(name="write_step_b16", kind="write", batch=16, tokens=1, history=32768, ragged=True, block=64, src="bf16"),
+        # a prompt chunk that begins and ends inside a block
+        dict(name="write_chunk_odd", kind="write", batch=3, tokens=1003, history=517, ragged=False, block=16, src="f32"),
+        # a whole 32K prompt of four requests, out of a bfloat16 prefill
+        dict(name="write_prompt_32k", kind="write", batch=4, tokens=32768, history=0, ragged=False, block=32,
+             src="bf16"),
+        # a short chat turn's single query
+        dict(name="quant_b1_2k", kind="quant", batch=1, heads=2, tokens=1, length=2048, ragged=False, block=64,
+             window=0, sinks=0),
+        # batched serving at 32K, the benchmark's layer
+        dict(name="quant_b16_32k", kind="quant", batch=16, heads=4, tokens=1, length=32768, ragged=False, block=64,
+             window=0, sinks=0),
+        # five requests of odd, different lengths, many query heads to a KV head
+        dict(name="quant_b5_ragged_20k", kind="quant", batch=5, heads=8, tokens=1, length=20011, ragged=True, block=32,
+             window=0, sinks=0),
+        # the sparse step's read: 1092 selected rows of 32K, 16 requests
+        dict(name="rows_b16_32k", kind="rows", batch=16, heads=4, length=32768, rows=1092, block=64),
+        # an 8K prompt at once, 32 query heads
+        dict(name="quant_prompt_8k", kind="quant", batch=1, heads=4, tokens=8192, length=8192, ragged=False, block=64,
+             window=0, sinks=0),
+        # a ragged chunk deep into a long prompt
+        dict(name="quant_chunk_30k", kind="quant", batch=1, heads=2, tokens=1000, length=30011, ragged=False, block=64,
+             window=0, sinks=0),
+        # streaming decode: four sinks and the last 4096 positions of eight 128K contexts
+        dict(name="window_b8_128k", kind="window", batch=8, heads=4, tokens=1, length=131072, ragged=False,
+             window=4096, sinks=4),
+        # a prompt through a sliding-window layer
+        dict(name="window_prompt_8k", kind="window", batch=2, heads=4, tokens=8192, length=8192, ragged=False,
+             window=1024, sinks=4),
+        # the same mask over the 8-bit cache, an odd chunk and an odd window
+        dict(name="quant_window_chunk", kind="quant", batch=2, heads=2, tokens=1501, length=12345, ragged=False,
+             block=32, window=2047, sinks=5),
+    ]
+
+
+def _log(rng, lo, hi):
+    """An integer spread over the logarithm of [lo, hi]."""
+    return min(hi, max(lo, round(math.exp(rng.uniform(math.log(lo), math.log(hi))))))
+
+
+def draw(rng):
+    kind = rng.choice(["write", "write", "quant", "quant", "quant", "rows", "window", "window"])
+    block = rng.choice([16, 32, 64])
+    if kind == "write":
+        if rng.random() < 0.4:
+            return dict(kind=kind, batch=_log(rng, 1, 32), tokens=_log(rng, 1, 8), history=_log(rng, 64, 32768),
+                        ragged=True, block=block, src=rng.choice(["bf16", "f16", "f32"]))
+        tokens = _log(rng, 16, 32768)
+        return dict(kind=kind, batch=_log(rng, 1, max(1, min(16, 4 * 32768 // tokens // 2))), tokens=tokens,
+                    history=rng.choice([0, _log(rng, 1, 16384)]), ragged=False, block=block,
+                    src=rng.choice(["bf16", "bf16", "f32"]))
+    heads = rng.choice([1, 2, 3, 4, 6, 8])
+    if kind == "rows":
+        length = _log(rng, 4096, 65536)
+        return dict(kind=kind, batch=_log(rng, 1, max(1, min(16, 16 * 32768 // length))), heads=heads, length=length,
+                    rows=_log(rng, 64, 2048), block=block)
+    masked = kind == "window" or rng.random() < 0.3
+    if rng.random() < 0.5:   # one query of every request
+        length = _log(rng, 1024, 131072)
+        c = dict(kind=kind, batch=_log(rng, 1, max(1, min(32, 14 * 32768 // length))), heads=heads, tokens=1,
+                 length=length, ragged=rng.random() < 0.4)
+    else:                    # a chunk
+        tokens = _log(rng, 128, 8192)
+        history = rng.choice([0, _log(rng, 64, 30000)]) if tokens <= 2048 else 0
+        most = 8192 * 8192 // (tokens * (tokens + 2 * history))
+        c = dict(kind=kind, batch=_log(rng, 1, max(1, min(4, most))), heads=rng.choice([1, 2, 3, 4]), tokens=tokens,
+                 length=tokens + history, ragged=False)
+    if kind == "quant":
+        c["block"] = block
+    return dict(c, window=_log(rng, 64, 8192) if masked else 0, sinks=rng.choice([0, 1, 4, 4, 64]) if masked else 0)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# inputs: made on the GPU from the seed alone
+# ---------------------------------------------------------------------------------------------------------------------
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _randn(gen, *shape, dtype=torch.bfloat16):
+    return torch.randn(*shape, generator=gen, device=DEV, dtype=dtype)
+
+
+def _codes(gen, B, C, block):
+    """A cache's codes and scales as a program holds them: N(0, 1) values over scales of 2^-8 to 2^-5."""
+    e = torch.randint(-8, -4, (B, G, -(-C // block)), generator=gen, device=DEV)
+    x = _randn(gen, B, G, C, D).mul_(32.0)
+    return x.clamp_(-448.0, 448.0).to(torch.float8_e4m3fn), torch.exp2(e.float())
+
+
+def _lengths(gen, case):
+    """A length per request, or one for all."""
+    L = case["length"]
+    if not case["ragged"]:
+        return L
+    return torch.randint(max(1, L // 4), L + 1, (case["batch"],), generator=gen, device=DEV).to(torch.int32)
+
+
+def prepare(case, seed):
+    gen = _gen(seed)
+    B, kind = case["batch"], case["kind"]
+    s = dict(kind=kind)
+    if kind == "write":
+        T, block, past = case["tokens"], case["block"], case["history"]
+        span = ((T - 1) // block + 2) * block if case["ragged"] else past % block + T
+        C = -(-(past + T) // block) * block + 2 * block
+        s["k8"], s["ks"] = _codes(gen, B, C, block)
+        s["v8"], s["vs"] = _codes(gen, B, C, block)
+        loud = torch.exp2(_randn(gen, 1, G, 1, D, dtype=torch.float32))
+        s["k"] = (_randn(gen, B, G, T, D, dtype=torch.float32) * loud).to(SRC[case["src"]])
+        s["v"] = _randn(gen, B, G, T, D, dtype=torch.float32).to(SRC[case["src"]])
+        start = torch.randint(past // 2, past + 1, (B,), generator=gen, device=DEV).to(torch.int32)
+        s["start"] = start if case["ragged"] else past
+        first = s["start"] - s["start"] % block
+        s["first"], s["span"], s["block"] = first, span, block
+        return s
+    L = case["length"]
+    h = case["heads"]
+    T = case.get("tokens", 1)
+    s["q"] = _randn(gen, B, G, h, T, D)
+    C = -(-(L + 1) // 64) * 64
+    if kind == "window":
+        s["k"], s["v"] = _randn(gen, B, G, C, D), _randn(gen, B, G, C, D)
+    else:
+        s["block"] = case["block"]
+        s["k8"], s["ks"] = _codes(gen, B, C, case["block"])
+        s["v8"], s["vs"] = _codes(gen, B, C, case["block"])
+    if kind == "rows":
+        picks = torch.rand(B, G, L, generator=gen, device=DEV).topk(case["rows"], dim=-1, sorted=False).indices
+        s["rows"] = picks.to(torch.int32)
+        return s
+    s["length"] = _lengths(gen, case)
+    s["window"], s["sinks"] = case["window"] or None, case["sinks"]
+    return s
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# one pass
+# ---------------------------------------------------------------------------------------------------------------------
+def run(s):
+    if own:
+        return _run_own(s)
+    if s["kind"] == "write":
+        k, v = _plain_write(s, "k"), _plain_write(s, "v")
+        return {"k": k, "v": v, "k_scale": s["ks"], "v_scale": s["vs"]}
+    if s["kind"] == "rows":
+        at = s["rows"].long()
+        k, v = (_plain_rows(_plain_values(s[x + "8"], s[x + "s"], s["block"]), at) for x in "kv")
+        return _plain_attention(s["q"], k, v, torch.ones((), dtype=torch.bool, device=DEV))
+    if s["kind"] == "quant":
+        k, v = (_plain_values(s[x + "8"], s[x + "s"], s["block"]) for x in "kv")
+    else:
+        k, v = s["k"].float(), s["v"].float()
+    return _plain_attention(s["q"], k, v, _plain_visible(s, k.shape[2]))
+
+
+def _run_own(s):
+    al = _package()
+    if s["kind"] == "window":
+        return al.window_attention(s["q"], s["k"], s["v"], window=s["window"], sinks=s["sinks"],
+                                   valid_length=s["length"])
+    cache = al.QuantCache(s["k8"], s["v8"], s["ks"], s["vs"], block=s["block"])
+    if s["kind"] == "write":
+        al.quantize_append(cache, s["k"], s["v"], s["start"])
+        k, v = al.dequantize_rows(cache, s["first"], s["span"])
+        return {"k": k, "v": v, "k_scale": s["ks"], "v_scale": s["vs"]}
+    if s["kind"] == "rows":
+        return al.quant_gather_attention(s["q"], cache, s["rows"])
+    return al.quant_attention(s["q"], cache, valid_length=s["length"], window=s["window"], sinks=s["sinks"])
+
+
+def _package():
+    if "attention_lab" not in sys.modules:
+        root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+        sys.path.insert(0, os.path.join(root, "attention-lab_amd"))
+    import attention_lab
+    return attention_lab
+
+
+def _plain_values(codes, scale, block):
+    """The values that codes stand for."""
+    return codes.float() * scale.repeat_interleave(block, dim=2)[:, :, :codes.shape[2], None]
+
+
+def _plain_e4m3(y):
+    """y (|y| <= 448) rounded to the nearest e4m3 value, ties to even: three bits behind the leading one, and steps of
+    2^-9 below 2^-6."""
+    step = torch.exp2((torch.frexp(y).exponent - 1).clamp(min=-6).float() - 3)
+    return torch.round(y / step) * step
+
+
+def _plain_rows(x, at):
+    return x.gather(2, at.unsqueeze(-1).expand(-1, -1, -1, D))
+
+
+def _plain_write(s, name):
+    codes, scale, x, block = s[name + "8"], s[name + "s"], s[name].float(), s["block"]
+    B, _, T, _ = x.shape
+    start = torch.as_tensor(s["start"], device=DEV).long().expand(B)
+    n = (T - 1) // block + 2                                     # blocks that T rows can touch
+    base = start // block
+    pos = (base.unsqueeze(1) * block + torch.arange(n * block, device=DEV))          # [B, n * block]
+    src = (pos - start.unsqueeze(1))
+    new = ((src >= 0) & (src < T)).view(B, 1, n, block, 1)
+    old = (src < 0).view(B, 1, n, block, 1)
+    at = pos.unsqueeze(1).expand(B, G, -1)
+    held = _plain_rows(codes.view(torch.uint8), at).view(codes.dtype).float().view(B, G, n, block, D)
+    x = _plain_rows(x, src.clamp(0, T - 1).unsqueeze(1).expand(B, G, -1)).view(B, G, n, block, D)
+    bad = ~torch.isfinite(x)
+    x = x.clamp(-LARGEST, LARGEST)
+    top = torch.where(new & ~bad, x.abs(), 0.0).amax(dim=(3, 4))
+    m, e = torch.frexp(top)                                      # top = m 2^e, m in [1/2, 1); 448 = 0.875 2^9
+    need = torch.where(top > 0, e - 9 + (m > 0.875).int(), LOWEST).clamp(min=LOWEST)
+    which = (base.unsqueeze(1) + torch.arange(n, device=DEV)).unsqueeze(1).expand(B, G, n)
+    was = scale.gather(2, which)
+    now = torch.where(old.any(dim=3).view(B, 1, n), torch.maximum(was, torch.exp2(need.float())),
+                      torch.exp2(need.float()))
+    now = torch.where(new.any(dim=3).view(B, 1, n), now, was)    # a block that no row reaches keeps its scale
+    unit = now.view(B, G, n, 1, 1)
+    fresh = torch.where(bad, float("nan"), _plain_e4m3(x / unit))
+    moved = _plain_e4m3(held * (was.view(B, G, n, 1, 1) / unit))
+    held = torch.where(new, fresh, torch.where(old, moved, held)).view(B, G, n * block, D)
+    codes.view(torch.uint8).scatter_(2, at.unsqueeze(-1).expand(-1, -1, -1, D),
+                                     held.to(codes.dtype).view(torch.uint8))
+    scale.scatter_(2, which, now)
+    return (held.view(B, G, n, block, D) * unit).view(B, G, -1, D)[:, :, :s["span"]].to(torch.bfloat16)
+
+
+def _plain_visible(s, C):
+    """Which of the C positions each query reads, [B or 1, 1, 1, T, C]."""
+    T = s["q"].shape[3]
+    length = torch.as_tensor(s["length"], device=DEV).long().view(-1, 1, 1, 1, 1)
+    p = length - T + torch.arange(T, device=DEV).view(1, 1, 1, T, 1)
+    j = torch.arange(C, device=DEV).view(1, 1, 1, 1, C)
+    seen = (j <= p) & (j < length)
+    return seen if s["window"] is None else seen & ((j > p - s["window"]) | (j < s["sinks"]))
+
+
+def _plain_attention(q, k, v, seen):
+    """Softmax attention of q [B, G, h, T, D] over the seen rows of k, v [B, G, C, D] in 32 bits."""
+    B, _, h, T, _ = q.shape
+    x = (q.float().view(B, G, h * T, D) @ k.transpose(2, 3).contiguous()).view(B, G, h, T, -1) * D ** -0.5
+    x = torch.where(seen, x, float("-inf"))
+    x = torch.exp(x - x.amax(dim=-1, keepdim=True))
+    out = (x.view(B, G, h * T, -1) @ v).view(B, G, h, T, D) / x.sum(dim=-1, keepdim=True)
+    return out.to(q.dtype)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# what a pass cannot do without
+# ---------------------------------------------------------------------------------------------------------------------
+def _pairs(T, L, window, sinks):
+    """(query, key) pairs of T queries at the last positions of L, and the distinct keys among them."""
+    if not window:
+        return T * (L - T) + T * (T + 1) // 2, L
+    n = 0
+    for p in range(L - T, L):
+        lo = max(0, p + 1 - window)
+        n += p + 1 - lo + min(sinks, lo)
+    lo = max(0, L - T + 1 - window)
+    return n, L - lo + min(sinks, lo)
+
+
+def work(case):
+    B, kind = case["batch"], case["kind"]
+    rows = B * G
+    if kind == "write":
+        T, block, past = case["tokens"], case["block"], case["history"]
+        held = block - 1 if case["ragged"] else past % block
+        span = ((T - 1) // block + 2) * block if case["ragged"] else past % block + T
+        e = torch.empty((), dtype=SRC[case["src"]]).element_size()
+        # in and out of the new rows, the old rows of the first block, and the read-back of what was written
+        return dict(bytes=2 * rows * D * (T * (e + 1) + held + span * 2), flops=2 * rows * D * 3 * T)
+    h = case["heads"]
+    if kind == "rows":
+        S = case["rows"]
+        return dict(bytes=rows * (S * (2 * D + 4) + 4 * h * D), flops=rows * 4 * h * S * D)
+    T, L = case["tokens"], case["length"]
+    if case["ragged"]:
+        L = L * 5 // 8       # the mean of the lengths
+    pairs, keys = _pairs(T, L, case["window"], case["sinks"])
+    e = 1 if kind == "quant" else 2
+    return dict(bytes=rows * (keys * 2 * D * e + 4 * h * T * D), flops=rows * h * pairs * 4 * D)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the same in 64 bits, from the definition
+# ---------------------------------------------------------------------------------------------------------------------
+def _exact_round(y):
+    """The e4m3 value nearest to y, by search among all of them (ties to the even code)."""
+    mantissa = torch.arange(8, device=DEV, dtype=torch.float64)
+    grid = torch.cat([mantissa * 2.0 ** -9] + [(8 + mantissa) * 2.0 ** (e - 3) for e in range(-6, 9)])[:127]
+    hi = torch.searchsorted(grid, y.abs().contiguous()).clamp(1, 126)
+    below, above = grid[hi - 1], grid[hi]
+    up = (y.abs() - below > above - y.abs()) | ((y.abs() - below == above - y.abs()) & (hi % 2 == 0))
+    return torch.copysign(torch.where(up, above, below), y)
+
+
+def _exact_write(s, name):
+    codes, scale, x, block = s[name + "8"], s[name + "s"], s[name], s["block"]
+    B, _, T, _ = x.shape
+    starts = s["start"].tolist() if isinstance(s["start"], torch.Tensor) else [s["start"]] * B
+    out = torch.zeros(B, G, s["span"], D, dtype=torch.float64, device=DEV)
+    scales = scale.double()
+    for b, start in enumerate(starts):
+        base = start - start % block
+        for j in range(base // block, -(-(base + s["span"]) // block)):
+            lo, hi = j * block, (j + 1) * block
+            c = codes[b, :, lo:hi].double()
+            n0, n1 = max(lo, start), min(hi, start + T)
+            if n0 < n1:
+                new = x[b, :, n0 - start:n1 - start].double()
+                top = new.abs().amax(dim=(1, 2))
+                e = torch.ceil(torch.log2(top / 448.0)).clamp(min=LOWEST)
+                e = torch.where(448.0 * torch.exp2(e - 1) >= top, e - 1, e).clamp(min=LOWEST)
+                unit = torch.exp2(e)
+                if start > lo:
+                    unit = torch.maximum(unit, scales[b, :, j])
+                    keep = c[:, :start - lo] * (scales[b, :, j] / unit).view(G, 1, 1)
+                    c[:, :start - lo] = _exact_round(keep)
+                c[:, n0 - lo:n1 - lo] = _exact_round(new / unit.view(G, 1, 1))
+                scales[b, :, j] = unit
+            m = min(hi - base, s["span"])
+            out[b, :, lo - base:m] = (c * scales[b, :, j].view(G, 1, 1))[:, :m - (lo - base)]
+    return out, scales
+
+
+def _exact_attention(s):
+    q = s["q"]
+    B, _, h, T, _ = q.shape
+    lengths = s["length"] if "length" in s else 0
+    lengths = lengths.tolist() if isinstance(lengths, torch.Tensor) else [lengths] * B
+    out = torch.empty(q.shape, dtype=torch.float64, device=DEV)
+    for b in range(B):
+        for g in range(G):
+            if s["kind"] == "window":
+                k, v = s["k"][b, g].double(), s["v"][b, g].double()
+            else:
+                at = torch.arange(s["k8"].shape[2], device=DEV) // s["block"]
+                k = s["k8"][b, g].double() * s["ks"][b, g].double()[at].unsqueeze(1)
+                v = s["v8"][b, g].double() * s["vs"][b, g].double()[at].unsqueeze(1)
+            if "rows" in s:
+                pick = s["rows"][b, g].long()
+                p = torch.softmax(q[b, g, :, 0].double() @ k[pick].t().contiguous() / math.sqrt(D), dim=-1)
+                out[b, g, :, 0] = p @ v[pick]
+                continue
+            L = lengths[b]
+            kt, v = k[:L].t().contiguous(), v[:L]
+            key = torch.arange(L, device=DEV)
+            step = max(1, (1 << 27) // (h * L))
+            for a in range(0, T, step):
+                z = min(T, a + step)
+                pos = torch.arange(L - T + a, L - T + z, device=DEV).unsqueeze(1)
+                gone = key > pos
+                if s["window"] is not None:
+                    gone = gone | ((pos - key >= s["window"]) & (key >= s["sinks"]))
+                x = (q[b, g, :, a:z].double() @ kt / math.sqrt(D)).masked_fill_(gone, float("-inf"))
+                out[b, g, :, a:z] = torch.softmax(x, dim=-1) @ v
+    return out
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if s["kind"] == "write":
+        if case["batch"] * case["tokens"] > 131072:
+            return None
+        k, ks = _exact_write(s, "k")
+        v, vs = _exact_write(s, "v")
+        return {"k": k, "v": v, "k_scale": ks, "v_scale": vs}
+    return _exact_attention(s)
