@@ -8,8 +8,8 @@ The kinds:
   window   attention over a bfloat16 cache with a sliding window and a few first tokens that stay visible
            (`window_attention`), one query or a chunk.
 
-The cache: codes in e4m3 [B, G, C, 128], a power-of-two scale for each block of 16, 32 or 64 positions, KV head and
-tensor. Shapes: 8 KV groups, head_dim 128, as in the Qwen3 shapes of bench.py; contexts from 1K to 128K, one request to
+The cache: codes in e4m3 [B, G, C, 128], and for each block of 16, 32 or 64 positions, KV head and tensor one scale
+2^(x - 127), kept as the byte x. Shapes: 8 KV groups, head_dim 128, as in the Qwen3 shapes of bench.py; contexts from 1K to 128K, one request to
 32, 1 to 8 query heads per KV group. Synthetic data: K, V and queries ~ N(0, 1), with a few loud channels in K, as
 rotated keys have them.
 
@@ -119,10 +119,10 @@ def _randn(gen, *shape, dtype=torch.bfloat16):
 
 
 def _codes(gen, B, C, block):
-    """A cache's codes and scales as a program holds them: N(0, 1) values over scales of 2^-8 to 2^-5."""
-    e = torch.randint(-8, -4, (B, G, -(-C // block)), generator=gen, device=DEV)
+    """A cache's codes and scale exponents as a program holds them: N(0, 1) values over scales of 2^-8 to 2^-5."""
+    e = torch.randint(127 - 8, 127 - 4, (B, G, -(-C // block)), generator=gen, device=DEV)
     x = _randn(gen, B, G, C, D).mul_(32.0)
-    return x.clamp_(-448.0, 448.0).to(torch.float8_e4m3fn), torch.exp2(e.float())
+    return x.clamp_(-448.0, 448.0).to(torch.float8_e4m3fn), e.to(torch.uint8)
 
 
 def _lengths(gen, case):
@@ -141,8 +141,8 @@ def prepare(case, seed):
         T, block, past = case["tokens"], case["block"], case["history"]
         span = ((T - 1) // block + 2) * block if case["ragged"] else past % block + T
         C = -(-(past + T) // block) * block + 2 * block
-        s["k8"], s["ks"] = _codes(gen, B, C, block)
-        s["v8"], s["vs"] = _codes(gen, B, C, block)
+        s["k8"], s["ke"] = _codes(gen, B, C, block)
+        s["v8"], s["ve"] = _codes(gen, B, C, block)
         loud = torch.exp2(_randn(gen, 1, G, 1, D, dtype=torch.float32))
         s["k"] = (_randn(gen, B, G, T, D, dtype=torch.float32) * loud).to(SRC[case["src"]])
         s["v"] = _randn(gen, B, G, T, D, dtype=torch.float32).to(SRC[case["src"]])
@@ -160,8 +160,8 @@ def prepare(case, seed):
         s["k"], s["v"] = _randn(gen, B, G, C, D), _randn(gen, B, G, C, D)
     else:
         s["block"] = case["block"]
-        s["k8"], s["ks"] = _codes(gen, B, C, case["block"])
-        s["v8"], s["vs"] = _codes(gen, B, C, case["block"])
+        s["k8"], s["ke"] = _codes(gen, B, C, case["block"])
+        s["v8"], s["ve"] = _codes(gen, B, C, case["block"])
     if kind == "rows":
         picks = torch.rand(B, G, L, generator=gen, device=DEV).topk(case["rows"], dim=-1, sorted=False).indices
         s["rows"] = picks.to(torch.int32)
@@ -179,13 +179,13 @@ def run(s):
         return _run_own(s)
     if s["kind"] == "write":
         k, v = _plain_write(s, "k"), _plain_write(s, "v")
-        return {"k": k, "v": v, "k_scale": s["ks"], "v_scale": s["vs"]}
+        return {"k": k, "v": v, "k_exp": s["ke"], "v_exp": s["ve"]}
     if s["kind"] == "rows":
         at = s["rows"].long()
-        k, v = (_plain_rows(_plain_values(s[x + "8"], s[x + "s"], s["block"]), at) for x in "kv")
+        k, v = (_plain_rows(_plain_values(s[x + "8"], s[x + "e"], s["block"]), at) for x in "kv")
         return _plain_attention(s["q"], k, v, torch.ones((), dtype=torch.bool, device=DEV))
     if s["kind"] == "quant":
-        k, v = (_plain_values(s[x + "8"], s[x + "s"], s["block"]) for x in "kv")
+        k, v = (_plain_values(s[x + "8"], s[x + "e"], s["block"]) for x in "kv")
     else:
         k, v = s["k"].float(), s["v"].float()
     return _plain_attention(s["q"], k, v, _plain_visible(s, k.shape[2]))
@@ -196,11 +196,11 @@ def _run_own(s):
     if s["kind"] == "window":
         return al.window_attention(s["q"], s["k"], s["v"], window=s["window"], sinks=s["sinks"],
                                    valid_length=s["length"])
-    cache = al.QuantCache(s["k8"], s["v8"], s["ks"], s["vs"], block=s["block"])
+    cache = al.QuantCache(s["k8"], s["v8"], s["ke"], s["ve"], block=s["block"])
     if s["kind"] == "write":
         al.quantize_append(cache, s["k"], s["v"], s["start"])
         k, v = al.dequantize_rows(cache, s["first"], s["span"])
-        return {"k": k, "v": v, "k_scale": s["ks"], "v_scale": s["vs"]}
+        return {"k": k, "v": v, "k_exp": s["ke"], "v_exp": s["ve"]}
     if s["kind"] == "rows":
         return al.quant_gather_attention(s["q"], cache, s["rows"])
     return al.quant_attention(s["q"], cache, valid_length=s["length"], window=s["window"], sinks=s["sinks"])
@@ -214,9 +214,13 @@ def _package():
     return attention_lab
 
 
-def _plain_values(codes, scale, block):
+def _plain_scale(x):
+    return torch.exp2(x.float() - 127.0)
+
+
+def _plain_values(codes, exponents, block):
     """The values that codes stand for."""
-    return codes.float() * scale.repeat_interleave(block, dim=2)[:, :, :codes.shape[2], None]
+    return codes.float() * _plain_scale(exponents).repeat_interleave(block, dim=2)[:, :, :codes.shape[2], None]
 
 
 def _plain_e4m3(y):
@@ -231,7 +235,7 @@ def _plain_rows(x, at):
 
 
 def _plain_write(s, name):
-    codes, scale, x, block = s[name + "8"], s[name + "s"], s[name].float(), s["block"]
+    codes, exponents, x, block = s[name + "8"], s[name + "e"], s[name].float(), s["block"]
     B, _, T, _ = x.shape
     start = torch.as_tensor(s["start"], device=DEV).long().expand(B)
     n = (T - 1) // block + 2                                     # blocks that T rows can touch
@@ -249,17 +253,17 @@ def _plain_write(s, name):
     m, e = torch.frexp(top)                                      # top = m 2^e, m in [1/2, 1); 448 = 0.875 2^9
     need = torch.where(top > 0, e - 9 + (m > 0.875).int(), LOWEST).clamp(min=LOWEST)
     which = (base.unsqueeze(1) + torch.arange(n, device=DEV)).unsqueeze(1).expand(B, G, n)
-    was = scale.gather(2, which)
-    now = torch.where(old.any(dim=3).view(B, 1, n), torch.maximum(was, torch.exp2(need.float())),
-                      torch.exp2(need.float()))
+    was = exponents.gather(2, which)
+    need = (need + 127).to(torch.uint8)
+    now = torch.where(old.any(dim=3).view(B, 1, n), torch.maximum(was, need), need)
     now = torch.where(new.any(dim=3).view(B, 1, n), now, was)    # a block that no row reaches keeps its scale
-    unit = now.view(B, G, n, 1, 1)
+    unit = _plain_scale(now).view(B, G, n, 1, 1)
     fresh = torch.where(bad, float("nan"), _plain_e4m3(x / unit))
-    moved = _plain_e4m3(held * (was.view(B, G, n, 1, 1) / unit))
+    moved = _plain_e4m3(held * (_plain_scale(was).view(B, G, n, 1, 1) / unit))
     held = torch.where(new, fresh, torch.where(old, moved, held)).view(B, G, n * block, D)
     codes.view(torch.uint8).scatter_(2, at.unsqueeze(-1).expand(-1, -1, -1, D),
                                      held.to(codes.dtype).view(torch.uint8))
-    scale.scatter_(2, which, now)
+    exponents.scatter_(2, which, now)
     return (held.view(B, G, n, block, D) * unit).view(B, G, -1, D)[:, :, :s["span"]].to(torch.bfloat16)
 
 
@@ -334,11 +338,11 @@ def _exact_round(y):
 
 
 def _exact_write(s, name):
-    codes, scale, x, block = s[name + "8"], s[name + "s"], s[name], s["block"]
+    codes, exponents, x, block = s[name + "8"], s[name + "e"], s[name], s["block"]
     B, _, T, _ = x.shape
     starts = s["start"].tolist() if isinstance(s["start"], torch.Tensor) else [s["start"]] * B
     out = torch.zeros(B, G, s["span"], D, dtype=torch.float64, device=DEV)
-    scales = scale.double()
+    scales = 2.0 ** (exponents.double() - 127.0)
     for b, start in enumerate(starts):
         base = start - start % block
         for j in range(base // block, -(-(base + s["span"]) // block)):
@@ -359,7 +363,7 @@ def _exact_write(s, name):
                 scales[b, :, j] = unit
             m = min(hi - base, s["span"])
             out[b, :, lo - base:m] = (c * scales[b, :, j].view(G, 1, 1))[:, :m - (lo - base)]
-    return out, scales
+    return out, (torch.log2(scales).round() + 127).to(torch.uint8)
 
 
 def _exact_attention(s):
@@ -374,8 +378,8 @@ def _exact_attention(s):
                 k, v = s["k"][b, g].double(), s["v"][b, g].double()
             else:
                 at = torch.arange(s["k8"].shape[2], device=DEV) // s["block"]
-                k = s["k8"][b, g].double() * s["ks"][b, g].double()[at].unsqueeze(1)
-                v = s["v8"][b, g].double() * s["vs"][b, g].double()[at].unsqueeze(1)
+                k, v = (s[x + "8"][b, g].double() * 2.0 ** (s[x + "e"][b, g].double()[at].unsqueeze(1) - 127.0)
+                        for x in "kv")
             if "rows" in s:
                 pick = s["rows"][b, g].long()
                 p = torch.softmax(q[b, g, :, 0].double() @ k[pick].t().contiguous() / math.sqrt(D), dim=-1)
@@ -401,7 +405,7 @@ def exact(case, seed):
     if s["kind"] == "write":
         if case["batch"] * case["tokens"] > 131072:
             return None
-        k, ks = _exact_write(s, "k")
-        v, vs = _exact_write(s, "v")
-        return {"k": k, "v": v, "k_scale": ks, "v_scale": vs}
+        k, ke = _exact_write(s, "k")
+        v, ve = _exact_write(s, "v")
+        return {"k": k, "v": v, "k_exp": ke, "v_exp": ve}
     return _exact_attention(s)
