@@ -16,6 +16,9 @@ from .selection import (FIXED_PREFIX, FIXED_RECENT, SelectionLayout, fixed_budge
 from .reference import dense_mask_reference, dense_reference  # noqa: E402
 from .sparse import flatten_cache, gather_attention, gather_rows, row_offsets, subset_attention  # noqa: E402
 from .full import FULL_BACKENDS, full_attention  # noqa: E402
+from .window import window_attention  # noqa: E402
+from .quant import (QuantCache, dequantize_rows, quant_attention, quant_gather_attention,  # noqa: E402
+                    quantize_append)
 from .indexer import GroupedIndexer, candidate_scores, project_keys, project_queries  # noqa: E402
 from .decode import (DecodeRequest, dense_decode_step, gathered_decode_step_kernel, prepare_request,  # noqa: E402
                      select_rows_kernel, select_rows_recent, select_rows_uniform, sparse_decode_step,
@@ -25,7 +28,8 @@ __all__ = [
     "FIXED_PREFIX", "FIXED_RECENT", "SelectionLayout", "fixed_budget", "legal_length", "selection_layout",
     "dense_reference", "dense_mask_reference",
     "flatten_cache", "gather_attention", "gather_rows", "row_offsets", "subset_attention",
-    "FULL_BACKENDS", "full_attention",
+    "FULL_BACKENDS", "full_attention", "window_attention",
+    "QuantCache", "dequantize_rows", "quant_attention", "quant_gather_attention", "quantize_append",
     "GroupedIndexer", "candidate_scores", "project_keys", "project_queries",
     "DecodeRequest", "dense_decode_step", "gathered_decode_step_kernel", "prepare_request", "select_rows_kernel",
     "select_rows_recent", "select_rows_uniform", "sparse_decode_step", "sparse_decode_step_kernel",

@@ -1,0 +1,170 @@
+"""Attention over a range of a cache on gfx950: every legal position, or a sliding window and a few first ones (sinks),
+for one query or a causal chunk, over a bfloat16 cache or an 8-bit one; and the row-list read of an 8-bit cache.
+
+The kernels behind `window_attention` (window.py) and `quant_attention` / `quant_gather_attention` (quant.py), which
+check their caches; this module checks what the reads share, chooses the split counts and launches. There is no state
+between calls: the split-K partials are allocated for the call, so calls on several streams, and captured graphs, share
+nothing. Launches go to the tensors' own device, on torch's current stream of it.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _native as nat
+from .hip_attend import HEAD_DIM
+
+MAX_H = 8           # query heads per KV group of the one-query kernels (the matrix core's 16 columns hold each twice)
+MAX_H_CHUNK = 16    # ... of the chunk kernel
+CHUNK_ROWS = 128    # (query, head) rows of the chunk kernel's workgroup
+CHUNK_KEYS = 64     # keys of its block
+TILE = 32           # rows a wave of the one-query kernel takes at a time
+MAX_SPLITS = 16
+MAX_P = 256
+INT_MAX = 2 ** 31 - 1
+
+
+def decode_partitions(BG: int, count: int) -> int:
+    """Split-K count of the one-query kernels for BG (b, g) rows of `count` positions each: about two workgroups per CU,
+    each at least one tile of 32 positions for every one of its four waves."""
+    return max(1, min(64, -(-512 // BG), count // (4 * TILE)))
+
+
+def chunk_splits(BG: int, h: int, T: int, keys: int) -> int:
+    """Workgroups that share a query tile's keys: one where the tiles give every CU one, else as many as bring the grid to
+    about two per CU, each at least 512 keys."""
+    tiles = BG * -(-T // (CHUNK_ROWS // h))
+    if tiles >= 256:
+        return 1
+    s = min(MAX_SPLITS, 512 // tiles, keys // 512)
+    return s if s >= 2 else 1
+
+
+def check_window(window, sinks):
+    """(window, sinks) for the kernels, window 0 for none."""
+    sinks = int(sinks)
+    if sinks < 0:
+        raise ValueError(f"sinks={sinks} must not be negative")
+    if window is None:
+        return 0, 0
+    window = int(window)
+    if window < 1:
+        raise ValueError(f"window={window} must be at least 1 (None: no window)")
+    return min(window, INT_MAX), min(sinks, INT_MAX)
+
+
+def check_query(q, B: int, G: int, device):
+    """q [B,G,h,T,128] bfloat16 on the cache's device -> (h, T)."""
+    if q.dim() != 5 or tuple(q.shape[:2]) != (B, G) or q.shape[4] != HEAD_DIM or q.dtype != torch.bfloat16:
+        raise ValueError(f"q must be a bfloat16 [B, G, h, T, {HEAD_DIM}] tensor with B, G = {B}, {G}, got {q.dtype} "
+                         f"{tuple(q.shape)}")
+    if q.device != device:
+        raise ValueError("q must live on the cache's device")
+    h = int(q.shape[2])
+    if not 1 <= h <= MAX_H_CHUNK:
+        raise ValueError(f"h={h} must be in [1, {MAX_H_CHUNK}]")
+    return h, int(q.shape[3])
+
+
+def check_lengths(lengths, B: int, device):
+    """A device tensor of one valid length (or start) per sequence."""
+    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous() \
+            or lengths.device != device:
+        raise ValueError(f"one value per sequence must be a contiguous int32 [{B}] tensor on the cache's device")
+    return lengths
+
+
+def check_out(out, q, dtype):
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("out_dtype must be float32 or bfloat16")
+    if out is None:
+        return torch.empty(q.shape, dtype=dtype, device=q.device)
+    if tuple(out.shape) != tuple(q.shape) or out.dtype != dtype or not out.is_contiguous() or out.device != q.device:
+        raise ValueError(f"out must be a contiguous {dtype} tensor shaped like q on its device")
+    return out
+
+
+def split_count(partitions, chosen: int, most: int) -> int:
+    """The caller's split count, checked, or the rule's."""
+    if partitions is None:
+        return chosen
+    if not 1 <= int(partitions) <= most:
+        raise ValueError(f"partitions must be in [1, {most}]")
+    return int(partitions)
+
+
+def _partials(words: int, device):
+    return torch.empty(words, dtype=torch.float32, device=device)
+
+
+def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: int, C: int, device, *, valid_length,
+                    query_start, window, sinks, scale, out, out_dtype, partitions):
+    """The reads of window_attention and quant_attention over a checked cache [B,G,C,128] at k_ptr / v_ptr (exp_ptrs: the
+    scale bytes of an 8-bit one, or (None, None))."""
+    if min(B, G, C) < 1:
+        raise ValueError(f"the cache must hold at least one sequence, group and position, got {B}, {G}, {C}")
+    h, T = check_query(q, B, G, device)
+    window, sinks = check_window(window, sinks)
+    lengths = None
+    if isinstance(valid_length, torch.Tensor):
+        lengths = check_lengths(valid_length, B, device)
+        if T != 1 or query_start is not None:
+            raise ValueError("a length per sequence goes with one query each, at its sequence's last position")
+        if h > MAX_H:
+            raise ValueError(f"a length per sequence takes h <= {MAX_H} query heads per group, got {h}")
+        legal, p0, seen = C, C - 1, C
+    else:
+        legal = C if valid_length is None else int(valid_length)
+        if not 0 < legal <= C:
+            raise ValueError(f"valid_length={legal} must be in (0, capacity={C}]")
+        p0 = legal - T if query_start is None else int(query_start)
+        if not 0 <= p0 < INT_MAX - T:
+            raise ValueError(f"query positions must be non-negative and below 2^31, got {p0}")
+        seen = min(legal, p0 + T)
+    if window:
+        seen = min(seen, window + T - 1 + min(sinks, seen))
+    q = q.contiguous()
+    sc = float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
+    stream = nat.stream_of(device)
+    if T == 1 and h <= MAX_H:
+        out = check_out(out, q, out_dtype)
+        P = split_count(partitions, decode_partitions(B * G, seen), MAX_P)
+        part = _partials(B * G * P * h * (HEAD_DIM + 2), device) if P > 1 else None
+        nat.call_on(device, "attnlab_range_decode", k_ptr, v_ptr, *exp_ptrs, block, q.data_ptr(), nat.ptr(lengths), legal,
+                    p0, window, sinks, B, G, h, C, P, sc, out.data_ptr(), int(out_dtype == torch.bfloat16),
+                    nat.ptr(part), stream)
+        return out
+    if out_dtype != torch.bfloat16:
+        raise ValueError("a chunk's outputs are bfloat16")
+    out = check_out(out, q, out_dtype)
+    if T == 0:
+        return out
+    splits = split_count(partitions, chunk_splits(B * G, h, T, seen), MAX_SPLITS)
+    nbytes = max(0, nat.lib().attnlab_range_prefill_part_bytes(B, G, h, T, splits))
+    part = _partials(nbytes // 4, device) if nbytes else None
+    nat.call_on(device, "attnlab_range_prefill", q.data_ptr(), k_ptr, v_ptr, *exp_ptrs, block, out.data_ptr(), B, G, h, T,
+                p0, legal, C, window, sinks, sc, splits, nat.ptr(part), nbytes, stream)
+    return out
+
+
+def listed_attention(q, cache, rows, *, scale, out, out_dtype, partitions):
+    """The row-list read of quant_gather_attention: rows int32 [B,G,S] contiguous, checked cache."""
+    B, G, C, device = cache.batch, cache.groups, cache.capacity, cache.device
+    h, T = check_query(q, B, G, device)
+    if T != 1:
+        raise ValueError("the row-list read takes one query position")
+    if h > MAX_H:
+        raise ValueError(f"the row-list read takes h <= {MAX_H} query heads per group, got {h}")
+    S = int(rows.shape[2])
+    if S < 1:
+        raise ValueError("at least one row must be selected")
+    out = check_out(out, q, out_dtype)
+    q = q.contiguous()
+    P = split_count(partitions, decode_partitions(B * G, S), MAX_P)
+    part = _partials(B * G * P * h * (HEAD_DIM + 2), device) if P > 1 else None
+    sc = float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
+    nat.call_on(device, "attnlab_quant_attend", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(),
+                cache.v_exp.data_ptr(), cache.block, q.data_ptr(), rows.data_ptr(), S, B, G, h, S, C, P, sc,
+                out.data_ptr(), int(out_dtype == torch.bfloat16), nat.ptr(part), nat.stream_of(device))
+    return out

@@ -1,0 +1,173 @@
+"""The 8-bit K/V cache: rows quantised as they are written, read back, and attended over in place.
+
+A `QuantCache` holds one layer's K and V as e4m3 codes [B,G,C,128] and one scale byte x per block of 16, 32 or 64
+positions, KV head and tensor; a value is code * 2^(x - 127), exact in bfloat16. Half the bytes of the bfloat16 cache,
+and so about half the time of every decode read, for a rounding of at most 2^-4 of each value (e4m3 keeps 4 significant
+bits; values below 2^-14 of their block's largest keep fewer).
+
+    cache = QuantCache.empty(B, G, C, device=dev)
+    quantize_append(cache, k_prompt, v_prompt, 0)                       # rows [0, T)
+    out = quant_attention(q_prompt, cache, valid_length=T)              # the causal chunk
+    quantize_append(cache, k_new, v_new, T)                             # one token
+    out = quant_attention(q_new, cache, valid_length=T + 1)             # one query, every legal position
+    out = quant_attention(q_new, cache, valid_length=T + 1, window=4096, sinks=4)
+    out = quant_gather_attention(q_new, cache, rows)                    # one query, the rows of a selection
+    k, v = dequantize_rows(cache, 0, T + 1)
+
+No counterpart in the reference, whose cache is bfloat16 or float32 (qwen_wrap.py:68-75); the reads have the semantics
+of full_attention (full.py:17-44) and gather_attention (sparse.py:63-67) over the values the codes stand for.
+Where a length or start per sequence is a device tensor, nothing is read back to the host, so a captured graph follows
+its later values.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _native as nat
+from . import hip_range
+from .hip_attend import HEAD_DIM
+
+BLOCKS = (16, 32, 64)
+_DTYPES = {torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16, torch.float32: nat.DT_F32}
+
+
+class QuantCache:
+    """One layer's K and V in 8 bits: k, v torch.float8_e4m3fn [B,G,C,128]; k_exp, v_exp uint8 [B,G,ceil(C/block)], the
+    scale of a block being 2^(x - 127). All four are contiguous tensors on one HIP device, used in place."""
+
+    __slots__ = ("k", "v", "k_exp", "v_exp", "block", "batch", "groups", "capacity", "device")
+
+    def __init__(self, k, v, k_exp, v_exp, *, block: int = 64):
+        if block not in BLOCKS:
+            raise ValueError(f"block must be one of {BLOCKS}, got {block!r}")
+        if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.dtype != torch.float8_e4m3fn or not k.is_contiguous() \
+                or not k.is_cuda:
+            raise ValueError(f"k must be a contiguous float8_e4m3fn [B, G, C, {HEAD_DIM}] tensor on a HIP device")
+        if v.shape != k.shape or v.dtype != k.dtype or not v.is_contiguous() or v.device != k.device:
+            raise ValueError("v must match k")
+        B, G, C, _ = k.shape
+        want = (B, G, -(-C // block))
+        for t, name in ((k_exp, "k_exp"), (v_exp, "v_exp")):
+            if tuple(t.shape) != want or t.dtype != torch.uint8 or not t.is_contiguous() or t.device != k.device:
+                raise ValueError(f"{name} must be a contiguous uint8 {list(want)} tensor on the cache's device")
+        self.k, self.v, self.k_exp, self.v_exp, self.block = k, v, k_exp, v_exp, int(block)
+        self.batch, self.groups, self.capacity, self.device = B, G, C, k.device
+
+    @classmethod
+    def empty(cls, batch: int, groups: int, capacity: int, *, block: int = 64, device) -> "QuantCache":
+        """A cache with nothing written: codes hold whatever the memory held, which no read of written rows meets."""
+        if block not in BLOCKS:
+            raise ValueError(f"block must be one of {BLOCKS}, got {block!r}")
+        if min(int(batch), int(groups), int(capacity)) < 1:
+            raise ValueError("batch, groups and capacity must be positive")
+        shape = (int(batch), int(groups), int(capacity), HEAD_DIM)
+        k, v = (torch.empty(shape, dtype=torch.float8_e4m3fn, device=device) for _ in "kv")
+        ke, ve = (torch.full((*shape[:2], -(-shape[2] // block)), 127, dtype=torch.uint8, device=device) for _ in "kv")
+        return cls(k, v, ke, ve, block=block)
+
+    def bytes(self) -> int:
+        return sum(t.numel() for t in (self.k, self.v, self.k_exp, self.v_exp))
+
+
+def _start(cache: QuantCache, start, length: int):
+    """(device tensor or None, int) of a start that is an int, checked here, or an int32 [B] device tensor."""
+    if isinstance(start, torch.Tensor):
+        return hip_range.check_lengths(start, cache.batch, cache.device), 0
+    start = int(start)
+    if start < 0 or start + length > cache.capacity:
+        raise ValueError(f"rows [{start}, {start + length}) outside the cache's capacity {cache.capacity}")
+    return None, start
+
+
+def _rows(x, dtype):
+    """x as the kernel takes it: unit stride along a row and 16-byte aligned rows (a copy where it has neither)."""
+    step = 16 // x.element_size()
+    if (x.stride(3) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) % step == 0 and x.stride(1) % step == 0
+            and x.stride(2) % step == 0):
+        return x
+    return x.contiguous()
+
+
+def quantize_append(cache: QuantCache, k, v, start=0) -> None:
+    """Write the rows k, v [B,G,T,128] (bfloat16, float16 or float32, any strides) at positions [start, start + T).
+
+    start: an int, or an int32 [B] device tensor with each sequence's own (rows outside [0, capacity) are then not
+    written). Every block's scale is the smallest power of two, 2^-110 at least, that its rows fit under; a block that
+    already holds rows before `start` keeps its scale unless a new row needs a larger one, and then its earlier codes
+    are moved to it. So a chunked write may round a value below 2^-6 of its scale twice where one write would round it
+    once; everything else is the same. Rows at and after start + T are no longer valid rows of the block they share.
+    NaN and infinity become NaN; finite values past 1.875 * 2^127 saturate.
+    """
+    want = (cache.batch, cache.groups)
+    if k.dim() != 4 or tuple(k.shape[:2]) != want or k.shape[3] != HEAD_DIM or v.shape != k.shape:
+        raise ValueError(f"k and v must be [B, G, T, {HEAD_DIM}] with B, G = {want}, got {tuple(k.shape)} and "
+                         f"{tuple(v.shape)}")
+    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+        raise ValueError(f"k and v must both be bfloat16, float16 or float32, got {k.dtype} and {v.dtype}")
+    if k.device != cache.device or v.device != cache.device:
+        raise ValueError("k and v must live on the cache's device")
+    T = int(k.shape[2])
+    starts, at = _start(cache, start, T)
+    k, v = _rows(k, k.dtype), _rows(v, v.dtype)
+    nat.call_on(cache.device, "attnlab_quant_append", k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(),
+                v.stride(0), v.stride(1), v.stride(2), _DTYPES[k.dtype], cache.k.data_ptr(), cache.v.data_ptr(),
+                cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), nat.ptr(starts), at, cache.batch, cache.groups, T,
+                cache.capacity, cache.block, nat.stream_of(cache.device))
+
+
+def dequantize_rows(cache: QuantCache, start=0, length=None, *, dtype=torch.bfloat16):
+    """The values of positions [start, start + length) -> (k, v), each [B,G,length,128] in `dtype` (bfloat16 and float32
+    exact, float16 rounded). start: an int, or an int32 [B] device tensor (positions outside the cache then give zeros;
+    length is required). length None: to the capacity."""
+    if dtype not in _DTYPES:
+        raise ValueError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
+    if length is None:
+        if isinstance(start, torch.Tensor):
+            raise ValueError("a start per sequence needs a length")
+        length = cache.capacity - int(start)
+    T = int(length)
+    if T < 0:
+        raise ValueError(f"length={T} must not be negative")
+    starts, at = _start(cache, start, T)
+    k, v = (torch.empty(cache.batch, cache.groups, T, HEAD_DIM, dtype=dtype, device=cache.device) for _ in "kv")
+    nat.call_on(cache.device, "attnlab_quant_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(),
+                cache.v_exp.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], nat.ptr(starts), at, cache.batch,
+                cache.groups, T, cache.capacity, cache.block, nat.stream_of(cache.device))
+    return k, v
+
+
+def quant_attention(q, cache: QuantCache, *, valid_length=None, query_start=None, window=None, sinks: int = 0,
+                    scale=None, out=None, out_dtype=torch.bfloat16, partitions=None):
+    """Attention of q [B,G,h,T,128] (bfloat16) over an 8-bit cache -> [B,G,h,T,128].
+
+    The T queries sit at consecutive positions from query_start (default: the last T legal ones); query at p reads
+    positions j <= p, j < valid_length, and with a window j > p - window or j < sinks. valid_length: an int (default:
+    the capacity), or for one query an int32 [B] device tensor with each sequence's length, clamped to [0, capacity],
+    its query at the last position. A query that reads no position gets zeros. One query takes h <= 8 at every form and
+    out_dtype float32 too; a chunk, and one query with h <= 16 and an int length, gives bfloat16. partitions overrides
+    the split-K count (one query: 1..256, a chunk: 1..16).
+    """
+    return hip_range.range_attention(q, cache.k.data_ptr(), cache.v.data_ptr(),
+                                     (cache.k_exp.data_ptr(), cache.v_exp.data_ptr()), cache.block, cache.batch,
+                                     cache.groups, cache.capacity, cache.device, valid_length=valid_length,
+                                     query_start=query_start, window=window, sinks=sinks, scale=scale, out=out,
+                                     out_dtype=out_dtype, partitions=partitions)
+
+
+def quant_gather_attention(q, cache: QuantCache, selected, selected_valid=None, *, scale=None, out=None,
+                           out_dtype=torch.bfloat16, partitions=None):
+    """gather_attention over an 8-bit cache: q [B,G,h,1,128] over the listed positions selected [B,G,S] (any integer
+    type), read in place. Slots with selected_valid False, and positions outside [0, capacity), are skipped; a position
+    listed twice counts twice; a query with no row gets zeros."""
+    if selected.dim() != 3 or tuple(selected.shape[:2]) != (cache.batch, cache.groups) or selected.is_floating_point():
+        raise ValueError(f"selected must be an integer [B, G, S] tensor with B, G = {cache.batch}, {cache.groups}")
+    if selected.device != cache.device:
+        raise ValueError("selected must live on the cache's device")
+    if selected_valid is not None:
+        if selected_valid.shape != selected.shape:
+            raise ValueError("selected_valid must match selected")
+        selected = torch.where(selected_valid.bool(), selected, -1)
+    if selected.dtype == torch.int64:   # a position past 32 bits is outside the cache, not another one
+        selected = selected.clamp(-1, cache.capacity)
+    return hip_range.listed_attention(q, cache, selected.to(torch.int32).contiguous(), scale=scale, out=out,
+                                      out_dtype=out_dtype, partitions=partitions)

@@ -17,13 +17,12 @@
 #include <type_traits>
 
 #include "common.h"
+#include "mfma_attend.h"
 
 namespace attnlab {
 namespace {
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x8_t __attribute__((ext_vector_type(8)));
 
@@ -406,9 +405,6 @@ __global__ __launch_bounds__(256) void project_keys_mfma(ProjectArgs a) {
 // 2.41 GHz takes 657 us. The form before this one (K and V through registers, V transposed by 4-byte LDS stores, two
 // barriers per block) took 642 us; the 1000-token chunk after 29011 (h=2) went from 309 to 264 us.
 // ---------------------------------------------------------------------------------------------------------------
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef uint32_t u32x2v_t __attribute__((ext_vector_type(2)));
-
 struct PrefillAttendArgs {
     const uint16_t* q;      // [BG, h, T, 128]
     const uint16_t* K;      // row j of bg at K + bg * kv_bg_stride + j * kv_row_stride
@@ -430,40 +426,6 @@ constexpr int kPrefillMaxSplits = 16;
 constexpr int kPaRows = 128;          // (query, head) rows per workgroup: 4 waves x 32
 constexpr int kPaKeys = 64;           // keys per block
 constexpr float kPaLazy = 8.0f;       // rescale O only when the running max grows by more than 2^8
-
-// two fp32 -> packed bf16 pair, round to nearest even (gfx950 converts in hardware: v_cvt_pk_bf16_f32)
-typedef __bf16 bf16x2v_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t pack_bf16x2(float x, float y) {
-    const bf16x2v_t v = {(__bf16)x, (__bf16)y};
-    return __builtin_bit_cast(uint32_t, v);
-}
-
-// 16 bytes per lane from global memory straight into LDS: the wave's 64 lanes fill the 1 KB at `lds` in lane order.
-__device__ __forceinline__ void load_lds16(const uint16_t* src, uint16_t* lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
-}
-
-// The same from a buffer of `bytes` bytes at `base` (wave-uniform), lane l from byte offset `off`; zeros past the end.
-__device__ __forceinline__ void load_lds16_buf(const uint16_t* base, uint32_t bytes, uint32_t off, uint16_t* lds) {
-    const __amdgpu_buffer_rsrc_t rsrc =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(base), 0, (int)bytes, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, (int)off, 0, 0, 0);
-}
-
-// the larger of x over lanes l and l ^ 32 (v_permlane32_swap, no LDS round trip)
-__device__ __forceinline__ float max_xor32(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-// Transposing LDS read (ds_read_b64_tr_b16): each 16 lanes read a 4 x 16 matrix of 16-bit elements, lane 4 e + j the
-// elements 4 j .. 4 j + 3 of row e; lane i receives column i.
-typedef short s16x4_t __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ u32x2v_t read_tr16(const char* lds) {
-    return __builtin_bit_cast(u32x2v_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                            (__attribute__((address_space(3))) s16x4_t*)lds));
-}
 
 // K and V blocks in LDS: 64 rows of 256 bytes, sixteen 16-byte chunks each, copied by load_lds16 (no registers, no
 // store instructions), so a row's chunks can only be permuted, not padded. K: chunk c of row j at slot c ^ (j & 15):

@@ -302,6 +302,74 @@ int attnlab_prefill_attend_split(const uint16_t* q, const uint16_t* K, const uin
                                  void* stream);
 
 /*
+ * The 8-bit K/V cache (no reference counterpart; it stands beside the bf16 cache of qwen_wrap.py:68-70). One tensor:
+ *   codes  [B, G, C, 128] e4m3 (1 sign, 4 exponent, 3 mantissa bits; largest 448; 0x7f and 0xff are NaN)
+ *   exp    [B, G, ceil(C / block)] one byte x per block of `block` positions (16, 32 or 64): the scale 2^(x - 127)
+ * and a value is code * scale, exact in bf16. attnlab_quant_append writes bytes of 17 to 247.
+ *
+ * attnlab_quant_append writes T rows of K and V at [start, start + T), or per sequence at [starts[b], starts[b] + T) with
+ * starts (int32 [B] on the device) given. k: element (b, g, t, e) at k + b k_b_stride + g k_g_stride + t k_t_stride + e
+ * (elements of `dtype`: ATTNLAB_DT_BF16, _F16 or _F32; rows 16-byte aligned; strides may be 0); v likewise. Per block:
+ *   need  = the smallest 2^e >= 2^-110 with max |finite new x| <= 448 * 2^e (|x| is limited to 1.875 * 2^127 first)
+ *   scale = need if the block holds no row before the first new one, else max(its scale, need)
+ *   code  = RNE_e4m3(x / scale), a non-finite x -> NaN; a block whose scale grew has its rows before the first new one
+ *           converted from their codes, RNE_e4m3(code * old scale / scale)
+ * Rows behind the new ones keep their codes (a block's scale may have changed under them: they are not valid rows).
+ * With `starts`, positions outside [0, C) are not written; with `start`, they are refused. One call owns its blocks:
+ * calls that write the same blocks must be ordered on one stream.
+ */
+int attnlab_quant_append(const void* k, int64_t k_b_stride, int64_t k_g_stride, int64_t k_t_stride, const void* v,
+                         int64_t v_b_stride, int64_t v_g_stride, int64_t v_t_stride, int dtype, uint8_t* k_codes,
+                         uint8_t* v_codes, uint8_t* k_exp, uint8_t* v_exp, const int32_t* starts, int start, int B,
+                         int G, int T, int C, int block, void* stream);
+
+/*
+ * Reads T rows of an 8-bit cache back as values: k_out, v_out [B, G, T, 128] in `dtype` (bf16 and fp32 exact, fp16
+ * rounded to nearest even), from start, or starts[b]; with `starts`, positions outside [0, C) give zeros.
+ */
+int attnlab_quant_read(const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_exp, const uint8_t* v_exp,
+                       void* k_out, void* v_out, int dtype, const int32_t* starts, int start, int B, int G, int T, int C,
+                       int block, void* stream);
+
+/*
+ * One query's attention over the legal positions of a cache, or those of a sliding window and a few first ones (sinks):
+ *   out[b,g,i] = sum_j softmax_j(scale * q[b,g,i] . K[b,g,j]) V[b,g,j]
+ *   over j < length, j <= q_pos, and with window > 0: j > q_pos - window or j < sinks.
+ * lengths (int32 [B] on the device, nullable): every sequence's own length, clamped to [0, C], its query at the last
+ * position; length and q_pos are then ignored. A query that reads no row, or whose scores are all -inf, gets zeros.
+ * K, V: [B, G, C, 128] bf16, or with k_exp and v_exp the 8-bit cache's codes (block: its positions to a scale byte;
+ * ignored without). q: [B, G, h, 128] bf16, 1 <= h <= 8. P split-K partitions (1..256): with P > 1, part must hold
+ * B * G * P * h * 130 floats and a second launch merges them. out: [B, G, h, 128], bf16 (RNE) when out_bf16 else fp32.
+ * The counterpart of full_attention for one query (full.py:17-44) with the window of a row list F = sinks + recent
+ * (selection.py:69-86) read by range.
+ */
+int attnlab_range_decode(const void* K, const void* V, const uint8_t* k_exp, const uint8_t* v_exp, int block,
+                         const uint16_t* q, const int32_t* lengths, int length, int64_t q_pos, int window, int sinks,
+                         int B, int G, int h, int C, int P, float scale, void* out, int out_bf16, float* part,
+                         void* stream);
+
+/*
+ * attnlab_attend over an 8-bit cache: one query's attention over listed rows. rows: [B*G, S] int32 positions (row
+ * stride rows_stride), S >= 1; positions outside [0, C) are skipped, never read, and a position listed twice counts
+ * twice. q, out, P, part, scale as in attnlab_range_decode.
+ */
+int attnlab_quant_attend(const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_exp, const uint8_t* v_exp,
+                         int block, const uint16_t* q, const int32_t* rows, int64_t rows_stride, int B, int G, int h,
+                         int S, int C, int P, float scale, void* out, int out_bf16, float* part, void* stream);
+
+/*
+ * The chunk form of attnlab_range_decode, on the matrix cores: T queries at positions q_pos0 + t, query t reading
+ * j <= q_pos0 + t, j < legal, and with window > 0: j > q_pos0 + t - window or j < sinks. q, out: [B, G, h, T, 128] bf16
+ * contiguous, 1 <= h <= 16; the caches as there. What a masked position holds (NaN, infinity) does not reach an
+ * output. splits (1..16): workgroups that share a query tile's key blocks; with more than one, part (16-byte aligned,
+ * attnlab_range_prefill_part_bytes bytes) holds their partials and a second launch merges them.
+ */
+int64_t attnlab_range_prefill_part_bytes(int B, int G, int h, int T, int splits);
+int attnlab_range_prefill(const uint16_t* q, const void* K, const void* V, const uint8_t* k_exp, const uint8_t* v_exp,
+                          int block, uint16_t* out, int B, int G, int h, int T, int q_pos0, int legal, int C, int window,
+                          int sinks, float scale, int splits, float* part, int64_t part_bytes, void* stream);
+
+/*
  * Workspace (bytes) of attnlab_sparse_decode_step for these sizes: candidate scores, row list, u, tiled-select
  * scratch and split-K partials, each 256-byte aligned, then the key lists of rows of 32769 to 131072 candidates. Its
  * contents need no initialisation. A step of such rows also takes a workspace without that last region (and then selects
