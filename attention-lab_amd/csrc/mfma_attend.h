@@ -37,12 +37,26 @@ __device__ __forceinline__ float max_xor32(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// the larger of x over lanes l and l ^ 16
+__device__ __forceinline__ float max_xor16(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // Transposing LDS read (ds_read_b64_tr_b16): each 16 lanes read a 4 x 16 matrix of 16-bit elements, lane 4 e + j the
 // elements 4 j .. 4 j + 3 of row e; lane i receives column i.
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ u32x2v_t read_tr16(const char* lds) {
     return __builtin_bit_cast(u32x2v_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                             (__attribute__((address_space(3))) s16x4_t*)lds));
+}
+
+// The same of 8-bit elements (ds_read_b64_tr_b8): each 16 lanes read an 8 x 16 matrix of bytes, lane 2 e + j the bytes
+// 8 j .. 8 j + 7 of row e; lane i receives column i.
+typedef int s32x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u32x2v_t read_tr8(const char* lds) {
+    return __builtin_bit_cast(u32x2v_t, __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                                            (__attribute__((address_space(3))) s32x2_t*)lds));
 }
 
 }  // namespace attnlab

@@ -3,20 +3,25 @@
 //   out[b,g,i] = sum_j softmax_j(scale q[b,g,i] . k_j) v_j    over j in [0, s) U [lo, n), or over the listed rows
 //
 // A wave takes 32 rows at a time: S^T[keys, heads] = K Q^T, two 16-key tiles of v_mfma_f32_16x16x32_bf16, then
-// O^T[dims, heads] += V^T P^T, eight 16-dim tiles. K's rows are read from memory in the operand's order (16 keys over
-// the lanes, a row's bytes over the four lane groups), so K goes from the load to the matrix core; V's rows are written
-// to the wave's own 8 KB of LDS and read transposed (ds_read_b64_tr_b16). Both are loaded a tile ahead, and a wave waits
-// for no other until the end. An 8-bit code becomes a bf16 exactly, its block's scale included, in the one conversion
-// (v_cvt_scalef32_pk_bf16_fp8).
+// O^T[dims, heads] += V^T P^T, eight 16-dim tiles. K's rows are loaded in the operand's order (16 keys over the lanes, a
+// row's bytes over the four lane groups) and go from the load to the matrix core; V's rows pass through the wave's own LDS
+// and are read transposed. Key 8 g + 4 t + i is row 4 g + i of tile t, so that a lane's eight weights are those of the
+// eight consecutive keys whose V it reads. The waves wait for each other only at the end.
+// An 8-bit code becomes a bf16 exactly, its block's scale included, in one conversion (v_cvt_scalef32_pk_bf16_fp8). The
+// matrix cores' own fp8 products would save K's, but they sum with about 16 bits (2^-16 of the summed magnitudes off on
+// N(0, 1) rows, 2^-13 on rows of mixed magnitudes, where the bf16 products stay within fp32's rounding).
 //
 // The 16 columns of a tile are 8 heads twice: columns 0..7 multiply V by P rounded to bf16, columns 8..15 by what that
 // rounding left, and the two are added at the end, so the weights keep 16 bits without a second product. Softmax is
-// online in the log2 domain with a lazy rescale; sums and outputs are fp32. The waves of a workgroup merge through LDS,
-// the P workgroups of a (b, g) through partials and a second small launch: no state outlives the call, so two graphs, or
-// two streams, share nothing.
+// online in the log2 domain; the running max moves, and sums are rescaled, only when a score passes it by 2^8, so most
+// tiles need no exchange between lanes. Sums and outputs are fp32. The waves of a workgroup merge through LDS, the P
+// workgroups of a (b, g) through partials and a second small launch: no state outlives the call, so two graphs, or two
+// streams, share nothing.
 //
-// Masked rows: their scores are replaced, and their V rows written as zeros, so whatever they hold (NaN, infinity) leaves
-// the output alone. A query with no row to read, or whose scores are all -inf, gets zeros.
+// Masked rows: their scores are replaced, and their V rows are zeros, so whatever they hold (NaN, infinity) leaves the
+// output alone. A query with no row to read, or whose scores are all -inf, gets zeros.
+#include <cfloat>
+
 #include "mfma_attend.h"
 #include "quant.h"
 
@@ -43,58 +48,124 @@ struct RangeArgs {
     const int32_t* lengths;   // [B] valid lengths, the query at the last position; or null: `n` and `qend`
     const int32_t* rows;      // [B * G, S] (listed rows)
     int64_t rows_stride;
-    int G, h, C, P, shift, nb;
+    int B, G, h, C, P, shift, nb;
     int n;                    // keys [0, n); the number of listed rows
     int64_t qend;             // the query's position + 1, where the window ends
     int window, sinks;        // window 0: none
     float scale_log2;
     void* out;
     int out_bf16;
-    float* part;              // [B * G, P, h, 130]: m, l, the unnormalised outputs (P > 1)
+    float* part;              // [slot, h, 130]: m, l, the unnormalised outputs (P > 1; B * G * P slots)
 };
 
-// One tile of a wave in flight. 8-bit: K two 16-byte loads a row (bytes 16 g .. and 64 + 16 g ..), V eight lanes a row;
-// bf16: twice as many. `ex`: lane l holds the scale byte of row l % 32, of K (l < 32) or V.
+// The rows a sequence of n keys reads: positions [0, s) and [lo, n), in aligned tiles of 32 (a scale block is 16 positions
+// or more, so a tile's eights share a scale); the second range's first tile may begin before lo.
+struct Span {
+    int s, lo, n;
+    __device__ __forceinline__ int first_tiles() const { return (s + kTile - 1) / kTile; }
+    __device__ __forceinline__ int from() const { return lo & ~(kTile - 1); }
+    __device__ __forceinline__ int tiles() const {
+        return first_tiles() + (n > lo ? (n - from() + kTile - 1) / kTile : 0);
+    }
+};
+__device__ __forceinline__ Span span_of(const RangeArgs& a, int n, int64_t qend) {
+    Span r{0, 0, n};
+    if (a.window > 0) {
+        r.s = min(a.sinks, n);
+        r.lo = (int)min((int64_t)n, max(qend - a.window, (int64_t)r.s));
+    }
+    return r;
+}
+__device__ __forceinline__ Span span_of_sequence(const RangeArgs& a, int b) {
+    const int n = min(max(a.lengths[b], 0), a.C);
+    return span_of(a, n, n);
+}
+
+// With a length per sequence and P > 1 the B P slots of a group go to the sequences by their tiles: sequence b takes
+// ceil(tiles_b / share), the share being the least (of 4 tiles or more) with which B (P - 1) slots would hold them all
+// evenly, so B more hold every remainder. Each workgroup works this out for itself, 64 sequences at a time.
+__device__ __forceinline__ int share_of(const RangeArgs& a) {
+    const int lane = threadIdx.x & 63;
+    uint32_t total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const uint32_t x = b0 + lane < a.B ? (uint32_t)span_of_sequence(a, b0 + lane).tiles() : 0u;
+        total += (uint32_t)__builtin_amdgcn_readlane((int)wave_incl_scan(x), 63);
+    }
+    const uint32_t even = (uint32_t)(a.B * (a.P - 1));
+    return (int)max((uint32_t)kWaves, (total + even - 1) / even);
+}
+// The sequence `by_slot` belongs to (or, by_slot < 0, `b` itself): b, its first slot and its number of slots. b = a.B where
+// the slot is nobody's.
+__device__ __forceinline__ void slots_of(const RangeArgs& a, int share, int by_slot, int& b, int& first, int& count) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+        const uint32_t x = b0 + lane < a.B ? (uint32_t)((span_of_sequence(a, b0 + lane).tiles() + share - 1) / share) : 0u;
+        const uint32_t to = wave_incl_scan(x) + (uint32_t)base;   // the slots of this lane's sequence end here
+        const uint64_t hit = by_slot < 0 ? (b >= b0 && b < b0 + 64 ? 1ull << (b - b0) : 0ull)
+                                         : __ballot((int)to > by_slot);
+        if (hit) {
+            const int at = __builtin_ctzll(hit);
+            b = b0 + at;
+            count = __builtin_amdgcn_readlane((int)x, at);
+            first = __builtin_amdgcn_readlane((int)to, at) - count;
+            return;
+        }
+        base = __builtin_amdgcn_readlane((int)to, 63);
+    }
+    b = a.B;
+    first = count = 0;
+}
+
+// One tile of a wave. 8-bit: K two 16-byte loads a row (bytes 16 g .. and 64 + 16 g ..), V eight lanes a row; bf16: twice
+// as many. Scale bytes: of this lane's K row of tile 0 and 1, and of V (of its eight keys; in a list of key
+// 8 g4 + n16 % 8).
 template <bool Q8>
 struct Tile {
     u32x4_t k[2][Q8 ? 2 : 4];
     u32x4_t v[Q8 ? 4 : 8];
-    uint32_t ex;
+    uint32_t kx[2], vx;
 };
 
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const uint8_t* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, (int)bytes, 0x00020000);
+}
+
 template <bool Q8, bool LIST>
-__global__ __launch_bounds__(256, 2) void range_attend(RangeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 3) void range_attend(RangeArgs a) {
     constexpr int kRow = Q8 ? kDim : 2 * kDim;          // bytes of a row
     constexpr int kLanes = kRow / 16;                   // lanes of a V row
+    constexpr int kKLoads = Q8 ? 2 : 4, kVLoads = Q8 ? 4 : 8;
     __shared__ __attribute__((aligned(1024))) uint16_t v_sh[kWaves][kTile * kDim];   // a wave's V tile; then the merge
     __shared__ float ml_sh[kWaves][16][2];
     __shared__ int list_sh[LIST ? kListChunk : 1];
-    const int lin = xcd_contiguous_block();
-    const int bg = lin / a.P, p = lin - bg * a.P;
+    __shared__ __attribute__((aligned(8))) uint8_t vx_sh[kWaves][kTile];
+    const int lin = __builtin_amdgcn_readfirstlane(xcd_contiguous_block());
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, g4 = lane >> 4;
 
-    // the entries 0 .. count - 1 of this (b, g): positions [0, s) and [lo, n), or the list
-    int s = 0, lo = 0, count = a.n;
-    if constexpr (!LIST) {
-        int n = a.n;
-        int64_t qend = a.qend;
-        if (a.lengths) {
-            n = min(max(a.lengths[bg / a.G], 0), a.C);
-            qend = n;
-        }
-        if (a.window > 0) {
-            s = min(a.sinks, n);
-            const int64_t from = qend - a.window;
-            lo = (int)min((int64_t)n, max(from, (int64_t)s));
-        }
-        count = s + n - lo;
+    // this workgroup's (b, g), its rows, and its tiles [t0, t1) of them
+    int bg, p, share;
+    Span rows{0, 0, a.n};   // the list's entries, or a range
+    if (!LIST && a.lengths && a.P > 1) {
+        const int g = lin / (a.B * a.P);
+        int b, first, count;
+        share = share_of(a);
+        slots_of(a, share, lin - g * a.B * a.P, b, first, count);
+        if (b >= a.B) return;
+        p = lin - g * a.B * a.P - first;
+        bg = b * a.G + g;
+        rows = span_of_sequence(a, b);
+    } else {
+        bg = lin / a.P;
+        p = lin - bg * a.P;
+        if constexpr (!LIST) rows = a.lengths ? span_of_sequence(a, bg / a.G) : span_of(a, a.n, a.qend);
+        share = (rows.tiles() + a.P - 1) / a.P;
     }
-    // partitions of whole tiles
-    const int tiles = (count + kTile - 1) / kTile;
-    const int per = ((tiles + a.P - 1) / a.P) * kTile;
-    const int e0 = (int)min((int64_t)p * per, (int64_t)count), e1 = min(e0 + per, count);
+    const int s = rows.s, lo = rows.lo, n = rows.n, from = rows.from();
+    const int na = rows.first_tiles(), tiles = rows.tiles();
+    const int t0 = (int)min((int64_t)p * share, (int64_t)tiles), t1 = min(t0 + share, tiles);
 
     // Q^T as the B operand: column n16 is head n16 % 8; its 8 dims of step kk, in the order K's bytes are loaded in
     bf16x8_t qb[4];
@@ -109,167 +180,225 @@ __global__ __launch_bounds__(256, 2) void range_attend(RangeArgs a) {
             qb[kk] = __builtin_bit_cast(bf16x8_t, w);
         }
     }
+    // the scale (log2 domain), made positive: a negative one flips the sign of q instead (exact), and zero becomes the
+    // smallest normal float, which gives the same weights while a masked key's -inf * scale stays -inf
+    const float sc = a.scale_log2 == 0.0f ? FLT_MIN : fabsf(a.scale_log2);
+    if (a.scale_log2 < 0.0f) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+            qb[kk] = __builtin_bit_cast(bf16x8_t, __builtin_bit_cast(u32x4_t, qb[kk]) ^ 0x80008000u);
+    }
     const uint8_t* Kb = a.K + (size_t)bg * a.C * kRow;
     const uint8_t* Vb = a.V + (size_t)bg * a.C * kRow;
     const uint8_t* keb = Q8 ? a.ke + (size_t)bg * a.nb : nullptr;
     const uint8_t* veb = Q8 ? a.ve + (size_t)bg * a.nb : nullptr;
+    // This lane's rows of a tile: K row 8 (n16 / 4) + 4 t + n16 % 4 of operand t; V rows u (64 / kLanes) + vrow.
+    const int krow = 8 * (n16 >> 2) + (n16 & 3), vrow = lane / kLanes;
+    // V in LDS. 8-bit: 128-byte rows of 8 chunks, chunk c of row r at c ^ (r / 2 % 8); bf16: 256-byte rows of 16 chunks,
+    // chunk c of row r at c ^ (4 (r % 4)): the rows that a transposing read takes together then lie in different banks
+    // (8-bit: lane 2 e + j of 16 reads 8 bytes of row 8 g4 + e and gets 8 rows of one dim; bf16: lane 4 e + j four
+    // elements of row 8 g4 + 4 t + e, and gets 4 rows).
+    char* vt = reinterpret_cast<char*>(v_sh[wave]);
+    const int vst = Q8 ? 128 * vrow + 16 * ((lane & 7) ^ (vrow >> 1)) : 256 * vrow + 16 * ((lane & 15) ^ (4 * (vrow & 3)));
+    const int vof8 = 128 * (8 * g4 + (n16 >> 1)) + 16 * (4 * (g4 & 1) + (n16 >> 2)) + 8 * (n16 & 1);
+    int vof[4];
+    if constexpr (!Q8) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) vof[x] = 256 * (8 * g4 + (n16 >> 2)) + 64 * (x ^ (n16 >> 2)) + 8 * (n16 & 3);
+    }
 
     float m = -INFINITY, l = 0.0f;
     f32x4_t o[8];
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    uint16_t* vt = v_sh[wave];
 
-    for (int c0 = e0; c0 < e1; c0 += LIST ? kListChunk : max(e1 - e0, 1)) {
-        const int clen = LIST ? min(kListChunk, e1 - c0) : e1 - c0;
+    int c0 = 0;   // first tile of the list chunk in LDS
+    // first position of a range's tile, the end of its range, and where the range begins
+    auto range_tile = [&](int t, int& base, int& end, int& begin) {
+        const bool first = t < na;
+        base = first ? kTile * t : from + kTile * (t - na);
+        end = first ? s : n;
+        begin = first ? 0 : lo;
+    };
+    auto entry = [&](int t, int r) -> int { return list_sh[kTile * (t - c0) + r]; };   // position of row r, or -1
+    auto issue = [&](int t, Tile<Q8>& f) {
         if constexpr (LIST) {
-            if (c0 != e0) __syncthreads();
-            const int32_t* src = a.rows + (size_t)bg * a.rows_stride + c0;
-            for (int i = tid; i < clen; i += 256) {
-                const int pos = src[i];
-                list_sh[i] = (unsigned)pos < (unsigned)a.C ? pos : -1;
-            }
-            __syncthreads();
-        }
-        const int nt = (clen + kTile - 1) / kTile;
-        // entry e of the chunk -> its position, or -1: past the chunk, or a listed position outside [0, C)
-        auto position = [&](int e) -> int {
-            if constexpr (LIST) return e < clen ? list_sh[e] : -1;
-            const int x = c0 + e;
-            return e < clen ? (x < s ? x : x - s + lo) : -1;
-        };
-        auto issue = [&](int t, Tile<Q8>& f) {
-            const int e = kTile * t;
+            int kp[2];
 #pragma unroll
             for (int t2 = 0; t2 < 2; ++t2) {
-                const uint8_t* r = Kb + (size_t)max(position(e + 16 * t2 + n16), 0) * kRow + 16 * g4;
+                kp[t2] = max(entry(t, krow + 4 * t2), 0);
+                f.kx[t2] = keb[kp[t2] >> a.shift];
+            }
+            f.vx = veb[max(entry(t, 8 * g4 + (n16 & 7)), 0) >> a.shift];
 #pragma unroll
-                for (int c = 0; c < (Q8 ? 2 : 4); ++c)
+            for (int t2 = 0; t2 < 2; ++t2) {
+                const uint8_t* r = Kb + (size_t)kp[t2] * kRow + 16 * g4;
+#pragma unroll
+                for (int c = 0; c < kKLoads; ++c)
                     f.k[t2][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(r + 64 * c));
             }
 #pragma unroll
-            for (int u = 0; u < (Q8 ? 4 : 8); ++u) {
-                const int row = u * (64 / kLanes) + lane / kLanes;
-                const uint8_t* r = Vb + (size_t)max(position(e + row), 0) * kRow + 16 * (lane % kLanes);
+            for (int u = 0; u < kVLoads; ++u) {
+                const uint8_t* r = Vb + (size_t)max(entry(t, (64 / kLanes) * u + vrow), 0) * kRow + 16 * (lane % kLanes);
                 f.v[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(r));
             }
-            if constexpr (Q8) f.ex = (lane < 32 ? keb : veb)[max(position(e + (lane & 31)), 0) >> a.shift];
-        };
-        auto compute = [&](int t, const Tile<Q8>& f) {
-            const int e = kTile * t;
-            const uint32_t ok = (uint32_t)__ballot(position(e + (lane & 31)) >= 0);   // rows of the tile to read
-            f32x4_t sc[2];
-#pragma unroll
-            for (int t2 = 0; t2 < 2; ++t2) {
-                sc[t2] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-                float ks = 1.0f;
-                if constexpr (Q8) ks = scale_of(__shfl(f.ex, 16 * t2 + n16, 64));
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    u32x4_t w;
-                    if constexpr (Q8) {
-                        const u32x4_t c = f.k[t2][kk >> 1];
-                        const uint32_t w0 = kk & 1 ? c.z : c.x, w1 = kk & 1 ? c.w : c.y;
-                        w = u32x4_t{e4m3_to_bf16x2<false>(w0, ks), e4m3_to_bf16x2<true>(w0, ks),
-                                    e4m3_to_bf16x2<false>(w1, ks), e4m3_to_bf16x2<true>(w1, ks)};
-                    } else {
-                        w = f.k[t2][kk];
-                    }
-                    sc[t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), qb[kk], sc[t2], 0,
-                                                                     0, 0);
-                }
+        } else {   // rows past the range read as zeros: the buffer ends there
+            int base, end, begin;
+            range_tile(t, base, end, begin);
+            const uint32_t bytes = (uint32_t)min(kTile, end - base) * kRow;
+            const __amdgpu_buffer_rsrc_t kr = buffer(Kb + (size_t)base * kRow, bytes);
+            const __amdgpu_buffer_rsrc_t vr = buffer(Vb + (size_t)base * kRow, bytes);
+            if constexpr (Q8) {
+                f.kx[0] = f.kx[1] = __builtin_amdgcn_raw_buffer_load_b8(buffer(keb, (uint32_t)a.nb),
+                                                                        (base + 8 * (n16 >> 2)) >> a.shift, 0, 0);
+                f.vx = __builtin_amdgcn_raw_buffer_load_b8(buffer(veb, (uint32_t)a.nb), (base + 8 * g4) >> a.shift, 0, 0);
             }
-            // this lane's scores: column n16, rows 16 t2 + 4 g4 + i
-            float bm = -INFINITY;
+            constexpr int kNt = 2;   // non-temporal
 #pragma unroll
             for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = sc[t2][i] * a.scale_log2;
-                    if (ok != 0xffffffffu && !(ok >> (16 * t2 + 4 * g4 + i) & 1)) x = -INFINITY;
-                    sc[t2][i] = x;
-                    bm = fmaxf(bm, x);
-                }
-            bm = fmaxf(bm, shfl_xor_f32(bm, 16));
-            bm = fmaxf(bm, shfl_xor_f32(bm, 32));
-            if (__any(bm > m + kLazy)) {
-                if (bm > m + kLazy) {   // also a column's first rows (m = -inf)
-                    const float al = fast_exp2(m - bm);
-                    l *= al;
+                for (int c = 0; c < kKLoads; ++c)
+                    f.k[t2][c] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                                                 kr, krow * kRow + 16 * g4 + 4 * t2 * kRow + 64 * c, 0, kNt));
 #pragma unroll
-                    for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[dt][i] *= al;
-                    m = bm;
-                }
-            }
-            const float mb = m == -INFINITY ? 0.0f : m;   // no score above -inf yet: every weight 0
-            uint32_t w4[4];
-#pragma unroll
-            for (int t2 = 0; t2 < 2; ++t2) {
-                float pr[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    pr[i] = fast_exp2(sc[t2][i] - mb);
-                    l += pr[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t hi = pack_bf16x2(pr[2 * i], pr[2 * i + 1]);
-                    const uint32_t rest = pack_bf16x2(pr[2 * i] - bf16_lo(hi), pr[2 * i + 1] - bf16_hi(hi));
-                    w4[2 * t2 + i] = n16 < 8 ? hi : rest;
-                }
-            }
-            const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{w4[0], w4[1], w4[2], w4[3]});
-            // V into LDS as bf16 rows of 16 chunks of 8; chunk c of row r at c ^ (4 (r & 3)), so that a transposing
-            // read's four rows lie in four different quarters of the banks
-#pragma unroll
-            for (int u = 0; u < (Q8 ? 4 : 8); ++u) {
-                const int row = u * (64 / kLanes) + lane / kLanes, c = lane % kLanes;
-                u32x4_t x = f.v[u];
-                if (ok != 0xffffffffu && !(ok >> row & 1)) x = u32x4_t{0, 0, 0, 0};
-                u32x4_t* dst = reinterpret_cast<u32x4_t*>(vt + row * kDim);
-                const int swz = 4 * (row & 3);
-                if constexpr (Q8) {
-                    const float vs = scale_of(__shfl(f.ex, 32 + row, 64));
-                    dst[(2 * c) ^ swz] = u32x4_t{e4m3_to_bf16x2<false>(x.x, vs), e4m3_to_bf16x2<true>(x.x, vs),
-                                                 e4m3_to_bf16x2<false>(x.y, vs), e4m3_to_bf16x2<true>(x.y, vs)};
-                    dst[(2 * c + 1) ^ swz] = u32x4_t{e4m3_to_bf16x2<false>(x.z, vs), e4m3_to_bf16x2<true>(x.z, vs),
-                                                     e4m3_to_bf16x2<false>(x.w, vs), e4m3_to_bf16x2<true>(x.w, vs)};
-                } else {
-                    dst[c ^ swz] = x;
-                }
-            }
-            // a wave's LDS operations take effect in order; these keep the compiler from moving them past each other
-            asm volatile("" ::: "memory");
-            const int j = n16 >> 2;   // row of the four this lane reads from, elements 4 (n16 % 4) ..
-#pragma unroll
-            for (int dt = 0; dt < 8; ++dt) {
-                u32x2v_t w[2];
-#pragma unroll
-                for (int t2 = 0; t2 < 2; ++t2) {
-                    const int row = 16 * t2 + 4 * g4 + j;
-                    const int slot = (2 * dt + ((n16 >> 1) & 1)) ^ (4 * (row & 3));
-                    w[t2] = read_tr16(reinterpret_cast<const char*>(vt) + 256 * row + 16 * slot + 8 * (n16 & 1));
-                }
-                const bf16x8_t va = __builtin_bit_cast(bf16x8_t, u32x4_t{w[0].x, w[0].y, w[1].x, w[1].y});
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pb, o[dt], 0, 0, 0);
-            }
-            asm volatile("" ::: "memory");
-        };
-        // tile t of the chunk belongs to wave t % kWaves; the next one is in flight while one is computed
-        Tile<Q8> f[2];
-        int t = wave;
-        if (t < nt) issue(t, f[0]);
-        while (t < nt) {
-            if (t + kWaves < nt) issue(t + kWaves, f[1]);
-            compute(t, f[0]);
-            t += kWaves;
-            if (t >= nt) break;
-            if (t + kWaves < nt) issue(t + kWaves, f[0]);
-            compute(t, f[1]);
-            t += kWaves;
+            for (int u = 0; u < kVLoads; ++u)
+                f.v[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, 16 * lane + 1024 * u, 0, kNt));
         }
+        // every load is on its way before the first result is waited for
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto compute = [&](int t, Tile<Q8>& f) {
+        uint32_t ok;   // rows of the tile to read
+        if constexpr (LIST) {
+            ok = (uint32_t)__ballot(entry(t, lane & 31) >= 0);
+        } else {
+            int base, end, begin;
+            range_tile(t, base, end, begin);
+            const int rows = end - base, skip = begin - base;
+            ok = rows >= kTile ? 0xffffffffu : (1u << rows) - 1u;
+            if (skip > 0) ok &= 0xffffffffu << skip;
+        }
+        f32x4_t sv[2];
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2) {
+            sv[t2] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            float ks = 1.0f;
+            if constexpr (Q8) ks = scale_of(f.kx[t2]);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                u32x4_t w;
+                if constexpr (Q8) {
+                    const u32x4_t c = f.k[t2][kk >> 1];
+                    const uint32_t w0 = kk & 1 ? c.z : c.x, w1 = kk & 1 ? c.w : c.y;
+                    w = u32x4_t{e4m3_to_bf16x2<false>(w0, ks), e4m3_to_bf16x2<true>(w0, ks),
+                                e4m3_to_bf16x2<false>(w1, ks), e4m3_to_bf16x2<true>(w1, ks)};
+                } else {
+                    w = f.k[t2][kk];
+                }
+                sv[t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), qb[kk], sv[t2], 0, 0, 0);
+            }
+        }
+        // V on its way to LDS while the scores are made
+        if (ok != 0xffffffffu) {
+            asm volatile("");   // a branch, not selects: few tiles are partial
+#pragma unroll
+            for (int u = 0; u < kVLoads; ++u)
+                if (!(ok >> ((64 / kLanes) * u + vrow) & 1)) f.v[u] = u32x4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < kVLoads; ++u) {
+            // 8-bit: r / 2 % 8 of row 8 u + vrow is vrow / 2 ^ 4 (u % 2)
+            const int at = Q8 ? (vst ^ (64 * (u & 1))) + 1024 * u : vst + 1024 * u;
+            *reinterpret_cast<u32x4_t*>(vt + at) = f.v[u];
+        }
+        if constexpr (LIST) {   // the scale bytes of V's 32 rows, to be read by eights
+            if (n16 < 8) vx_sh[wave][8 * g4 + n16] = (uint8_t)f.vx;
+        }
+        // this lane's scores: column n16, keys 8 g4 + 4 t2 + i
+        if (ok != 0xffffffffu) {
+            asm volatile("");
+#pragma unroll
+            for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!(ok >> (8 * g4 + 4 * t2 + i) & 1)) sv[t2][i] = -INFINITY;
+        }
+        float bm = -INFINITY;
+#pragma unroll
+        for (int t2 = 0; t2 < 2; ++t2)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) bm = fmaxf(bm, sv[t2][i]);
+        if (__any(bm * sc > m + kLazy)) {
+            bm = max_xor32(max_xor16(bm)) * sc;
+            if (bm > m + kLazy) {   // also a column's first rows (m = -inf)
+                const float al = fast_exp2(m - bm);
+                l *= al;
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[dt][i] *= al;
+                m = bm;
+            }
+        }
+        const float nm = m == -INFINITY ? 0.0f : -m;   // no score above -inf yet: every weight 0
+        float pr[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pr[i] = fast_exp2(fmaf(sv[i >> 2][i & 3], sc, nm));
+        l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+        // a wave's LDS operations take effect in order; these keep the compiler from moving them past each other
+        asm volatile("" ::: "memory");
+        if constexpr (LIST) {   // V's rows have scales of their own: they go into the weights
+            const uint2 x = *reinterpret_cast<const uint2*>(&vx_sh[wave][8 * g4]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pr[i] *= scale_of((i < 4 ? x.x : x.y) >> (8 * (i & 3)) & 255u);
+        }
+        uint32_t w4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t hi = pack_bf16x2(pr[2 * i], pr[2 * i + 1]);
+            const uint32_t rest = pack_bf16x2(pr[2 * i] - bf16_lo(hi), pr[2 * i + 1] - bf16_hi(hi));
+            w4[i] = n16 < 8 ? hi : rest;
+        }
+        const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{w4[0], w4[1], w4[2], w4[3]});
+        const float vs = Q8 && !LIST ? scale_of(f.vx) : 1.0f;
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+            u32x4_t w;
+            if constexpr (Q8) {
+                const u32x2v_t c = read_tr8(vt + (vof8 ^ (16 * dt)));
+                w = u32x4_t{e4m3_to_bf16x2<false>(c.x, vs), e4m3_to_bf16x2<true>(c.x, vs), e4m3_to_bf16x2<false>(c.y, vs),
+                            e4m3_to_bf16x2<true>(c.y, vs)};
+            } else {
+                const char* r = vt + vof[dt >> 1] + 32 * (dt & 1);
+                const u32x2v_t w0 = read_tr16(r), w1 = read_tr16(r + 4 * 256);
+                w = u32x4_t{w0.x, w0.y, w1.x, w1.y};
+            }
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), pb, o[dt], 0, 0, 0);
+        }
+        asm volatile("" ::: "memory");
+    };
+    auto walk = [&](int ta, int tb) {   // tile t of [ta, tb) belongs to wave (t - ta) % kWaves
+        for (int t = ta + wave; t < tb; t += kWaves) {
+            Tile<Q8> f;
+            issue(t, f);
+            compute(t, f);
+        }
+    };
+    if constexpr (LIST) {
+        for (c0 = t0; c0 < t1; c0 += kListChunk / kTile) {
+            const int tb = min(c0 + kListChunk / kTile, t1);
+            const int32_t* src = a.rows + (size_t)bg * a.rows_stride + (size_t)kTile * c0;
+            const int len = min(kTile * (tb - c0), n - kTile * c0);
+            if (c0 != t0) __syncthreads();
+            for (int i = tid; i < kTile * (tb - c0); i += 64 * kWaves) {
+                const int pos = i < len ? src[i] : -1;
+                list_sh[i] = (unsigned)pos < (unsigned)a.C ? pos : -1;
+            }
+            __syncthreads();
+            walk(c0, tb);
+        }
+    } else {
+        walk(t0, t1);
     }
     l += shfl_xor_f32(l, 16);
     l += shfl_xor_f32(l, 32);
@@ -286,7 +415,7 @@ __global__ __launch_bounds__(256, 2) void range_attend(RangeArgs a) {
     for (int dt = 0; dt < 8; ++dt)
         *reinterpret_cast<f32x4_t*>(red + (wave * 16 + n16) * kDim + 16 * dt + 4 * g4) = o[dt];
     __syncthreads();
-    for (int idx = tid; idx < a.h * kDim; idx += 256) {
+    for (int idx = tid; idx < a.h * kDim; idx += 64 * kWaves) {
         const int i = idx / kDim, d = idx - i * kDim;
         float ms = -INFINITY;
 #pragma unroll
@@ -306,7 +435,7 @@ __global__ __launch_bounds__(256, 2) void range_attend(RangeArgs a) {
             if (a.out_bf16) reinterpret_cast<uint16_t*>(a.out)[at] = f32_to_bf16_rne(r);
             else reinterpret_cast<float*>(a.out)[at] = r;
         } else {
-            float* pp = a.part + (((size_t)bg * a.P + p) * a.h + i) * kPartWords;
+            float* pp = a.part + ((size_t)lin * a.h + i) * kPartWords;
             if (d == 0) {
                 pp[0] = ms;
                 pp[1] = ls;
@@ -316,25 +445,39 @@ __global__ __launch_bounds__(256, 2) void range_attend(RangeArgs a) {
     }
 }
 
-// The partials of every (b, g, head) merged in partition order: thread -> (head, dim).
-__global__ __launch_bounds__(128) void range_combine(RangeArgs a) {
-    const int lin = xcd_contiguous_block();
-    const int bg = lin / a.h, i = lin - bg * a.h, d = threadIdx.x;
-    const float* pb = a.part + ((size_t)bg * a.P * a.h + i) * kPartWords;
+// The partials of a (b, g, head) merged: W waves (one for every four slots, at most eight) take every W-th slot, four of
+// them in flight at once, and meet in LDS; lane l holds dims 2 l, 2 l + 1. Every sum's order is fixed by the slots' numbers.
+constexpr int kMergeWaves = 8;
+__global__ __launch_bounds__(64 * kMergeWaves) void range_combine(RangeArgs a) {
+    const int W = blockDim.x >> 6;
+    __shared__ float ml_sh[kMergeWaves][2];
+    __shared__ float2 acc_sh[kMergeWaves][64];
+    const int bg = blockIdx.x / a.h, i = blockIdx.x - bg * a.h;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int first = bg * a.P, count = a.P;
+    if (a.lengths) {
+        int b = bg / a.G;
+        slots_of(a, share_of(a), -1, b, first, count);
+        first += (bg - b * a.G) * a.B * a.P;
+    }
+    const float* pb = a.part + ((size_t)first * a.h + i) * kPartWords;
     const size_t step = (size_t)a.h * kPartWords;
-    float ms = -INFINITY, ls = 0.0f, as = 0.0f;
-    constexpr int kGroup = 8;   // partials in flight
-    for (int p0 = 0; p0 < a.P; p0 += kGroup) {
-        float mv[kGroup], lv[kGroup], av[kGroup];
+    float ms = -INFINITY, ls = 0.0f;
+    float2 as = make_float2(0.0f, 0.0f);
+    constexpr int kGroup = 4;   // slots in flight
+    for (int p0 = wave; p0 < count; p0 += kGroup * W) {
+        float mv[kGroup], lv[kGroup];
+        float2 av[kGroup];
 #pragma unroll
         for (int u = 0; u < kGroup; ++u) {
             mv[u] = -INFINITY;
-            lv[u] = av[u] = 0.0f;
-            if (p0 + u < a.P) {
-                const float* pp = pb + (p0 + u) * step;
+            lv[u] = 0.0f;
+            av[u] = make_float2(0.0f, 0.0f);
+            if (p0 + u * W < count) {
+                const float* pp = pb + (p0 + u * W) * step;
                 mv[u] = pp[0];
                 lv[u] = pp[1];
-                av[u] = pp[2 + d];
+                av[u] = *reinterpret_cast<const float2*>(pp + 2 + 2 * lane);
             }
         }
         float mn = ms;
@@ -342,30 +485,54 @@ __global__ __launch_bounds__(128) void range_combine(RangeArgs a) {
         for (int u = 0; u < kGroup; ++u) mn = fmaxf(mn, mv[u]);
         const float w0 = ms == -INFINITY ? 1.0f : fast_exp2(ms - mn);
         ls *= w0;
-        as *= w0;
+        as.x *= w0;
+        as.y *= w0;
 #pragma unroll
         for (int u = 0; u < kGroup; ++u) {
             const float w = mv[u] == -INFINITY ? (lv[u] == 0.0f ? 0.0f : 1.0f) : fast_exp2(mv[u] - mn);
             ls += w * lv[u];
-            as += w * av[u];
+            as.x += w * av[u].x;
+            as.y += w * av[u].y;
         }
         ms = mn;
     }
-    const float r = ls == 0.0f ? 0.0f : as / ls;
-    const size_t at = ((size_t)bg * a.h + i) * kDim + d;
-    if (a.out_bf16) reinterpret_cast<uint16_t*>(a.out)[at] = f32_to_bf16_rne(r);
-    else reinterpret_cast<float*>(a.out)[at] = r;
+    if (lane == 0) {
+        ml_sh[wave][0] = ms;
+        ml_sh[wave][1] = ls;
+    }
+    acc_sh[wave][lane] = as;
+    __syncthreads();
+    if (wave != 0) return;
+    float mt = ms;
+    for (int w = 1; w < W; ++w) mt = fmaxf(mt, ml_sh[w][0]);
+    float lt = 0.0f;
+    float2 at = make_float2(0.0f, 0.0f);
+    for (int w = 0; w < W; ++w) {
+        const float mw = ml_sh[w][0], lw = ml_sh[w][1];
+        const float x = mw == -INFINITY ? (lw == 0.0f ? 0.0f : 1.0f) : fast_exp2(mw - mt);
+        lt += x * lw;
+        at.x += x * acc_sh[w][lane].x;
+        at.y += x * acc_sh[w][lane].y;
+    }
+    if (lt == 0.0f) {
+        at = make_float2(0.0f, 0.0f);
+        lt = 1.0f;
+    }
+    const size_t to = ((size_t)bg * a.h + i) * kDim + 2 * lane;
+    if (a.out_bf16) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + to) = pack_bf16x2(at.x / lt, at.y / lt);
+    else *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + to) = make_float2(at.x / lt, at.y / lt);
 }
 
 template <bool LIST>
-int launch_range(const RangeArgs& a, int B, hipStream_t s) {
-    const int64_t blocks = (int64_t)B * a.G * a.P;
+int launch_range(const RangeArgs& a, hipStream_t s) {
+    const int64_t blocks = (int64_t)a.B * a.G * a.P;
     ATTNLAB_REQUIRE(blocks < (int64_t)1 << 31, "grid of %lld workgroups is too large", (long long)blocks);
-    const dim3 grid((unsigned)blocks), wg(256);
+    const dim3 grid((unsigned)blocks), wg(64 * kWaves);
     if constexpr (LIST) hipLaunchKernelGGL((range_attend<true, true>), grid, wg, 0, s, a);
     else if (a.ke) hipLaunchKernelGGL((range_attend<true, false>), grid, wg, 0, s, a);
     else hipLaunchKernelGGL((range_attend<false, false>), grid, wg, 0, s, a);
-    if (a.P > 1) hipLaunchKernelGGL(range_combine, dim3((unsigned)(B * a.G * a.h)), dim3(kDim), 0, s, a);
+    if (a.P > 1) hipLaunchKernelGGL(range_combine, dim3((unsigned)(a.B * a.G * a.h)),
+                                    dim3(64 * (a.P <= 4 ? 1 : a.P <= 8 ? 2 : a.P <= 16 ? 4 : kMergeWaves)), 0, s, a);
     return check_launch(LIST ? "range_attend (rows)" : "range_attend");
 }
 
@@ -387,8 +554,10 @@ int check_range(const void* K, const void* V, const uint8_t* k_exp, const uint8_
 }
 
 RangeArgs range_args(const void* K, const void* V, const uint8_t* k_exp, const uint8_t* v_exp, int block,
-                     const uint16_t* q, int G, int h, int C, int P, float scale, void* out, int out_bf16, float* part) {
+                     const uint16_t* q, int B, int G, int h, int C, int P, float scale, void* out, int out_bf16,
+                     float* part) {
     RangeArgs a{};
+    a.B = B;
     a.K = static_cast<const uint8_t*>(K);
     a.V = static_cast<const uint8_t*>(V);
     a.ke = k_exp;
@@ -424,13 +593,13 @@ extern "C" int attnlab_range_decode(const void* K, const void* V, const uint8_t*
     ATTNLAB_REQUIRE(lengths != nullptr || q_pos >= 0, "the query's position %lld must not be negative",
                     (long long)q_pos);
     ATTNLAB_REQUIRE(window >= 0 && sinks >= 0, "window=%d and sinks=%d must not be negative", window, sinks);
-    RangeArgs a = range_args(K, V, k_exp, v_exp, block, q, G, h, C, P, scale, out, out_bf16, part);
+    RangeArgs a = range_args(K, V, k_exp, v_exp, block, q, B, G, h, C, P, scale, out, out_bf16, part);
     a.lengths = lengths;
     a.n = lengths ? 0 : (int)(q_pos + 1 < length ? q_pos + 1 : length);   // causal: no key past the query
     a.qend = q_pos + 1;
     a.window = window;
     a.sinks = sinks;
-    return launch_range<false>(a, B, reinterpret_cast<hipStream_t>(stream));
+    return launch_range<false>(a, reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int attnlab_quant_attend(const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_exp,
@@ -442,9 +611,9 @@ extern "C" int attnlab_quant_attend(const uint8_t* k_codes, const uint8_t* v_cod
     if (rc) return rc;
     ATTNLAB_REQUIRE(S >= 1, "at least one row must be selected (S=%d)", S);
     ATTNLAB_REQUIRE(rows != nullptr && rows_stride >= S, "rows must hold S=%d positions per (b, g)", S);
-    RangeArgs a = range_args(k_codes, v_codes, k_exp, v_exp, block, q, G, h, C, P, scale, out, out_bf16, part);
+    RangeArgs a = range_args(k_codes, v_codes, k_exp, v_exp, block, q, B, G, h, C, P, scale, out, out_bf16, part);
     a.rows = rows;
     a.rows_stride = rows_stride;
     a.n = S;
-    return launch_range<true>(a, B, reinterpret_cast<hipStream_t>(stream));
+    return launch_range<true>(a, reinterpret_cast<hipStream_t>(stream));
 }
