@@ -22,7 +22,7 @@ from .quant import (QuantCache, dequantize_rows, quant_attention, quant_gather_a
 from .indexer import GroupedIndexer, candidate_scores, project_keys, project_queries  # noqa: E402
 from .decode import (DecodeRequest, dense_decode_step, gathered_decode_step_kernel, prepare_request,  # noqa: E402
                      select_rows_kernel, select_rows_recent, select_rows_uniform, sparse_decode_step,
-                     sparse_decode_step_kernel)
+                     sparse_decode_step_kernel, sparse_decode_step_quant)
 
 __all__ = [
     "FIXED_PREFIX", "FIXED_RECENT", "SelectionLayout", "fixed_budget", "legal_length", "selection_layout",
@@ -33,4 +33,5 @@ __all__ = [
     "GroupedIndexer", "candidate_scores", "project_keys", "project_queries",
     "DecodeRequest", "dense_decode_step", "gathered_decode_step_kernel", "prepare_request", "select_rows_kernel",
     "select_rows_recent", "select_rows_uniform", "sparse_decode_step", "sparse_decode_step_kernel",
+    "sparse_decode_step_quant",
 ]

@@ -59,8 +59,8 @@ SIGNATURES = {
     "attnlab_prefill_attend_split": (_i, [_p, _p, _p, _i64, _i, _p] + [_i] * 8 + [_f, _i, _p, _i64, _p]),
     "attnlab_quant_append": (_i, ([_p] + [_i64] * 3) * 2 + [_i] + [_p] * 5 + [_i] * 6 + [_p]),
     "attnlab_quant_read": (_i, [_p] * 6 + [_i, _p] + [_i] * 6 + [_p]),
-    "attnlab_range_decode": (_i, [_p] * 4 + [_i, _p, _p, _i, _i64] + [_i] * 7 + [_f, _p, _i, _p, _p]),
-    "attnlab_quant_attend": (_i, [_p] * 4 + [_i, _p, _p, _i64] + [_i] * 6 + [_f, _p, _i, _p, _p]),
+    "attnlab_range_decode": (_i, [_p] * 4 + [_i, _p, _p, _i, _i64] + [_i] * 7 + [_f, _p, _i, _p, _p, _p]),
+    "attnlab_quant_attend": (_i, [_p] * 4 + [_i, _p, _p, _i64] + [_i] * 6 + [_f, _p, _i, _p, _p, _p]),
     "attnlab_range_prefill_part_bytes": (_i64, [_i] * 5),
     "attnlab_range_prefill": (_i, [_p] * 5 + [_i, _p] + [_i] * 9 + [_f, _i, _p, _i64, _p]),
     "attnlab_sparse_decode_workspace": (_i64, [_i] * 8),

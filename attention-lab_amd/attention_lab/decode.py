@@ -10,6 +10,7 @@ module is a drop-in for it; the torch ops under each function are replaced by th
   reference's order (F first, then the candidates by descending score).
 * `gathered_decode_step_kernel` - the attend kernel on a given flat row list.
 * `dense_decode_step` - the dense decode kernel.
+* `sparse_decode_step_quant` - the sparse step over an 8-bit K/V cache: score, select, row-list read, a launch or two each.
 
 The `backend` arguments are validated as in the reference and otherwise ignored: the HIP kernels are the backend.
 The selection tie order is defined (equal scores: lower position first) where torch.topk leaves it open. Only
@@ -24,7 +25,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _native as nat
-from . import hip_attend, hip_score, hip_select
+from . import hip_attend, hip_range, hip_score, hip_select
 from .indexer import GroupedIndexer
 from .selection import FIXED_PREFIX, FIXED_RECENT, SelectionLayout, fixed_budget, legal_length, selection_layout
 from .sparse import check_flat, row_offsets
@@ -186,7 +187,7 @@ def select_rows_uniform(fixed_rows, off_lo, lo: int, hi: int, k: int, *, rng) ->
     return torch.cat([fixed_rows, rel + off_lo], dim=-1).reshape(-1)
 
 
-def _positions_from_flat(rows, B, G, S, C, device):
+def positions_from_flat(rows, B, G, S, C, device):
     off = row_offsets(B, G, C, device)
     pos = rows.view(B, G, S) - off
     return pos.to(torch.int32).contiguous()
@@ -202,7 +203,7 @@ def gathered_decode_step_kernel(q_main, k_cache, v_cache, rows, selected_count: 
     check_flat(k_cache)
     check_flat(v_cache)
     C = int(k_cache.shape[2])
-    pos = _positions_from_flat(rows, B, G, selected_count, C, k_cache.device)
+    pos = positions_from_flat(rows, B, G, selected_count, C, k_cache.device)
     q = q_main.reshape(B, G, h, d).contiguous()
     out = hip_attend.attend(q, k_cache, v_cache, pos, scale=scale, out_dtype=q_main.dtype)
     return out.view(B, G, h, 1, d)
@@ -295,6 +296,58 @@ def sparse_decode_step_kernel(q_main, q_pre, k_cache, v_cache, zT, wq_t_scaled, 
              zT.data_ptr(), wq_c.data_ptr(), wk_c.data_ptr(), nat.ptr(k_new), B, G, h, r,
              C, lo, hi, legal, k, wc, sc, order, P, state.data_ptr(), ws.data_ptr(), ws.numel(), None, nat.ptr(flat),
              out.data_ptr(), nat.stream_of(device))
+    return (out, flat) if return_rows else out
+
+
+_QUANT_WS = nat.Workspace()   # the select state of sparse_decode_step_quant
+
+
+def sparse_decode_step_quant(q_main, q_pre, cache, zT, wq_t_scaled, wk, fixed_rows, off_lo, lo: int, hi: int, k: int,
+                             selected_count: int, *, k_pre_new=None, write_col: int = -1, scale=None,
+                             return_rows: bool = False, canonical_order: bool = False, partitions=None, workspace=None):
+    """sparse_decode_step_kernel over an 8-bit K/V cache (quant.QuantCache of capacity C, the table's): z column write, u,
+    candidate scan and top-k as there, over a bfloat16 or float32 index table, then the row-list read of the codes. No
+    counterpart in the reference. The new key's and value's rows are the caller's to append (quantize_append)."""
+    B, G, h, T, d = q_main.shape
+    if T != 1:
+        raise ValueError("a decode step takes exactly one new query position")
+    C = cache.capacity
+    if (B, G, d) != (cache.batch, cache.groups, hip_attend.HEAD_DIM):
+        raise ValueError(f"q_main {tuple(q_main.shape)} does not match a cache of B, G = {cache.batch}, {cache.groups}")
+    if zT.dim() != 4 or tuple(zT.shape[:2]) != (B, G) or zT.shape[3] != C:
+        raise ValueError("zT must be a [B, G, r, C] tensor matching the cache")
+    if q_pre.numel() != q_main.numel():
+        raise ValueError("q_pre must hold q_main's elements")
+    lo, hi, k, S = int(lo), int(hi), int(k), int(selected_count)
+    legal = _layout_from_rows(fixed_rows, lo, hi, k, S)
+    if legal > C:
+        raise ValueError(f"legal length {legal} exceeds capacity {C}")
+    if not 0 <= k <= hi - lo:
+        raise ValueError(f"need 0 <= k <= {hi - lo}, got {k}")
+    check_standard_f(fixed_rows, off_lo, lo, hi, legal, C)
+    k_new, wc = None, -1
+    if k_pre_new is not None:
+        if tuple(k_pre_new.shape) != (B, G, 1, d) or k_pre_new.dtype != zT.dtype:
+            raise ValueError(f"k_pre_new must be a {zT.dtype} [B, G, 1, d] tensor")
+        k_new = k_pre_new.reshape(B, G, d).contiguous()
+        wc = int(write_col) if write_col >= 0 else C + int(write_col)
+    score = dict(wk=wk.contiguous(), q_cat=q_pre.reshape(B, G, h * d).contiguous(), wq_t=wq_t_scaled.contiguous(),
+                 k_new=k_new, write_col=wc)
+    if k == 0:
+        if k_new is not None:
+            hip_score.score_grouped(zT, lo, lo, **score)   # nothing is a candidate, but the new key gets its column
+        flat = fixed_rows.reshape(-1)
+        pos = positions_from_flat(flat, B, G, S, C, cache.device)
+    else:
+        W = nat.SELECT_STATE_WORDS
+        wsp = _QUANT_WS if workspace is None else workspace
+        state = wsp.bytes(cache.device, B * G * W * 4, "state")[:B * G * W * 4].view(torch.int32).view(B, G, W)
+        s = hip_score.score_grouped(zT, lo, hi, state=state, **score)
+        order = _order(canonical_order or not return_rows)   # the order shows only in rows that leave the call
+        pos, flat = hip_select.select_rows(s, lo, hi, legal, k, C, order=order, want_flat=return_rows, state=state,
+                                           workspace=wsp)
+    out = hip_range.listed_attention(q_main, cache, pos, scale=scale, out=None, out_dtype=torch.bfloat16,
+                                     partitions=partitions)
     return (out, flat) if return_rows else out
 
 

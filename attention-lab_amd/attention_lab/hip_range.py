@@ -2,9 +2,12 @@
 for one query or a causal chunk, over a bfloat16 cache or an 8-bit one; and the row-list read of an 8-bit cache.
 
 The kernels behind `window_attention` (window.py) and `quant_attention` / `quant_gather_attention` (quant.py), which
-check their caches; this module checks what the reads share, chooses the split counts and launches. There is no state
-between calls: the split-K partials are allocated for the call, so calls on several streams, and captured graphs, share
-nothing. Launches go to the tensors' own device, on torch's current stream of it.
+check their caches; this module checks what the reads share, chooses the split counts and launches, on the tensors' own
+device and torch's current stream of it.
+
+The split-K partials are allocated for each call. The last workgroup of a (b, g) to arrive merges them where a counter
+tells it that it is: counters belong to a stream, whose calls follow one another and leave them zero. A captured call
+takes a second launch for the merge instead (the same sums), so a graph shares nothing with other graphs or calls.
 """
 from __future__ import annotations
 
@@ -22,13 +25,24 @@ CHUNK_KEYS = 64     # keys of its block
 TILE = 32           # rows a wave of the one-query kernel takes at a time
 MAX_SPLITS = 16
 MAX_P = 256
+MERGE_SLOTS = 16    # partials the last workgroup to arrive merges itself; more take a second launch
 INT_MAX = 2 ** 31 - 1
 
 
-def decode_partitions(BG: int, count: int) -> int:
-    """Split-K count of the one-query kernels for BG (b, g) rows of `count` positions each: about two workgroups per CU,
-    each at least one tile of 32 positions for every one of its four waves."""
-    return max(1, min(64, -(-512 // BG), count // (4 * TILE)))
+def decode_partitions(BG: int, count: int, ragged: bool = False) -> int:
+    """Split-K count of the one-query kernels for BG (b, g) rows of `count` positions each: one workgroup per CU, or two
+    where that leaves each at least 48 tiles of 32 positions, and at least one tile for every one of its four waves.
+    Measured on MI355X (graph replay, 8-bit): one per CU against two, BG=8 at 8K 10.3 / 11.9 us, at 20K 14.0 / 15.8;
+    BG=32 at 4K 12.4 / 14.6; BG=64, 4K windows in bfloat16, 27.3 / 29.4; and the longer ones BG=24 at 20K 28.3 / 26.6,
+    BG=128 at 32K 162 / 158.
+    ragged (a length per sequence): the slots that the kernel deals out by the sequences' lengths, about two workgroups
+    per CU with the half slot that every sequence's remainder takes (BG=40 to 20K: 31.9 us, 36.3 with half as many more;
+    BG=128 to 8K: 41.6 against 45.2)."""
+    tiles = -(-count // TILE)
+    BG = max(BG, 1)
+    if ragged:
+        return max(2, min(64, (512 + BG // 2) // BG))
+    return max(1, min(64, (512 if BG * tiles >= 256 * 48 else 256) // BG, count // (4 * TILE)))
 
 
 def chunk_splits(BG: int, h: int, T: int, keys: int) -> int:
@@ -56,15 +70,16 @@ def check_window(window, sinks):
 
 def check_query(q, B: int, G: int, device):
     """q [B,G,h,T,128] bfloat16 on the cache's device -> (h, T)."""
-    if q.dim() != 5 or tuple(q.shape[:2]) != (B, G) or q.shape[4] != HEAD_DIM or q.dtype != torch.bfloat16:
+    shape = q.shape
+    if len(shape) != 5 or shape[0] != B or shape[1] != G or shape[4] != HEAD_DIM or q.dtype != torch.bfloat16:
         raise ValueError(f"q must be a bfloat16 [B, G, h, T, {HEAD_DIM}] tensor with B, G = {B}, {G}, got {q.dtype} "
-                         f"{tuple(q.shape)}")
+                         f"{tuple(shape)}")
     if q.device != device:
         raise ValueError("q must live on the cache's device")
-    h = int(q.shape[2])
+    h = shape[2]
     if not 1 <= h <= MAX_H_CHUNK:
         raise ValueError(f"h={h} must be in [1, {MAX_H_CHUNK}]")
-    return h, int(q.shape[3])
+    return h, shape[3]
 
 
 def check_lengths(lengths, B: int, device):
@@ -79,7 +94,8 @@ def check_out(out, q, dtype):
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("out_dtype must be float32 or bfloat16")
     if out is None:
-        return torch.empty(q.shape, dtype=dtype, device=q.device)
+        # q is contiguous where it stands for the layout: empty_like is half the time of an empty with its arguments
+        return torch.empty_like(q) if dtype == torch.bfloat16 else torch.empty_like(q, dtype=dtype)
     if tuple(out.shape) != tuple(q.shape) or out.dtype != dtype or not out.is_contiguous() or out.device != q.device:
         raise ValueError(f"out must be a contiguous {dtype} tensor shaped like q on its device")
     return out
@@ -94,8 +110,22 @@ def split_count(partitions, chosen: int, most: int) -> int:
     return int(partitions)
 
 
-def _partials(words: int, device):
-    return torch.empty(words, dtype=torch.float32, device=device)
+_ARRIVALS: dict = {}   # (device index, stream) -> its counters, zeroed once, left zero by every call
+COUNTERS = 4096        # (b, g) rows that they serve; more take the second launch
+
+
+def _split_k(P: int, BG: int, h: int, device, stream: int, counted: bool):
+    """(partials, counters' address) of a one-query call split over P workgroups."""
+    if P == 1:
+        return None, None
+    part = torch.empty(BG * P * h * (HEAD_DIM + 2), dtype=torch.float32, device=device)
+    if not counted or P > MERGE_SLOTS or BG > COUNTERS or torch._C._cuda_isCurrentStreamCapturing():
+        return part, None
+    key = (device.index, stream)
+    counters = _ARRIVALS.get(key)
+    if counters is None:
+        counters = _ARRIVALS[key] = torch.zeros(COUNTERS, dtype=torch.int32, device=device)
+    return part, counters.data_ptr()
 
 
 def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: int, C: int, device, *, valid_length,
@@ -129,11 +159,11 @@ def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: 
     stream = nat.stream_of(device)
     if T == 1 and h <= MAX_H:
         out = check_out(out, q, out_dtype)
-        P = split_count(partitions, decode_partitions(B * G, seen), MAX_P)
-        part = _partials(B * G * P * h * (HEAD_DIM + 2), device) if P > 1 else None
+        P = split_count(partitions, decode_partitions(B * G, seen, lengths is not None), MAX_P)
+        part, arrive = _split_k(P, B * G, h, device, stream, lengths is None)
         nat.call_on(device, "attnlab_range_decode", k_ptr, v_ptr, *exp_ptrs, block, q.data_ptr(), nat.ptr(lengths), legal,
                     p0, window, sinks, B, G, h, C, P, sc, out.data_ptr(), int(out_dtype == torch.bfloat16),
-                    nat.ptr(part), stream)
+                    nat.ptr(part), arrive, stream)
         return out
     if out_dtype != torch.bfloat16:
         raise ValueError("a chunk's outputs are bfloat16")
@@ -142,7 +172,7 @@ def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: 
         return out
     splits = split_count(partitions, chunk_splits(B * G, h, T, seen), MAX_SPLITS)
     nbytes = max(0, nat.lib().attnlab_range_prefill_part_bytes(B, G, h, T, splits))
-    part = _partials(nbytes // 4, device) if nbytes else None
+    part = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
     nat.call_on(device, "attnlab_range_prefill", q.data_ptr(), k_ptr, v_ptr, *exp_ptrs, block, out.data_ptr(), B, G, h, T,
                 p0, legal, C, window, sinks, sc, splits, nat.ptr(part), nbytes, stream)
     return out
@@ -159,12 +189,13 @@ def listed_attention(q, cache, rows, *, scale, out, out_dtype, partitions):
     S = int(rows.shape[2])
     if S < 1:
         raise ValueError("at least one row must be selected")
-    out = check_out(out, q, out_dtype)
     q = q.contiguous()
+    out = check_out(out, q, out_dtype)
     P = split_count(partitions, decode_partitions(B * G, S), MAX_P)
-    part = _partials(B * G * P * h * (HEAD_DIM + 2), device) if P > 1 else None
+    stream = nat.stream_of(device)
+    part, arrive = _split_k(P, B * G, h, device, stream, True)
     sc = float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
     nat.call_on(device, "attnlab_quant_attend", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(),
                 cache.v_exp.data_ptr(), cache.block, q.data_ptr(), rows.data_ptr(), S, B, G, h, S, C, P, sc,
-                out.data_ptr(), int(out_dtype == torch.bfloat16), nat.ptr(part), nat.stream_of(device))
+                out.data_ptr(), int(out_dtype == torch.bfloat16), nat.ptr(part), arrive, stream)
     return out

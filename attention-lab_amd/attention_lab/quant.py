@@ -40,18 +40,20 @@ class QuantCache:
     def __init__(self, k, v, k_exp, v_exp, *, block: int = 64):
         if block not in BLOCKS:
             raise ValueError(f"block must be one of {BLOCKS}, got {block!r}")
-        if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.dtype != torch.float8_e4m3fn or not k.is_contiguous() \
+        shape = k.shape
+        if len(shape) != 4 or shape[3] != HEAD_DIM or k.dtype != torch.float8_e4m3fn or not k.is_contiguous() \
                 or not k.is_cuda:
             raise ValueError(f"k must be a contiguous float8_e4m3fn [B, G, C, {HEAD_DIM}] tensor on a HIP device")
-        if v.shape != k.shape or v.dtype != k.dtype or not v.is_contiguous() or v.device != k.device:
+        device = k.device
+        if v.shape != shape or v.dtype != torch.float8_e4m3fn or not v.is_contiguous() or v.device != device:
             raise ValueError("v must match k")
-        B, G, C, _ = k.shape
+        B, G, C, _ = shape
         want = (B, G, -(-C // block))
         for t, name in ((k_exp, "k_exp"), (v_exp, "v_exp")):
-            if tuple(t.shape) != want or t.dtype != torch.uint8 or not t.is_contiguous() or t.device != k.device:
+            if t.shape != want or t.dtype != torch.uint8 or not t.is_contiguous() or t.device != device:
                 raise ValueError(f"{name} must be a contiguous uint8 {list(want)} tensor on the cache's device")
         self.k, self.v, self.k_exp, self.v_exp, self.block = k, v, k_exp, v_exp, int(block)
-        self.batch, self.groups, self.capacity, self.device = B, G, C, k.device
+        self.batch, self.groups, self.capacity, self.device = B, G, C, device
 
     @classmethod
     def empty(cls, batch: int, groups: int, capacity: int, *, block: int = 64, device) -> "QuantCache":
@@ -79,13 +81,14 @@ def _start(cache: QuantCache, start, length: int):
     return None, start
 
 
-def _rows(x, dtype):
-    """x as the kernel takes it: unit stride along a row and 16-byte aligned rows (a copy where it has neither)."""
-    step = 16 // x.element_size()
-    if (x.stride(3) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) % step == 0 and x.stride(1) % step == 0
-            and x.stride(2) % step == 0):
-        return x
-    return x.contiguous()
+def _rows(x, step: int):
+    """(x as the kernel takes it, its three outer strides): unit stride along a row and 16-byte aligned rows of `step`
+    elements to 16 bytes (a copy where it has neither)."""
+    sb, sg, st, sd = x.stride()
+    if sd != 1 or (sb | sg | st) % step or x.data_ptr() % 16:
+        x = x.contiguous()
+        sb, sg, st, _ = x.stride()
+    return x, sb, sg, st
 
 
 def quantize_append(cache: QuantCache, k, v, start=0) -> None:
@@ -98,21 +101,24 @@ def quantize_append(cache: QuantCache, k, v, start=0) -> None:
     once; everything else is the same. Rows at and after start + T are no longer valid rows of the block they share.
     NaN and infinity become NaN; finite values past 1.875 * 2^127 saturate.
     """
-    want = (cache.batch, cache.groups)
-    if k.dim() != 4 or tuple(k.shape[:2]) != want or k.shape[3] != HEAD_DIM or v.shape != k.shape:
-        raise ValueError(f"k and v must be [B, G, T, {HEAD_DIM}] with B, G = {want}, got {tuple(k.shape)} and "
-                         f"{tuple(v.shape)}")
-    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+    shape = k.shape
+    if len(shape) != 4 or shape[0] != cache.batch or shape[1] != cache.groups or shape[3] != HEAD_DIM or v.shape != shape:
+        raise ValueError(f"k and v must be [B, G, T, {HEAD_DIM}] with B, G = {cache.batch}, {cache.groups}, got "
+                         f"{tuple(shape)} and {tuple(v.shape)}")
+    dtype = _DTYPES.get(k.dtype)
+    if dtype is None or v.dtype != k.dtype:
         raise ValueError(f"k and v must both be bfloat16, float16 or float32, got {k.dtype} and {v.dtype}")
-    if k.device != cache.device or v.device != cache.device:
+    device = cache.device
+    if k.device != device or v.device != device:
         raise ValueError("k and v must live on the cache's device")
-    T = int(k.shape[2])
+    T = shape[2]
     starts, at = _start(cache, start, T)
-    k, v = _rows(k, k.dtype), _rows(v, v.dtype)
-    nat.call_on(cache.device, "attnlab_quant_append", k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(),
-                v.stride(0), v.stride(1), v.stride(2), _DTYPES[k.dtype], cache.k.data_ptr(), cache.v.data_ptr(),
-                cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), nat.ptr(starts), at, cache.batch, cache.groups, T,
-                cache.capacity, cache.block, nat.stream_of(cache.device))
+    step = 4 if dtype == nat.DT_F32 else 8
+    k, *k_strides = _rows(k, step)
+    v, *v_strides = _rows(v, step)
+    nat.call_on(device, "attnlab_quant_append", k.data_ptr(), *k_strides, v.data_ptr(), *v_strides, dtype,
+                cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), nat.ptr(starts), at,
+                cache.batch, cache.groups, T, cache.capacity, cache.block, nat.stream_of(device))
 
 
 def dequantize_rows(cache: QuantCache, start=0, length=None, *, dtype=torch.bfloat16):

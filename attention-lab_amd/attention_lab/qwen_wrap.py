@@ -16,7 +16,10 @@ How this build arranges it:
   (attnlab_project_keys); a dense decode step reads every legal position on the dense decode kernel; a sparse decode
   step asks the state's selector strategy for its read. The index selector (D0) is one fused HIP step per layer
   (z column, u, scan, top-k, gather-free attend); the recent (B) and uniform (C) selectors build their row list on
-  the host, as the reference does, and read it with the gather-free attend.
+  the host, as the reference does, and read it with the gather-free attend. A windowed state (mode "window", no
+  counterpart in the reference) reads the sinks and the recent window in prefill and decode alike.
+* Formats. The K/V cache is bfloat16 (kv_format "bfloat16") or 8-bit (kv_format "e4m3": a QuantCache per layer, rows
+  quantised as they are appended, every read over the codes). The index table, the plans and the selection are the same.
 * Plans. F and the candidate domain of a step are built once per step (`build_step_plan`) from device tensors the
   cache keeps, and tagged as the selection rule's F so the HIP step takes them without a device read.
 
@@ -32,12 +35,15 @@ from dataclasses import dataclass, field
 import torch
 from torch import nn
 
-from .decode import (gathered_decode_step_kernel, select_rows_recent, select_rows_uniform, sparse_decode_step_kernel,
-                     tag_standard_f)
+from .decode import (gathered_decode_step_kernel, positions_from_flat, select_rows_recent, select_rows_uniform,
+                     sparse_decode_step_kernel, sparse_decode_step_quant, tag_standard_f)
 from .full import full_attention
+from .hip_range import check_window
 from .indexer import GroupedIndexer, project_keys
+from .quant import QuantCache, quant_attention, quant_gather_attention, quantize_append
 from .selection import FIXED_PREFIX, FIXED_RECENT, fixed_budget, selection_layout
 from .sparse import row_offsets
+from .window import window_attention
 
 try:  # transformers is needed by this module only; the rest of the package imports without it
     from transformers.models.qwen3.modeling_qwen3 import apply_rotary_pos_emb
@@ -49,6 +55,8 @@ except ImportError as _e:  # pragma: no cover
 MASK_BYPASS = {"full_attention": None}
 SELECTORS = ("index", "recent", "uniform")   # D0, B, C
 PHASES = ("prefill", "decode")
+MODES = ("full", "sparse", "window")
+KV_FORMATS = ("bfloat16", "e4m3")   # the first: the dtype the cache is given
 SLOT_ALIGN = 8   # rows per (b, g) are allocated in multiples of this: 16 bytes of a bfloat16 index-table row
 
 
@@ -89,12 +97,18 @@ class _AppendLedger:
 class LabCache:
     """Static per-layer K/V [B,G,slots,d] and optional index tables zT [B,G,r,slots] with one legal length for all
     layers (reference qwen_wrap.py:52-139). Allocated with torch.empty: slots at or past valid_length hold whatever the
-    memory held (tests poison them) and no read or selection may touch them; slots past `capacity` are padding."""
+    memory held (tests poison them) and no read or selection may touch them; slots past `capacity` are padding.
+
+    kv_format "e4m3" holds K and V in 8 bits: k[l] and v[l] are codes, quant[l] the layer's QuantCache (its scale bytes
+    for blocks of kv_block positions), and rows are quantised as they are written. `dtype` is then the rows' own."""
 
     def __init__(self, *, layers: int, batch: int, groups: int, capacity: int, head_dim: int, index_dim=None, device,
-                 dtype=torch.float32, index_dtype=None):
+                 dtype=torch.float32, index_dtype=None, kv_format: str = "bfloat16", kv_block: int = 64):
         if int(capacity) <= 0 or int(layers) <= 0:
             raise ValueError("capacity and layers must be positive")
+        if kv_format not in KV_FORMATS:
+            raise ValueError(f"kv_format must be one of {KV_FORMATS}")
+        self.kv_format, self.kv_block = kv_format, int(kv_block)
         self.layers, self.batch, self.groups = int(layers), int(batch), int(groups)
         self.capacity, self.head_dim = int(capacity), int(head_dim)
         self.slots = -(-self.capacity // SLOT_ALIGN) * SLOT_ALIGN
@@ -102,8 +116,13 @@ class LabCache:
         self.device, self.dtype = torch.device(device), dtype
         self.index_dtype = dtype if index_dtype is None else index_dtype
         kv_shape = (self.layers, self.batch, self.groups, self.slots, self.head_dim)
-        self._store = {"k": torch.empty(kv_shape, device=self.device, dtype=dtype),
-                       "v": torch.empty(kv_shape, device=self.device, dtype=dtype)}
+        kv_dtype = torch.float8_e4m3fn if kv_format == "e4m3" else dtype
+        self._store = {"k": torch.empty(kv_shape, device=self.device, dtype=kv_dtype),
+                       "v": torch.empty(kv_shape, device=self.device, dtype=kv_dtype)}
+        if kv_format == "e4m3":
+            exp_shape = (*kv_shape[:3], -(-self.slots // self.kv_block))
+            for name in ("k_exp", "v_exp"):
+                self._store[name] = torch.full(exp_shape, 127, device=self.device, dtype=torch.uint8)
         if self.index_dim is not None:
             self._store["z"] = torch.empty(self.layers, self.batch, self.groups, self.index_dim, self.slots,
                                            device=self.device, dtype=self.index_dtype)
@@ -121,6 +140,10 @@ class LabCache:
         self.k = list(self._store["k"].unbind(0))
         self.v = list(self._store["v"].unbind(0))
         self.z = list(self._store["z"].unbind(0)) if "z" in self._store else None
+        self.quant = None
+        if self.kv_format == "e4m3":
+            self.quant = [QuantCache(k, v, ke, ve, block=self.kv_block) for k, v, ke, ve in
+                          zip(self.k, self.v, self._store["k_exp"].unbind(0), self._store["v_exp"].unbind(0))]
 
     @property
     def has_index(self) -> bool:
@@ -146,14 +169,22 @@ class LabCache:
         self._ledger.record(layer, start, length)
         return start
 
+    def write(self, layer: int, start: int, k_main: torch.Tensor, v: torch.Tensor) -> None:
+        """K/V rows into the slots [start, start + T) of a layer, in the cache's format."""
+        if self.quant is not None:
+            quantize_append(self.quant[layer], k_main, v, start)
+            return
+        T = int(k_main.shape[2])
+        self.k[layer][:, :, start:start + T].copy_(k_main)
+        self.v[layer][:, :, start:start + T].copy_(v)
+
     def append(self, layer: int, k_main: torch.Tensor, v: torch.Tensor, z=None) -> None:
         """Write this layer's T new rows at [valid_length, valid_length + T); exactly once per layer per forward."""
         T = int(k_main.shape[2])
         if z is not None and not self.has_index:
             raise RuntimeError("this cache was created without an index table")
         start = self.reserve(layer, T)
-        self.k[layer][:, :, start:start + T].copy_(k_main)
-        self.v[layer][:, :, start:start + T].copy_(v)
+        self.write(layer, start, k_main, v)
         if z is not None:
             self.z[layer][..., start:start + T].copy_(z)
 
@@ -182,7 +213,8 @@ class LabCache:
     def bytes(self) -> dict:
         """Bytes held (padding slots included)."""
         size = {name: t.numel() * t.element_size() for name, t in self._store.items()}
-        kv, z = size["k"] + size["v"], size.get("z", 0)
+        z = size.get("z", 0)
+        kv = sum(size.values()) - z
         return {"kv_bytes": kv, "index_bytes": z, "total_bytes": kv + z}
 
 
@@ -246,6 +278,13 @@ class _IndexSelector:
         l, cache = attn.layer_idx, state.cache
         idx = state.indexers[l]
         B, G, h, _, d = q5.shape
+        if cache.quant is not None:
+            res = sparse_decode_step_quant(
+                q5, q_pre.reshape(B, G, h, 1, d).to(idx.wk.dtype), cache.quant[l], cache.z[l], idx.wq_t_scaled, idx.wk,
+                plan.fixed_rows, plan.off_lo, plan.lo, plan.hi, plan.k, plan.selected_count,
+                k_pre_new=k_pre.to(idx.wk.dtype), write_col=plan.write_col, scale=attn.scaling,
+                return_rows=state.record_selection, canonical_order=state.canonical_order)
+            return res if state.record_selection else (res, None)
         res = sparse_decode_step_kernel(
             q5, q_pre.reshape(B, G, h, 1, d).to(idx.wk.dtype), cache.k[l], cache.v[l], cache.z[l], idx.wq_t_scaled,
             idx.wk, plan.fixed_rows, plan.off_lo, plan.lo, plan.hi, plan.k, plan.selected_count,
@@ -267,8 +306,12 @@ class _ListedSelector:
         if state.canonical_order:
             B, G = q5.shape[:2]
             rows = rows.view(B, G, plan.selected_count).sort(dim=-1).values.reshape(-1)
-        out = gathered_decode_step_kernel(q5, state.cache.k[l], state.cache.v[l], rows, plan.selected_count,
-                                          scale=attn.scaling)
+        cache = state.cache
+        if cache.quant is not None:
+            B, G = q5.shape[:2]
+            pos = positions_from_flat(rows, B, G, plan.selected_count, cache.slots, cache.device)
+            return quant_gather_attention(q5, cache.quant[l], pos, scale=attn.scaling), rows
+        out = gathered_decode_step_kernel(q5, cache.k[l], cache.v[l], rows, plan.selected_count, scale=attn.scaling)
         return out, rows
 
 
@@ -298,13 +341,15 @@ _SELECTOR_IMPL = {"index": _IndexSelector, "recent": _RecentSelector, "uniform":
 # ---------------------------------------------------------------------------------------------------------------------
 # state
 # ---------------------------------------------------------------------------------------------------------------------
-def _read_config_layers(cache: LabCache, indexers, mode: str, selector: str, sparse_layers):
+def _read_config_layers(cache: LabCache, indexers, mode: str, selector: str, sparse_layers, window):
     """Validate a read configuration against its cache and return the sparse layer set (None: every layer). The
     messages are the contract's; this function's own rule is that a configuration is checked in full before any state
     is built, cheapest property first."""
     problems = []
-    if mode not in ("full", "sparse"):
-        problems.append("mode must be 'full' or 'sparse'")
+    if mode not in MODES:
+        problems.append(f"mode must be one of {MODES}")
+    elif (mode == "window") != (window is not None):
+        problems.append("mode 'window' goes with a window, and a window with it")
     if selector not in SELECTORS:
         problems.append(f"selector must be one of {SELECTORS}")
     if indexers is not None and len(indexers) != cache.layers:
@@ -339,15 +384,16 @@ class _RequestBudget:
 
 
 class LabState:
-    """One read configuration (reference qwen_wrap.py:189-256): the cache, the per-layer indexers, the mode (full or
-    sparse), the selector of a sparse read and the plan and phase of the forward in flight. The request's budget
+    """One read configuration (reference qwen_wrap.py:189-256): the cache, the per-layer indexers, the mode (full, sparse
+    or window, the last with its window and sinks), the selector of a sparse read and the plan and phase of the forward in flight. The request's budget
     (rho, k0, the first step's legal length, the request count) lives in a `_RequestBudget`; the reference's attribute
     names read through to it."""
 
     def __init__(self, cache: LabCache, indexers=None, *, mode: str = "full", selector: str = "index",
                  decode_backend: str = "sdpa_fold", prefill_backend: str = "sdpa_fold", uniform_seed: int = 0,
-                 sparse_layers=None, cache_guard=None, canonical_order=False):
-        self.sparse_layers = _read_config_layers(cache, indexers, mode, selector, sparse_layers)
+                 sparse_layers=None, cache_guard=None, canonical_order=False, window=None, sinks: int = FIXED_PREFIX):
+        self.sparse_layers = _read_config_layers(cache, indexers, mode, selector, sparse_layers, window)
+        self.window, self.sinks = check_window(window, sinks) if window is not None else (None, 0)
         self.cache, self.indexers = cache, indexers
         self.mode, self.selector = mode, selector
         self.selector_impl = _SELECTOR_IMPL[selector]()
@@ -431,18 +477,26 @@ class LabAttention(nn.Module):
         l, cache = self.layer_idx, st.cache
         T = int(k_main.shape[2])
         start = cache.reserve(l, T)
-        cache.k[l][:, :, start:start + T].copy_(k_main)
-        cache.v[l][:, :, start:start + T].copy_(v)
+        cache.write(l, start, k_main, v)
         if cache.has_index and st.indexers is not None:
             wk = st.indexers[l].wk
             project_keys(k_pre.to(wk.dtype), wk, out=cache.z[l], col0=start)
         return start
 
+    def _read_range(self, st, q5, legal: int, backend: str):
+        """The read of every legal position, or of the state's window and sinks, in the cache's format."""
+        l, cache = self.layer_idx, st.cache
+        if cache.quant is not None:
+            return quant_attention(q5, cache.quant[l], valid_length=legal, window=st.window, sinks=st.sinks,
+                                   scale=self.scaling)
+        if st.window is not None:
+            return window_attention(q5, cache.k[l], cache.v[l], window=st.window, sinks=st.sinks, valid_length=legal,
+                                    scale=self.scaling)
+        return full_attention(q5, cache.k[l], cache.v[l], valid_length=legal, backend=backend, scale=self.scaling)
+
     def _read_prefill(self, st, q5, k_pre, k_main, v):
         start = self._write_keys(st, k_main, v, k_pre)
-        l, T = self.layer_idx, int(q5.shape[3])
-        return full_attention(q5, st.cache.k[l], st.cache.v[l], valid_length=start + T, backend=st.prefill_backend,
-                              scale=self.scaling)
+        return self._read_range(st, q5, start + int(q5.shape[3]), st.prefill_backend)
 
     def _read_decode(self, st, q5, q_pre, k_pre, k_main, v):
         if q5.shape[3] != 1:
@@ -450,8 +504,7 @@ class LabAttention(nn.Module):
         l, cache = self.layer_idx, st.cache
         if not st.reads_sparse(l):
             start = self._write_keys(st, k_main, v, k_pre)
-            return full_attention(q5, cache.k[l], cache.v[l], valid_length=start + 1, backend=st.decode_backend,
-                                  scale=self.scaling)
+            return self._read_range(st, q5, start + 1, st.decode_backend)
         plan = st.plan
         if plan is None or plan.legal_length != cache.valid_length + 1:
             raise RuntimeError("sparse decode needs a StepPlan built for this step's legal length")
@@ -535,11 +588,12 @@ def _param_device_dtype(model, device, dtype):
 
 
 def make_cache(model, capacity: int, *, with_index: bool, index_dim: int = 32, batch: int = 1, dtype=None, device=None,
-               index_dtype=None) -> LabCache:
+               index_dtype=None, kv_format: str = "bfloat16", kv_block: int = 64) -> LabCache:
     geo = geometry_of(model)
     device, dtype = _param_device_dtype(model, device, dtype)
     return LabCache(layers=geo.layers, batch=batch, groups=geo.groups, capacity=capacity, head_dim=geo.head_dim,
-                    index_dim=index_dim if with_index else None, device=device, dtype=dtype, index_dtype=index_dtype)
+                    index_dim=index_dim if with_index else None, device=device, dtype=dtype, index_dtype=index_dtype,
+                    kv_format=kv_format, kv_block=kv_block)
 
 
 def make_indexers(model, *, r: int = 32, seed: int = 0, dtype=None, device=None) -> list[GroupedIndexer]:
@@ -551,11 +605,13 @@ def make_indexers(model, *, r: int = 32, seed: int = 0, dtype=None, device=None)
 
 
 def make_state(model, capacity: int, mode: str, *, selector: str = "index", r: int = 32, seed: int = 0, batch: int = 1,
-               **kw) -> LabState:
+               kv_format: str = "bfloat16", kv_block: int = 64, **kw) -> LabState:
     """A: mode "full". D0: mode "sparse" with the index selector (index table and indexers). B / C: mode "sparse" with
-    selector "recent" / "uniform" (neither an index table nor indexers)."""
+    selector "recent" / "uniform" (neither an index table nor indexers). A sliding window: mode "window" with window=
+    and sinks=. kv_format "e4m3": the same reads over an 8-bit cache."""
     indexed = mode == "sparse" and selector == "index"
-    cache = make_cache(model, capacity, with_index=indexed, index_dim=r, batch=batch)
+    cache = make_cache(model, capacity, with_index=indexed, index_dim=r, batch=batch, kv_format=kv_format,
+                       kv_block=kv_block)
     return LabState(cache, make_indexers(model, r=r, seed=seed) if indexed else None, mode=mode, selector=selector,
                     **kw)
 

@@ -141,9 +141,12 @@ def load_bank(run_dir, metadata: dict, geometry, *, device, initial: bool = Fals
     return FrozenBank(indexes, identity=identity)
 
 
-def make_trained_state(model, capacity: int, bank: FrozenBank, *, sparse_layers=None, mode: str = "sparse"):
-    """A LabState over a float32 index cache, guarded by the bank, with every row list in ascending order."""
+def make_trained_state(model, capacity: int, bank: FrozenBank, *, sparse_layers=None, mode: str = "sparse",
+                       kv_format: str = "bfloat16", kv_block: int = 64):
+    """A LabState over a float32 index cache, guarded by the bank, with every row list in ascending order (kv_format,
+    kv_block: of the K/V cache, as in qwen_wrap.make_cache)."""
     from .qwen_wrap import LabState, make_cache
-    cache = make_cache(model, capacity, with_index=True, index_dim=bank.indexes[0].r, index_dtype=torch.float32)
+    cache = make_cache(model, capacity, with_index=True, index_dim=bank.indexes[0].r, index_dtype=torch.float32,
+                       kv_format=kv_format, kv_block=kv_block)
     return LabState(cache, bank.indexes, mode=mode, selector="index", sparse_layers=sparse_layers,
                     cache_guard=bank.guard, canonical_order=True)

@@ -53,15 +53,6 @@ __device__ __forceinline__ void merge_state(float& m, float& l, float& m2, float
     m = mn;
 }
 
-// A partial's words for the in-kernel merge, written and read at system scope (past the L2 of the writing XCD).
-__device__ __forceinline__ void store_coherent(float* p, float v) {
-    __hip_atomic_store(reinterpret_cast<uint32_t*>(p), __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-}
-__device__ __forceinline__ float load_coherent(const float* p) {
-    return __uint_as_float(__hip_atomic_load(reinterpret_cast<const uint32_t*>(p), __ATOMIC_RELAXED,
-                                             __HIP_MEMORY_SCOPE_SYSTEM));
-}
-
 __device__ __forceinline__ void store_out(const AttendArgs& a, size_t idx, float v) {
     if (a.out_bf16) reinterpret_cast<uint16_t*>(a.out)[idx] = f32_to_bf16_rne(v);
     else reinterpret_cast<float*>(a.out)[idx] = v;

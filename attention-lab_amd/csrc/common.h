@@ -86,6 +86,15 @@ __device__ __forceinline__ float shfl_xor_f32(float x, int mask) { return __shfl
 // exp2 on the hardware transcendental unit (v_exp_f32); exp2(-inf) = 0.
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// A partial's words for the in-kernel merge, written and read at system scope (past the L2 of the writing XCD).
+__device__ __forceinline__ void store_coherent(float* p, float v) {
+    __hip_atomic_store(reinterpret_cast<uint32_t*>(p), __float_as_uint(v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+__device__ __forceinline__ float load_coherent(const float* p) {
+    return __uint_as_float(__hip_atomic_load(reinterpret_cast<const uint32_t*>(p), __ATOMIC_RELAXED,
+                                             __HIP_MEMORY_SCOPE_SYSTEM));
+}
+
 // Workgroups of a launch are dealt to MI355X's 8 XCDs round robin (workgroup b runs on XCD b % 8), each with its own
 // L2. This renumbers them so that XCD x gets the contiguous logical range [x * n / 8, (x + 1) * n / 8) when the grid
 // size n is a multiple of 8: kernels that split the same rows the same way then touch a row's data from one XCD.

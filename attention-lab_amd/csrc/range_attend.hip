@@ -55,6 +55,8 @@ struct RangeArgs {
     float scale_log2;
     void* out;
     int out_bf16;
+    uint32_t* arrive;         // [B * G] arrival counters, zero on entry and left zero: the last workgroup of a (b, g) merges
+                              // its partials (P <= kMergeSlots, no lengths); null: a second launch does
     float* part;              // [slot, h, 130]: m, l, the unnormalised outputs (P > 1; B * G * P slots)
 };
 
@@ -127,6 +129,68 @@ struct Tile {
     uint32_t kx[2], vx;
 };
 
+// Slots whose partials the last workgroup of a (b, g) to arrive merges itself; more take a launch of their own.
+constexpr int kMergeSlots = 16;
+
+// A partial's weight against the maximum mt. No score above -inf (m = -inf): nothing to add, unless they were NaN.
+__device__ __forceinline__ float slot_weight(float m, float l, float mt) {
+    return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : fast_exp2(m - mt);
+}
+
+// `count` partials `step` words apart merged in order, eight in flight: lane l holds dims 2 l, 2 l + 1. COHERENT: written
+// by workgroups of this launch, read past the caches of this XCD.
+template <bool COHERENT>
+__device__ __forceinline__ void merge_slots(const float* pb, size_t step, int count, float& m, float& l, float2& o) {
+    constexpr int kGroup = 8;
+    const int lane = threadIdx.x & 63;
+    m = -INFINITY;
+    l = 0.0f;
+    o = make_float2(0.0f, 0.0f);
+    for (int p0 = 0; p0 < count; p0 += kGroup) {
+        float mv[kGroup], lv[kGroup];
+        float2 ov[kGroup];
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {   // past the last slot: that one again, with no weight
+            const float* pp = pb + min(p0 + u, count - 1) * step;
+            if constexpr (COHERENT) {
+                mv[u] = load_coherent(pp);
+                lv[u] = load_coherent(pp + 1);
+                ov[u] = make_float2(load_coherent(pp + 2 + 2 * lane), load_coherent(pp + 3 + 2 * lane));
+            } else {
+                const float2 ml = *reinterpret_cast<const float2*>(pp);
+                mv[u] = ml.x;
+                lv[u] = ml.y;
+                ov[u] = *reinterpret_cast<const float2*>(pp + 2 + 2 * lane);
+            }
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) mn = fmaxf(mn, mv[u]);
+        const float w0 = slot_weight(m, l, mn);
+        l *= w0;
+        o.x *= w0;
+        o.y *= w0;
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {
+            if (p0 + u < count) {
+                const float w = slot_weight(mv[u], lv[u], mn);
+                l += w * lv[u];
+                o.x += w * ov[u].x;
+                o.y += w * ov[u].y;
+            }
+        }
+        m = mn;
+    }
+}
+
+// Outputs 2 l, 2 l + 1 of a (b, g, head); zeros where nothing was summed.
+__device__ __forceinline__ void store_row(const RangeArgs& a, size_t row, float l, float2 o) {
+    const float2 r = l == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(o.x / l, o.y / l);
+    const size_t to = row * kDim + 2 * (threadIdx.x & 63);
+    if (a.out_bf16) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + to) = pack_bf16x2(r.x, r.y);
+    else *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + to) = r;
+}
+
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const uint8_t* base, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, (int)bytes, 0x00020000);
 }
@@ -140,6 +204,7 @@ __global__ __launch_bounds__(64 * kWaves, 3) void range_attend(RangeArgs a) {
     __shared__ float ml_sh[kWaves][16][2];
     __shared__ int list_sh[LIST ? kListChunk : 1];
     __shared__ __attribute__((aligned(8))) uint8_t vx_sh[kWaves][kTile];
+    __shared__ uint32_t last_sh;
     const int lin = __builtin_amdgcn_readfirstlane(xcd_contiguous_block());
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -415,112 +480,95 @@ __global__ __launch_bounds__(64 * kWaves, 3) void range_attend(RangeArgs a) {
     for (int dt = 0; dt < 8; ++dt)
         *reinterpret_cast<f32x4_t*>(red + (wave * 16 + n16) * kDim + 16 * dt + 4 * g4) = o[dt];
     __syncthreads();
-    for (int idx = tid; idx < a.h * kDim; idx += 64 * kWaves) {
-        const int i = idx / kDim, d = idx - i * kDim;
+    const bool merge_here = a.P > 1 && a.arrive != nullptr;
+    for (int i = wave; i < a.h; i += kWaves) {   // wave -> head, lane l -> dims 2 l, 2 l + 1
         float ms = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) ms = fmaxf(ms, ml_sh[w][i][0]);
-        float ls = 0.0f, as = 0.0f;
+        float ls = 0.0f;
+        float2 os = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float mw = ml_sh[w][i][0], lw = ml_sh[w][i][1];
-            // a wave without a finite score has m = -inf: nothing to add, unless its scores were NaN
-            const float ww = mw == -INFINITY ? (lw == 0.0f ? 0.0f : 1.0f) : fast_exp2(mw - ms);
-            ls += ww * lw;
-            as += ww * (red[(w * 16 + i) * kDim + d] + red[(w * 16 + 8 + i) * kDim + d]);
+            const float x = slot_weight(ml_sh[w][i][0], ml_sh[w][i][1], ms);
+            const float2 hi = *reinterpret_cast<const float2*>(red + (w * 16 + i) * kDim + 2 * lane);
+            const float2 rest = *reinterpret_cast<const float2*>(red + (w * 16 + 8 + i) * kDim + 2 * lane);
+            ls += x * ml_sh[w][i][1];
+            os.x += x * (hi.x + rest.x);
+            os.y += x * (hi.y + rest.y);
         }
         if (a.P == 1) {
-            const float r = ls == 0.0f ? 0.0f : as / ls;
-            const size_t at = ((size_t)bg * a.h + i) * kDim + d;
-            if (a.out_bf16) reinterpret_cast<uint16_t*>(a.out)[at] = f32_to_bf16_rne(r);
-            else reinterpret_cast<float*>(a.out)[at] = r;
-        } else {
-            float* pp = a.part + ((size_t)lin * a.h + i) * kPartWords;
-            if (d == 0) {
-                pp[0] = ms;
-                pp[1] = ls;
+            store_row(a, (size_t)bg * a.h + i, ls, os);
+            continue;
+        }
+        float* pp = a.part + ((size_t)lin * a.h + i) * kPartWords;
+        if (merge_here) {   // written through to memory, so the merging workgroup reads them on any XCD
+            if (lane == 0) {
+                store_coherent(pp, ms);
+                store_coherent(pp + 1, ls);
             }
-            pp[2 + d] = as;
+            store_coherent(pp + 2 + 2 * lane, os.x);
+            store_coherent(pp + 3 + 2 * lane, os.y);
+        } else {
+            if (lane == 0) *reinterpret_cast<float2*>(pp) = make_float2(ms, ls);
+            *reinterpret_cast<float2*>(pp + 2 + 2 * lane) = os;
         }
     }
+    if (!merge_here) return;
+    // Arrival: every partial store of this workgroup has completed before its count (the wait and the barrier), so the
+    // workgroup that counts P - 1 before itself finds every partial in memory. It leaves the counter zero.
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0)
+        last_sh = __hip_atomic_fetch_add(a.arrive + bg, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(a.P - 1);
+    __syncthreads();
+    if (!last_sh) return;
+    for (int i = wave; i < a.h; i += kWaves) {
+        float m2, l2;
+        float2 o2;
+        merge_slots<true>(a.part + ((size_t)bg * a.P * a.h + i) * kPartWords, (size_t)a.h * kPartWords, a.P, m2, l2, o2);
+        store_row(a, (size_t)bg * a.h + i, l2, o2);
+    }
+    if (tid == 0) __hip_atomic_store(a.arrive + bg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The partials of a (b, g, head) merged: W waves (one for every four slots, at most eight) take every W-th slot, four of
-// them in flight at once, and meet in LDS; lane l holds dims 2 l, 2 l + 1. Every sum's order is fixed by the slots' numbers.
-constexpr int kMergeWaves = 8;
-__global__ __launch_bounds__(64 * kMergeWaves) void range_combine(RangeArgs a) {
-    const int W = blockDim.x >> 6;
-    __shared__ float ml_sh[kMergeWaves][2];
-    __shared__ float2 acc_sh[kMergeWaves][64];
+// The partials of a (b, g, head) merged: one wave up to kMergeSlots slots, the sums those of the merge inside
+// range_attend; past them four waves that take every fourth slot and meet in LDS.
+__global__ __launch_bounds__(256) void range_combine(RangeArgs a) {
+    __shared__ float ml_sh[4][2];
+    __shared__ float2 acc_sh[4][64];
     const int bg = blockIdx.x / a.h, i = blockIdx.x - bg * a.h;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
     int first = bg * a.P, count = a.P;
     if (a.lengths) {
         int b = bg / a.G;
         slots_of(a, share_of(a), -1, b, first, count);
         first += (bg - b * a.G) * a.B * a.P;
     }
-    const float* pb = a.part + ((size_t)first * a.h + i) * kPartWords;
     const size_t step = (size_t)a.h * kPartWords;
-    float ms = -INFINITY, ls = 0.0f;
-    float2 as = make_float2(0.0f, 0.0f);
-    constexpr int kGroup = 4;   // slots in flight
-    for (int p0 = wave; p0 < count; p0 += kGroup * W) {
-        float mv[kGroup], lv[kGroup];
-        float2 av[kGroup];
-#pragma unroll
-        for (int u = 0; u < kGroup; ++u) {
-            mv[u] = -INFINITY;
-            lv[u] = 0.0f;
-            av[u] = make_float2(0.0f, 0.0f);
-            if (p0 + u * W < count) {
-                const float* pp = pb + (p0 + u * W) * step;
-                mv[u] = pp[0];
-                lv[u] = pp[1];
-                av[u] = *reinterpret_cast<const float2*>(pp + 2 + 2 * lane);
-            }
+    float m, l;
+    float2 o;
+    merge_slots<false>(a.part + ((size_t)first * a.h + i) * kPartWords + wave * step, W * step, (count - wave + W - 1) / W,
+                       m, l, o);
+    if (W > 1) {
+        if (lane == 0) {
+            ml_sh[wave][0] = m;
+            ml_sh[wave][1] = l;
         }
-        float mn = ms;
-#pragma unroll
-        for (int u = 0; u < kGroup; ++u) mn = fmaxf(mn, mv[u]);
-        const float w0 = ms == -INFINITY ? 1.0f : fast_exp2(ms - mn);
-        ls *= w0;
-        as.x *= w0;
-        as.y *= w0;
-#pragma unroll
-        for (int u = 0; u < kGroup; ++u) {
-            const float w = mv[u] == -INFINITY ? (lv[u] == 0.0f ? 0.0f : 1.0f) : fast_exp2(mv[u] - mn);
-            ls += w * lv[u];
-            as.x += w * av[u].x;
-            as.y += w * av[u].y;
+        acc_sh[wave][lane] = o;
+        __syncthreads();
+        if (wave != 0) return;
+        float mt = m;
+        for (int w = 1; w < W; ++w) mt = fmaxf(mt, ml_sh[w][0]);
+        l = 0.0f;
+        o = make_float2(0.0f, 0.0f);
+        for (int w = 0; w < W; ++w) {
+            const float x = slot_weight(ml_sh[w][0], ml_sh[w][1], mt);
+            l += x * ml_sh[w][1];
+            o.x += x * acc_sh[w][lane].x;
+            o.y += x * acc_sh[w][lane].y;
         }
-        ms = mn;
     }
-    if (lane == 0) {
-        ml_sh[wave][0] = ms;
-        ml_sh[wave][1] = ls;
-    }
-    acc_sh[wave][lane] = as;
-    __syncthreads();
-    if (wave != 0) return;
-    float mt = ms;
-    for (int w = 1; w < W; ++w) mt = fmaxf(mt, ml_sh[w][0]);
-    float lt = 0.0f;
-    float2 at = make_float2(0.0f, 0.0f);
-    for (int w = 0; w < W; ++w) {
-        const float mw = ml_sh[w][0], lw = ml_sh[w][1];
-        const float x = mw == -INFINITY ? (lw == 0.0f ? 0.0f : 1.0f) : fast_exp2(mw - mt);
-        lt += x * lw;
-        at.x += x * acc_sh[w][lane].x;
-        at.y += x * acc_sh[w][lane].y;
-    }
-    if (lt == 0.0f) {
-        at = make_float2(0.0f, 0.0f);
-        lt = 1.0f;
-    }
-    const size_t to = ((size_t)bg * a.h + i) * kDim + 2 * lane;
-    if (a.out_bf16) *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + to) = pack_bf16x2(at.x / lt, at.y / lt);
-    else *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.out) + to) = make_float2(at.x / lt, at.y / lt);
+    store_row(a, (size_t)bg * a.h + i, l, o);
 }
 
 template <bool LIST>
@@ -531,8 +579,8 @@ int launch_range(const RangeArgs& a, hipStream_t s) {
     if constexpr (LIST) hipLaunchKernelGGL((range_attend<true, true>), grid, wg, 0, s, a);
     else if (a.ke) hipLaunchKernelGGL((range_attend<true, false>), grid, wg, 0, s, a);
     else hipLaunchKernelGGL((range_attend<false, false>), grid, wg, 0, s, a);
-    if (a.P > 1) hipLaunchKernelGGL(range_combine, dim3((unsigned)(a.B * a.G * a.h)),
-                                    dim3(64 * (a.P <= 4 ? 1 : a.P <= 8 ? 2 : a.P <= 16 ? 4 : kMergeWaves)), 0, s, a);
+    if (a.P > 1 && a.arrive == nullptr)
+        hipLaunchKernelGGL(range_combine, dim3((unsigned)(a.B * a.G * a.h)), dim3(a.P <= kMergeSlots ? 64 : 256), 0, s, a);
     return check_launch(LIST ? "range_attend (rows)" : "range_attend");
 }
 
@@ -549,13 +597,14 @@ int check_range(const void* K, const void* V, const uint8_t* k_exp, const uint8_
     ATTNLAB_REQUIRE(K && V && q && out, "K, V, q and out must be device pointers");
     ATTNLAB_REQUIRE(((reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V) | reinterpret_cast<uintptr_t>(q)) &
                      15) == 0, "K, V and q must be 16-byte aligned");
-    ATTNLAB_REQUIRE(P == 1 || part != nullptr, "P > 1 needs the partial buffer");
+    ATTNLAB_REQUIRE(P == 1 || (part != nullptr && (reinterpret_cast<uintptr_t>(part) & 7) == 0),
+                    "P > 1 needs the partial buffer, 8-byte aligned");
     return ATTNLAB_OK;
 }
 
 RangeArgs range_args(const void* K, const void* V, const uint8_t* k_exp, const uint8_t* v_exp, int block,
                      const uint16_t* q, int B, int G, int h, int C, int P, float scale, void* out, int out_bf16,
-                     float* part) {
+                     float* part, uint32_t* arrive) {
     RangeArgs a{};
     a.B = B;
     a.K = static_cast<const uint8_t*>(K);
@@ -575,6 +624,7 @@ RangeArgs range_args(const void* K, const void* V, const uint8_t* k_exp, const u
     a.out = out;
     a.out_bf16 = out_bf16;
     a.part = part;
+    a.arrive = P > 1 && P <= kMergeSlots ? arrive : nullptr;
     return a;
 }
 
@@ -586,15 +636,16 @@ using namespace attnlab;
 extern "C" int attnlab_range_decode(const void* K, const void* V, const uint8_t* k_exp, const uint8_t* v_exp, int block,
                                     const uint16_t* q, const int32_t* lengths, int length, int64_t q_pos, int window,
                                     int sinks, int B, int G, int h, int C, int P, float scale, void* out, int out_bf16,
-                                    float* part, void* stream) {
+                                    float* part, uint32_t* arrive, void* stream) {
     const int rc = check_range(K, V, k_exp, v_exp, block, q, B, G, h, C, P, out, part);
     if (rc) return rc;
     ATTNLAB_REQUIRE(lengths != nullptr || (0 <= length && length <= C), "valid length %d outside [0, C=%d]", length, C);
     ATTNLAB_REQUIRE(lengths != nullptr || q_pos >= 0, "the query's position %lld must not be negative",
                     (long long)q_pos);
     ATTNLAB_REQUIRE(window >= 0 && sinks >= 0, "window=%d and sinks=%d must not be negative", window, sinks);
-    RangeArgs a = range_args(K, V, k_exp, v_exp, block, q, B, G, h, C, P, scale, out, out_bf16, part);
+    RangeArgs a = range_args(K, V, k_exp, v_exp, block, q, B, G, h, C, P, scale, out, out_bf16, part, arrive);
     a.lengths = lengths;
+    if (lengths) a.arrive = nullptr;   // the sequences' slots are counted on the device
     a.n = lengths ? 0 : (int)(q_pos + 1 < length ? q_pos + 1 : length);   // causal: no key past the query
     a.qend = q_pos + 1;
     a.window = window;
@@ -605,13 +656,13 @@ extern "C" int attnlab_range_decode(const void* K, const void* V, const uint8_t*
 extern "C" int attnlab_quant_attend(const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_exp,
                                     const uint8_t* v_exp, int block, const uint16_t* q, const int32_t* rows,
                                     int64_t rows_stride, int B, int G, int h, int S, int C, int P, float scale,
-                                    void* out, int out_bf16, float* part, void* stream) {
+                                    void* out, int out_bf16, float* part, uint32_t* arrive, void* stream) {
     ATTNLAB_REQUIRE(k_exp && v_exp, "the scale bytes must be device pointers");
     const int rc = check_range(k_codes, v_codes, k_exp, v_exp, block, q, B, G, h, C, P, out, part);
     if (rc) return rc;
     ATTNLAB_REQUIRE(S >= 1, "at least one row must be selected (S=%d)", S);
     ATTNLAB_REQUIRE(rows != nullptr && rows_stride >= S, "rows must hold S=%d positions per (b, g)", S);
-    RangeArgs a = range_args(k_codes, v_codes, k_exp, v_exp, block, q, B, G, h, C, P, scale, out, out_bf16, part);
+    RangeArgs a = range_args(k_codes, v_codes, k_exp, v_exp, block, q, B, G, h, C, P, scale, out, out_bf16, part, arrive);
     a.rows = rows;
     a.rows_stride = rows_stride;
     a.n = S;

@@ -339,23 +339,27 @@ int attnlab_quant_read(const uint8_t* k_codes, const uint8_t* v_codes, const uin
  * position; length and q_pos are then ignored. A query that reads no row, or whose scores are all -inf, gets zeros.
  * K, V: [B, G, C, 128] bf16, or with k_exp and v_exp the 8-bit cache's codes (block: its positions to a scale byte;
  * ignored without). q: [B, G, h, 128] bf16, 1 <= h <= 8. P split-K partitions (1..256): with P > 1, part must hold
- * B * G * P * h * 130 floats and a second launch merges them. out: [B, G, h, 128], bf16 (RNE) when out_bf16 else fp32.
+ * B * G * P * h * 130 floats, 8-byte aligned, for their partials. They are merged by the last workgroup of a (b, g) to
+ * arrive where arrive (uint32 [B*G], zero on entry, left zero, not shared with a call that may overlap) is given, P <= 16
+ * and there are no lengths; by a second launch otherwise, with the same result. out: [B, G, h, 128], bf16 (RNE) when
+ * out_bf16 else fp32.
  * The counterpart of full_attention for one query (full.py:17-44) with the window of a row list F = sinks + recent
  * (selection.py:69-86) read by range.
  */
 int attnlab_range_decode(const void* K, const void* V, const uint8_t* k_exp, const uint8_t* v_exp, int block,
                          const uint16_t* q, const int32_t* lengths, int length, int64_t q_pos, int window, int sinks,
                          int B, int G, int h, int C, int P, float scale, void* out, int out_bf16, float* part,
-                         void* stream);
+                         uint32_t* arrive, void* stream);
 
 /*
  * attnlab_attend over an 8-bit cache: one query's attention over listed rows. rows: [B*G, S] int32 positions (row
  * stride rows_stride), S >= 1; positions outside [0, C) are skipped, never read, and a position listed twice counts
- * twice. q, out, P, part, scale as in attnlab_range_decode.
+ * twice. q, out, P, part, arrive, scale as in attnlab_range_decode.
  */
 int attnlab_quant_attend(const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_exp, const uint8_t* v_exp,
                          int block, const uint16_t* q, const int32_t* rows, int64_t rows_stride, int B, int G, int h,
-                         int S, int C, int P, float scale, void* out, int out_bf16, float* part, void* stream);
+                         int S, int C, int P, float scale, void* out, int out_bf16, float* part, uint32_t* arrive,
+                         void* stream);
 
 /*
  * The chunk form of attnlab_range_decode, on the matrix cores: T queries at positions q_pos0 + t, query t reading

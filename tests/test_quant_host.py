@@ -67,9 +67,9 @@ APPEND = dict(k=16, kb=1024, kg=256, kt=128, v=16, vb=1024, vg=256, vt=128, dtyp
 READ = dict(kc=16, vc=16, ke=16, ve=16, ko=16, vo=16, dtype=0, starts=None, start=0, B=1, G=2, T=4, C=64, block=16,
             stream=None)
 DECODE = dict(K=16, V=16, ke=16, ve=16, block=16, q=16, lengths=None, length=10, q_pos=9, window=0, sinks=0, B=1, G=2,
-              h=2, C=64, P=1, scale=0.1, out=16, out_bf16=1, part=None, stream=None)
+              h=2, C=64, P=1, scale=0.1, out=16, out_bf16=1, part=None, arrive=None, stream=None)
 ROWS = dict(K=16, V=16, ke=16, ve=16, block=16, q=16, rows=16, rows_stride=8, B=1, G=2, h=2, S=8, C=64, P=1, scale=0.1,
-            out=16, out_bf16=1, part=None, stream=None)
+            out=16, out_bf16=1, part=None, arrive=None, stream=None)
 CHUNK = dict(q=16, K=16, V=16, ke=16, ve=16, block=16, out=16, B=1, G=2, h=2, T=4, q_pos0=0, legal=4, C=64, window=0,
              sinks=0, scale=0.1, splits=1, part=None, part_bytes=0, stream=None)
 REFUSED = [
