@@ -219,42 +219,58 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
 
-    auto block = [&](int kb, const uint16_t* ks, const uint16_t* vs) {
+    auto block = [&](int kb, const uint16_t* kt, const uint16_t* vt) {
         // no key of the block is visible to a row of this wave
         if (kb >= kend_wave || (a.window > 0 && kb >= a.sinks && kb + kKeys - 1 <= wfirst - a.window)) return;
+        const char* ks = reinterpret_cast<const char*>(kt);
+        const char* vs = reinterpret_cast<const char*>(vt);
         f32x16_t s[2];
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[kt][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                const bf16x8_t ka = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4_t*>(
-                                                                     reinterpret_cast<const char*>(ks) + 8192 * kt + kof[kk]));
-                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, qb[kk], s[kt], 0, 0, 0);
+            for (int x = 0; x < 2; ++x) {
+                const bf16x8_t ka = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4_t*>(ks + 8192 * x + kof[kk]));
+                s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, qb[kk], s[x], 0, 0, 0);
             }
-        // this lane's scores: row R, keys kb + 32 kt + 8 (i / 4) + 4 g + i % 4
-        const bool whole = kb + kKeys - 1 <= wfirst && kb + kKeys <= a.legal &&
-                           (a.window == 0 || kb + kKeys <= a.sinks || kb > wlast - a.window);
-        if (!whole) {
-            const int from = a.window > 0 ? pos - a.window : -1;   // visible: key > from, or a sink
+        // this lane's scores: row R, keys kb + 4 g + c, c = 32 x + 8 (i / 4) + i % 4. The bounds that a block needs are
+        // applied apart, each a compare with a constant and a select
+        const int at = kb + 4 * g;
+        if (kb + kKeys - 1 > wfirst || kb + kKeys > a.legal) {
+            const int most = min(pos, a.legal - 1) - at;
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = kb + 32 * kt + 8 * (i >> 2) + 4 * g + (i & 3);
-                    if (key > pos || key >= a.legal || (key <= from && key >= a.sinks)) s[kt][i] = -INFINITY;
-                }
+                for (int i = 0; i < 16; ++i) s[x][i] = 32 * x + 8 * (i >> 2) + (i & 3) <= most ? s[x][i] : -INFINITY;
+        }
+        if (a.window > 0 && kb <= wlast - a.window && kb + kKeys > a.sinks) {
+            const int from = pos - a.window - at;   // visible: c > from, or c < sink
+            if (kb >= a.sinks) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[x][i] = 32 * x + 8 * (i >> 2) + (i & 3) > from ? s[x][i] : -INFINITY;
+            } else {
+                const int sink = a.sinks - at;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int c = 32 * x + 8 * (i >> 2) + (i & 3);
+                        s[x][i] = (c > from) | (c < sink) ? s[x][i] : -INFINITY;
+                    }
+            }
         }
         float bm = -INFINITY;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) bm = fmaxf(bm, s[kt][i]);
+            for (int i = 0; i < 16; ++i) bm = fmaxf(bm, s[x][i]);
         bm = max_xor32(bm) * sc;
-        if (bm > m_run + kLazy) {   // also the first block of the row (m_run = -inf)
+        if (bm > m_run + kLazy) {   // also the first keys of the row (m_run = -inf)
             const float al = fast_exp2(m_run - bm);   // exp2(-inf) = 0
             l_run *= al;
 #pragma unroll
@@ -264,7 +280,7 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
             m_run = bm;
         }
         // P^T (bf16: the matrix core's operand; the sum l is of the unrounded weights) as the B operand of
-        // O^T += V^T P^T, one per 16-key step ks: tile ks / 2, accumulators 8 (ks % 2) .. + 7
+        // O^T += V^T P^T, one per 16-key step ks2: tile ks2 / 2, accumulators 8 (ks2 % 2) .. + 7
         bf16x8_t pb[4];
         // no score above -inf in the row yet: weights 0, or NaN for a NaN score
         const float nm = m_run == -INFINITY ? 0.0f : -m_run;
@@ -285,7 +301,7 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
         for (int ks2 = 0; ks2 < 4; ++ks2) {
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt) {
-                const char* vp = reinterpret_cast<const char*>(vs) + 4096 * ks2 + vof[dt];
+                const char* vp = vs + 4096 * ks2 + vof[dt];
                 const u32x2v_t lo4 = read_tr16(vp), hi4 = read_tr16(vp + 8 * 256);
                 const bf16x8_t va = __builtin_bit_cast(bf16x8_t, u32x4_t{lo4.x, lo4.y, hi4.x, hi4.y});
                 o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pb[ks2], o[dt], 0, 0, 0);
