@@ -48,8 +48,8 @@ def decode_partitions(BG: int, count: int, ragged: bool = False) -> int:
 def chunk_splits(BG: int, h: int, T: int, keys: int) -> int:
     """Workgroups that share a query tile's keys (`keys`: those the longest tile reads): one where the tiles give every CU
     more than one, else as many as bring the grid to about two per CU, each at least 512 keys. MI355X, 8-bit: 1000 queries
-    (h=2) after 29011, 128 tiles, 754 us in one, 387 in two, 268 in four, 278 in eight; a 2K prompt (h=2), 256 tiles, 59
-    us in one, 46 in two; 1501 queries under a 2047 window (B=2, h=2), 384 tiles, 82 us in one, 87 in two."""
+    (h=2) after 29011, 128 tiles, 583 us in one, 300 in two, 256 in four, 262 in eight; a 2K prompt (h=2), 256 tiles, 46
+    us in one, 41 in two; 1501 queries under a 2047 window (B=2, h=2), 384 tiles, 77 us in one, 79 in two."""
     tiles = BG * -(-T // (CHUNK_ROWS // h))
     if tiles > 256:
         return 1

@@ -4,15 +4,17 @@
 //
 // A workgroup owns 128 (query, head) rows, 128 / h consecutive queries with all h heads, and walks blocks of 64 keys: the
 // blocks of the sinks, then those from the first query's window on. Per block S^T = K Q^T, the softmax on its
-// accumulators, O^T += V^T P^T (v_mfma_f32_32x32x16_bf16; a row's softmax state and outputs stay in lanes n and n + 32),
-// with K and V as bf16 tiles in LDS, a block ahead, one barrier a block. The bf16 cache is copied into LDS directly; an
-// 8-bit one passes through registers, 32 codes a thread and tensor, each converted once for all four waves (exactly, its
-// scale included), while the block before it is computed.
+// accumulators, O^T += V^T P^T (v_mfma_f32_32x32x16_bf16; a row's softmax state and outputs stay in lanes n and n + 32).
+// K and V are copied into LDS in the cache's own format without passing through registers, a block ahead, one barrier a
+// block; an 8-bit operand becomes bf16 (exactly, its scale included) as it is read, which costs each wave 128 conversions
+// a block and halves what it reads from LDS.
 //
 // A masked key has weight zero, but zero times a V row that holds NaN or infinity is NaN. Rows past the visible range are
-// written as zeros; inside it a key can be masked for one row and visible to the next, so a row whose result is not
-// finite is computed again key by key, over its visible keys alone (row_again).
+// copied as zeros; inside it a key can be masked for one row and visible to the next. So a workgroup with a result that is
+// not finite takes its rows again, looks over the blocks that have masked keys and multiplies those that hold such values
+// by way of flags.
 #include <cfloat>
+#include <type_traits>
 
 #include "mfma_attend.h"
 #include "quant.h"
@@ -46,60 +48,26 @@ struct RangePrefillArgs {
     float* part;            // [BG, h, T, splits, 132]
 };
 
-// A row's outputs from the formula over the block's visible keys, one at a time, by one wave: lane l holds dims 2 l and
-// 2 l + 1.
-template <bool Q8>
-__device__ __forceinline__ void row_again(const RangePrefillArgs& a, int bg, int pos, int kb, float q0, float q1,
-                                          float& m, float& l, float& a0, float& a1) {
-    const int lane = threadIdx.x & 63;
-    for (int j = 0; j < kKeys; ++j) {
-        const int key = kb + j;
-        if (key > pos || key >= a.legal) break;
-        if (a.window > 0 && key <= pos - a.window && key >= a.sinks) continue;
-        float k0, k1, v0, v1;
-        const size_t at = ((size_t)bg * a.C + key) * kDim + 2 * lane;
-        if constexpr (Q8) {
-            const float ks = scale_of(a.ke[(size_t)bg * a.nb + (key >> a.shift)]);
-            const float vs = scale_of(a.ve[(size_t)bg * a.nb + (key >> a.shift)]);
-            const qf32x2_t kk = e4m3_to_f32x2<false>(*reinterpret_cast<const uint16_t*>((const uint8_t*)a.K + at));
-            const qf32x2_t vv = e4m3_to_f32x2<false>(*reinterpret_cast<const uint16_t*>((const uint8_t*)a.V + at));
-            k0 = kk.x * ks;
-            k1 = kk.y * ks;
-            v0 = vv.x * vs;
-            v1 = vv.y * vs;
-        } else {
-            const uint32_t kk = *reinterpret_cast<const uint32_t*>((const uint16_t*)a.K + at);
-            const uint32_t vv = *reinterpret_cast<const uint32_t*>((const uint16_t*)a.V + at);
-            k0 = bf16_lo(kk);
-            k1 = bf16_hi(kk);
-            v0 = bf16_lo(vv);
-            v1 = bf16_hi(vv);
-        }
-        float x = q0 * k0 + q1 * k1;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
-        x *= a.scale_log2;
-        if (x > m) {
-            const float al = fast_exp2(m - x);
-            l *= al;
-            a0 *= al;
-            a1 *= al;
-            m = x;
-        }
-        const float p = fast_exp2(x - (m == -INFINITY ? 0.0f : m));
-        l += p;
-        a0 += p * v0;
-        a1 += p * v1;
-    }
+// NaN and infinity among two packed bf16: the pair with those elements zeroed, and a pair of flags (1.0 or 0).
+__device__ __forceinline__ uint32_t bf16x2_finite(uint32_t w, uint32_t& flags) {
+    const uint32_t lo = (w & 0x00007f80u) == 0x00007f80u ? 0x0000ffffu : 0u;
+    const uint32_t hi = (w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
+    flags = (lo & 0x3f80u) | (hi & 0x3f800000u);
+    return w & ~(lo | hi);
 }
 
-// K and V blocks in LDS: 64 rows of 256 bytes, sixteen 16-byte chunks each, permuted within the row so that the operand
-// reads meet no bank twice. K: chunk c of row j at slot c ^ (j & 15) (16 rows, one chunk). V: chunk c of row j at slot
-// c ^ (4 (j & 3)) (a transposing read takes 4 chunks of 4 consecutive rows).
+// K and V blocks in LDS: 64 rows in 16-byte chunks, permuted within the row so that the reads meet no bank twice.
+// bf16, 16 chunks: K's chunk c of row j at slot c ^ (j & 15) (a read takes 16 rows, one chunk), V's at c ^ (4 (j & 3)) (a
+// transposing read takes 4 chunks of 4 consecutive rows). 8-bit, 8 chunks: both at c ^ (j / 2 % 8) (K: 16 rows, one
+// chunk; V: one chunk of 8 consecutive rows).
+// Key 16 z + 8 g + 4 a + b of a 32-key tile is row 16 z + 8 a + 4 g + b of its product, so that a lane's weights are those
+// of eight consecutive keys, the ones whose V its operand holds.
 template <bool SPLIT, bool Q8>
 __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
-    __shared__ __attribute__((aligned(1024))) uint16_t kt0[kKeys * kDim], vt0[kKeys * kDim];
-    __shared__ __attribute__((aligned(1024))) uint16_t kt1[kKeys * kDim], vt1[kKeys * kDim];
+    constexpr int kRow = Q8 ? kDim : 2 * kDim;   // bytes of a row
+    __shared__ __attribute__((aligned(1024))) char kt0[kKeys * kRow], vt0[kKeys * kRow];
+    __shared__ __attribute__((aligned(1024))) char kt1[kKeys * kRow], vt1[kKeys * kRow];
+    __shared__ int again;
     const int lin = xcd_contiguous_block();
     // the query tiles of a (b, g) in reverse: without a window the later ones read more keys, so they start first
     const int nsp = SPLIT ? a.splits : 1;
@@ -116,11 +84,16 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
     const int t = t0 + R / a.h, head = R % a.h;
     const int tc = min(t, tend - 1);             // rows past the last query repeat it and are not written
     const int pos = a.q_pos0 + tc;
-    bf16x8_t qb[8];                              // B operand of S^T: row R, dims 16 kk + 8 g .. + 7
+    // B operand of S^T: row R, in step kk dims 16 kk + 8 g .. + 7 (8-bit: 32 (kk / 2) + 16 g + 8 (kk % 2) .., two steps to
+    // a 16-byte read of K)
+    bf16x8_t qb[8];
     {
-        const uint16_t* qr = a.q + (((size_t)bg * a.h + head) * a.T + tc) * kDim + 8 * g;
+        const uint16_t* qr = a.q + (((size_t)bg * a.h + head) * a.T + tc) * kDim;
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) qb[kk] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4_t*>(qr + 16 * kk));
+        for (int kk = 0; kk < 8; ++kk) {
+            const int d = Q8 ? 32 * (kk >> 1) + 16 * g + 8 * (kk & 1) : 16 * kk + 8 * g;
+            qb[kk] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4_t*>(qr + d));
+        }
     }
     // the tile's keys: blocks [0, na) for the sinks, then [bw, ceil(kend / 64)) from the first query's window on
     const int kend = min(a.legal, a.q_pos0 + tend);
@@ -138,70 +111,58 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
     const int wlast = a.q_pos0 + min(t0 + __builtin_amdgcn_readfirstlane((32 * wave + 31) / a.h), tend - 1);
     const int kend_wave = min(a.legal, wlast + 1);
 
-    // staging. bf16: load u of wave w fills rows 16 u + 4 w .. + 3 of a tile, lane l slot l % 16 of row l / 16 of them, from
-    // a buffer of those 4 rows (rows past kend give zeros)
-    const int srow = 4 * wave + (lane >> 4);
-    const uint32_t koff = 256u * (lane >> 4) + 16u * ((lane & 15) ^ srow);
-    const uint32_t voff = 256u * (lane >> 4) + 16u * ((lane & 15) ^ ((lane >> 4) << 2));
-    const uint16_t* Kb = reinterpret_cast<const uint16_t*>(a.K) + (size_t)bg * a.C * kDim;
-    const uint16_t* Vb = reinterpret_cast<const uint16_t*>(a.V) + (size_t)bg * a.C * kDim;
-    auto copy = [&](int kb, uint16_t* kt, uint16_t* vt) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int row = kb + 16 * u + 4 * wave;
-            const uint32_t bytes = 256u * (uint32_t)__builtin_amdgcn_readfirstlane(max(min(kend - row, 4), 0));
-            load_lds16_buf(Kb + (size_t)row * kDim, bytes, koff, kt + (16 * u + 4 * wave) * kDim);
-            load_lds16_buf(Vb + (size_t)row * kDim, bytes, voff, vt + (16 * u + 4 * wave) * kDim);
-        }
-    };
-    // 8-bit: 16 codes of rows tid / 8 and 32 + tid / 8 of each tensor through registers
-    const uint8_t* K8 = reinterpret_cast<const uint8_t*>(a.K) + (size_t)bg * a.C * kDim;
-    const uint8_t* V8 = reinterpret_cast<const uint8_t*>(a.V) + (size_t)bg * a.C * kDim;
+    // staging: a load of a wave fills 1 KB of a tile, kPer rows, lane l slot l % kSlots of row l / kSlots of them, from a
+    // buffer of those rows (rows past kend give zeros)
+    constexpr int kSlots = kRow / 16, kPer = 64 / kSlots, kLoads = kKeys / kPer / 4;
+    const int srow = lane / kSlots, slot = lane % kSlots;
+    const int kswz = Q8 ? 4 * (wave & 1) + (srow >> 1) : 4 * wave + srow, vswz = Q8 ? kswz : 4 * srow;
+    const uint32_t koff = kRow * srow + 16 * (slot ^ kswz), voff = kRow * srow + 16 * (slot ^ vswz);
+    const char* Kb = reinterpret_cast<const char*>(a.K) + (size_t)bg * a.C * kRow;
+    const char* Vb = reinterpret_cast<const char*>(a.V) + (size_t)bg * a.C * kRow;
     const uint8_t* keb = Q8 ? a.ke + (size_t)bg * a.nb : nullptr;
     const uint8_t* veb = Q8 ? a.ve + (size_t)bg * a.nb : nullptr;
-    u32x4_t rk[2], rv[2];
-    uint32_t xk[2], xv[2];
-    auto fetch = [&](int kb) {
+    const int last = (a.C - 1) >> a.shift;   // the last scale byte
+    uint32_t kx[2], vx[4];                   // the next block's scale bytes: K, of this lane's rows; V, of 16 keys each
+    auto copy = [&](int kb, char* kt, char* vt) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = kb + 32 * u + (tid >> 3);
-            const int rc = min(row, kend - 1);
-            rk[u] = *reinterpret_cast<const u32x4_t*>(K8 + (size_t)rc * kDim + 16 * (tid & 7));
-            rv[u] = *reinterpret_cast<const u32x4_t*>(V8 + (size_t)rc * kDim + 16 * (tid & 7));
-            xk[u] = keb[rc >> a.shift];
-            xv[u] = veb[rc >> a.shift];
-            if (row >= kend) rk[u] = rv[u] = u32x4_t{0, 0, 0, 0};
+        for (int u = 0; u < kLoads; ++u) {
+            const int part = 4 * u + wave, row = kb + kPer * part;
+            const uint32_t bytes = kRow * (uint32_t)__builtin_amdgcn_readfirstlane(max(min(kend - row, kPer), 0));
+            load_lds16_buf(reinterpret_cast<const uint16_t*>(Kb + (size_t)row * kRow), bytes, koff,
+                           reinterpret_cast<uint16_t*>(kt + 1024 * part));
+            load_lds16_buf(reinterpret_cast<const uint16_t*>(Vb + (size_t)row * kRow), bytes, voff,
+                           reinterpret_cast<uint16_t*>(vt + 1024 * part));
+        }
+        if constexpr (Q8) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) kx[x] = keb[min((kb + 32 * x + (n & 16)) >> a.shift, last)];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) vx[x] = veb[min((kb + 16 * x) >> a.shift, last)];
         }
     };
-    auto expand = [&](uint16_t* kt, uint16_t* vt) {
+    // operand reads, as byte offsets into a tile. K: this lane's key of a 32-key tile, bf16 chunk 2 kk + g (8-bit: chunk
+    // 2 (kk / 2) + g). V: bf16 rows 16 ks + 8 g + 4 hf + e, dims 32 dt + 16 (lane / 16 % 2) + 4 j .. + 3, e = lane % 16 / 4,
+    // j = lane % 4; 8-bit rows 16 ks + 8 g + e, bytes 32 dt + 16 (lane / 16 % 2) + 8 j .. + 7, e = lane % 16 / 2,
+    // j = lane % 2. `pin` keeps the compiler from holding a copy of each per tile.
+    const int key = (n & 16) + 8 * ((n >> 2) & 1) + 4 * ((n >> 3) & 1) + (n & 3);
+    constexpr int kKof = Q8 ? 4 : 8;
+    uint32_t kof[kKof], vof[4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = 32 * u + (tid >> 3), c = 2 * (tid & 7);
-            auto put = [&](uint16_t* tile, int swz, const u32x4_t& w, float s) {
-                u32x4_t* dst = reinterpret_cast<u32x4_t*>(tile + row * kDim);
-                dst[c ^ swz] = u32x4_t{e4m3_to_bf16x2<false>(w.x, s), e4m3_to_bf16x2<true>(w.x, s),
-                                       e4m3_to_bf16x2<false>(w.y, s), e4m3_to_bf16x2<true>(w.y, s)};
-                dst[(c + 1) ^ swz] = u32x4_t{e4m3_to_bf16x2<false>(w.z, s), e4m3_to_bf16x2<true>(w.z, s),
-                                             e4m3_to_bf16x2<false>(w.w, s), e4m3_to_bf16x2<true>(w.w, s)};
-            };
-            put(kt, row & 15, rk[u], scale_of(xk[u]));
-            put(vt, 4 * (row & 3), rv[u], scale_of(xv[u]));
-        }
-    };
-    // operand reads, as byte offsets into a tile: K row 32 kt + n, chunk 2 kk + g; V rows 16 ks + 8 hf + 4 g + e, dims
-    // 32 dt + 16 (lane / 16 % 2) + 4 j .. + 3, e = lane % 16 / 4, j = lane % 4. `pin` keeps the compiler from holding a
-    // copy of each per tile.
-    uint32_t kof[8], vof[4];
-    const int ve = (lane >> 2) & 3;
+    for (int kk = 0; kk < kKof; ++kk) kof[kk] = kRow * key + 16 * ((2 * kk + g) ^ (Q8 ? (key >> 1) & 7 : key & 15));
+    const int ve = Q8 ? (lane & 15) >> 1 : (lane & 15) >> 2;
 #pragma unroll
-    for (int kk = 0; kk < 8; ++kk) kof[kk] = 256 * n + 16 * ((2 * kk) ^ g ^ (n & 15));
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt) vof[dt] = 256 * (4 * g + ve) + 64 * (dt ^ ve) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    for (int dt = 0; dt < 4; ++dt)
+        vof[dt] = Q8 ? kRow * (8 * g + ve) + 16 * ((2 * dt + ((lane >> 4) & 1)) ^ (4 * g + (ve >> 1))) + 8 * (lane & 1)
+                     : kRow * (8 * g + ve) + 64 * (dt ^ ve) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
     auto pin = [&]() {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) asm volatile("" : "+v"(kof[kk]));
+        for (int kk = 0; kk < kKof; ++kk) asm volatile("" : "+v"(kof[kk]));
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt) asm volatile("" : "+v"(vof[dt]));
+    };
+    auto widen = [&](uint32_t w0, uint32_t w1, float scale) {   // eight codes as a bf16 operand
+        return __builtin_bit_cast(bf16x8_t, u32x4_t{e4m3_to_bf16x2<false>(w0, scale), e4m3_to_bf16x2<true>(w0, scale),
+                                                    e4m3_to_bf16x2<false>(w1, scale), e4m3_to_bf16x2<true>(w1, scale)});
     };
 
     float m_run = -INFINITY, l_run = 0.0f;
@@ -219,50 +180,88 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
 
-    auto block = [&](int kb, const uint16_t* kt, const uint16_t* vt) {
+    auto block = [&](auto careful, int kb, const char* ks, const char* vs, const float (&ksc)[2], const float (&vsc)[4])
+                     __attribute__((always_inline)) {
         // no key of the block is visible to a row of this wave
         if (kb >= kend_wave || (a.window > 0 && kb >= a.sinks && kb + kKeys - 1 <= wfirst - a.window)) return;
-        const char* ks = reinterpret_cast<const char*>(kt);
-        const char* vs = reinterpret_cast<const char*>(vt);
+        // whether a key is masked for some row of the wave: past its position or the legal keys, or ahead of its window
+        const bool ahead = kb + kKeys - 1 > wfirst || kb + kKeys > a.legal;
+        const bool behind = a.window > 0 && kb <= wlast - a.window && kb + kKeys > a.sinks;
+        auto value = [&](int ks2, int dt) -> bf16x8_t {   // V^T's operand of 16-key step ks2, dims 32 dt ..
+            const char* vp = vs + 16 * kRow * ks2 + vof[dt];
+            if constexpr (Q8) {
+                const u32x2v_t w = read_tr8(vp);
+                return widen(w.x, w.y, vsc[ks2]);
+            } else {
+                const u32x2v_t lo4 = read_tr16(vp), hi4 = read_tr16(vp + 4 * kRow);
+                return __builtin_bit_cast(bf16x8_t, u32x4_t{lo4.x, lo4.y, hi4.x, hi4.y});
+            }
+        };
+        bool spoilt = false;   // some V of a block with masked keys is NaN or infinite
+        if (careful && (ahead || behind)) {
+            float chk = 0.0f;  // 0 times it, which is NaN
+#pragma unroll
+            for (int ks2 = 0; ks2 < 4; ++ks2)
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) {
+                    const u32x4_t w = __builtin_bit_cast(u32x4_t, value(ks2, dt));
+                    chk = dot2_bf16(w.x, 0u, chk);
+                    chk = dot2_bf16(w.y, 0u, chk);
+                    chk = dot2_bf16(w.z, 0u, chk);
+                    chk = dot2_bf16(w.w, 0u, chk);
+                    __builtin_amdgcn_sched_barrier(0);   // an operand at a time: registers
+                }
+            spoilt = __any(chk != 0.0f);
+        }
         f32x16_t s[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
+        for (int kk = 0; kk < kKof; ++kk)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const bf16x8_t ka = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4_t*>(ks + 8192 * x + kof[kk]));
-                s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, qb[kk], s[x], 0, 0, 0);
+                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(ks + 32 * kRow * x + kof[kk]);
+                if constexpr (Q8) {
+                    s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(w.x, w.y, ksc[x]), qb[2 * kk], s[x], 0, 0, 0);
+                    s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(w.z, w.w, ksc[x]), qb[2 * kk + 1], s[x], 0, 0, 0);
+                } else {
+                    s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, w), qb[kk], s[x], 0, 0, 0);
+                }
             }
-        // this lane's scores: row R, keys kb + 4 g + c, c = 32 x + 8 (i / 4) + i % 4. The bounds that a block needs are
+        // this lane's scores: row R, keys kb + 8 g + c, c = 32 x + 16 (i / 8) + i % 8. The bounds that a block needs are
         // applied apart, each a compare with a constant and a select
-        const int at = kb + 4 * g;
-        if (kb + kKeys - 1 > wfirst || kb + kKeys > a.legal) {
+        const int at = kb + 8 * g;
+        if (ahead) {
             const int most = min(pos, a.legal - 1) - at;
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[x][i] = 32 * x + 8 * (i >> 2) + (i & 3) <= most ? s[x][i] : -INFINITY;
+                for (int i = 0; i < 16; ++i) s[x][i] = 32 * x + 16 * (i >> 3) + (i & 7) <= most ? s[x][i] : -INFINITY;
         }
-        if (a.window > 0 && kb <= wlast - a.window && kb + kKeys > a.sinks) {
+        if (behind) {
             const int from = pos - a.window - at;   // visible: c > from, or c < sink
             if (kb >= a.sinks) {
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[x][i] = 32 * x + 8 * (i >> 2) + (i & 3) > from ? s[x][i] : -INFINITY;
+                    for (int i = 0; i < 16; ++i) s[x][i] = 32 * x + 16 * (i >> 3) + (i & 7) > from ? s[x][i] : -INFINITY;
             } else {
                 const int sink = a.sinks - at;
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int c = 32 * x + 8 * (i >> 2) + (i & 3);
+                        const int c = 32 * x + 16 * (i >> 3) + (i & 7);
                         s[x][i] = (c > from) | (c < sink) ? s[x][i] : -INFINITY;
                     }
             }
+        }
+        uint32_t see = 0;   // a spoilt block's visible keys, a bit for each of this lane's scores
+        if (careful && spoilt) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) see |= s[i >> 4][i & 15] == -INFINITY ? 0u : 1u << i;
         }
         float bm = -INFINITY;
 #pragma unroll
@@ -297,89 +296,90 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
             }
             pb[ks2] = __builtin_bit_cast(bf16x8_t, u32x4_t{w4[0], w4[1], w4[2], w4[3]});
         }
+        if (!careful || !spoilt) {
 #pragma unroll
-        for (int ks2 = 0; ks2 < 4; ++ks2) {
+            for (int ks2 = 0; ks2 < 4; ++ks2)
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt)
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value(ks2, dt), pb[ks2], o[dt], 0, 0, 0);
+        } else {   // the finite values' products, and NaN where a visible key's value is not finite
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt) {
-                const char* vp = vs + 4096 * ks2 + vof[dt];
-                const u32x2v_t lo4 = read_tr16(vp), hi4 = read_tr16(vp + 8 * 256);
-                const bf16x8_t va = __builtin_bit_cast(bf16x8_t, u32x4_t{lo4.x, lo4.y, hi4.x, hi4.y});
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pb[ks2], o[dt], 0, 0, 0);
+                f32x16_t f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) f[i] = 0.0f;
+#pragma unroll
+                for (int ks2 = 0; ks2 < 4; ++ks2) {
+                    u32x4_t v = __builtin_bit_cast(u32x4_t, value(ks2, dt)), flag, one;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t bits;
+                        v[e] = bf16x2_finite(v[e], bits);
+                        flag[e] = bits;
+                        const uint32_t two = see >> (8 * ks2 + 2 * e);
+                        one[e] = (two & 1u ? 0x3f80u : 0u) | (two & 2u ? 0x3f800000u : 0u);
+                    }
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v), pb[ks2], o[dt], 0, 0, 0);
+                    f = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, flag),
+                                                                __builtin_bit_cast(bf16x8_t, one), f, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[dt][i] = f[i] > 0.0f ? __builtin_nanf("") : o[dt][i];
             }
         }
     };
-    // Two tile pairs: the next block's copies (or its loads into registers) are issued when every wave has left the tiles
-    // they overwrite, the barrier that also publishes the current block, and land while it is computed.
-    if constexpr (Q8) {
-        auto publish = [&]() {
-            __builtin_amdgcn_s_waitcnt(0xc07f);   // lgkmcnt(0): this wave's LDS stores and reads are done
-            asm volatile("s_barrier" ::: "memory");
-            pin();
-        };
-        if (i0 < i1) {
-            fetch(first_key(i0));
-            expand(kt0, vt0);
+    // Two tile pairs: the next block's copies are issued when every wave has left the tiles they overwrite, the barrier that
+    // also publishes the current block, and land while it is computed. The pairs are separate arrays, so that the
+    // compiler knows a block's reads apart from the copies in flight.
+    float ksc[2] = {1.0f, 1.0f}, vsc[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+    auto publish = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0): this wave's copies have landed, its reads are done
+        asm volatile("s_barrier" ::: "memory");
+        pin();
+        if constexpr (Q8) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) ksc[x] = scale_of(kx[x]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) vsc[x] = scale_of(vx[x]);
         }
-        for (int i = i0; i < i1; i += 2) {
-            publish();
-            if (i + 1 < i1) fetch(first_key(i + 1));
-            block(first_key(i), kt0, vt0);
-            if (i + 1 >= i1) break;
-            expand(kt1, vt1);
-            publish();
-            if (i + 2 < i1) fetch(first_key(i + 2));
-            block(first_key(i + 1), kt1, vt1);
-            if (i + 2 < i1) expand(kt0, vt0);
-        }
-    } else {
-        auto publish = [&]() {
-            __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0): this wave's copies have landed, its reads are done
-            asm volatile("s_barrier" ::: "memory");
-            pin();
-        };
-        if (i0 < i1) copy(first_key(i0), kt0, vt0);
-        for (int i = i0; i < i1; i += 2) {
-            publish();
-            if (i + 1 < i1) copy(first_key(i + 1), kt1, vt1);
-            block(first_key(i), kt0, vt0);
-            if (i + 1 >= i1) break;
-            publish();
-            if (i + 2 < i1) copy(first_key(i + 2), kt0, vt0);
-            block(first_key(i + 1), kt1, vt1);
-        }
+    };
+    if (tid == 0) again = 0;   // published by the first block's barrier
+    if (i0 < i1) copy(first_key(i0), kt0, vt0);
+    for (int i = i0; i < i1; i += 2) {
+        publish();
+        if (i + 1 < i1) copy(first_key(i + 1), kt1, vt1);
+        block(std::false_type{}, first_key(i), kt0, vt0, ksc, vsc);
+        if (i + 1 >= i1) break;
+        publish();
+        if (i + 2 < i1) copy(first_key(i + 2), kt0, vt0);
+        block(std::false_type{}, first_key(i + 1), kt1, vt1, ksc, vsc);
     }
-    const float l_tot = l_run + shfl_xor_f32(l_run, 32);
-    const bool row = t < tend;
-    // a row whose result is not finite: from its visible keys alone
-    float finite = 0.0f * l_tot;
+    // A result that is not finite: a visible key's doing, or zero weights times a masked one's values. All rows again, with
+    // the blocks that have masked keys looked over (two to three times the time, where there are such values).
+    float finite = 0.0f * l_run;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) finite = fmaf(0.0f, o[dt][i], finite);
-    const uint64_t bad2 = __ballot(row && finite != 0.0f);
-    const uint32_t bad = (uint32_t)bad2 | (uint32_t)(bad2 >> 32);
-    for (uint32_t left = bad; left; left &= left - 1) {
-        const int r = 32 * wave + __builtin_ctz(left);
-        const int rt = t0 + r / a.h, rh = r % a.h;
-        const uint16_t* qr = a.q + (((size_t)bg * a.h + rh) * a.T + rt) * kDim;
-        const uint32_t qw = *reinterpret_cast<const uint32_t*>(qr + 2 * lane);
-        float m = -INFINITY, l = 0.0f, a0 = 0.0f, a1 = 0.0f;
-        for (int i = i0; i < i1; ++i)
-            row_again<Q8>(a, bg, a.q_pos0 + rt, first_key(i), bf16_lo(qw), bf16_hi(qw), m, l, a0, a1);
-        if constexpr (SPLIT) {
-            float* pp = a.part + ((((size_t)bg * a.h + rh) * a.T + rt) * a.splits + sp) * kPart;
-            if (lane == 0) {
-                pp[0] = m;
-                pp[1] = l;
-            }
-            *reinterpret_cast<float2*>(pp + 4 + 2 * lane) = make_float2(a0, a1);
-        } else {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            *reinterpret_cast<uint32_t*>(a.out + (((size_t)bg * a.h + rh) * a.T + rt) * kDim + 2 * lane) =
-                pack_bf16x2(a0 * inv, a1 * inv);
+    if (__any(finite != 0.0f) && lane == 0) again = 1;
+    __syncthreads();
+    if (again) {
+        m_run = -INFINITY;
+        l_run = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
+        for (int i = i0; i < i1; ++i) {
+            copy(first_key(i), kt0, vt0);
+            publish();
+            block(std::true_type{}, first_key(i), kt0, vt0, ksc, vsc);
+            __syncthreads();
         }
     }
-    if (!row || (bad >> n & 1)) return;
+    const float l_tot = l_run + shfl_xor_f32(l_run, 32);
+    if (t >= tend) return;
     if constexpr (SPLIT) {   // this split's partial: m (log2 domain, scaled), l and the unnormalised outputs
         float* pp = a.part + ((((size_t)bg * a.h + head) * a.T + t) * a.splits + sp) * kPart;
         if (g == 0) {
