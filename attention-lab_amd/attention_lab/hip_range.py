@@ -5,9 +5,10 @@ The kernels behind `window_attention` (window.py) and `quant_attention` / `quant
 check their caches; this module checks what the reads share, chooses the split counts and launches, on the tensors' own
 device and torch's current stream of it.
 
-The split-K partials are allocated for each call. The last workgroup of a (b, g) to arrive merges them where a counter
-tells it that it is: counters belong to a stream, whose calls follow one another and leave them zero. A captured call
-takes a second launch for the merge instead (the same sums), so a graph shares nothing with other graphs or calls.
+The last workgroup of a (b, g) to arrive merges its split-K partials where a counter tells it that it is: the counters and
+partials of such single launches belong to a stream, whose launches follow one another and leave the counters zero. Other
+calls, a captured one among them, allocate partials of their own and take a second launch for the merge (the same sums),
+so a graph shares nothing with other graphs or calls.
 """
 from __future__ import annotations
 
@@ -112,22 +113,34 @@ def split_count(partitions, chosen: int, most: int) -> int:
     return int(partitions)
 
 
-_ARRIVALS: dict = {}   # (device index, stream) -> its counters, zeroed once, left zero by every call
-COUNTERS = 4096        # (b, g) rows that they serve; more take the second launch
+_MERGES: dict = {}      # (device index, stream) -> its counters, zeroed once and left zero by every call, and partials
+COUNTERS = 4096         # (b, g) rows that they serve
+PARTIALS = 8 * 512      # (slot, head) partials: one or two workgroups per CU of eight heads, 2.1 MB
+PART_WORDS = HEAD_DIM + 2
 
 
 def _split_k(P: int, BG: int, h: int, device, stream: int, counted: bool):
-    """(partials, counters' address) of a one-query call split over P workgroups."""
+    """(tensor to hold on to, partials' address, counters' address) of a one-query call split over P workgroups."""
     if P == 1:
-        return None, None
-    part = torch.empty(BG * P * h * (HEAD_DIM + 2), dtype=torch.float32, device=device)
-    if not counted or P > MERGE_SLOTS or BG > COUNTERS or torch._C._cuda_isCurrentStreamCapturing():
-        return part, None
-    key = (device.index, stream)
-    counters = _ARRIVALS.get(key)
-    if counters is None:
-        counters = _ARRIVALS[key] = torch.zeros(COUNTERS, dtype=torch.int32, device=device)
-    return part, counters.data_ptr()
+        return None, None, None
+    rows = BG * P * h
+    if counted and P <= MERGE_SLOTS and BG <= COUNTERS and rows <= PARTIALS and not _capturing(device):
+        buf = _MERGES.get((device.index, stream))
+        if buf is None:
+            buf = _MERGES[device.index, stream] = torch.zeros(COUNTERS + PARTIALS * PART_WORDS, dtype=torch.int32,
+                                                              device=device)
+        at = buf.data_ptr()
+        return buf, at + 4 * COUNTERS, at
+    part = torch.empty(rows * PART_WORDS, dtype=torch.float32, device=device)
+    return part, part.data_ptr(), None
+
+
+def _capturing(device) -> bool:
+    """torch's current stream on `device` is being captured."""
+    if device.index == torch._C._cuda_getDevice():
+        return torch._C._cuda_isCurrentStreamCapturing()
+    with torch.cuda.device(device):
+        return torch._C._cuda_isCurrentStreamCapturing()
 
 
 def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: int, C: int, device, *, valid_length,
@@ -162,10 +175,10 @@ def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: 
     if T == 1 and h <= MAX_H:
         out = check_out(out, q, out_dtype)
         P = split_count(partitions, decode_partitions(B * G, seen, lengths is not None), MAX_P)
-        part, arrive = _split_k(P, B * G, h, device, stream, lengths is None)
+        held, part, arrive = _split_k(P, B * G, h, device, stream, lengths is None)
         nat.call_on(device, "attnlab_range_decode", k_ptr, v_ptr, *exp_ptrs, block, q.data_ptr(), nat.ptr(lengths), legal,
                     p0, window, sinks, B, G, h, C, P, sc, out.data_ptr(), int(out_dtype == torch.bfloat16),
-                    nat.ptr(part), arrive, stream)
+                    part, arrive, stream)
         return out
     if out_dtype != torch.bfloat16:
         raise ValueError("a chunk's outputs are bfloat16")
@@ -195,9 +208,9 @@ def listed_attention(q, cache, rows, *, scale, out, out_dtype, partitions):
     out = check_out(out, q, out_dtype)
     P = split_count(partitions, decode_partitions(B * G, S), MAX_P)
     stream = nat.stream_of(device)
-    part, arrive = _split_k(P, B * G, h, device, stream, True)
+    held, part, arrive = _split_k(P, B * G, h, device, stream, True)
     sc = float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
     nat.call_on(device, "attnlab_quant_attend", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(),
                 cache.v_exp.data_ptr(), cache.block, q.data_ptr(), rows.data_ptr(), S, B, G, h, S, C, P, sc,
-                out.data_ptr(), int(out_dtype == torch.bfloat16), nat.ptr(part), arrive, stream)
+                out.data_ptr(), int(out_dtype == torch.bfloat16), part, arrive, stream)
     return out

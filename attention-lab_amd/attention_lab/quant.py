@@ -28,6 +28,7 @@ from . import hip_range
 from .hip_attend import HEAD_DIM
 
 BLOCKS = (16, 32, 64)
+_POSITIONS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 _DTYPES = {torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16, torch.float32: nat.DT_F32}
 
 
@@ -162,18 +163,21 @@ def quant_attention(q, cache: QuantCache, *, valid_length=None, query_start=None
 
 def quant_gather_attention(q, cache: QuantCache, selected, selected_valid=None, *, scale=None, out=None,
                            out_dtype=torch.bfloat16, partitions=None):
-    """gather_attention over an 8-bit cache: q [B,G,h,1,128] over the listed positions selected [B,G,S] (any integer
-    type), read in place. Slots with selected_valid False, and positions outside [0, capacity), are skipped; a position
-    listed twice counts twice; a query with no row gets zeros."""
-    if selected.dim() != 3 or tuple(selected.shape[:2]) != (cache.batch, cache.groups) or selected.is_floating_point():
-        raise ValueError(f"selected must be an integer [B, G, S] tensor with B, G = {cache.batch}, {cache.groups}")
+    """gather_attention over an 8-bit cache: q [B,G,h,1,128] over the listed positions selected [B,G,S] (signed
+    integers or uint8), read in place. Slots with selected_valid False, and positions outside [0, capacity), are skipped;
+    a position listed twice counts twice; a query with no row gets zeros."""
+    if selected.dim() != 3 or tuple(selected.shape[:2]) != (cache.batch, cache.groups) \
+            or selected.dtype not in _POSITIONS:
+        raise ValueError(f"selected must be an integer [B, G, S] tensor with B, G = {cache.batch}, {cache.groups}, got "
+                         f"{selected.dtype} {tuple(selected.shape)}")
     if selected.device != cache.device:
         raise ValueError("selected must live on the cache's device")
-    if selected_valid is not None:
-        if selected_valid.shape != selected.shape:
-            raise ValueError("selected_valid must match selected")
-        selected = torch.where(selected_valid.bool(), selected, -1)
+    if selected_valid is not None and selected_valid.shape != selected.shape:
+        raise ValueError("selected_valid must match selected")
     if selected.dtype == torch.int64:   # a position past 32 bits is outside the cache, not another one
         selected = selected.clamp(-1, cache.capacity)
-    return hip_range.listed_attention(q, cache, selected.to(torch.int32).contiguous(), scale=scale, out=out,
-                                      out_dtype=out_dtype, partitions=partitions)
+    selected = selected.to(torch.int32)   # before the -1 of the slots to skip, which unsigned types do not hold
+    if selected_valid is not None:
+        selected = torch.where(selected_valid.bool(), selected, -1)
+    return hip_range.listed_attention(q, cache, selected.contiguous(), scale=scale, out=out, out_dtype=out_dtype,
+                                      partitions=partitions)

@@ -418,6 +418,89 @@ def test_masked_places_never_matter(gpu, kind, poison):
     restore()
 
 
+@pytest.mark.parametrize("dtype", [torch.int8, torch.uint8, torch.int16])
+def test_listed_rows_of_narrow_types(gpu, dtype):
+    """A skipped slot is no position in any type: 255 is what -1 would be in uint8."""
+    B, G, C, h, S = 1, 2, 300, 2, 40
+    cache, k, v = random_cache(gpu, 6, B, G, C, 32)
+    q = randn(18, B, G, h, 1, 128)
+    rows = torch.randint(0, 100, (B, G, S), generator=gen(S))
+    valid = torch.rand(rows.shape, generator=gen(2)) < 0.5
+    valid[0, 1] = False
+    masked = np.where(valid.numpy(), rows.numpy(), -1)
+    qf = f64(q)[:, :, :, 0]
+    got = quant_gather_attention(q.to(gpu), cache, rows.to(dtype).to(gpu), valid.to(gpu), out_dtype=torch.float32)
+    check(got, oq.listed_attention(qf, k, v, masked, SCALE)[:, :, :, None],
+          oq.listed_attention(qf, k, np.abs(v), masked, SCALE)[:, :, :, None], top_score(f64(q), k), chunk=False,
+          what=str(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bool, torch.float32, torch.complex64, torch.uint16, torch.uint32, torch.uint64])
+def test_listed_rows_of_other_types_are_refused(gpu, dtype):
+    cache, _, _ = random_cache(gpu, 6, 1, 2, 64, 32)
+    q = randn(18, 1, 2, 2, 1, 128).to(gpu)
+    with pytest.raises(ValueError, match="integer"):
+        quant_gather_attention(q, cache, torch.zeros(1, 2, 8, dtype=dtype, device=gpu))
+
+
+@pytest.mark.parametrize("kind", ["bf16", 16])
+@pytest.mark.parametrize("B,G,C,h,partitions", [(130, 1, 200, 1, None), (130, 1, 200, 1, 256), (65, 2, 90, 3, 2),
+                                                (5, 1, 3000, 2, 256)])
+def test_a_length_for_each_of_many_sequences(gpu, kind, B, G, C, h, partitions):
+    """More sequences than a wave has lanes, more partitions than tiles, empty sequences among them."""
+    call, k, v, _ = a_cache(gpu, kind, 12, B, G, C)
+    q = randn(19, B, G, h, 1, 128)
+    lengths = torch.randint(0, C + 1, (B,), generator=gen(B))
+    lengths[::9] = 0
+    lengths[1], lengths[-1] = C, 1
+    got = call(q.to(gpu), valid_length=lengths.to(torch.int32).to(gpu), window=None, sinks=0, out_dtype=torch.float32,
+               partitions=partitions)
+    S = top_score(f64(q), k)
+    for b in range(B):
+        if lengths[b] == 0:
+            assert not got[b].any()
+            continue
+        w, a = expect(q[b:b + 1], k[b:b + 1], v[b:b + 1], int(lengths[b]), int(lengths[b]) - 1, None, 0)
+        check(got[b:b + 1], w, a, S, chunk=False, what=f"b={b}")
+
+
+@pytest.mark.parametrize("B,G,C,h,partitions", [(4200, 1, 40, 1, 2), (40, 2, 600, 8, 16), (8, 4, 600, 8, 16)])
+def test_more_rows_than_the_shared_partials_hold(gpu, B, G, C, h, partitions):
+    """Past the counters, past the partials, and at the partials' last row; repeated, so the counters are zero again."""
+    call, k, v, _ = a_cache(gpu, 32, 13, B, G, C)
+    q = randn(20, B, G, h, 1, 128)
+    first = call(q.to(gpu), window=None, sinks=0, out_dtype=torch.float32, partitions=partitions)
+    w, a = expect(q, k, v, C, C - 1, None, 0)
+    check(first, w, a, top_score(f64(q), k), chunk=False, what="first")
+    for _ in range(3):
+        again = call(q.to(gpu), window=None, sinks=0, out_dtype=torch.float32, partitions=partitions)
+        assert torch.equal(first, again)
+
+
+@pytest.mark.parametrize("kind", ["bf16", 16, 64])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (200, 0), (65, 70)])
+@pytest.mark.parametrize("partitions", [1, 3])
+def test_chunk_with_values_that_are_not_numbers(gpu, kind, window, sinks, partitions):
+    """NaN rows of V inside the chunk and its history: the queries that see one get NaN, every other one its output."""
+    B, G, h, T, past = 1, 2, 2, 300, 700
+    C = past + T + 20
+    call, k, v, (_, vt) = a_cache(gpu, kind, 14, B, G, C)
+    q = randn(21, B, G, h, T, 128)
+    spoilt = [past + T - 2, past + T + 3] + ([] if window is None else [past + 3, sinks + 7])
+    for p in spoilt:
+        v[0, 1, p] = np.nan
+        if kind == "bf16":
+            vt[0, 1, p] = math.nan
+        else:
+            vt.view(torch.uint8)[0, 1, p] = 0x7f
+    L = past + T
+    got = call(q.to(gpu), valid_length=L, query_start=past, window=window, sinks=sinks, partitions=partitions)
+    w, _ = expect(q, k, v, L, past, window, sinks)
+    _, a = expect(q, k, np.nan_to_num(v), L, past, window, sinks)
+    assert np.isnan(w).any() and not np.isnan(w[0, 0]).any() and not np.isnan(w).all(axis=(2, 3, 4)).any()
+    check(got, w, a, top_score(f64(q), k), chunk=True, what=f"{kind} {window} {sinks}")
+
+
 @pytest.mark.parametrize("kind", ["bf16", 16])
 def test_large_scores_and_minus_infinity(gpu, kind):
     """Scores hundreds apart; a query whose every score is -inf gets zeros (bfloat16 cache)."""
