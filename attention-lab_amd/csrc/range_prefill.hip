@@ -58,8 +58,8 @@ __device__ __forceinline__ uint32_t bf16x2_finite(uint32_t w, uint32_t& flags) {
 
 // K and V blocks in LDS: 64 rows in 16-byte chunks, permuted within the row so that the reads meet no bank twice.
 // bf16, 16 chunks: K's chunk c of row j at slot c ^ (j & 15) (a read takes 16 rows, one chunk), V's at c ^ (4 (j & 3)) (a
-// transposing read takes 4 chunks of 4 consecutive rows). 8-bit, 8 chunks: both at c ^ (j / 2 % 8) (K: 16 rows, one
-// chunk; V: one chunk of 8 consecutive rows).
+// transposing read takes 4 chunks of 4 consecutive rows). 8-bit, 8 chunks: K's at c ^ (j / 2 % 8) (16 rows, one chunk),
+// V's at c ^ (2 (j / 2 % 4)) (half a wave takes two chunks of 8 consecutive rows).
 // Key 16 z + 8 g + 4 a + b of a 32-key tile is row 16 z + 8 a + 4 g + b of its product, so that a lane's weights are those
 // of eight consecutive keys, the ones whose V its operand holds.
 template <bool SPLIT, bool Q8>
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
     // buffer of those rows (rows past kend give zeros)
     constexpr int kSlots = kRow / 16, kPer = 64 / kSlots, kLoads = kKeys / kPer / 4;
     const int srow = lane / kSlots, slot = lane % kSlots;
-    const int kswz = Q8 ? 4 * (wave & 1) + (srow >> 1) : 4 * wave + srow, vswz = Q8 ? kswz : 4 * srow;
+    const int kswz = Q8 ? 4 * (wave & 1) + (srow >> 1) : 4 * wave + srow, vswz = Q8 ? 2 * (srow >> 1) : 4 * srow;
     const uint32_t koff = kRow * srow + 16 * (slot ^ kswz), voff = kRow * srow + 16 * (slot ^ vswz);
     const char* Kb = reinterpret_cast<const char*>(a.K) + (size_t)bg * a.C * kRow;
     const char* Vb = reinterpret_cast<const char*>(a.V) + (size_t)bg * a.C * kRow;
@@ -152,7 +152,7 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
     const int ve = Q8 ? (lane & 15) >> 1 : (lane & 15) >> 2;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
-        vof[dt] = Q8 ? kRow * (8 * g + ve) + 16 * ((2 * dt + ((lane >> 4) & 1)) ^ (4 * g + (ve >> 1))) + 8 * (lane & 1)
+        vof[dt] = Q8 ? kRow * (8 * g + ve) + 16 * ((2 * dt + ((lane >> 4) & 1)) ^ (2 * (ve >> 1))) + 8 * (lane & 1)
                      : kRow * (8 * g + ve) + 64 * (dt ^ ve) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
     auto pin = [&]() {
 #pragma unroll
@@ -218,11 +218,22 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
         for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[x][i] = 0.0f;
+        // K's reads stay kAhead steps ahead of their products (left to the compiler, one read: an 8K prompt 519 us, 511 so;
+        // the same for V, or V's ahead of the softmax, gave nothing more)
+        constexpr int kAhead = 3;
+        u32x4_t kw[kKof][2];
+        auto read_k = [&](int kk) __attribute__((always_inline)) {
 #pragma unroll
-        for (int kk = 0; kk < kKof; ++kk)
+            for (int x = 0; x < 2; ++x) kw[kk][x] = *reinterpret_cast<const u32x4_t*>(ks + 32 * kRow * x + kof[kk]);
+        };
+#pragma unroll
+        for (int kk = 0; kk < kAhead; ++kk) read_k(kk);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int kk = 0; kk < kKof; ++kk) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const u32x4_t w = *reinterpret_cast<const u32x4_t*>(ks + 32 * kRow * x + kof[kk]);
+                const u32x4_t w = kw[kk][x];
                 if constexpr (Q8) {
                     s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(w.x, w.y, ksc[x]), qb[2 * kk], s[x], 0, 0, 0);
                     s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(widen(w.z, w.w, ksc[x]), qb[2 * kk + 1], s[x], 0, 0, 0);
@@ -230,6 +241,11 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
                     s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, w), qb[kk], s[x], 0, 0, 0);
                 }
             }
+            if (kk + kAhead < kKof) {
+                read_k(kk + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
         // this lane's scores: row R, keys kb + 8 g + c, c = 32 x + 16 (i / 8) + i % 8. The bounds that a block needs are
         // applied apart, each a compare with a constant and a select
         const int at = kb + 8 * g;
