@@ -47,15 +47,17 @@ def decode_partitions(BG: int, count: int, ragged: bool = False) -> int:
 
 
 def chunk_splits(BG: int, h: int, T: int, keys: int) -> int:
-    """Workgroups that share a query tile's keys (`keys`: those the longest tile reads): one where the tiles give every CU
-    more than one, else as many as bring the grid to about two per CU, each at least 512 keys. MI355X, 8-bit: 1000 queries
-    (h=2) after 29011, 128 tiles, 583 us in one, 300 in two, 256 in four, 262 in eight; a 2K prompt (h=2), 256 tiles, 46
-    us in one, 41 in two; 1501 queries under a 2047 window (B=2, h=2), 384 tiles, 77 us in one, 79 in two."""
+    """Workgroups that share a query tile's keys (`keys`: those the longest tile reads). Two workgroups per CU where that
+    leaves each 1024 keys or more, else one per CU with at least 320: a share writes and reads back 67 KB of partials, and
+    a grid between one and two per CU takes as long as two. MI355X, 8-bit, us for splits of 1, 2, 4, 8: 1000 queries (h=2)
+    after 29011, 128 tiles, 549, 290, 250, 256; a 2K prompt (h=2), 256 tiles, 45, 40, 46; a 1K prompt (h=4), 256 tiles,
+    27, 33, 41; 200 queries (h=4) after 2500, 56 tiles, 55, 38, 30, 33; 300 (h=3) after 700, 64 tiles, 25, 22, 22, 28; 512
+    (h=4) after none, 128 tiles, 16, 22, 26; 1501 under a window of 2047, 384 tiles, 76, 78."""
     tiles = BG * -(-T // (CHUNK_ROWS // h))
-    if tiles > 256:
-        return 1
-    s = min(MAX_SPLITS, 512 // tiles, keys // 512)
-    return s if s >= 2 else 1
+    s = min(MAX_SPLITS, 512 // tiles)
+    if keys < 1024 * s:
+        s = min(MAX_SPLITS, 256 // tiles, keys // 320)
+    return max(s, 1)
 
 
 def check_window(window, sinks):
