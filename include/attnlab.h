@@ -365,7 +365,7 @@ int attnlab_quant_attend(const uint8_t* k_codes, const uint8_t* v_codes, const u
  * The chunk form of attnlab_range_decode, on the matrix cores: T queries at positions q_pos0 + t, query t reading
  * j <= q_pos0 + t, j < legal, and with window > 0: j > q_pos0 + t - window or j < sinks. q, out: [B, G, h, T, 128] bf16
  * contiguous, 1 <= h <= 16; the caches as there. What a masked position holds (NaN, infinity) does not reach an
- * output. splits (1..16): workgroups that share a query tile's key blocks; with more than one, part (16-byte aligned,
+ * output; a query that sees a value that is not finite gets outputs that are not (infinity may become NaN). splits (1..16): workgroups that share a query tile's key blocks; with more than one, part (16-byte aligned,
  * attnlab_range_prefill_part_bytes bytes) holds their partials and a second launch merges them.
  */
 int64_t attnlab_range_prefill_part_bytes(int B, int G, int h, int T, int splits);
