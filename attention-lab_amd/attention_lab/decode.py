@@ -314,6 +314,7 @@ def sparse_decode_step_quant(q_main, q_pre, cache, zT, wq_t_scaled, wk, fixed_ro
     C = cache.capacity
     if (B, G, d) != (cache.batch, cache.groups, hip_attend.HEAD_DIM):
         raise ValueError(f"q_main {tuple(q_main.shape)} does not match a cache of B, G = {cache.batch}, {cache.groups}")
+    hip_range.check_listed(q_main, B, G, cache.device, partitions)   # the read's refusals, before the table is written
     if zT.dim() != 4 or tuple(zT.shape[:2]) != (B, G) or zT.shape[3] != C:
         raise ValueError("zT must be a [B, G, r, C] tensor matching the cache")
     if q_pre.numel() != q_main.numel():

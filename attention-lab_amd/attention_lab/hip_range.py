@@ -87,6 +87,17 @@ def check_query(q, B: int, G: int, device):
     return h, shape[3]
 
 
+def check_listed(q, B: int, G: int, device, partitions) -> int:
+    """q and the split count of a row-list read -> h."""
+    h, T = check_query(q, B, G, device)
+    if T != 1:
+        raise ValueError("the row-list read takes one query position")
+    if h > MAX_H:
+        raise ValueError(f"the row-list read takes h <= {MAX_H} query heads per group, got {h}")
+    split_count(partitions, 1, MAX_P)
+    return h
+
+
 def check_lengths(lengths, B: int, device):
     """A device tensor of one valid length (or start) per sequence."""
     if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous() \
@@ -198,11 +209,7 @@ def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: 
 def listed_attention(q, cache, rows, *, scale, out, out_dtype, partitions):
     """The row-list read of quant_gather_attention: rows int32 [B,G,S] contiguous, checked cache."""
     B, G, C, device = cache.batch, cache.groups, cache.capacity, cache.device
-    h, T = check_query(q, B, G, device)
-    if T != 1:
-        raise ValueError("the row-list read takes one query position")
-    if h > MAX_H:
-        raise ValueError(f"the row-list read takes h <= {MAX_H} query heads per group, got {h}")
+    h = check_listed(q, B, G, device, partitions)
     S = int(rows.shape[2])
     if S < 1:
         raise ValueError("at least one row must be selected")

@@ -28,6 +28,7 @@ from . import hip_range
 from .hip_attend import HEAD_DIM
 
 BLOCKS = (16, 32, 64)
+SMALLEST = 127 - 110   # the scale byte of 2^-110
 _POSITIONS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
 _DTYPES = {torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16, torch.float32: nat.DT_F32}
 
@@ -58,14 +59,15 @@ class QuantCache:
 
     @classmethod
     def empty(cls, batch: int, groups: int, capacity: int, *, block: int = 64, device) -> "QuantCache":
-        """A cache with nothing written: codes hold whatever the memory held, which no read of written rows meets."""
+        """A cache with nothing written: codes hold whatever the memory held, which no read of written rows meets, and the
+        scales are the smallest, so that a first write inside a block takes the scale it needs."""
         if block not in BLOCKS:
             raise ValueError(f"block must be one of {BLOCKS}, got {block!r}")
         if min(int(batch), int(groups), int(capacity)) < 1:
             raise ValueError("batch, groups and capacity must be positive")
         shape = (int(batch), int(groups), int(capacity), HEAD_DIM)
         k, v = (torch.empty(shape, dtype=torch.float8_e4m3fn, device=device) for _ in "kv")
-        ke, ve = (torch.full((*shape[:2], -(-shape[2] // block)), 127, dtype=torch.uint8, device=device) for _ in "kv")
+        ke, ve = (torch.full((*shape[:2], -(-shape[2] // block)), SMALLEST, dtype=torch.uint8, device=device) for _ in "kv")
         return cls(k, v, ke, ve, block=block)
 
     def bytes(self) -> int:

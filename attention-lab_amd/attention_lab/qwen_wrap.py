@@ -40,7 +40,7 @@ from .decode import (gathered_decode_step_kernel, positions_from_flat, select_ro
 from .full import full_attention
 from .hip_range import check_window
 from .indexer import GroupedIndexer, project_keys
-from .quant import QuantCache, quant_attention, quant_gather_attention, quantize_append
+from .quant import BLOCKS, SMALLEST, QuantCache, quant_attention, quant_gather_attention, quantize_append
 from .selection import FIXED_PREFIX, FIXED_RECENT, fixed_budget, selection_layout
 from .sparse import row_offsets
 from .window import window_attention
@@ -108,6 +108,8 @@ class LabCache:
             raise ValueError("capacity and layers must be positive")
         if kv_format not in KV_FORMATS:
             raise ValueError(f"kv_format must be one of {KV_FORMATS}")
+        if kv_format == "e4m3" and kv_block not in BLOCKS:
+            raise ValueError(f"kv_block must be one of {BLOCKS}, got {kv_block!r}")
         self.kv_format, self.kv_block = kv_format, int(kv_block)
         self.layers, self.batch, self.groups = int(layers), int(batch), int(groups)
         self.capacity, self.head_dim = int(capacity), int(head_dim)
@@ -122,7 +124,7 @@ class LabCache:
         if kv_format == "e4m3":
             exp_shape = (*kv_shape[:3], -(-self.slots // self.kv_block))
             for name in ("k_exp", "v_exp"):
-                self._store[name] = torch.full(exp_shape, 127, device=self.device, dtype=torch.uint8)
+                self._store[name] = torch.full(exp_shape, SMALLEST, device=self.device, dtype=torch.uint8)
         if self.index_dim is not None:
             self._store["z"] = torch.empty(self.layers, self.batch, self.groups, self.index_dim, self.slots,
                                            device=self.device, dtype=self.index_dtype)

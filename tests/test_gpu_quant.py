@@ -168,6 +168,17 @@ def test_append_extreme_device_starts(gpu):
     assert (f64(dequantize_rows(cache, st, 1)[0]) == 0).all()
 
 
+def test_a_first_write_inside_a_block_takes_its_own_scale(gpu):
+    """A sequence that begins inside a block of an empty cache: small rows keep their precision."""
+    cache = QuantCache.empty(1, 1, 64, block=64, device=gpu)
+    x = randn(3, 1, 1, 20, 128) * 2.0 ** -12
+    quantize_append(cache, x.to(gpu), x.to(gpu), 7)
+    for t in dequantize_rows(cache, 7, 20, dtype=torch.float32):
+        top = float(x.abs().max())
+        err = (t.cpu().double() - x.double()).abs()
+        assert bool((err <= 2.0 ** -4 * x.double().abs() + 2.0 ** -17 * top).all())
+
+
 def test_append_takes_any_strides(gpu):
     B, G, T, block = 2, 4, 50, 16
     base = randn(3, B, T, G, 128)

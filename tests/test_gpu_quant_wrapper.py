@@ -93,6 +93,24 @@ def test_sparse_step_refusals(gpu):
             call()
 
 
+def test_a_refused_sparse_step_leaves_the_table(gpu):
+    """The read's own refusals come before the new key's column is written."""
+    G, d = 2, 128
+    cache = QuantCache.empty(1, G, 400, device=gpu)
+    req = prepare_request(1, G, 400, valid_length=300, query_position=299, rho=0.1, device=gpu)
+    lay = req.layout
+    args = (req.fixed_rows, req.off_lo, lay.candidate_lo, lay.candidate_hi, req.k, req.selected_count)
+    for h, dtype, kw, match in ((2, torch.float32, {}, "bfloat16"), (2, torch.bfloat16, dict(partitions=257), "partitions"),
+                                (9, torch.bfloat16, {}, "h <= 8")):
+        idx = GroupedIndexer(G, h, d, 32, device=gpu, dtype=torch.bfloat16, seed=3)
+        q = torch.ones(1, G, h, 1, d, dtype=torch.bfloat16, device=gpu)
+        z = torch.zeros(1, G, 32, 400, dtype=torch.bfloat16, device=gpu)
+        with pytest.raises(ValueError, match=match):
+            sparse_decode_step_quant(q.to(dtype), q, cache, z, idx.wq_t_scaled, idx.wk, *args, k_pre_new=q[:, :, :1, 0],
+                                     write_col=299, **kw)
+        assert not z.any()
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # the wrapper
 # ---------------------------------------------------------------------------------------------------------------------

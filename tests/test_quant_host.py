@@ -159,3 +159,12 @@ def test_argument_types_survive_the_binding():
     assert _native.SIGNATURES["attnlab_quant_attend"][1][7] is ctypes.c_int64
     assert [i for i, t in enumerate(_native.SIGNATURES["attnlab_quant_append"][1]) if t is ctypes.c_int64] == [1, 2, 3, 5,
                                                                                                                 6, 7]
+
+
+@pytest.mark.parametrize("block", [0, 8, 48, 128, -64])
+def test_wrapper_cache_refuses_other_blocks(block):
+    pytest.importorskip("transformers")
+    from attention_lab.qwen_wrap import LabCache
+    with pytest.raises(ValueError, match="kv_block must be one of"):
+        LabCache(layers=1, batch=1, groups=1, capacity=64, head_dim=128, device="cpu", dtype=torch.bfloat16,
+                 kv_format="e4m3", kv_block=block)
