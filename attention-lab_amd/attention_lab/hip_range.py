@@ -30,20 +30,21 @@ MERGE_SLOTS = 16    # partials the last workgroup to arrive merges itself; more 
 INT_MAX = 2 ** 31 - 1
 
 
-def decode_partitions(BG: int, count: int, ragged: bool = False) -> int:
+def decode_partitions(BG: int, count: int, ragged: bool = False, listed: bool = False) -> int:
     """Split-K count of the one-query kernels for BG (b, g) rows of `count` positions each: one workgroup per CU, or two
-    where that leaves each at least 48 tiles of 32 positions, and at least one tile for every one of its four waves.
-    Measured on MI355X (graph replay, 8-bit): one per CU against two, BG=8 at 8K 10.3 / 11.9 us, at 20K 14.0 / 15.8;
-    BG=32 at 4K 12.4 / 14.6; BG=64, 4K windows in bfloat16, 27.3 / 29.4; and the longer ones BG=24 at 20K 28.3 / 26.6,
-    BG=128 at 32K 162 / 158.
+    where that leaves each at least 48 tiles of 32 positions, and at least two tiles for every one of its four waves (one
+    of listed rows). Measured on MI355X (graph replay, 8-bit): one per CU against two, BG=8 at 8K 10.3 / 11.9 us, at 20K
+    14.0 / 15.8; BG=32 at 4K 12.4 / 14.6; BG=64, 4K windows in bfloat16, 27.3 / 29.4; and the longer ones BG=24 at 20K
+    28.3 / 26.6, BG=128 at 32K 162 / 158. Two tiles a wave against one: BG=8 at 2K 8.2 / 9.1, at 512 7.2 / 7.3; of 1092
+    listed rows, BG=16, 12.0 / 11.5.
     ragged (a length per sequence): the slots that the kernel deals out by the sequences' lengths, about two workgroups
     per CU with the half slot that every sequence's remainder takes (BG=40 to 20K: 31.9 us, 36.3 with half as many more;
     BG=128 to 8K: 41.6 against 45.2)."""
-    tiles = -(-count // TILE)
     BG = max(BG, 1)
     if ragged:
         return max(2, min(64, (512 + BG // 2) // BG))
-    return max(1, min(64, (512 if BG * tiles >= 256 * 48 else 256) // BG, count // (4 * TILE)))
+    tiles = -(-count // TILE)
+    return max(1, min(64, (512 if BG * tiles >= 256 * 48 else 256) // BG, count // ((4 if listed else 8) * TILE)))
 
 
 def chunk_splits(BG: int, h: int, T: int, keys: int) -> int:
@@ -215,7 +216,7 @@ def listed_attention(q, cache, rows, *, scale, out, out_dtype, partitions):
         raise ValueError("at least one row must be selected")
     q = q.contiguous()
     out = check_out(out, q, out_dtype)
-    P = split_count(partitions, decode_partitions(B * G, S), MAX_P)
+    P = split_count(partitions, decode_partitions(B * G, S, listed=True), MAX_P)
     stream = nat.stream_of(device)
     held, part, arrive = _split_k(P, B * G, h, device, stream, True)
     sc = float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)

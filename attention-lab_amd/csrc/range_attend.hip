@@ -21,8 +21,9 @@
 // What bounds it: the bytes of the rows. A CU streams about 26 GB/s whatever the number of its waves or loads in flight
 // (6.7 TB/s over 256), which 16 requests of 32K (8 groups, h=4) reach: 8-bit 158 us, 6.8 TB/s. Eight 128K caches with a
 // window of 4096 over bf16: 25.6 us, 5.2 TB/s; five of 5K to 20K (h=8): 29 us; 1092 listed rows of 16 requests: 15 us,
-// 2.4 TB/s of rows apart; one request of 2K: the launch. Three waves a SIMD with one tile each beat two with two, and four
-// waves a workgroup eight or sixteen.
+// 2.5 TB/s of rows apart; one request of 2K: 8 us, the latencies
+// of a launch (5.2 with one tile a wave and nothing to merge) and of the merge. Ranges take three waves a SIMD with one tile
+// each over two with two, and four waves a workgroup over eight or sixteen.
 //
 // Masked rows: their scores are replaced, and their V rows are zeros, so whatever they hold (NaN, infinity) leaves the
 // output alone. A query with no row to read, or whose scores are all -inf, gets zeros.
@@ -202,7 +203,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const uint8_t* base, ui
 }
 
 template <bool Q8, bool LIST>
-__global__ __launch_bounds__(64 * kWaves, 3) void range_attend(RangeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, LIST ? 2 : 3) void range_attend(RangeArgs a) {
     constexpr int kRow = Q8 ? kDim : 2 * kDim;          // bytes of a row
     constexpr int kLanes = kRow / 16;                   // lanes of a V row
     constexpr int kKLoads = Q8 ? 2 : 4, kVLoads = Q8 ? 4 : 8;
@@ -449,10 +450,24 @@ __global__ __launch_bounds__(64 * kWaves, 3) void range_attend(RangeArgs a) {
         asm volatile("" ::: "memory");
     };
     auto walk = [&](int ta, int tb) {   // tile t of [ta, tb) belongs to wave (t - ta) % kWaves
-        for (int t = ta + wave; t < tb; t += kWaves) {
-            Tile<Q8> f;
-            issue(t, f);
-            compute(t, f);
+        int t = ta + wave;
+        if constexpr (LIST) {
+            // a tile ahead, at two waves a SIMD: 1092 rows of 16 requests 14.9 us for 15.8 (ranges gain nothing by it)
+            Tile<Q8> f0, f1;
+            if (t < tb) issue(t, f0);
+            for (; t < tb; t += 2 * kWaves) {
+                if (t + kWaves < tb) issue(t + kWaves, f1);
+                compute(t, f0);
+                if (t + kWaves >= tb) break;
+                if (t + 2 * kWaves < tb) issue(t + 2 * kWaves, f0);
+                compute(t + kWaves, f1);
+            }
+        } else {
+            for (; t < tb; t += kWaves) {
+                Tile<Q8> f;
+                issue(t, f);
+                compute(t, f);
+            }
         }
     };
     if constexpr (LIST) {
