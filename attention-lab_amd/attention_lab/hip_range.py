@@ -28,6 +28,7 @@ MAX_SPLITS = 16
 MAX_P = 256
 MERGE_SLOTS = 16    # partials the last workgroup to arrive merges itself; more take a second launch
 INT_MAX = 2 ** 31 - 1
+DEFAULT_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 
 def decode_partitions(BG: int, count: int, ragged: bool = False, listed: bool = False) -> int:
@@ -108,11 +109,13 @@ def check_lengths(lengths, B: int, device):
 
 
 def check_out(out, q, dtype):
+    if out is None and dtype is torch.bfloat16:
+        # q is contiguous where it stands for the layout: empty_like is half the time of an empty with its arguments
+        return torch.empty_like(q)
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("out_dtype must be float32 or bfloat16")
     if out is None:
-        # q is contiguous where it stands for the layout: empty_like is half the time of an empty with its arguments
-        return torch.empty_like(q) if dtype == torch.bfloat16 else torch.empty_like(q, dtype=dtype)
+        return torch.empty_like(q, dtype=dtype)
     if tuple(out.shape) != tuple(q.shape) or out.dtype != dtype or not out.is_contiguous() or out.device != q.device:
         raise ValueError(f"out must be a contiguous {dtype} tensor shaped like q on its device")
     return out
@@ -157,17 +160,21 @@ def _capturing(device) -> bool:
         return torch._C._cuda_isCurrentStreamCapturing()
 
 
-def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: int, C: int, device, *, valid_length,
+# The host's part of a call is most of a small one's time, so the checks below look only at what the call gives.
+def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: int, C: int, device, valid_length,
                     query_start, window, sinks, scale, out, out_dtype, partitions):
     """The reads of window_attention and quant_attention over a checked cache [B,G,C,128] at k_ptr / v_ptr (exp_ptrs: the
     scale bytes of an 8-bit one, or (None, None))."""
-    if min(B, G, C) < 1:
+    if not (B and G and C):
         raise ValueError(f"the cache must hold at least one sequence, group and position, got {B}, {G}, {C}")
     h, T = check_query(q, B, G, device)
-    window, sinks = check_window(window, sinks)
+    if window is not None or sinks:
+        window, sinks = check_window(window, sinks)
+    else:
+        window = sinks = 0
     lengths = None
     if isinstance(valid_length, torch.Tensor):
-        lengths = check_lengths(valid_length, B, device)
+        lengths = check_lengths(valid_length, B, device).data_ptr()
         if T != 1 or query_start is not None:
             raise ValueError("a length per sequence goes with one query each, at its sequence's last position")
         if h > MAX_H:
@@ -180,30 +187,32 @@ def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: 
         p0 = legal - T if query_start is None else int(query_start)
         if not 0 <= p0 < INT_MAX - T:
             raise ValueError(f"query positions must be non-negative and below 2^31, got {p0}")
-        seen = min(legal, p0 + T)
+        seen = legal if query_start is None else min(legal, p0 + T)
     if window:   # what the query, or a chunk's workgroup, reads
         seen = min(seen, window + min(T, CHUNK_ROWS // h) - 1 + min(sinks, seen))
     q = q.contiguous()
-    sc = float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
+    sc = DEFAULT_SCALE if scale is None else float(scale)
     stream = nat.stream_of(device)
     if T == 1 and h <= MAX_H:
         out = check_out(out, q, out_dtype)
-        P = split_count(partitions, decode_partitions(B * G, seen, lengths is not None), MAX_P)
+        P = decode_partitions(B * G, seen, lengths is not None) if partitions is None else split_count(partitions, 1, MAX_P)
         held, part, arrive = _split_k(P, B * G, h, device, stream, lengths is None)
-        nat.call_on(device, "attnlab_range_decode", k_ptr, v_ptr, *exp_ptrs, block, q.data_ptr(), nat.ptr(lengths), legal,
-                    p0, window, sinks, B, G, h, C, P, sc, out.data_ptr(), int(out_dtype == torch.bfloat16),
-                    part, arrive, stream)
+        nat.call_on(device, "attnlab_range_decode", k_ptr, v_ptr, *exp_ptrs, block, q.data_ptr(), lengths, legal, p0, window,
+                    sinks, B, G, h, C, P, sc, out.data_ptr(), out_dtype == torch.bfloat16, part, arrive, stream)
         return out
     if out_dtype != torch.bfloat16:
         raise ValueError("a chunk's outputs are bfloat16")
     out = check_out(out, q, out_dtype)
     if T == 0:
         return out
-    splits = split_count(partitions, chunk_splits(B * G, h, T, seen), MAX_SPLITS)
-    nbytes = max(0, nat.lib().attnlab_range_prefill_part_bytes(B, G, h, T, splits))
-    part = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+    splits = chunk_splits(B * G, h, T, seen) if partitions is None else split_count(partitions, 1, MAX_SPLITS)
+    nbytes, part = 0, None
+    if splits > 1:
+        nbytes = nat.lib().attnlab_range_prefill_part_bytes(B, G, h, T, splits)
+        held = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+        part = held.data_ptr()
     nat.call_on(device, "attnlab_range_prefill", q.data_ptr(), k_ptr, v_ptr, *exp_ptrs, block, out.data_ptr(), B, G, h, T,
-                p0, legal, C, window, sinks, sc, splits, nat.ptr(part), nbytes, stream)
+                p0, legal, C, window, sinks, sc, splits, part, nbytes, stream)
     return out
 
 
@@ -219,7 +228,7 @@ def listed_attention(q, cache, rows, *, scale, out, out_dtype, partitions):
     P = split_count(partitions, decode_partitions(B * G, S, listed=True), MAX_P)
     stream = nat.stream_of(device)
     held, part, arrive = _split_k(P, B * G, h, device, stream, True)
-    sc = float(1.0 / math.sqrt(HEAD_DIM) if scale is None else scale)
+    sc = DEFAULT_SCALE if scale is None else float(scale)
     nat.call_on(device, "attnlab_quant_attend", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(),
                 cache.v_exp.data_ptr(), cache.block, q.data_ptr(), rows.data_ptr(), S, B, G, h, S, C, P, sc,
                 out.data_ptr(), int(out_dtype == torch.bfloat16), part, arrive, stream)

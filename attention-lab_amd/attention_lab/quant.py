@@ -42,18 +42,17 @@ class QuantCache:
     def __init__(self, k, v, k_exp, v_exp, *, block: int = 64):
         if block not in BLOCKS:
             raise ValueError(f"block must be one of {BLOCKS}, got {block!r}")
-        shape = k.shape
-        if len(shape) != 4 or shape[3] != HEAD_DIM or k.dtype != torch.float8_e4m3fn or not k.is_contiguous() \
-                or not k.is_cuda:
+        shape, device = k.shape, k.device
+        B, G, C, d = shape if len(shape) == 4 else (0, 0, 0, 0)
+        if d != HEAD_DIM or k.dtype != torch.float8_e4m3fn or not k.is_contiguous() or not k.is_cuda:
             raise ValueError(f"k must be a contiguous float8_e4m3fn [B, G, C, {HEAD_DIM}] tensor on a HIP device")
-        device = k.device
         if v.shape != shape or v.dtype != torch.float8_e4m3fn or not v.is_contiguous() or v.device != device:
             raise ValueError("v must match k")
-        B, G, C, _ = shape
-        want = (B, G, -(-C // block))
-        for t, name in ((k_exp, "k_exp"), (v_exp, "v_exp")):
+        want = torch.Size((B, G, -(-C // block)))
+        for t in (k_exp, v_exp):
             if t.shape != want or t.dtype != torch.uint8 or not t.is_contiguous() or t.device != device:
-                raise ValueError(f"{name} must be a contiguous uint8 {list(want)} tensor on the cache's device")
+                raise ValueError(f"{'k_exp' if t is k_exp else 'v_exp'} must be a contiguous uint8 {list(want)} tensor on "
+                                 f"the cache's device")
         self.k, self.v, self.k_exp, self.v_exp, self.block = k, v, k_exp, v_exp, int(block)
         self.batch, self.groups, self.capacity, self.device = B, G, C, device
 
@@ -75,9 +74,9 @@ class QuantCache:
 
 
 def _start(cache: QuantCache, start, length: int):
-    """(device tensor or None, int) of a start that is an int, checked here, or an int32 [B] device tensor."""
+    """(address or None, int) of a start that is an int32 [B] device tensor, or an int, checked here."""
     if isinstance(start, torch.Tensor):
-        return hip_range.check_lengths(start, cache.batch, cache.device), 0
+        return hip_range.check_lengths(start, cache.batch, cache.device).data_ptr(), 0
     start = int(start)
     if start < 0 or start + length > cache.capacity:
         raise ValueError(f"rows [{start}, {start + length}) outside the cache's capacity {cache.capacity}")
@@ -85,13 +84,15 @@ def _start(cache: QuantCache, start, length: int):
 
 
 def _rows(x, step: int):
-    """(x as the kernel takes it, its three outer strides): unit stride along a row and 16-byte aligned rows of `step`
-    elements to 16 bytes (a copy where it has neither)."""
+    """(x as the kernel takes it, its address and three outer strides): unit stride along a row and 16-byte aligned rows of
+    `step` elements to 16 bytes (a copy where it has neither)."""
     sb, sg, st, sd = x.stride()
-    if sd != 1 or (sb | sg | st) % step or x.data_ptr() % 16:
+    at = x.data_ptr()
+    if sd != 1 or (sb | sg | st) % step or at % 16:
         x = x.contiguous()
         sb, sg, st, _ = x.stride()
-    return x, sb, sg, st
+        at = x.data_ptr()
+    return x, at, sb, sg, st
 
 
 def quantize_append(cache: QuantCache, k, v, start=0) -> None:
@@ -105,7 +106,8 @@ def quantize_append(cache: QuantCache, k, v, start=0) -> None:
     NaN and infinity become NaN; finite values past 1.875 * 2^127 saturate.
     """
     shape = k.shape
-    if len(shape) != 4 or shape[0] != cache.batch or shape[1] != cache.groups or shape[3] != HEAD_DIM or v.shape != shape:
+    B, G, T, d = shape if len(shape) == 4 else (0, 0, 0, 0)
+    if B != cache.batch or G != cache.groups or d != HEAD_DIM or v.shape != shape:
         raise ValueError(f"k and v must be [B, G, T, {HEAD_DIM}] with B, G = {cache.batch}, {cache.groups}, got "
                          f"{tuple(shape)} and {tuple(v.shape)}")
     dtype = _DTYPES.get(k.dtype)
@@ -114,21 +116,21 @@ def quantize_append(cache: QuantCache, k, v, start=0) -> None:
     device = cache.device
     if k.device != device or v.device != device:
         raise ValueError("k and v must live on the cache's device")
-    T = shape[2]
     starts, at = _start(cache, start, T)
     step = 4 if dtype == nat.DT_F32 else 8
-    k, *k_strides = _rows(k, step)
-    v, *v_strides = _rows(v, step)
-    nat.call_on(device, "attnlab_quant_append", k.data_ptr(), *k_strides, v.data_ptr(), *v_strides, dtype,
-                cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), nat.ptr(starts), at,
-                cache.batch, cache.groups, T, cache.capacity, cache.block, nat.stream_of(device))
+    k, k_at, kb, kg, kt = _rows(k, step)
+    v, v_at, vb, vg, vt = _rows(v, step)
+    nat.call_on(device, "attnlab_quant_append", k_at, kb, kg, kt, v_at, vb, vg, vt, dtype, cache.k.data_ptr(),
+                cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), starts, at, B, G, T, cache.capacity,
+                cache.block, nat.stream_of(device))
 
 
 def dequantize_rows(cache: QuantCache, start=0, length=None, *, dtype=torch.bfloat16):
     """The values of positions [start, start + length) -> (k, v), each [B,G,length,128] in `dtype` (bfloat16 and float32
     exact, float16 rounded). start: an int, or an int32 [B] device tensor (positions outside the cache then give zeros;
     length is required). length None: to the capacity."""
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise ValueError(f"dtype must be bfloat16, float16 or float32, got {dtype}")
     if length is None:
         if isinstance(start, torch.Tensor):
@@ -138,10 +140,12 @@ def dequantize_rows(cache: QuantCache, start=0, length=None, *, dtype=torch.bflo
     if T < 0:
         raise ValueError(f"length={T} must not be negative")
     starts, at = _start(cache, start, T)
-    k, v = (torch.empty(cache.batch, cache.groups, T, HEAD_DIM, dtype=dtype, device=cache.device) for _ in "kv")
-    nat.call_on(cache.device, "attnlab_quant_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(),
-                cache.v_exp.data_ptr(), k.data_ptr(), v.data_ptr(), _DTYPES[dtype], nat.ptr(starts), at, cache.batch,
-                cache.groups, T, cache.capacity, cache.block, nat.stream_of(cache.device))
+    B, G, device = cache.batch, cache.groups, cache.device
+    k = torch.empty((B, G, T, HEAD_DIM), dtype=dtype, device=device)
+    v = torch.empty_like(k)
+    nat.call_on(device, "attnlab_quant_read", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(),
+                cache.v_exp.data_ptr(), k.data_ptr(), v.data_ptr(), code, starts, at, B, G, T, cache.capacity, cache.block,
+                nat.stream_of(device))
     return k, v
 
 
@@ -158,9 +162,8 @@ def quant_attention(q, cache: QuantCache, *, valid_length=None, query_start=None
     """
     return hip_range.range_attention(q, cache.k.data_ptr(), cache.v.data_ptr(),
                                      (cache.k_exp.data_ptr(), cache.v_exp.data_ptr()), cache.block, cache.batch,
-                                     cache.groups, cache.capacity, cache.device, valid_length=valid_length,
-                                     query_start=query_start, window=window, sinks=sinks, scale=scale, out=out,
-                                     out_dtype=out_dtype, partitions=partitions)
+                                     cache.groups, cache.capacity, cache.device, valid_length, query_start, window, sinks,
+                                     scale, out, out_dtype, partitions)
 
 
 def quant_gather_attention(q, cache: QuantCache, selected, selected_valid=None, *, scale=None, out=None,

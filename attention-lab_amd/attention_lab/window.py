@@ -28,6 +28,5 @@ def window_attention(q, k, v, *, window, sinks: int = FIXED_PREFIX, valid_length
     if v.shape != k.shape or v.dtype != k.dtype or not v.is_contiguous() or v.device != k.device:
         raise ValueError("v must match k")
     B, G, C, _ = k.shape
-    return hip_range.range_attention(q, k.data_ptr(), v.data_ptr(), (None, None), 0, B, G, C, k.device,
-                                     valid_length=valid_length, query_start=query_start, window=window, sinks=sinks,
-                                     scale=scale, out=out, out_dtype=out_dtype, partitions=partitions)
+    return hip_range.range_attention(q, k.data_ptr(), v.data_ptr(), (None, None), 0, B, G, C, k.device, valid_length,
+                                     query_start, window, sinks, scale, out, out_dtype, partitions)
