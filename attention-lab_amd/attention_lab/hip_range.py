@@ -5,10 +5,10 @@ The kernels behind `window_attention` (window.py) and `quant_attention` / `quant
 check their caches; this module checks what the reads share, chooses the split counts and launches, on the tensors' own
 device and torch's current stream of it.
 
-The last workgroup of a (b, g) to arrive merges its split-K partials where a counter tells it that it is: the counters and
-partials of such single launches belong to a stream, whose launches follow one another and leave the counters zero. Other
-calls, a captured one among them, allocate partials of their own and take a second launch for the merge (the same sums),
-so a graph shares nothing with other graphs or calls.
+The last workgroup of a (b, g) to arrive merges its split-K partials where a counter tells it that it is: the counters
+and partials of such single launches belong to a stream, whose launches follow one another and leave the counters zero.
+Other calls, a captured one among them, allocate partials of their own and take a second launch for the merge (the same
+sums), so a graph shares nothing with other graphs or calls.
 """
 from __future__ import annotations
 
@@ -33,28 +33,32 @@ DEFAULT_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 def decode_partitions(BG: int, count: int, ragged: bool = False, listed: bool = False) -> int:
     """Split-K count of the one-query kernels for BG (b, g) rows of `count` positions each: one workgroup per CU, or two
-    where that leaves each at least 48 tiles of 32 positions, and at least two tiles for every one of its four waves (one
-    of listed rows). Measured on MI355X (graph replay, 8-bit): one per CU against two, BG=8 at 8K 10.3 / 11.9 us, at 20K
-    14.0 / 15.8; BG=32 at 4K 12.4 / 14.6; BG=64, 4K windows in bfloat16, 27.3 / 29.4; and the longer ones BG=24 at 20K
-    28.3 / 26.6, BG=128 at 32K 162 / 158. Two tiles a wave against one: BG=8 at 2K 8.2 / 9.1, at 512 7.2 / 7.3; of 1092
-    listed rows, BG=16, 12.0 / 11.5.
-    ragged (a length per sequence): the slots that the kernel deals out by the sequences' lengths, about two workgroups
-    per CU with the half slot that every sequence's remainder takes (BG=40 to 20K: 31.9 us, 36.3 with half as many more;
-    BG=128 to 8K: 41.6 against 45.2)."""
+    where that leaves each at least 48 tiles of 32 positions, and at least two tiles for every one of its four waves
+    (one of listed rows). Measured on MI355X (graph replay, 8-bit): one per CU against two, BG=8 at 8K 10.3 / 11.9 us, at
+    20K 14.0 / 15.8; BG=32 at 4K 12.4 / 14.6; BG=64, 4K windows in bfloat16, 27.3 / 29.4; and the longer ones BG=24 at
+    20K 28.3 / 26.6, BG=128 at 32K 162 / 158. Two tiles a wave against one: BG=8 at 2K 8.2 / 9.1, at 512 7.2 / 7.3; of
+    1092 listed rows, BG=16, 12.0 / 11.5.
+    ragged (a length per sequence, `count` by the capacity): the slots that the kernel deals out by the sequences'
+    lengths, with the half slot that every sequence's remainder takes: two workgroups per CU, or four where two leave a
+    tenth of the chip idle; at most one to 128 positions. BG=40 to 20K: 13 slots 30.5 us, 16 35.9; BG=128 to 32K: 4 (448
+    of 512 places) 129, 8 (960 of 1024) 122; BG=256 to 2K: 2 31.0, 4 27.2; BG=8 of 2K: 16 9.7, 64 9.9."""
     BG = max(BG, 1)
     if ragged:
-        return max(2, min(64, (512 + BG // 2) // BG))
+        P = (512 + BG // 2) // BG
+        if P * BG - BG // 2 < 460:
+            P = (1024 + BG // 2) // BG
+        return max(2, min(64, P, count // (4 * TILE)))
     tiles = -(-count // TILE)
     return max(1, min(64, (512 if BG * tiles >= 256 * 48 else 256) // BG, count // ((4 if listed else 8) * TILE)))
 
 
 def chunk_splits(BG: int, h: int, T: int, keys: int) -> int:
     """Workgroups that share a query tile's keys (`keys`: those the longest tile reads). Two workgroups per CU where that
-    leaves each 1024 keys or more, else one per CU with at least 320: a share writes and reads back 67 KB of partials, and
-    a grid between one and two per CU takes as long as two. MI355X, 8-bit, us for splits of 1, 2, 4, 8: 1000 queries (h=2)
-    after 29011, 128 tiles, 549, 290, 250, 256; a 2K prompt (h=2), 256 tiles, 45, 40, 46; a 1K prompt (h=4), 256 tiles,
-    27, 33, 41; 200 queries (h=4) after 2500, 56 tiles, 55, 38, 30, 33; 300 (h=3) after 700, 64 tiles, 25, 22, 22, 28; 512
-    (h=4) after none, 128 tiles, 16, 22, 26; 1501 under a window of 2047, 384 tiles, 76, 78."""
+    leaves each 1024 keys or more, else one per CU with at least 320: a share writes and reads back 67 KB of partials,
+    and a grid between one and two per CU takes as long as two. MI355X, 8-bit, us for splits of 1, 2, 4, 8: 1000 queries
+    (h=2) after 29011, 128 tiles, 549, 290, 250, 256; a 2K prompt (h=2), 256 tiles, 45, 40, 46; a 1K prompt (h=4), 256
+    tiles, 27, 33, 41; 200 queries (h=4) after 2500, 56 tiles, 55, 38, 30, 33; 300 (h=3) after 700, 64 tiles, 25, 22, 22,
+    28; 512 (h=4) after none, 128 tiles, 16, 22, 26; 1501 under a window of 2047, 384 tiles, 76, 78."""
     tiles = BG * -(-T // (CHUNK_ROWS // h))
     s = min(MAX_SPLITS, 512 // tiles)
     if keys < 1024 * s:
@@ -132,8 +136,11 @@ def split_count(partitions, chosen: int, most: int) -> int:
 
 _MERGES: dict = {}      # (device index, stream) -> its counters, zeroed once and left zero by every call, and partials
 COUNTERS = 4096         # (b, g) rows that they serve
-PARTIALS = 8 * 512      # (slot, head) partials: one or two workgroups per CU of eight heads, 2.1 MB
+PARTIALS = 8 * 1024     # (slot, head) partials: up to four workgroups per CU of eight heads, 4.3 MB
 PART_WORDS = HEAD_DIM + 2
+# Positions to read, by the capacity, up to which a ragged call merges in its one launch: 32 x 2K takes 1 us less on the GPU
+# and a launch less on the host, five of 20K 2 us more (a sequence of many slots is merged by one workgroup).
+RAGGED_MERGE = 1 << 19
 
 
 def _split_k(P: int, BG: int, h: int, device, stream: int, counted: bool):
@@ -196,7 +203,7 @@ def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: 
     if T == 1 and h <= MAX_H:
         out = check_out(out, q, out_dtype)
         P = decode_partitions(B * G, seen, lengths is not None) if partitions is None else split_count(partitions, 1, MAX_P)
-        held, part, arrive = _split_k(P, B * G, h, device, stream, lengths is None)
+        held, part, arrive = _split_k(P, B * G, h, device, stream, lengths is None or B * G * seen <= RAGGED_MERGE)
         nat.call_on(device, "attnlab_range_decode", k_ptr, v_ptr, *exp_ptrs, block, q.data_ptr(), lengths, legal, p0, window,
                     sinks, B, G, h, C, P, sc, out.data_ptr(), out_dtype == torch.bfloat16, part, arrive, stream)
         return out

@@ -63,7 +63,7 @@ struct RangeArgs {
     void* out;
     int out_bf16;
     uint32_t* arrive;         // [B * G] arrival counters, zero on entry and left zero: the last workgroup of a (b, g) merges
-                              // its partials (P <= kMergeSlots, no lengths); null: a second launch does
+                              // its partials (P <= kMergeSlots); null: a second launch does
     float* part;              // [slot, h, 130]: m, l, the unnormalised outputs (P > 1; B * G * P slots)
 };
 
@@ -91,8 +91,8 @@ __device__ __forceinline__ Span span_of_sequence(const RangeArgs& a, int b) {
 }
 
 // With a length per sequence and P > 1 the B P slots of a group go to the sequences by their tiles: sequence b takes
-// ceil(tiles_b / share), the share being the least (of 4 tiles or more) with which B (P - 1) slots would hold them all
-// evenly, so B more hold every remainder. Each workgroup works this out for itself, 64 sequences at a time.
+// ceil(tiles_b / share), one at least, the share being the least (of 4 tiles or more) with which B (P - 1) slots would hold
+// them all evenly, so B more hold every remainder. Each workgroup works this out for itself, 64 sequences at a time.
 __device__ __forceinline__ int share_of(const RangeArgs& a) {
     const int lane = threadIdx.x & 63;
     uint32_t total = 0;
@@ -109,7 +109,8 @@ __device__ __forceinline__ void slots_of(const RangeArgs& a, int share, int by_s
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int b0 = 0; b0 < a.B; b0 += 64) {
-        const uint32_t x = b0 + lane < a.B ? (uint32_t)((span_of_sequence(a, b0 + lane).tiles() + share - 1) / share) : 0u;
+        const uint32_t x =
+            b0 + lane < a.B ? (uint32_t)max((span_of_sequence(a, b0 + lane).tiles() + share - 1) / share, 1) : 0u;
         const uint32_t to = wave_incl_scan(x) + (uint32_t)base;   // the slots of this lane's sequence end here
         const uint64_t hit = by_slot < 0 ? (b >= b0 && b < b0 + 64 ? 1ull << (b - b0) : 0ull)
                                          : __ballot((int)to > by_slot);
@@ -218,13 +219,13 @@ __global__ __launch_bounds__(64 * kWaves, LIST ? 2 : 3) void range_attend(RangeA
     const int n16 = lane & 15, g4 = lane >> 4;
 
     // this workgroup's (b, g), its rows, and its tiles [t0, t1) of them
-    int bg, p, share;
+    int bg, p, share, slots = a.P;
     Span rows{0, 0, a.n};   // the list's entries, or a range
     if (!LIST && a.lengths && a.P > 1) {
         const int g = lin / (a.B * a.P);
-        int b, first, count;
+        int b, first;
         share = share_of(a);
-        slots_of(a, share, lin - g * a.B * a.P, b, first, count);
+        slots_of(a, share, lin - g * a.B * a.P, b, first, slots);
         if (b >= a.B) return;
         p = lin - g * a.B * a.P - first;
         bg = b * a.G + g;
@@ -501,7 +502,7 @@ __global__ __launch_bounds__(64 * kWaves, LIST ? 2 : 3) void range_attend(RangeA
     for (int dt = 0; dt < 8; ++dt)
         *reinterpret_cast<f32x4_t*>(red + (wave * 16 + n16) * kDim + 16 * dt + 4 * g4) = o[dt];
     __syncthreads();
-    const bool merge_here = a.P > 1 && a.arrive != nullptr;
+    const bool alone = a.P == 1 || (a.arrive != nullptr && slots == 1), merge_here = a.arrive != nullptr && slots > 1;
     for (int i = wave; i < a.h; i += kWaves) {   // wave -> head, lane l -> dims 2 l, 2 l + 1
         float ms = -INFINITY;
 #pragma unroll
@@ -517,7 +518,7 @@ __global__ __launch_bounds__(64 * kWaves, LIST ? 2 : 3) void range_attend(RangeA
             os.x += x * (hi.x + rest.x);
             os.y += x * (hi.y + rest.y);
         }
-        if (a.P == 1) {
+        if (alone) {
             store_row(a, (size_t)bg * a.h + i, ls, os);
             continue;
         }
@@ -536,17 +537,17 @@ __global__ __launch_bounds__(64 * kWaves, LIST ? 2 : 3) void range_attend(RangeA
     }
     if (!merge_here) return;
     // Arrival: every partial store of this workgroup has completed before its count (the wait and the barrier), so the
-    // workgroup that counts P - 1 before itself finds every partial in memory. It leaves the counter zero.
+    // workgroup that counts all others before itself finds every partial in memory. It leaves the counter zero.
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (tid == 0)
-        last_sh = __hip_atomic_fetch_add(a.arrive + bg, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(a.P - 1);
+        last_sh = __hip_atomic_fetch_add(a.arrive + bg, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(slots - 1);
     __syncthreads();
     if (!last_sh) return;
     for (int i = wave; i < a.h; i += kWaves) {
         float m2, l2;
         float2 o2;
-        merge_slots<true>(a.part + ((size_t)bg * a.P * a.h + i) * kPartWords, (size_t)a.h * kPartWords, a.P, m2, l2, o2);
+        merge_slots<true>(a.part + ((size_t)(lin - p) * a.h + i) * kPartWords, (size_t)a.h * kPartWords, slots, m2, l2, o2);
         store_row(a, (size_t)bg * a.h + i, l2, o2);
     }
     if (tid == 0) __hip_atomic_store(a.arrive + bg, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -666,7 +667,6 @@ extern "C" int attnlab_range_decode(const void* K, const void* V, const uint8_t*
     ATTNLAB_REQUIRE(window >= 0 && sinks >= 0, "window=%d and sinks=%d must not be negative", window, sinks);
     RangeArgs a = range_args(K, V, k_exp, v_exp, block, q, B, G, h, C, P, scale, out, out_bf16, part, arrive);
     a.lengths = lengths;
-    if (lengths) a.arrive = nullptr;   // the sequences' slots are counted on the device
     a.n = lengths ? 0 : (int)(q_pos + 1 < length ? q_pos + 1 : length);   // causal: no key past the query
     a.qend = q_pos + 1;
     a.window = window;

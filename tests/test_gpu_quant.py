@@ -475,6 +475,36 @@ def test_a_length_for_each_of_many_sequences(gpu, kind, B, G, C, h, partitions):
         check(got[b:b + 1], w, a, S, chunk=False, what=f"b={b}")
 
 
+@pytest.mark.parametrize("kind", ["bf16", 64])
+@pytest.mark.parametrize("B,C,h,partitions", [(1, 2112, 2, None), (4, 2112, 8, 16), (32, 700, 3, 4), (2, 9000, 1, 8)])
+def test_a_length_each_in_one_launch_and_in_two(gpu, kind, B, C, h, partitions):
+    """Small ragged calls merge in their launch and captured ones in a second: the same bits, whatever the lengths, call
+    after call (the counters return to zero)."""
+    G = 2
+    call, k, v, _ = a_cache(gpu, kind, 22, B, G, C)
+    q = randn(23, B, G, h, 1, 128).to(gpu)
+    lengths = torch.zeros(B, dtype=torch.int32, device=gpu)
+    read = lambda: call(q, valid_length=lengths, window=None, sinks=0, out_dtype=torch.float32,  # noqa: E731
+                        partitions=partitions)
+    read()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = read()
+    S = top_score(f64(q), k)
+    for fill in ([C] * B, [0] * B, [1] * B, [C if b == B // 2 else 40 for b in range(B)],
+                 torch.randint(0, C + 1, (B,), generator=gen(B)).tolist()):
+        lengths.copy_(torch.tensor(fill, dtype=torch.int32))
+        eager = read()
+        graph.replay()
+        assert torch.equal(eager, out)
+        b = B // 2
+        if fill[b] == 0:
+            assert not eager.any()
+        else:
+            w, a = expect(q[b:b + 1], k[b:b + 1], v[b:b + 1], fill[b], fill[b] - 1, None, 0)
+            check(eager[b:b + 1], w, a, S, chunk=False, what=str(fill[b]))
+
+
 @pytest.mark.parametrize("B,G,C,h,partitions", [(4200, 1, 40, 1, 2), (40, 2, 600, 8, 16), (8, 4, 600, 8, 16)])
 def test_more_rows_than_the_shared_partials_hold(gpu, B, G, C, h, partitions):
     """Past the counters, past the partials, and at the partials' last row; repeated, so the counters are zero again."""

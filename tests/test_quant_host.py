@@ -148,6 +148,8 @@ def test_python_refusals_without_a_device():
 @pytest.mark.parametrize("n", [0, 1, 127, 128, 4100, 131072])
 def test_split_rules_stay_in_range(BG, n):
     assert 1 <= hip_range.decode_partitions(BG, n) <= 256
+    assert 1 <= hip_range.decode_partitions(BG, n, listed=True) <= 256
+    assert 2 <= hip_range.decode_partitions(BG, n, ragged=True) <= 256
     for h in (1, 3, 16):
         for T in (1, 33, 8192):
             assert 1 <= hip_range.chunk_splits(BG, h, T, n) <= hip_range.MAX_SPLITS
