@@ -33,11 +33,12 @@ DEFAULT_SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 def decode_partitions(BG: int, count: int, ragged: bool = False, listed: bool = False) -> int:
     """Split-K count of the one-query kernels for BG (b, g) rows of `count` positions each: one workgroup per CU, or two
-    where that leaves each at least 48 tiles of 32 positions, and at least two tiles for every one of its four waves
-    (one of listed rows). Measured on MI355X (graph replay, 8-bit): one per CU against two, BG=8 at 8K 10.3 / 11.9 us, at
-    20K 14.0 / 15.8; BG=32 at 4K 12.4 / 14.6; BG=64, 4K windows in bfloat16, 27.3 / 29.4; and the longer ones BG=24 at
-    20K 28.3 / 26.6, BG=128 at 32K 162 / 158. Two tiles a wave against one: BG=8 at 2K 8.2 / 9.1, at 512 7.2 / 7.3; of
-    1092 listed rows, BG=16, 12.0 / 11.5.
+    where that leaves one more than a seventh of the CUs idle or each of two 48 tiles of 32 positions; and at least two
+    tiles for every one of a workgroup's four waves (one of listed rows). Measured on MI355X (graph replay, 8-bit), one
+    per CU against two: BG=8 at 8K 10.3 / 11.9 us, at 64K 27.6 / 31.9; BG=32 at 16K 27.8 / 31.0; BG=64 at 8K 27.5 /
+    30.0, at 12K 38.8 / 38.2, at 20K 55.6 / 54.6; BG=128 at 32K 162 / 158; BG=56 (224 workgroups of one) at 4K 17.3 /
+    18.3; BG=96 (192) at 4K 25.9 / 23.0; BG=160 (160) at 2K 25.8 / 21.4. Two tiles a wave against one: BG=8 at 2K 8.2 /
+    9.1, at 512 7.2 / 7.3; of 1092 listed rows, BG=16, 12.0 / 11.5.
     ragged (a length per sequence, `count` by the capacity): the slots that the kernel deals out by the sequences'
     lengths, with the half slot that every sequence's remainder takes: two workgroups per CU, or four where two leave a
     tenth of the chip idle; at most one to 128 positions. BG=40 to 20K: 13 slots 30.5 us, 16 35.9; BG=128 to 32K: 4 (448
@@ -48,8 +49,10 @@ def decode_partitions(BG: int, count: int, ragged: bool = False, listed: bool = 
         if P * BG - BG // 2 < 460:
             P = (1024 + BG // 2) // BG
         return max(2, min(64, P, count // (4 * TILE)))
-    tiles = -(-count // TILE)
-    return max(1, min(64, (512 if BG * tiles >= 256 * 48 else 256) // BG, count // ((4 if listed else 8) * TILE)))
+    P = 256 // BG
+    if BG * count >= 512 * 48 * TILE or P * BG < 220:
+        P = 512 // BG
+    return max(1, min(64, P, count // ((4 if listed else 8) * TILE)))
 
 
 def chunk_splits(BG: int, h: int, T: int, keys: int) -> int:
