@@ -20,10 +20,10 @@
 //
 // What bounds it: the bytes of the rows. A CU streams about 26 GB/s whatever the number of its waves or loads in flight
 // (6.7 TB/s over 256), which 16 requests of 32K (8 groups, h=4) reach: 8-bit 158 us, 6.8 TB/s. Eight 128K caches with a
-// window of 4096 over bf16: 25.6 us, 5.2 TB/s; five of 5K to 20K (h=8): 29 us; 1092 listed rows of 16 requests: 15 us,
-// 2.5 TB/s of rows apart; one request of 2K: 8 us, the latencies
-// of a launch (5.2 with one tile a wave and nothing to merge) and of the merge. Ranges take three waves a SIMD with one tile
-// each over two with two, and four waves a workgroup over eight or sixteen.
+// window of 4096 over bf16: 25.6 us, 5.2 TB/s; five of 5K to 20K (h=8): 29.5 us; 1092 listed rows of 16 requests: 14.1 us,
+// 2.6 TB/s of rows apart; one request of 2K: 8 us, the latencies of a launch (5.2 with one tile a wave and nothing to merge)
+// and of the merge. Ranges take three waves a SIMD with one tile each over two with two, and four waves a workgroup over
+// eight or sixteen.
 //
 // Masked rows: their scores are replaced, and their V rows are zeros, so whatever they hold (NaN, infinity) leaves the
 // output alone. A query with no row to read, or whose scores are all -inf, gets zeros.
