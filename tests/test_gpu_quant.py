@@ -12,6 +12,7 @@ oracle (what a relative error of every weight and of their sum moves an output b
 from __future__ import annotations
 
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -688,6 +689,35 @@ def test_two_graphs_and_two_streams(gpu):
         torch.cuda.synchronize()
         for o, e, w in zip(outs, eager, want):
             assert torch.equal(o, w) and all(torch.equal(x, w) for x in e)
+
+
+@pytest.mark.parametrize("own_streams", [False, True])
+def test_calls_from_two_threads(gpu, own_streams):
+    """Two host threads that read at once, each on its own stream or both on one: the results of one after the other."""
+    B, G, C, h = 2, 4, 3000, 4
+    call, _, _, _ = a_cache(gpu, 32, 24, B, G, C)
+    qs = [randn(60 + i, B, G, h, 1, 128).to(gpu) for i in range(8)]
+    want = [call(q, window=None, sinks=0, partitions=8) for q in qs]
+    torch.cuda.synchronize()
+    shared, failed = torch.cuda.Stream(), []
+
+    def reads():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream() if own_streams else shared):
+                for _ in range(25):
+                    got = [call(q, window=None, sinks=0, partitions=8) for q in qs]
+                torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(g, w) for g, w in zip(got, want)):
+                failed.append("another result")
+        except Exception as e:  # noqa: BLE001 - a thread's exception would be lost
+            failed.append(e)
+
+    threads = [threading.Thread(target=reads) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
 
 
 def test_refusals(gpu):
