@@ -11,9 +11,9 @@
 //
 // What bounds it: the matrix cores are busy 46 % of the time at about 2.1 GHz, the vector units 60 % with the softmax and
 // the conversions; LDS reads wait between (without them the kernel took 320 us where it took 535, without the copies 428).
-// An 8K prompt (8 groups, h=4; 0.55 TFLOP) takes 511 us over bf16 (1.08 PFLOP/s) and 520 to 536 over 8 bits, where tiles
-// widened on their way into LDS took 562. 1000 queries after 29011 (h=2), 8-bit: 250 us (0.97 PFLOP/s); 1501 queries,
-// window 2047, 8-bit: 76; two 8K prompts (h=4) with a window of 1024 over bf16: 308. A wave with 64 rows halves the reads
+// An 8K prompt (8 groups, h=4; 0.55 TFLOP) takes 509 us over bf16 (1.08 PFLOP/s) and 516 to 530 over 8 bits, where tiles
+// widened on their way into LDS took 562. 1000 queries after 29011 (h=2), 8-bit: 246 us (0.98 PFLOP/s); 1501 queries,
+// window 2047, 8-bit: 75; two 8K prompts (h=4) with a window of 1024 over bf16: 308. A wave with 64 rows halves the reads
 // per product and holds too many registers (632 us and 828); eight waves over 256 rows are 3 % faster on long prompts and
 // coarser on short ones; equal runs of all tiles' blocks for each workgroup balance the chip and write twice the partials
 // (86 us for 76 under the window); a wave's priority, half blocks or V read ahead gave nothing.
@@ -121,32 +121,35 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
     const int kend_wave = min(a.legal, wlast + 1);
 
     // staging: a load of a wave fills 1 KB of a tile, kPer rows, lane l slot l % kSlots of row l / kSlots of them, from a
-    // buffer of those rows (rows past kend give zeros)
+    // buffer of the block's rows (those past kend give zeros)
     constexpr int kSlots = kRow / 16, kPer = 64 / kSlots, kLoads = kKeys / kPer / 4;
     const int srow = lane / kSlots, slot = lane % kSlots;
     const int kswz = Q8 ? 4 * (wave & 1) + (srow >> 1) : 4 * wave + srow, vswz = Q8 ? 2 * (srow >> 1) : 4 * srow;
-    const uint32_t koff = kRow * srow + 16 * (slot ^ kswz), voff = kRow * srow + 16 * (slot ^ vswz);
+    const uint32_t koff = 1024 * wave + kRow * srow + 16 * (slot ^ kswz), voff = 1024 * wave + kRow * srow + 16 * (slot ^ vswz);
     const char* Kb = reinterpret_cast<const char*>(a.K) + (size_t)bg * a.C * kRow;
     const char* Vb = reinterpret_cast<const char*>(a.V) + (size_t)bg * a.C * kRow;
     const uint8_t* keb = Q8 ? a.ke + (size_t)bg * a.nb : nullptr;
     const uint8_t* veb = Q8 ? a.ve + (size_t)bg * a.nb : nullptr;
-    const int last = (a.C - 1) >> a.shift;   // the last scale byte
-    uint32_t kx[2], vx[4];                   // the next block's scale bytes: K, of this lane's rows; V, of 16 keys each
+    const __amdgpu_buffer_rsrc_t ker = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(keb), 0, a.nb, 0x00020000);
+    const __amdgpu_buffer_rsrc_t ver = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(veb), 0, a.nb, 0x00020000);
+    uint32_t kx[2], vx;   // the next block's scale bytes: K, of this lane's rows; V, of 16 keys in each of lanes 0 .. 3
     auto copy = [&](int kb, char* kt, char* vt) {
+        const uint32_t bytes = kRow * (uint32_t)min(kend - kb, kKeys);
+        const char* Kt = Kb + (size_t)kb * kRow;
+        const char* Vt = Vb + (size_t)kb * kRow;
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
-            const int part = 4 * u + wave, row = kb + kPer * part;
-            const uint32_t bytes = kRow * (uint32_t)__builtin_amdgcn_readfirstlane(max(min(kend - row, kPer), 0));
-            load_lds16_buf(reinterpret_cast<const uint16_t*>(Kb + (size_t)row * kRow), bytes, koff,
-                           reinterpret_cast<uint16_t*>(kt + 1024 * part));
-            load_lds16_buf(reinterpret_cast<const uint16_t*>(Vb + (size_t)row * kRow), bytes, voff,
-                           reinterpret_cast<uint16_t*>(vt + 1024 * part));
+            const int at = 4096 * u;
+            load_lds16_buf(reinterpret_cast<const uint16_t*>(Kt), bytes, koff + at,
+                           reinterpret_cast<uint16_t*>(kt + 1024 * wave + at));
+            load_lds16_buf(reinterpret_cast<const uint16_t*>(Vt), bytes, voff + at,
+                           reinterpret_cast<uint16_t*>(vt + 1024 * wave + at));
         }
-        if constexpr (Q8) {
+        if constexpr (Q8) {   // past the last byte: zero, of rows that are zeros
 #pragma unroll
-            for (int x = 0; x < 2; ++x) kx[x] = keb[min((kb + 32 * x + (n & 16)) >> a.shift, last)];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) vx[x] = veb[min((kb + 16 * x) >> a.shift, last)];
+            for (int x = 0; x < 2; ++x)
+                kx[x] = __builtin_amdgcn_raw_buffer_load_b8(ker, (kb + 32 * x + (n & 16)) >> a.shift, 0, 0);
+            vx = __builtin_amdgcn_raw_buffer_load_b8(ver, (kb + 16 * (lane & 3)) >> a.shift, 0, 0);
         }
     };
     // operand reads, as byte offsets into a tile. K: this lane's key of a 32-key tile, bf16 chunk 2 kk + g (8-bit: chunk
@@ -366,7 +369,7 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) ksc[x] = scale_of(kx[x]);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) vsc[x] = scale_of(vx[x]);
+            for (int x = 0; x < 4; ++x) vsc[x] = scale_of((uint32_t)__builtin_amdgcn_readlane((int)vx, x));
         }
     };
     if (tid == 0) again = 0;   // published by the first block's barrier
