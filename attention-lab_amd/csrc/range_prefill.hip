@@ -9,9 +9,9 @@
 // block; an 8-bit operand becomes bf16 (exactly, its scale included) as it is read, which costs each wave 128 conversions
 // a block and halves what it reads from LDS.
 //
-// What bounds it: the matrix cores are busy 46 % of the time at about 2.1 GHz, the vector units 60 % with the softmax and
+// What bounds it: the matrix cores are busy 50 % of the time at about 2.1 GHz, the vector units 60 % with the softmax and
 // the conversions; LDS reads wait between (without them the kernel took 320 us where it took 535, without the copies 428).
-// An 8K prompt (8 groups, h=4; 0.55 TFLOP) takes 509 us over bf16 (1.08 PFLOP/s) and 516 to 530 over 8 bits, where tiles
+// An 8K prompt (8 groups, h=4; 0.55 TFLOP) takes 509 us over bf16 (1.08 PFLOP/s) and 516 over 8 bits, where tiles
 // widened on their way into LDS took 562. 1000 queries after 29011 (h=2), 8-bit: 246 us (0.98 PFLOP/s); 1501 queries,
 // window 2047, 8-bit: 75; two 8K prompts (h=4) with a window of 1024 over bf16: 308. A wave with 64 rows halves the reads
 // per product and holds too many registers (632 us and 828); eight waves over 256 rows are 3 % faster on long prompts and
