@@ -141,9 +141,13 @@ _MERGES: dict = {}      # (device index, stream) -> its counters, zeroed once an
 COUNTERS = 4096         # (b, g) rows that they serve
 PARTIALS = 8 * 1024     # (slot, head) partials: up to four workgroups per CU of eight heads, 4.3 MB
 PART_WORDS = HEAD_DIM + 2
-# Positions to read, by the capacity, up to which a ragged call merges in its one launch: 32 x 2K takes 1 us less on the GPU
-# and a launch less on the host, five of 20K 2 us more (a sequence of many slots is merged by one workgroup).
-RAGGED_MERGE = 1 << 19
+
+def _merge_here(h: int, P: int, positions: int, ragged: bool) -> bool:
+    """Whether a call merges in its own launch (P <= MERGE_SLOTS), which spares the host a launch (3.5 us) and, for few
+    partials, the GPU up to 1 us. Long reads with many partials merge faster in a launch of their own: h=8, P=16, BG=16 at
+    16K 18.6 us for 22.2 (at 4K, BG=8, 10.2 for 12.8, but the host's part is 9 or 12.5); with a length per sequence, whose
+    merge is the workgroup's with the most slots, 40 x 20K 30.5 for 32.8, 256 x 2K 31.0 for 30.1."""
+    return positions <= 1 << 19 if ragged else h * P <= 64 or positions <= 1 << 17
 
 
 def _split_k(P: int, BG: int, h: int, device, stream: int, counted: bool):
@@ -206,7 +210,7 @@ def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: 
     if T == 1 and h <= MAX_H:
         out = check_out(out, q, out_dtype)
         P = decode_partitions(B * G, seen, lengths is not None) if partitions is None else split_count(partitions, 1, MAX_P)
-        held, part, arrive = _split_k(P, B * G, h, device, stream, lengths is None or B * G * seen <= RAGGED_MERGE)
+        held, part, arrive = _split_k(P, B * G, h, device, stream, _merge_here(h, P, B * G * seen, lengths is not None))
         nat.call_on(device, "attnlab_range_decode", k_ptr, v_ptr, *exp_ptrs, block, q.data_ptr(), lengths, legal, p0, window,
                     sinks, B, G, h, C, P, sc, out.data_ptr(), out_dtype == torch.bfloat16, part, arrive, stream)
         return out
@@ -237,7 +241,7 @@ def listed_attention(q, cache, rows, *, scale, out, out_dtype, partitions):
     out = check_out(out, q, out_dtype)
     P = split_count(partitions, decode_partitions(B * G, S, listed=True), MAX_P)
     stream = nat.stream_of(device)
-    held, part, arrive = _split_k(P, B * G, h, device, stream, True)
+    held, part, arrive = _split_k(P, B * G, h, device, stream, _merge_here(h, P, B * G * S, False))
     sc = DEFAULT_SCALE if scale is None else float(scale)
     nat.call_on(device, "attnlab_quant_attend", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(),
                 cache.v_exp.data_ptr(), cache.block, q.data_ptr(), rows.data_ptr(), S, B, G, h, S, C, P, sc,
