@@ -142,6 +142,7 @@ COUNTERS = 4096         # (b, g) rows that they serve
 PARTIALS = 8 * 1024     # (slot, head) partials: up to four workgroups per CU of eight heads, 4.3 MB
 PART_WORDS = HEAD_DIM + 2
 
+
 def _merge_here(h: int, P: int, positions: int, ragged: bool) -> bool:
     """Whether a call merges in its own launch (P <= MERGE_SLOTS), which spares the host a launch (3.5 us) and, for few
     partials, the GPU up to 1 us. Long reads with many partials merge faster in a launch of their own: h=8, P=16, BG=16 at
