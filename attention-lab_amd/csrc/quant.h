@@ -1,5 +1,5 @@
 // The 8-bit K/V cache's element format, shared by the kernels that write it (quant.hip) and read it (range_attend.hip,
-// prefill.hip): e4m3 codes (1 sign, 4 exponent, 3 mantissa bits; largest 448, smallest step 2^-9, 0x7f / 0xff NaN) and
+// range_prefill.hip): e4m3 codes (1 sign, 4 exponent, 3 mantissa bits; largest 448, smallest step 2^-9, 0x7f / 0xff NaN) and
 // one scale 2^(x - 127) per block of positions, KV head and tensor, kept as the byte x.
 //
 // A scale that is a power of two keeps every conversion exact: x * 2^-e and code * 2^e round nothing in fp32 or bf16

@@ -137,7 +137,8 @@ struct Tile {
     uint32_t kx[2], vx;
 };
 
-// Slots whose partials the last workgroup of a (b, g) to arrive merges itself; more take a launch of their own.
+// P up to which the last workgroup of a (b, g) to arrive merges its partials (with lengths, a sequence can have more slots
+// than P); past it they take a launch of their own.
 constexpr int kMergeSlots = 16;
 
 // A partial's weight against the maximum mt. No score above -inf (m = -inf): nothing to add, unless they were NaN.
