@@ -96,6 +96,16 @@ def check_query(q, B: int, G: int, device):
     return h, shape[3]
 
 
+def aligned_query(q):
+    """(q contiguous at a 16-byte aligned address, that address): a copy where it is not."""
+    q = q.contiguous()
+    at = q.data_ptr()
+    if at % 16:
+        q = q.clone()
+        at = q.data_ptr()
+    return q, at
+
+
 def check_listed(q, B: int, G: int, device, partitions) -> int:
     """q and the split count of a row-list read -> h."""
     h, T = check_query(q, B, G, device)
@@ -205,14 +215,14 @@ def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: 
         seen = legal if query_start is None else min(legal, p0 + T)
     if window:   # what the query, or a chunk's workgroup, reads
         seen = min(seen, window + min(T, CHUNK_ROWS // h) - 1 + min(sinks, seen))
-    q = q.contiguous()
+    q, q_at = aligned_query(q)
     sc = DEFAULT_SCALE if scale is None else float(scale)
     stream = nat.stream_of(device)
     if T == 1 and h <= MAX_H:
         out = check_out(out, q, out_dtype)
         P = decode_partitions(B * G, seen, lengths is not None) if partitions is None else split_count(partitions, 1, MAX_P)
         held, part, arrive = _split_k(P, B * G, h, device, stream, _merge_here(h, P, B * G * seen, lengths is not None))
-        nat.call_on(device, "attnlab_range_decode", k_ptr, v_ptr, *exp_ptrs, block, q.data_ptr(), lengths, legal, p0, window,
+        nat.call_on(device, "attnlab_range_decode", k_ptr, v_ptr, *exp_ptrs, block, q_at, lengths, legal, p0, window,
                     sinks, B, G, h, C, P, sc, out.data_ptr(), out_dtype == torch.bfloat16, part, arrive, stream)
         return out
     if out_dtype != torch.bfloat16:
@@ -226,7 +236,7 @@ def range_attention(q, k_ptr: int, v_ptr: int, exp_ptrs, block: int, B: int, G: 
         nbytes = nat.lib().attnlab_range_prefill_part_bytes(B, G, h, T, splits)
         held = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
         part = held.data_ptr()
-    nat.call_on(device, "attnlab_range_prefill", q.data_ptr(), k_ptr, v_ptr, *exp_ptrs, block, out.data_ptr(), B, G, h, T,
+    nat.call_on(device, "attnlab_range_prefill", q_at, k_ptr, v_ptr, *exp_ptrs, block, out.data_ptr(), B, G, h, T,
                 p0, legal, C, window, sinks, sc, splits, part, nbytes, stream)
     return out
 
@@ -238,13 +248,13 @@ def listed_attention(q, cache, rows, *, scale, out, out_dtype, partitions):
     S = int(rows.shape[2])
     if S < 1:
         raise ValueError("at least one row must be selected")
-    q = q.contiguous()
+    q, q_at = aligned_query(q)
     out = check_out(out, q, out_dtype)
     P = split_count(partitions, decode_partitions(B * G, S, listed=True), MAX_P)
     stream = nat.stream_of(device)
     held, part, arrive = _split_k(P, B * G, h, device, stream, _merge_here(h, P, B * G * S, False))
     sc = DEFAULT_SCALE if scale is None else float(scale)
     nat.call_on(device, "attnlab_quant_attend", cache.k.data_ptr(), cache.v.data_ptr(), cache.k_exp.data_ptr(),
-                cache.v_exp.data_ptr(), cache.block, q.data_ptr(), rows.data_ptr(), S, B, G, h, S, C, P, sc,
+                cache.v_exp.data_ptr(), cache.block, q_at, rows.data_ptr(), S, B, G, h, S, C, P, sc,
                 out.data_ptr(), int(out_dtype == torch.bfloat16), part, arrive, stream)
     return out

@@ -85,13 +85,16 @@ def _start(cache: QuantCache, start, length: int):
 
 def _rows(x, step: int):
     """(x as the kernel takes it, its address and three outer strides): unit stride along a row and 16-byte aligned rows of
-    `step` elements to 16 bytes (a copy where it has neither)."""
+    `step` elements to 16 bytes (a copy where it has neither). A dimension of one position has no stride: torch may keep
+    any there."""
     sb, sg, st, sd = x.stride()
     at = x.data_ptr()
     if sd != 1 or (sb | sg | st) % step or at % 16:
-        x = x.contiguous()
-        sb, sg, st, _ = x.stride()
-        at = x.data_ptr()
+        sb, sg, st = (0 if n == 1 else s for n, s in zip(x.shape[:3], (sb, sg, st)))
+        if sd != 1 or (sb | sg | st) % step or at % 16:
+            x = x.clone(memory_format=torch.contiguous_format)   # contiguous() is x itself where only its address is odd
+            sb, sg, st, _ = x.stride()
+            at = x.data_ptr()
     return x, at, sb, sg, st
 
 

@@ -615,7 +615,7 @@ int launch_range(const RangeArgs& a, hipStream_t s) {
 }
 
 int check_range(const void* K, const void* V, const uint8_t* k_exp, const uint8_t* v_exp, int block, const uint16_t* q,
-                int B, int G, int h, int C, int P, const void* out, const float* part) {
+                int B, int G, int h, int C, int P, const void* out, int out_bf16, const float* part) {
     if (k_exp || v_exp) {
         const int rc = check_quant_cache(K, V, k_exp, v_exp, B, G, C, block);
         if (rc) return rc;
@@ -627,6 +627,8 @@ int check_range(const void* K, const void* V, const uint8_t* k_exp, const uint8_
     ATTNLAB_REQUIRE(K && V && q && out, "K, V, q and out must be device pointers");
     ATTNLAB_REQUIRE(((reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V) | reinterpret_cast<uintptr_t>(q)) &
                      15) == 0, "K, V and q must be 16-byte aligned");
+    ATTNLAB_REQUIRE((reinterpret_cast<uintptr_t>(out) & (out_bf16 ? 3 : 7)) == 0,
+                    "out must be aligned to two of its elements (stored in pairs)");
     ATTNLAB_REQUIRE(P == 1 || (part != nullptr && (reinterpret_cast<uintptr_t>(part) & 7) == 0),
                     "P > 1 needs the partial buffer, 8-byte aligned");
     return ATTNLAB_OK;
@@ -667,7 +669,7 @@ extern "C" int attnlab_range_decode(const void* K, const void* V, const uint8_t*
                                     const uint16_t* q, const int32_t* lengths, int length, int64_t q_pos, int window,
                                     int sinks, int B, int G, int h, int C, int P, float scale, void* out, int out_bf16,
                                     float* part, uint32_t* arrive, void* stream) {
-    const int rc = check_range(K, V, k_exp, v_exp, block, q, B, G, h, C, P, out, part);
+    const int rc = check_range(K, V, k_exp, v_exp, block, q, B, G, h, C, P, out, out_bf16, part);
     if (rc) return rc;
     ATTNLAB_REQUIRE(lengths != nullptr || (0 <= length && length <= C), "valid length %d outside [0, C=%d]", length, C);
     ATTNLAB_REQUIRE(lengths != nullptr || q_pos >= 0, "the query's position %lld must not be negative",
@@ -687,7 +689,7 @@ extern "C" int attnlab_quant_attend(const uint8_t* k_codes, const uint8_t* v_cod
                                     int64_t rows_stride, int B, int G, int h, int S, int C, int P, float scale,
                                     void* out, int out_bf16, float* part, uint32_t* arrive, void* stream) {
     ATTNLAB_REQUIRE(k_exp && v_exp, "the scale bytes must be device pointers");
-    const int rc = check_range(k_codes, v_codes, k_exp, v_exp, block, q, B, G, h, C, P, out, part);
+    const int rc = check_range(k_codes, v_codes, k_exp, v_exp, block, q, B, G, h, C, P, out, out_bf16, part);
     if (rc) return rc;
     ATTNLAB_REQUIRE(S >= 1, "at least one row must be selected (S=%d)", S);
     ATTNLAB_REQUIRE(rows != nullptr && rows_stride >= S, "rows must hold S=%d positions per (b, g)", S);

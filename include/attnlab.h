@@ -341,7 +341,8 @@ int attnlab_quant_read(const uint8_t* k_codes, const uint8_t* v_codes, const uin
  * ignored without). q: [B, G, h, 128] bf16, 1 <= h <= 8. P split-K partitions (1..256): with P > 1, part must hold
  * B * G * P * h * 130 floats, 8-byte aligned, for their partials. They are merged by the last workgroup of a (b, g) to
  * arrive where arrive (uint32 [B*G], zero on entry, left zero, not shared with a call that may overlap) is given and
- * P <= 16; by a second launch otherwise, with the same result. out: [B, G, h, 128], bf16 (RNE) when out_bf16 else fp32.
+ * P <= 16; by a second launch otherwise, with the same result. out: [B, G, h, 128], bf16 (RNE) when out_bf16 else fp32,
+ * aligned to two elements.
  * The counterpart of full_attention for one query (full.py:17-44) with the window of a row list F = sinks + recent
  * (selection.py:69-86) read by range.
  */

@@ -170,3 +170,21 @@ def test_wrapper_cache_refuses_other_blocks(block):
     with pytest.raises(ValueError, match="kv_block must be one of"):
         LabCache(layers=1, batch=1, groups=1, capacity=64, head_dim=128, device="cpu", dtype=torch.bfloat16,
                  kv_format="e4m3", kv_block=block)
+
+
+@pytest.mark.parametrize("entry,args", [("attnlab_range_decode", DECODE), ("attnlab_quant_attend", ROWS)])
+@pytest.mark.parametrize("out,bf16", [(18, 1), (17, 1), (20, 0), (18, 0)])
+def test_outputs_off_their_pairs_are_refused(native_lib, entry, args, out, bf16):
+    with pytest.raises(ValueError, match="out must be aligned"):
+        _native.call(entry, *dict(args, out=out, out_bf16=bf16).values())
+
+
+def test_rows_are_copied_only_where_their_address_or_strides_are_odd():
+    from attention_lab.quant import _rows
+    x = torch.zeros(2, 3, 5, 128, dtype=torch.bfloat16)
+    odd = torch.zeros(x.numel() + 1, dtype=torch.bfloat16)[1:].view(x.shape)
+    wide = torch.zeros(1, 1, 1, 131, dtype=torch.bfloat16)[..., :128]
+    for t, kept in ((x, True), (x.transpose(1, 2), True), (x[:, :, :1], True), (wide, True), (odd, False),
+                    (x.transpose(2, 3).contiguous().transpose(2, 3), False)):
+        got, at, *strides = _rows(t, 8)
+        assert (got is t) == kept and at % 16 == 0 and not any(s % 8 for s in strides) and torch.equal(got, t)
