@@ -157,7 +157,8 @@ def quant_attention(q, cache: QuantCache, *, valid_length=None, query_start=None
     """Attention of q [B,G,h,T,128] (bfloat16) over an 8-bit cache -> [B,G,h,T,128].
 
     The T queries sit at consecutive positions from query_start (default: the last T legal ones); query at p reads
-    positions j <= p, j < valid_length, and with a window j > p - window or j < sinks. valid_length: an int (default:
+    positions j <= p, j < valid_length, and with a window j > p - window or j < sinks. Sums are fp32 under weights of at
+    most 1: n rows of values below 2^128 / n have finite outputs. valid_length: an int (default:
     the capacity), or for one query an int32 [B] device tensor with each sequence's length, clamped to [0, capacity],
     its query at the last position. A query that reads no position gets zeros. One query takes h <= 8 at every form and
     out_dtype float32 too; a chunk, and one query with h <= 16 and an int length, gives bfloat16. partitions overrides

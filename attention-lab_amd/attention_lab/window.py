@@ -18,7 +18,8 @@ def window_attention(q, k, v, *, window, sinks: int = FIXED_PREFIX, valid_length
 
     The T queries sit at consecutive positions from query_start (default: the last T legal ones); query at p reads
     positions j <= p, j < valid_length with j > p - window or j < sinks, by their original positions. window None:
-    every legal position. valid_length: an int (default: the capacity), or for one query an int32 [B] device tensor
+    every legal position. Sums are fp32 under weights of at most 1: n rows of values below 2^128 / n have finite outputs.
+    valid_length: an int (default: the capacity), or for one query an int32 [B] device tensor
     with each sequence's length, clamped to [0, C], its query at the last position. A query that reads no position
     gets zeros. One query takes h <= 8 at every form and out_dtype float32 too; a chunk, and one query with h <= 16 and
     an int length, gives bfloat16. partitions overrides the split-K count (one query: 1..256, a chunk: 1..16).

@@ -13,8 +13,9 @@
 //
 // The 16 columns of a tile are 8 heads twice: columns 0..7 multiply V by P rounded to bf16, columns 8..15 by what that
 // rounding left, and the two are added at the end, so the weights keep 16 bits without a second product. Softmax is
-// online in the log2 domain; the running max moves, and sums are rescaled, only when a score passes it by 2^8, so most
-// tiles need no exchange between lanes. Sums and outputs are fp32. The waves of a workgroup merge through LDS, the P
+// online in the log2 domain; a row's shift m is set 2^8 above its largest score so far and moves, with the sums rescaled,
+// only when a score passes it, so most tiles need no exchange between lanes and no weight is above 1: n rows of values
+// below 2^128 / n have finite sums, as with the exact maximum. Sums and outputs are fp32. The waves of a workgroup merge through LDS, the P
 // workgroups of a (b, g) through partials: the last to arrive merges them in split order, or, without counters, a second
 // small launch does, with the same sums.
 //
@@ -43,7 +44,7 @@ constexpr int kDim = 128;
 constexpr int kWaves = 4;
 constexpr int kTile = 32;           // rows a wave takes at a time
 constexpr int kListChunk = 2048;    // listed positions staged in LDS at a time
-constexpr float kLazy = 8.0f;       // the running max grows only by more than 2^8
+constexpr float kLazy = 8.0f;       // the shift lies 2^8 above the largest score when it is set
 constexpr int kPartWords = kDim + 2;
 
 struct RangeArgs {
@@ -409,9 +410,10 @@ __global__ __launch_bounds__(64 * kWaves, LIST ? 2 : 3) void range_attend(RangeA
         for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
             for (int i = 0; i < 4; ++i) bm = fmaxf(bm, sv[t2][i]);
-        if (__any(bm * sc > m + kLazy)) {
+        if (__any(bm * sc > m)) {
             bm = max_xor32(max_xor16(bm)) * sc;
-            if (bm > m + kLazy) {   // also a column's first rows (m = -inf)
+            if (bm > m) {   // also a column's first rows (m = -inf)
+                bm += kLazy;
                 const float al = fast_exp2(m - bm);
                 l *= al;
 #pragma unroll

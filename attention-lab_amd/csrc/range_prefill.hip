@@ -38,7 +38,8 @@ namespace {
 constexpr int kDim = 128;
 constexpr int kRows = 128;          // (query, head) rows per workgroup: 4 waves x 32
 constexpr int kKeys = 64;           // keys per block
-constexpr float kLazy = 8.0f;       // rescale O only when the running max grows by more than 2^8
+constexpr float kLazy = 8.0f;       // a row's shift is set 2^8 above its largest score and moves when one passes it: few
+                                    // rescales, and no weight above 1, so n rows of values below 2^128 / n have finite sums
 constexpr int kPart = 132;          // m, l, two unused words (16-byte aligned rows), the 128 unnormalised outputs
 constexpr int kMaxSplits = 16;
 
@@ -297,7 +298,8 @@ __global__ __launch_bounds__(256, 2) void range_prefill(RangePrefillArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) bm = fmaxf(bm, s[x][i]);
         bm = max_xor32(bm) * sc;
-        if (bm > m_run + kLazy) {   // also the first keys of the row (m_run = -inf)
+        if (bm > m_run) {   // also the first keys of the row (m_run = -inf)
+            bm += kLazy;
             const float al = fast_exp2(m_run - bm);   // exp2(-inf) = 0
             l_run *= al;
 #pragma unroll

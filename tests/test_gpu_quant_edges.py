@@ -1,12 +1,17 @@
-"""The 8-bit cache and the windowed read at the edges of what they take: rows and queries at any address."""
+"""The 8-bit cache and the windowed read at the edges of what they take: rows and queries at any address, and values near the
+largest. Tolerances as in test_gpu_quant.py."""
 from __future__ import annotations
+
+import math
 
 import numpy as np
 import pytest
 import torch
 
-from attention_lab import dequantize_rows, quant_attention, quant_gather_attention, quantize_append, window_attention
-from test_gpu_quant import bytes_of, random_cache, randn
+from attention_lab import (QuantCache, dequantize_rows, quant_attention, quant_gather_attention, quantize_append,
+                           window_attention)
+from oracle import quant as oq
+from test_gpu_quant import bytes_of, check, f64, random_cache, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -73,3 +78,59 @@ def test_an_output_whose_rows_are_not_aligned_is_refused(gpu, dtype, elements):
     with pytest.raises(ValueError, match="aligned"):
         quant_attention(q, cache, out=out, out_dtype=dtype)
     assert not out.any()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# values near the largest: weights are at most 1, so n rows of less than 2^128 / n have finite sums
+# ---------------------------------------------------------------------------------------------------------------------
+def loud_rows(gpu, kind, C):
+    """K rows that score 0 up to 128 and 7.5 (log2) behind, V rows of one sign up to 1.875 * 2^118; the call and both."""
+    g = torch.Generator().manual_seed(3)
+    k = torch.zeros(1, 2, C, 128)
+    k[:, :, 128:, 0] = 7.5
+    codes = torch.randint(0x38, 0x40, (1, 2, C, 128), generator=g).to(torch.uint8)      # 1 to 1.875
+    v = codes.view(torch.float8_e4m3fn).double() * 2.0 ** 118
+    if kind == "bf16":
+        kd, vd = k.to(torch.bfloat16).to(gpu), v.to(torch.bfloat16).to(gpu)
+        return (lambda q, **kw: window_attention(q, kd, vd, window=None, **kw)), f64(k), f64(v), None
+    nb = -(-C // kind)
+    cache = QuantCache(k.to(torch.float8_e4m3fn).to(gpu), codes.to(gpu).view(torch.float8_e4m3fn),
+                       torch.full((1, 2, nb), 127, dtype=torch.uint8, device=gpu),
+                       torch.full((1, 2, nb), 127 + 118, dtype=torch.uint8, device=gpu), block=kind)
+    return (lambda q, **kw: quant_attention(q, cache, **kw)), f64(k), f64(v), cache
+
+
+@pytest.mark.parametrize("kind", ["bf16", 16, 64])
+@pytest.mark.parametrize("T", [1, 20])
+@pytest.mark.parametrize("partitions", [1, 2])
+def test_loud_values_have_finite_outputs(gpu, kind, T, partitions):
+    C = 300
+    call, k, v, cache = loud_rows(gpu, kind, C)
+    q = torch.zeros(1, 2, 2, T, 128, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    scale = math.log(2.0)
+    want = oq.range_attention(f64(q), k, v, C, C - T, None, 0, scale)
+    assert np.isfinite(want.astype(np.float32)).all()
+    for dt in (torch.bfloat16, torch.float32) if T == 1 else (torch.bfloat16,):
+        got = call(q.to(gpu), scale=scale, out_dtype=dt, partitions=partitions)
+        check(got, want, want, 7.5, chunk=T > 1, what=f"{kind} {dt}")
+    if T == 1 and cache is not None:
+        rows = torch.randperm(C, generator=torch.Generator().manual_seed(1))[:250].view(1, 1, -1).expand(1, 2, -1)
+        rows = rows.sort(dim=-1).values     # the quiet rows first
+        want = oq.listed_attention(f64(q)[:, :, :, 0], k, v, rows.numpy(), scale)[:, :, :, None]
+        got = quant_gather_attention(q.to(gpu), cache, rows.to(gpu), scale=scale, partitions=partitions)
+        check(got, want, want, 7.5, chunk=False, what="rows")
+
+
+@pytest.mark.parametrize("T", [1, 5])
+def test_one_row_of_the_largest_value(gpu, T):
+    """What the append stores at most, 1.875 * 2^127, is read as it is."""
+    cache = QuantCache.empty(1, 1, 64, block=16, device=gpu)
+    x = torch.full((1, 1, 1, 128), 3.4e38, device=gpu)
+    quantize_append(cache, torch.zeros_like(x), x, 0)
+    q = randn(1, 1, 1, 2, T, 128).to(gpu)
+    got = quant_attention(q, cache, valid_length=1, query_start=0)
+    assert (f64(got) == 1.875 * 2.0 ** 127).all()
+    if T == 1:
+        got = quant_gather_attention(q, cache, torch.zeros(1, 1, 1, dtype=torch.int32, device=gpu), out_dtype=torch.float32)
+        assert (f64(got) == 1.875 * 2.0 ** 127).all()
