@@ -35,7 +35,9 @@ _DTYPES = {torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16, torch.float32
 
 class QuantCache:
     """One layer's K and V in 8 bits: k, v torch.float8_e4m3fn [B,G,C,128]; k_exp, v_exp uint8 [B,G,ceil(C/block)], the
-    scale of a block being 2^(x - 127). All four are contiguous tensors on one HIP device, used in place."""
+    scale of a block being 2^(x - 127). All four are contiguous tensors on one HIP device, used in place. Scale bytes are 17
+    to 247, as quantize_append writes them; those of blocks that hold no row a read takes may be any, but a first write
+    that begins inside a block takes the block's byte for that of rows before it (`empty` sets the smallest)."""
 
     __slots__ = ("k", "v", "k_exp", "v_exp", "block", "batch", "groups", "capacity", "device")
 

@@ -26,8 +26,8 @@
 // and of the merge. Ranges take three waves a SIMD with one tile each over two with two, and four waves a workgroup over
 // eight or sixteen.
 //
-// Masked rows: their scores are replaced, and their V rows are zeros, so whatever they hold (NaN, infinity) leaves the
-// output alone. A query with no row to read, or whose scores are all -inf, gets zeros.
+// Masked rows: their scores are replaced, and their V rows are zeros of scale 1, so whatever they and their scale bytes hold
+// (NaN, infinity) leaves the output alone. A query with no row to read, or whose scores are all -inf, gets zeros.
 #include <cfloat>
 
 #include "mfma_attend.h"
@@ -311,7 +311,10 @@ __global__ __launch_bounds__(64 * kWaves, LIST ? 2 : 3) void range_attend(RangeA
                 kp[t2] = max(entry(t, krow + 4 * t2), 0);
                 f.kx[t2] = keb[kp[t2] >> a.shift];
             }
-            f.vx = veb[max(entry(t, 8 * g4 + (n16 & 7)), 0) >> a.shift];
+            // a skipped slot has no scale byte: its weight is zero, and zero times the scale of some byte would be NaN
+            const int vp = entry(t, 8 * g4 + (n16 & 7));
+            const uint32_t vx = veb[max(vp, 0) >> a.shift];
+            f.vx = vp < 0 ? 127u : vx;
 #pragma unroll
             for (int t2 = 0; t2 < 2; ++t2) {
                 const uint8_t* r = Kb + (size_t)kp[t2] * kRow + 16 * g4;
@@ -443,7 +446,8 @@ __global__ __launch_bounds__(64 * kWaves, LIST ? 2 : 3) void range_attend(RangeA
             w4[i] = n16 < 8 ? hi : rest;
         }
         const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{w4[0], w4[1], w4[2], w4[3]});
-        const float vs = Q8 && !LIST ? scale_of(f.vx) : 1.0f;
+        // 8-bit: the scale of this lane's eight keys. Where all are masked it can be any byte, one that is no number among them
+        const float vs = Q8 && !LIST && (ok >> (8 * g4) & 255u) != 0 ? scale_of(f.vx) : 1.0f;
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
             u32x4_t w;

@@ -1,5 +1,5 @@
-"""The 8-bit cache and the windowed read at the edges of what they take: rows and queries at any address, and values near the
-largest. Tolerances as in test_gpu_quant.py."""
+"""The 8-bit cache and the windowed read at the edges of what they take: rows and queries at any address, values near the
+largest, and scale bytes of blocks that no row read lies in. Tolerances as in test_gpu_quant.py."""
 from __future__ import annotations
 
 import math
@@ -134,3 +134,44 @@ def test_one_row_of_the_largest_value(gpu, T):
     if T == 1:
         got = quant_gather_attention(q, cache, torch.zeros(1, 1, 1, dtype=torch.int32, device=gpu), out_dtype=torch.float32)
         assert (f64(got) == 1.875 * 2.0 ** 127).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# scale bytes of blocks that no row read lies in
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("byte", [0, 255])
+@pytest.mark.parametrize("block", [16, 32, 64])
+def test_scale_bytes_of_unread_blocks_never_matter(gpu, byte, block):
+    """A cache of the caller's own tensors need not have set the scale bytes of blocks that hold no row yet, or that no
+    query reads: whatever they are, and whatever the codes there, the outputs are the same."""
+    B, G, h, C = 1, 2, 3, 256
+    cache, _, _ = random_cache(gpu, 5, B, G, C, block)
+    spoilt, _, _ = random_cache(gpu, 5, B, G, C, block)
+
+    def spoil(keep):
+        """Every block without a position of `keep`: its scale byte, and zeros and other codes in its rows."""
+        used = torch.zeros(C, dtype=torch.bool)
+        used[list(keep)] = True
+        for j in range(C // block):
+            if not used[block * j:block * j + block].any():
+                for t in (spoilt.k_exp, spoilt.v_exp):
+                    t[:, :, j] = byte
+                for t in (spoilt.k, spoilt.v):
+                    t.view(torch.uint8)[:, :, block * j:block * j + block:2] = 0
+
+    q = randn(17, B, G, h, 1, 128).to(gpu)
+    rows = torch.tensor([-1, 130, 200, C, 131, -7, 255, 130] * 9, dtype=torch.int32, device=gpu).expand(B, G, -1)
+    spoil((130, 131, 200, 255))
+    for P in (1, 2):
+        assert torch.equal(quant_gather_attention(q, spoilt, rows, partitions=P),
+                           quant_gather_attention(q, cache, rows, partitions=P))
+    for L, window, sinks in ((130, None, 0), (131, 20, 3), (200, 17, 0)):
+        for T in (1, 9):
+            keep = set(range(sinks)) | set(range(max(0, L - T - window + 1) if window else 0, L))
+            spoilt, _, _ = random_cache(gpu, 5, B, G, C, block)
+            spoil(keep)
+            qq = randn(18, B, G, h, T, 128).to(gpu)
+            for P in (1, 2):
+                read = lambda c: quant_attention(qq, c, valid_length=L, window=window, sinks=sinks, partitions=P)  # noqa: E731, B023
+                assert torch.equal(read(spoilt), read(cache)), (L, window, sinks, T, P)
+
