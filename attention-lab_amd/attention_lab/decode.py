@@ -19,7 +19,9 @@ one (trained.py:78-81); other inputs raise ValueError.
 """
 from __future__ import annotations
 
+import contextlib
 import math
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -299,7 +301,28 @@ def sparse_decode_step_kernel(q_main, q_pre, k_cache, v_cache, zT, wq_t_scaled, 
     return (out, flat) if return_rows else out
 
 
-_QUANT_WS = nat.Workspace()   # the select state of sparse_decode_step_quant
+# Select state and scratch of sparse_decode_step_quant: the score launch adds into the state and the select launch takes it
+# out again, so both belong to one stream, and no other thread's launches on it may come between them.
+_QUANT_WS: dict = {}      # (device index, stream) -> (Workspace, lock)
+
+
+class _GraphScratch:
+    """The workspace of a captured step: memory of its graph's own, the state zeroed by every replay."""
+
+    @staticmethod
+    def bytes(device, nbytes: int, tag: str):
+        return (torch.zeros if tag == "state" else torch.empty)(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
+def _step_workspace(device, workspace):
+    """(workspace, lock to hold from the score launch to the select's) of a step on torch's current stream."""
+    if workspace is not None:
+        return workspace, contextlib.nullcontext()
+    if hip_range.capturing(device):
+        return _GraphScratch, contextlib.nullcontext()
+    key = (device.index, nat.stream_of(device))
+    held = _QUANT_WS.get(key)
+    return _QUANT_WS.setdefault(key, (nat.Workspace(), threading.Lock())) if held is None else held
 
 
 def sparse_decode_step_quant(q_main, q_pre, cache, zT, wq_t_scaled, wk, fixed_rows, off_lo, lo: int, hi: int, k: int,
@@ -307,7 +330,12 @@ def sparse_decode_step_quant(q_main, q_pre, cache, zT, wq_t_scaled, wk, fixed_ro
                              return_rows: bool = False, canonical_order: bool = False, partitions=None, workspace=None):
     """sparse_decode_step_kernel over an 8-bit K/V cache (quant.QuantCache of capacity C, the table's): z column write, u,
     candidate scan and top-k as there, over a bfloat16 or float32 index table, then the row-list read of the codes. No
-    counterpart in the reference. The new key's and value's rows are the caller's to append (quantize_append)."""
+    counterpart in the reference. The new key's and value's rows are the caller's to append (quantize_append).
+
+    workspace: None, or a _native.Workspace for the select state and scratch, whose calls must follow one another on one
+    stream. By default every stream has its own, threads that share a stream take turns, and a captured call's belongs to
+    its graph, so steps on other streams, in other threads and graphs share nothing.
+    """
     B, G, h, T, d = q_main.shape
     if T != 1:
         raise ValueError("a decode step takes exactly one new query position")
@@ -315,8 +343,8 @@ def sparse_decode_step_quant(q_main, q_pre, cache, zT, wq_t_scaled, wk, fixed_ro
     if (B, G, d) != (cache.batch, cache.groups, hip_attend.HEAD_DIM):
         raise ValueError(f"q_main {tuple(q_main.shape)} does not match a cache of B, G = {cache.batch}, {cache.groups}")
     hip_range.check_listed(q_main, B, G, cache.device, partitions)   # the read's refusals, before the table is written
-    if zT.dim() != 4 or tuple(zT.shape[:2]) != (B, G) or zT.shape[3] != C:
-        raise ValueError("zT must be a [B, G, r, C] tensor matching the cache")
+    if zT.dim() != 4 or tuple(zT.shape[:2]) != (B, G) or zT.shape[3] != C or zT.device != cache.device:
+        raise ValueError("zT must be a [B, G, r, C] tensor matching the cache, on its device")
     if q_pre.numel() != q_main.numel():
         raise ValueError("q_pre must hold q_main's elements")
     lo, hi, k, S = int(lo), int(hi), int(k), int(selected_count)
@@ -340,13 +368,20 @@ def sparse_decode_step_quant(q_main, q_pre, cache, zT, wq_t_scaled, wk, fixed_ro
         flat = fixed_rows.reshape(-1)
         pos = positions_from_flat(flat, B, G, S, C, cache.device)
     else:
-        W = nat.SELECT_STATE_WORDS
-        wsp = _QUANT_WS if workspace is None else workspace
-        state = wsp.bytes(cache.device, B * G * W * 4, "state")[:B * G * W * 4].view(torch.int32).view(B, G, W)
-        s = hip_score.score_grouped(zT, lo, hi, state=state, **score)
+        nb = B * G * nat.SELECT_STATE_WORDS * 4
         order = _order(canonical_order or not return_rows)   # the order shows only in rows that leave the call
-        pos, flat = hip_select.select_rows(s, lo, hi, legal, k, C, order=order, want_flat=return_rows, state=state,
-                                           workspace=wsp)
+        wsp, lock = _step_workspace(cache.device, workspace)
+        with lock:
+            state = wsp.bytes(cache.device, nb, "state")[:nb].view(torch.int32).view(B, G, -1)
+            scratch = hip_select.reserve(cache.device, B * G, hi - lo, k, order, wsp)
+            rows = torch.empty(B, G, S, dtype=torch.int32, device=cache.device)
+            try:
+                s = hip_score.score_grouped(zT, lo, hi, state=state, **score)
+                pos, flat = hip_select.select_rows(s, lo, hi, legal, k, C, order=order, rows=rows, want_flat=return_rows,
+                                                   state=state, scratch=scratch)
+            except BaseException:
+                state.zero_()   # of what the score added and no select will take out
+                raise
     out = hip_range.listed_attention(q_main, cache, pos, scale=scale, out=None, out_dtype=torch.bfloat16,
                                      partitions=partitions)
     return (out, flat) if return_rows else out

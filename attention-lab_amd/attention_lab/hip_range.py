@@ -166,7 +166,7 @@ def _split_k(P: int, BG: int, h: int, device, stream: int, counted: bool):
     if P == 1:
         return None, None, None
     rows = BG * P * h
-    if counted and P <= MERGE_SLOTS and BG <= COUNTERS and rows <= PARTIALS and not _capturing(device):
+    if counted and P <= MERGE_SLOTS and BG <= COUNTERS and rows <= PARTIALS and not capturing(device):
         buf = _MERGES.get((device.index, stream))
         if buf is None:
             buf = _MERGES[device.index, stream] = torch.zeros(COUNTERS + PARTIALS * PART_WORDS, dtype=torch.int32,
@@ -177,7 +177,7 @@ def _split_k(P: int, BG: int, h: int, device, stream: int, counted: bool):
     return part, part.data_ptr(), None
 
 
-def _capturing(device) -> bool:
+def capturing(device) -> bool:
     """torch's current stream on `device` is being captured."""
     if device.index == torch._C._cuda_getDevice():
         return torch._C._cuda_isCurrentStreamCapturing()

@@ -185,13 +185,13 @@ def score_grouped(zT, lo: int, hi: int, *, wk=None, q_cat=None, wq_t=None, u=Non
     if zT.dtype == torch.float32:
         if u is None and u_out is None and M > 0:
             u_out = torch.empty(B, G, r, dtype=torch.float32, device=zT.device)
-        nat.call("attnlab_score_grouped_f32", zT.data_ptr(), nat.ptr(k_new), nat.ptr(wk), nat.ptr(q_cat),
-                 nat.ptr(wq_t), nat.ptr(u), nat.ptr(u_out), out.data_ptr(), out.shape[2], B, G, r, C, d, hd, lo, hi,
-                 write_col if k_new is not None else 0, nat.ptr(state), nat.stream_of(zT.device))
+        nat.call_on(zT.device, "attnlab_score_grouped_f32", zT.data_ptr(), nat.ptr(k_new), nat.ptr(wk), nat.ptr(q_cat),
+                    nat.ptr(wq_t), nat.ptr(u), nat.ptr(u_out), out.data_ptr(), out.shape[2], B, G, r, C, d, hd, lo, hi,
+                    write_col if k_new is not None else 0, nat.ptr(state), nat.stream_of(zT.device))
         return out[..., :M]
-    nat.call("attnlab_score_grouped", zT.data_ptr(), nat.ptr(k_new), nat.ptr(wk), nat.ptr(q_cat), nat.ptr(wq_t),
-             nat.ptr(u), nat.ptr(u_out), out.data_ptr(), out.shape[2], B, G, r, C, d, hd, lo, hi,
-             write_col if k_new is not None else 0, 1, nat.ptr(state), nat.stream_of(zT.device))
+    nat.call_on(zT.device, "attnlab_score_grouped", zT.data_ptr(), nat.ptr(k_new), nat.ptr(wk), nat.ptr(q_cat),
+                nat.ptr(wq_t), nat.ptr(u), nat.ptr(u_out), out.data_ptr(), out.shape[2], B, G, r, C, d, hd, lo, hi,
+                write_col if k_new is not None else 0, 1, nat.ptr(state), nat.stream_of(zT.device))
     return out[..., :M]
 
 

@@ -80,8 +80,14 @@ def topk(scores, k: int, *, order: str = "score", tiled=None, workspace=None):
     return val[:, :k].reshape(*lead, k), idx[:, :k].reshape(*lead, k)
 
 
+def reserve(device, rows: int, M: int, k: int, order: str, workspace=None):
+    """The scratch of a tiled select of k > 0 of M candidates in each of `rows` rows."""
+    nbytes = nat.lib().attnlab_select_scratch_bytes(rows, M, k, _order_code(order))
+    return (_WS if workspace is None else workspace).bytes(device, nbytes, "scratch")
+
+
 def select_rows(scores, lo: int, hi: int, legal: int, k: int, capacity: int, *, order: str = "position",
-                rows=None, want_flat: bool = False, state=None, tiled: bool = True, workspace=None):
+                rows=None, want_flat: bool = False, state=None, tiled: bool = True, workspace=None, scratch=None):
     """Row list of one decode step from candidate scores [B, G, hi-lo] (fp32, unit column stride).
 
     Returns (rows int32 [B, G, S] original positions, flat int64 [B*G*S] row ids of the flattened cache or None),
@@ -89,7 +95,8 @@ def select_rows(scores, lo: int, hi: int, legal: int, k: int, capacity: int, *, 
     first and then the candidates by descending score, like cat(fixed_rows, topk.indices) in decode.py:93.
     state: the select state score_grouped(..., state=) filled for these scores (cleared here), or None. With a state
     and tiled=True the keys are classified by a grid of 4096-key tiles and each row resolved by one workgroup (same
-    result as the single-workgroup select, in either order). Score order takes any k.
+    result as the single-workgroup select, in either order). Score order takes any k. scratch: what `reserve` gave for
+    this call, for a caller that holds it before the scores are made.
     """
     if scores.dim() != 3 or scores.dtype != torch.float32 or not scores.is_cuda or scores.stride(2) != 1:
         raise ValueError("scores must be a float32 [B, G, M] tensor with unit column stride on a HIP device")
@@ -116,13 +123,11 @@ def select_rows(scores, lo: int, hi: int, legal: int, k: int, capacity: int, *, 
     if state is not None and (state.dtype != torch.int32 or tuple(state.shape) != (B, G, W)
                               or not state.is_contiguous() or state.device != scores.device):
         raise ValueError(f"state must be a contiguous int32 [{B}, {G}, {W}] tensor on the scores' device")
-    scratch = None
-    if k > 0 and ((state is not None and tiled) or (code == nat.ORDER_SCORE and k > LDS_SORT_K)):
-        nbytes = nat.lib().attnlab_select_scratch_bytes(B * G, M, k, code)
-        scratch = (_WS if workspace is None else workspace).bytes(scores.device, nbytes, "scratch")
-    nat.call("attnlab_select_rows", scores.data_ptr(), stride, B, G, lo, hi, legal, k, capacity, code,
-             rows.data_ptr(), S, nat.ptr(flat), nat.ptr(state), nat.ptr(scratch),
-             0 if scratch is None else scratch.numel(), nat.stream_of(scores.device))
+    if scratch is None and k > 0 and ((state is not None and tiled) or (code == nat.ORDER_SCORE and k > LDS_SORT_K)):
+        scratch = reserve(scores.device, B * G, M, k, order, workspace)
+    nat.call_on(scores.device, "attnlab_select_rows", scores.data_ptr(), stride, B, G, lo, hi, legal, k, capacity, code,
+                rows.data_ptr(), S, nat.ptr(flat), nat.ptr(state), nat.ptr(scratch),
+                0 if scratch is None else scratch.numel(), nat.stream_of(scores.device))
     return rows, flat
 
 

@@ -188,3 +188,57 @@ def test_rows_are_copied_only_where_their_address_or_strides_are_odd():
                     (x.transpose(2, 3).contiguous().transpose(2, 3), False)):
         got, at, *strides = _rows(t, 8)
         assert (got is t) == kept and at % 16 == 0 and not any(s % 8 for s in strides) and torch.equal(got, t)
+
+
+def test_steps_that_share_a_stream_take_turns(monkeypatch):
+    """Two host threads on one stream: no launch of one comes between the other's score and select, which meet in the
+    select state; the launches are stand-ins here."""
+    import contextlib
+    import threading
+    import time
+    from types import SimpleNamespace
+    from attention_lab import decode, hip_score, hip_select
+    events = []
+
+    def score(zT, lo, hi, *, state, **kw):
+        events.append(("score", threading.get_ident(), state.data_ptr()))
+        time.sleep(0.02)
+        return torch.zeros(1, 1, hi - lo)
+
+    def select(s, *args, rows, **kw):
+        events.append(("select", threading.get_ident(), 0))
+        return rows, None
+
+    monkeypatch.setattr(hip_score, "score_grouped", score)
+    monkeypatch.setattr(hip_select, "select_rows", select)
+    monkeypatch.setattr(hip_select, "reserve", lambda *a: None)
+    monkeypatch.setattr(hip_range, "capturing", lambda device: False)
+    monkeypatch.setattr(hip_range, "check_listed", lambda *a: 1)
+    monkeypatch.setattr(hip_range, "listed_attention", lambda q, *a, **k: q)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    stream = threading.local()
+    monkeypatch.setattr(_native, "stream_of", lambda device: getattr(stream, "of", 0))
+    monkeypatch.setattr(decode, "_QUANT_WS", {})
+    cache = SimpleNamespace(capacity=400, batch=1, groups=1, device=torch.device("cpu"))
+    q = torch.zeros(1, 1, 1, 1, 128, dtype=torch.bfloat16)
+    req = decode.prepare_request(1, 1, 400, valid_length=300, query_position=299, rho=0.1, device="cpu")
+    lay = req.layout
+
+    def run(of):
+        stream.of = of
+        for _ in range(4):
+            decode.sparse_decode_step_quant(q, q, cache, torch.zeros(1, 1, 32, 400, dtype=torch.bfloat16),
+                                            torch.zeros(1, 128, 32), torch.zeros(1, 32, 128), req.fixed_rows, req.off_lo,
+                                            lay.candidate_lo, lay.candidate_hi, req.k, req.selected_count)
+
+    for streams, shared in (((7, 7), True), ((7, 8), False)):
+        events.clear()
+        threads = [threading.Thread(target=run, args=(s,)) for s in streams]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert len(events) == 16 and len({p for n, _, p in events if n == "score"}) == (1 if shared else 2)
+        if shared:
+            assert all(a[0] == "score" and b[0] == "select" and a[1] == b[1] for a, b in zip(events[::2], events[1::2]))
+    assert isinstance(decode._step_workspace(cache.device, object())[1], contextlib.nullcontext)
