@@ -17,7 +17,7 @@ import torch
 LIB_NAME = "libattnlab.so"
 # ATTNLAB_LIB names another build of the same library (the host-sanitized debug build); unset, the in-tree one
 LIB_PATH = os.environ.get("ATTNLAB_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 11
+ABI_VERSION = 12
 # select state per (b, g) row: the first-digit histogram of the top-k (2048 bins, top 11 bits of the order-preserving
 # score key), 64 super-bin counts of 32 bins each, then 64 arrival counters of the step's attend partitions
 # (ATTNLAB_SELECT_STATE_WORDS)
@@ -58,6 +58,7 @@ SIGNATURES = {
     "attnlab_prefill_part_bytes": (_i64, [_i] * 5),
     "attnlab_prefill_attend_split": (_i, [_p, _p, _p, _i64, _i, _p] + [_i] * 8 + [_f, _i, _p, _i64, _p]),
     "attnlab_quant_append": (_i, ([_p] + [_i64] * 3) * 2 + [_i] + [_p] * 5 + [_i] * 6 + [_p]),
+    "attnlab_quant_append_kept": (_i, ([_p] + [_i64] * 3) * 2 + [_p] * 4 + [_i] * 6 + [_p, _p, _i, _p]),
     "attnlab_quant_read": (_i, [_p] * 6 + [_i, _p] + [_i] * 6 + [_p]),
     "attnlab_range_decode": (_i, [_p] * 4 + [_i, _p, _p, _i, _i64] + [_i] * 7 + [_f, _p, _i, _p, _p, _p]),
     "attnlab_quant_attend": (_i, [_p] * 4 + [_i, _p, _p, _i64] + [_i] * 6 + [_f, _p, _i, _p, _p, _p]),

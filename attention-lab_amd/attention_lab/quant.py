@@ -100,16 +100,8 @@ def _rows(x, step: int):
     return x, at, sb, sg, st
 
 
-def quantize_append(cache: QuantCache, k, v, start=0) -> None:
-    """Write the rows k, v [B,G,T,128] (bfloat16, float16 or float32, any strides) at positions [start, start + T).
-
-    start: an int, or an int32 [B] device tensor with each sequence's own (rows outside [0, capacity) are then not
-    written). Every block's scale is the smallest power of two, 2^-110 at least, that its rows fit under; a block that
-    already holds rows before `start` keeps its scale unless a new row needs a larger one, and then its earlier codes
-    are moved to it. So a chunked write may round a value below 2^-6 of its scale twice where one write would round it
-    once; everything else is the same. Rows at and after start + T are no longer valid rows of the block they share.
-    NaN and infinity become NaN; finite values past 1.875 * 2^127 saturate.
-    """
+def _check_rows(cache: QuantCache, k, v):
+    """(dtype code, T) of the rows k, v [B,G,T,128] of a write."""
     shape = k.shape
     B, G, T, d = shape if len(shape) == 4 else (0, 0, 0, 0)
     if B != cache.batch or G != cache.groups or d != HEAD_DIM or v.shape != shape:
@@ -118,16 +110,60 @@ def quantize_append(cache: QuantCache, k, v, start=0) -> None:
     dtype = _DTYPES.get(k.dtype)
     if dtype is None or v.dtype != k.dtype:
         raise ValueError(f"k and v must both be bfloat16, float16 or float32, got {k.dtype} and {v.dtype}")
-    device = cache.device
-    if k.device != device or v.device != device:
+    if k.device != cache.device or v.device != cache.device:
         raise ValueError("k and v must live on the cache's device")
+    return dtype, T
+
+
+def quantize_append(cache: QuantCache, k, v, start=0) -> None:
+    """Write the rows k, v [B,G,T,128] (bfloat16, float16 or float32, any strides) at positions [start, start + T).
+
+    start: an int, or an int32 [B] device tensor with each sequence's own (rows outside [0, capacity) are then not
+    written). Every block's scale is the smallest power of two, 2^-110 at least, that its rows fit under; a block that
+    already holds rows before `start` keeps its scale unless a new row needs a larger one, and then its earlier codes
+    are moved to it. So a chunked write may round a value below 2^-6 of its scale twice where one write would round it
+    once; everything else is the same. Rows at and after start + T are no longer valid rows of the block they share, but a
+    block that grew for rows since discarded keeps that scale and rounding (qwen_wrap.LabCache.rollback undoes it).
+    NaN and infinity become NaN; finite values past 1.875 * 2^127 saturate.
+    """
+    dtype, T = _check_rows(cache, k, v)
+    device = cache.device
     starts, at = _start(cache, start, T)
     step = 4 if dtype == nat.DT_F32 else 8
     k, k_at, kb, kg, kt = _rows(k, step)
     v, v_at, vb, vg, vt = _rows(v, step)
     nat.call_on(device, "attnlab_quant_append", k_at, kb, kg, kt, v_at, vb, vg, vt, dtype, cache.k.data_ptr(),
-                cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), starts, at, B, G, T, cache.capacity,
-                cache.block, nat.stream_of(device))
+                cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), starts, at, cache.batch, cache.groups, T,
+                cache.capacity, cache.block, nat.stream_of(device))
+
+
+class KeptRows:
+    """The last R rows written to a cache as they came: position p in slot p % R of k, v (bfloat16 [B,G,R,128], contiguous).
+    What a cache that takes rows back writes them again from."""
+
+    __slots__ = ("cache", "k", "v", "rows")
+
+    def __init__(self, cache: QuantCache, k, v):
+        self.cache, self.k, self.v, self.rows = cache, k, v, int(k.shape[2]) if k.dim() == 4 else 0
+        for t in (k, v):
+            if tuple(t.shape) != (cache.batch, cache.groups, self.rows, HEAD_DIM) or t.dtype != torch.bfloat16 \
+                    or not t.is_contiguous() or t.device != cache.device or not self.rows:
+                raise ValueError(f"kept rows must be two contiguous bfloat16 [{cache.batch}, {cache.groups}, R, {HEAD_DIM}] "
+                                 f"tensors of R >= 1 on the cache's device")
+
+
+def append_kept(kept: KeptRows, k, v, start: int) -> None:
+    """quantize_append of bfloat16 rows to the kept rows' cache; the last of them are kept too."""
+    cache = kept.cache
+    dtype, T = _check_rows(cache, k, v)
+    if dtype != nat.DT_BF16:
+        raise ValueError(f"rows to keep must be bfloat16, got {k.dtype}")
+    _, at = _start(cache, int(start), T)
+    k, k_at, kb, kg, kt = _rows(k, 8)
+    v, v_at, vb, vg, vt = _rows(v, 8)
+    nat.call_on(cache.device, "attnlab_quant_append_kept", k_at, kb, kg, kt, v_at, vb, vg, vt, cache.k.data_ptr(),
+                cache.v.data_ptr(), cache.k_exp.data_ptr(), cache.v_exp.data_ptr(), at, cache.batch, cache.groups, T,
+                cache.capacity, cache.block, kept.k.data_ptr(), kept.v.data_ptr(), kept.rows, nat.stream_of(cache.device))
 
 
 def dequantize_rows(cache: QuantCache, start=0, length=None, *, dtype=torch.bfloat16):

@@ -26,10 +26,12 @@ How this build arranges it:
 Projections, q_norm / k_norm, RoPE, MLP, norms, embeddings and lm_head are the installed transformers model's. The
 K/V cache must be bfloat16 with head_dim 128 for the kernels (other dtypes raise from the ops); the index table is
 bfloat16, or float32 for a trained bank (trained.py). A token's slot is its absolute position; a rollback shortens the
-legal range and leaves the old suffix in memory where no read or selection reaches it.
+legal range and leaves the old suffix in memory where no read or selection reaches it (in an 8-bit cache it also undoes what
+the suffix did to the block that it began in).
 """
 from __future__ import annotations
 
+import copy
 from dataclasses import dataclass, field
 
 import torch
@@ -40,7 +42,8 @@ from .decode import (gathered_decode_step_kernel, positions_from_flat, select_ro
 from .full import full_attention
 from .hip_range import check_window
 from .indexer import GroupedIndexer, project_keys
-from .quant import BLOCKS, SMALLEST, QuantCache, quant_attention, quant_gather_attention, quantize_append
+from .quant import (BLOCKS, SMALLEST, KeptRows, QuantCache, append_kept, quant_attention, quant_gather_attention,
+                    quantize_append)
 from .selection import FIXED_PREFIX, FIXED_RECENT, fixed_budget, selection_layout
 from .sparse import row_offsets
 from .window import window_attention
@@ -94,13 +97,80 @@ class _AppendLedger:
         return _AppendLedger(self.layers, list(self.writes), list(self.last_write), self.pending)
 
 
+KEEP_BLOCKS = 4   # blocks of an 8-bit cache whose last rows are kept as they came
+
+
+class _Rollback:
+    """What an 8-bit cache needs to take rows back: a block's scale grows for a louder row, and its earlier codes are rounded
+    again, so shortening the legal range alone would leave discarded rows' mark on the rows before them. Kept as they came
+    (bfloat16, in the cache's store): the last `ring` rows written (position p in slot p % ring), and those of the block
+    that the last forward of more than one token ended in (`pin`), where requests are replayed from. A block's codes and
+    scale follow from its rows and where each write began."""
+
+    def __init__(self, block: int, slots: int):
+        self.block = block
+        self.ring = block * min(KEEP_BLOCKS, -(-slots // block))
+        self.lo = 0               # the rows [lo, valid length) are in the ring
+        self.starts: list = []    # where the forwards behind the legal rows began
+        self.pin = (0, 0)         # the positions [a, b) of the pinned rows
+
+    def copy(self) -> "_Rollback":
+        new = copy.copy(self)
+        new.starts = list(self.starts)
+        return new
+
+    def wrote(self, end: int) -> None:
+        """A layer's rows up to `end` went into the ring."""
+        self.lo = max(self.lo, end - self.ring)
+
+    def advance(self, start: int, length: int, store) -> None:
+        """A forward of every layer is done."""
+        end = start + length
+        if length == 0:
+            return
+        self.starts.append(start)
+        a = end - end % self.block
+        if length > 1 and a < end:
+            self.pin = (a, end)
+            for x in "kv":
+                store[x + "_pin"][:, :, :, :end - a].copy_(self.rows(store[x + "_ring"], a, end))
+
+    def rows(self, ring, a: int, b: int):
+        """The ring's rows [a, b) of one block."""
+        at = a % self.ring
+        return ring[:, :, :, at:at + b - a]
+
+    def rollback(self, length: int, store) -> None:
+        """Bring the block that the legal range will end in to what it was at that length."""
+        a = length - length % self.block
+        pinned = self.pin[0] == a and self.pin[1] >= length
+        if a < length and a < self.lo and not pinned:
+            raise ValueError(f"rollback to {length}: an 8-bit cache keeps the rows that the block of {self.block} would need "
+                             f"for its last {self.ring} positions and for the last forward of several tokens; roll back "
+                             f"to {a}, a multiple of the block, and write the rows from there again")
+        if a < length and a < self.lo:
+            for x in "kv":
+                self.rows(store[x + "_ring"], a, length).copy_(store[x + "_pin"][:, :, :, :length - a])
+        self.lo = min(self.lo, a)
+        self.starts = [s for s in self.starts if s < length]
+        self.pin = (a, length) if pinned and a < length else self.pin if self.pin[1] <= length else (0, 0)
+        if a == length:
+            return
+        layers = lambda t: t.view(-1, *t.shape[2:])  # noqa: E731 - every layer's block in one launch a write
+        cache = QuantCache(*(layers(store[n]) for n in ("k", "v", "k_exp", "v_exp")), block=self.block)
+        bounds = [a, *(s for s in self.starts if s > a), length]
+        for b, e in zip(bounds, bounds[1:]):
+            quantize_append(cache, *(layers(self.rows(store[x + "_ring"], b, e)) for x in "kv"), b)
+
+
 class LabCache:
     """Static per-layer K/V [B,G,slots,d] and optional index tables zT [B,G,r,slots] with one legal length for all
     layers (reference qwen_wrap.py:52-139). Allocated with torch.empty: slots at or past valid_length hold whatever the
     memory held (tests poison them) and no read or selection may touch them; slots past `capacity` are padding.
 
     kv_format "e4m3" holds K and V in 8 bits: k[l] and v[l] are codes, quant[l] the layer's QuantCache (its scale bytes
-    for blocks of kv_block positions), and rows are quantised as they are written. `dtype` is then the rows' own."""
+    for blocks of kv_block positions), and rows are quantised as they are written. `dtype` is then the rows' own. The last
+    rows are kept as they came too, for `rollback` (160 KB a layer, request and KV head with blocks of 64)."""
 
     def __init__(self, *, layers: int, batch: int, groups: int, capacity: int, head_dim: int, index_dim=None, device,
                  dtype=torch.float32, index_dtype=None, kv_format: str = "bfloat16", kv_block: int = 64):
@@ -125,6 +195,11 @@ class LabCache:
             exp_shape = (*kv_shape[:3], -(-self.slots // self.kv_block))
             for name in ("k_exp", "v_exp"):
                 self._store[name] = torch.full(exp_shape, SMALLEST, device=self.device, dtype=torch.uint8)
+            self._undo = _Rollback(self.kv_block, self.slots)
+            for name, rows in (("ring", self._undo.ring), ("pin", self.kv_block)):
+                for x in "kv":
+                    self._store[f"{x}_{name}"] = torch.empty(*kv_shape[:3], rows, self.head_dim, device=self.device,
+                                                             dtype=torch.bfloat16)
         if self.index_dim is not None:
             self._store["z"] = torch.empty(self.layers, self.batch, self.groups, self.index_dim, self.slots,
                                            device=self.device, dtype=self.index_dtype)
@@ -146,6 +221,8 @@ class LabCache:
         if self.kv_format == "e4m3":
             self.quant = [QuantCache(k, v, ke, ve, block=self.kv_block) for k, v, ke, ve in
                           zip(self.k, self.v, self._store["k_exp"].unbind(0), self._store["v_exp"].unbind(0))]
+            self._kept = [KeptRows(c, k, v) for c, k, v in
+                          zip(self.quant, self._store["k_ring"].unbind(0), self._store["v_ring"].unbind(0))]
 
     @property
     def has_index(self) -> bool:
@@ -173,10 +250,11 @@ class LabCache:
 
     def write(self, layer: int, start: int, k_main: torch.Tensor, v: torch.Tensor) -> None:
         """K/V rows into the slots [start, start + T) of a layer, in the cache's format."""
-        if self.quant is not None:
-            quantize_append(self.quant[layer], k_main, v, start)
-            return
         T = int(k_main.shape[2])
+        if self.quant is not None:
+            append_kept(self._kept[layer], k_main.to(torch.bfloat16), v.to(torch.bfloat16), start)
+            self._undo.wrote(start + T)
+            return
         self.k[layer][:, :, start:start + T].copy_(k_main)
         self.v[layer][:, :, start:start + T].copy_(v)
 
@@ -193,14 +271,24 @@ class LabCache:
     def advance(self, T: int) -> None:
         """Commit a forward of T tokens once every layer has appended it."""
         self._ledger.commit(int(T))
+        if self.quant is not None:
+            self._undo.advance(self.valid_length, int(T), self._store)
         self.valid_length += int(T)
 
     def rollback(self, length: int) -> None:
-        """Shorten the legal range; the old suffix stays in memory, outside every read and selection."""
+        """Shorten the legal range; the old suffix stays in memory, outside every read and selection.
+
+        An 8-bit cache's last block goes back to the codes and scales it had at that length, as if the discarded rows had
+        never been written. For that it keeps rows as they came: it can be rolled back to any length within KEEP_BLOCKS - 1
+        blocks of the furthest position written, in the block that the last forward of several tokens ended in (up to its
+        end), and to any multiple of kv_block. Another length raises ValueError and changes nothing.
+        """
         if not 0 <= int(length) <= self.valid_length:
             raise ValueError(f"rollback to {length} outside [0, {self.valid_length}]")
         if self._ledger.pending is not None:
             raise RuntimeError("rollback during a forward")
+        if self.quant is not None and int(length) < self.valid_length:
+            self._undo.rollback(int(length), self._store)
         self.valid_length = int(length)
 
     def clone(self) -> "LabCache":
@@ -210,14 +298,17 @@ class LabCache:
         new._store = {name: t.clone() for name, t in self._store.items()}
         new._bind_views()
         new._ledger = self._ledger.copy()
+        if new.quant is not None:
+            new._undo = self._undo.copy()
         return new
 
     def bytes(self) -> dict:
-        """Bytes held (padding slots included)."""
+        """Bytes held (padding slots included); rows kept for a rollback count in the total alone."""
         size = {name: t.numel() * t.element_size() for name, t in self._store.items()}
         z = size.get("z", 0)
-        kv = sum(size.values()) - z
-        return {"kv_bytes": kv, "index_bytes": z, "total_bytes": kv + z}
+        kept = sum(n for name, n in size.items() if name.endswith(("_ring", "_pin")))
+        total = sum(size.values())
+        return {"kv_bytes": total - z - kept, "index_bytes": z, "total_bytes": total}
 
 
 # ---------------------------------------------------------------------------------------------------------------------

@@ -5,7 +5,8 @@
 //   need = the smallest scale with max |finite x in N| <= 448 * scale      scale = O empty ? need : max(old scale, need)
 //   code(x) = RNE_e4m3(x / scale), non-finite x -> NaN                     O's codes move to the new scale if it grew
 // so a block's scale grows only when a louder row arrives, by a power of two, and a row in it is converted once more.
-// Rows of the block from start + T on keep their bytes.
+// Rows of the block from start + T on keep their bytes. A caller that will take rows back keeps the last ones as they came
+// (KEEP): a block's state follows from its rows and where each write began, so writing them again restores it.
 //
 // One workgroup of four waves owns 64 aligned positions of one (b, g) and one tensor, hence whole blocks of 16, 32 or
 // 64: no block is shared, nothing is atomic. Each wave holds its 16 rows in registers (16 bytes a lane and load, a row
@@ -28,6 +29,8 @@ struct AppendArgs {
     uint8_t* exps[2];                 // [B, G, nb]
     const int32_t* starts;            // one per sequence, or null: `start`
     int start, G, T, C, shift, nb, spans;
+    uint16_t* keep[2];                // [B, G, ring, 128] bf16: the rows as they came, position p in slot p % ring (KEEP)
+    int ring;
 };
 
 // Eight elements of a row as floats.
@@ -57,7 +60,12 @@ __device__ __forceinline__ void load8(const void* base, int64_t off, float (&v)[
     }
 }
 
-template <int DT>
+// Two floats that are bf16 numbers as a packed pair.
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    return __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xffff0000u);
+}
+
+template <int DT, bool KEEP>
 __global__ __launch_bounds__(256) void quant_append(AppendArgs a) {
     __shared__ float top_sh[4];
     const int side = blockIdx.x & 1;                   // K, V
@@ -114,6 +122,12 @@ __global__ __launch_bounds__(256) void quant_append(AppendArgs a) {
     for (int u = 0; u < 4; ++u) {
         if (!fresh[u]) continue;
         const int64_t pos = span0 + 16 * wave + 4 * u + (lane >> 4);
+        if constexpr (KEEP) {   // of rows that share a slot, the last
+            if (pos >= end - a.ring)
+                *reinterpret_cast<u32x4_t*>(a.keep[side] + ((int64_t)bg * a.ring + pos % a.ring) * kDim + 8 * chunk) =
+                    u32x4_t{bf16_pair(v[u][0], v[u][1]), bf16_pair(v[u][2], v[u][3]), bf16_pair(v[u][4], v[u][5]),
+                            bf16_pair(v[u][6], v[u][7])};
+        }
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {   // an infinity stays one (it becomes a NaN code), a finite value saturates
@@ -211,11 +225,13 @@ int check_quant_cache(const void* k_codes, const void* v_codes, const void* k_ex
 
 using namespace attnlab;
 
-extern "C" int attnlab_quant_append(const void* k, int64_t k_b_stride, int64_t k_g_stride, int64_t k_t_stride,
-                                    const void* v, int64_t v_b_stride, int64_t v_g_stride, int64_t v_t_stride,
-                                    int dtype, uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_exp, uint8_t* v_exp,
-                                    const int32_t* starts, int start, int B, int G, int T, int C, int block,
-                                    void* stream) {
+namespace {
+
+// keep_rows 0: no rows are kept.
+int run_append(const void* k, int64_t k_b_stride, int64_t k_g_stride, int64_t k_t_stride, const void* v,
+               int64_t v_b_stride, int64_t v_g_stride, int64_t v_t_stride, int dtype, uint8_t* k_codes, uint8_t* v_codes,
+               uint8_t* k_exp, uint8_t* v_exp, const int32_t* starts, int start, int B, int G, int T, int C, int block,
+               uint16_t* k_keep, uint16_t* v_keep, int keep_rows, void* stream) {
     const int rc = check_quant_cache(k_codes, v_codes, k_exp, v_exp, B, G, C, block);
     if (rc) return rc;
     ATTNLAB_REQUIRE(dtype == ATTNLAB_DT_BF16 || dtype == ATTNLAB_DT_F16 || dtype == ATTNLAB_DT_F32,
@@ -230,7 +246,8 @@ extern "C" int attnlab_quant_append(const void* k, int64_t k_b_stride, int64_t k
                                                          v_g_stride | v_t_stride) % step == 0,
                     "the rows of k and v must be 16-byte aligned");
     AppendArgs a{{k, v}, {k_b_stride, v_b_stride}, {k_g_stride, v_g_stride}, {k_t_stride, v_t_stride},
-                 {k_codes, v_codes}, {k_exp, v_exp}, starts, start, G, T, C, block_shift(block), 0, 0};
+                 {k_codes, v_codes}, {k_exp, v_exp}, starts, start, G, T, C, block_shift(block), 0, 0,
+                 {k_keep, v_keep}, keep_rows};
     a.nb = (C + block - 1) / block;
     // aligned spans that T rows touch: at any start, or at the one given
     a.spans = starts ? (int)(((int64_t)T + 62) / kSpan + 1) : (start + T - 1) / kSpan - start / kSpan + 1;
@@ -238,10 +255,33 @@ extern "C" int attnlab_quant_append(const void* k, int64_t k_b_stride, int64_t k
     ATTNLAB_REQUIRE(blocks < (int64_t)1 << 31, "grid of %lld workgroups is too large", (long long)blocks);
     const dim3 grid((unsigned)blocks), wg(256);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    if (dtype == ATTNLAB_DT_BF16) hipLaunchKernelGGL(quant_append<ATTNLAB_DT_BF16>, grid, wg, 0, s, a);
-    else if (dtype == ATTNLAB_DT_F16) hipLaunchKernelGGL(quant_append<ATTNLAB_DT_F16>, grid, wg, 0, s, a);
-    else hipLaunchKernelGGL(quant_append<ATTNLAB_DT_F32>, grid, wg, 0, s, a);
+    if (keep_rows) hipLaunchKernelGGL((quant_append<ATTNLAB_DT_BF16, true>), grid, wg, 0, s, a);
+    else if (dtype == ATTNLAB_DT_BF16) hipLaunchKernelGGL((quant_append<ATTNLAB_DT_BF16, false>), grid, wg, 0, s, a);
+    else if (dtype == ATTNLAB_DT_F16) hipLaunchKernelGGL((quant_append<ATTNLAB_DT_F16, false>), grid, wg, 0, s, a);
+    else hipLaunchKernelGGL((quant_append<ATTNLAB_DT_F32, false>), grid, wg, 0, s, a);
     return check_launch("quant_append");
+}
+
+}  // namespace
+
+extern "C" int attnlab_quant_append(const void* k, int64_t k_b_stride, int64_t k_g_stride, int64_t k_t_stride,
+                                    const void* v, int64_t v_b_stride, int64_t v_g_stride, int64_t v_t_stride,
+                                    int dtype, uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_exp, uint8_t* v_exp,
+                                    const int32_t* starts, int start, int B, int G, int T, int C, int block,
+                                    void* stream) {
+    return run_append(k, k_b_stride, k_g_stride, k_t_stride, v, v_b_stride, v_g_stride, v_t_stride, dtype, k_codes, v_codes,
+                      k_exp, v_exp, starts, start, B, G, T, C, block, nullptr, nullptr, 0, stream);
+}
+
+extern "C" int attnlab_quant_append_kept(const uint16_t* k, int64_t k_b_stride, int64_t k_g_stride, int64_t k_t_stride,
+                                         const uint16_t* v, int64_t v_b_stride, int64_t v_g_stride, int64_t v_t_stride,
+                                         uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_exp, uint8_t* v_exp, int start,
+                                         int B, int G, int T, int C, int block, uint16_t* k_keep, uint16_t* v_keep,
+                                         int keep_rows, void* stream) {
+    ATTNLAB_REQUIRE(keep_rows >= 1 && k_keep && v_keep && aligned(k_keep, 16) && aligned(v_keep, 16),
+                    "the kept rows (%d) must be 16-byte aligned device buffers of at least one row", keep_rows);
+    return run_append(k, k_b_stride, k_g_stride, k_t_stride, v, v_b_stride, v_g_stride, v_t_stride, ATTNLAB_DT_BF16, k_codes,
+                      v_codes, k_exp, v_exp, nullptr, start, B, G, T, C, block, k_keep, v_keep, keep_rows, stream);
 }
 
 extern "C" int attnlab_quant_read(const uint8_t* k_codes, const uint8_t* v_codes, const uint8_t* k_exp,

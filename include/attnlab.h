@@ -324,6 +324,17 @@ int attnlab_quant_append(const void* k, int64_t k_b_stride, int64_t k_g_stride, 
                          int G, int T, int C, int block, void* stream);
 
 /*
+ * attnlab_quant_append of bf16 rows at one start that also keeps the last of them as they came: position p's row in slot
+ * p % keep_rows of k_keep, v_keep [B, G, keep_rows, 128] bf16 (16-byte aligned), for p >= start + T - keep_rows. A block's
+ * codes and scale follow from its rows and the starts of the writes that brought them, so appending the kept rows again,
+ * write by write from the block's first position, undoes what later rows did to it.
+ */
+int attnlab_quant_append_kept(const uint16_t* k, int64_t k_b_stride, int64_t k_g_stride, int64_t k_t_stride,
+                              const uint16_t* v, int64_t v_b_stride, int64_t v_g_stride, int64_t v_t_stride,
+                              uint8_t* k_codes, uint8_t* v_codes, uint8_t* k_exp, uint8_t* v_exp, int start, int B, int G,
+                              int T, int C, int block, uint16_t* k_keep, uint16_t* v_keep, int keep_rows, void* stream);
+
+/*
  * Reads T rows of an 8-bit cache back as values: k_out, v_out [B, G, T, 128] in `dtype` (bf16 and fp32 exact, fp16
  * rounded to nearest even), from start, or starts[b]; with `starts`, positions outside [0, C) give zeros.
  */

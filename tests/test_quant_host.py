@@ -242,3 +242,17 @@ def test_steps_that_share_a_stream_take_turns(monkeypatch):
         if shared:
             assert all(a[0] == "score" and b[0] == "select" and a[1] == b[1] for a, b in zip(events[::2], events[1::2]))
     assert isinstance(decode._step_workspace(cache.device, object())[1], contextlib.nullcontext)
+
+
+KEPT = dict(k=16, kb=1024, kg=256, kt=128, v=16, vb=1024, vg=256, vt=128, kc=16, vc=16, ke=16, ve=16, start=0, B=1, G=2,
+            T=4, C=64, block=16, kk=16, vk=16, rows=32, stream=None)
+
+
+@pytest.mark.parametrize("change,match", [(dict(kk=None), "kept rows"), (dict(vk=8), "kept rows"), (dict(rows=0), "kept rows"),
+                                          (dict(start=61), "outside"), (dict(start=-1), "outside"), (dict(k=8), "aligned"),
+                                          (dict(T=-1), "negative"), (dict(block=8), "block")])
+def test_kept_rows_refused_before_any_launch(native_lib, change, match):
+    assert len(KEPT) == len(_native.SIGNATURES["attnlab_quant_append_kept"][1])
+    with pytest.raises(ValueError, match=match):
+        _native.call("attnlab_quant_append_kept", *dict(KEPT, **change).values())
+    _native.call("attnlab_quant_append_kept", *dict(KEPT, T=0).values())
