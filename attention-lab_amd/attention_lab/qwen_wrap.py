@@ -40,7 +40,8 @@ from torch import nn
 from .decode import (gathered_decode_step_kernel, positions_from_flat, select_rows_recent, select_rows_uniform,
                      sparse_decode_step_kernel, sparse_decode_step_quant, tag_standard_f)
 from .full import full_attention
-from .hip_range import check_window
+from .hip_attend import HEAD_DIM
+from .hip_range import MAX_H, MAX_H_CHUNK, check_window
 from .indexer import GroupedIndexer, project_keys
 from .quant import (BLOCKS, SMALLEST, KeptRows, QuantCache, append_kept, quant_attention, quant_gather_attention,
                     quantize_append)
@@ -180,6 +181,8 @@ class LabCache:
             raise ValueError(f"kv_format must be one of {KV_FORMATS}")
         if kv_format == "e4m3" and kv_block not in BLOCKS:
             raise ValueError(f"kv_block must be one of {BLOCKS}, got {kv_block!r}")
+        if kv_format == "e4m3" and (dtype != torch.bfloat16 or int(head_dim) != HEAD_DIM):
+            raise ValueError(f"kv_format 'e4m3' holds bfloat16 rows of head_dim {HEAD_DIM}, got {dtype} and {head_dim}")
         self.kv_format, self.kv_block = kv_format, int(kv_block)
         self.layers, self.batch, self.groups = int(layers), int(batch), int(groups)
         self.capacity, self.head_dim = int(capacity), int(head_dim)
@@ -434,6 +437,14 @@ _SELECTOR_IMPL = {"index": _IndexSelector, "recent": _RecentSelector, "uniform":
 # ---------------------------------------------------------------------------------------------------------------------
 # state
 # ---------------------------------------------------------------------------------------------------------------------
+def _head_problems(h: int, mode: str, kv_format: str) -> list:
+    """What keeps h query heads per KV group from the reads of a configuration."""
+    most = MAX_H if mode == "sparse" and kv_format == "e4m3" else MAX_H_CHUNK
+    if h <= most or (mode != "window" and kv_format != "e4m3"):
+        return []
+    return [f"mode {mode!r} over a {kv_format} cache takes at most {most} query heads per KV group, got {h}"]
+
+
 def _read_config_layers(cache: LabCache, indexers, mode: str, selector: str, sparse_layers, window):
     """Validate a read configuration against its cache and return the sparse layer set (None: every layer). The
     messages are the contract's; this function's own rule is that a configuration is checked in full before any state
@@ -443,12 +454,16 @@ def _read_config_layers(cache: LabCache, indexers, mode: str, selector: str, spa
         problems.append(f"mode must be one of {MODES}")
     elif (mode == "window") != (window is not None):
         problems.append("mode 'window' goes with a window, and a window with it")
+    elif mode == "window" and (cache.dtype != torch.bfloat16 or cache.head_dim != HEAD_DIM):
+        problems.append(f"mode 'window' reads a cache of bfloat16 rows of head_dim {HEAD_DIM}")
     if selector not in SELECTORS:
         problems.append(f"selector must be one of {SELECTORS}")
     if indexers is not None and len(indexers) != cache.layers:
         problems.append("one indexer per layer")
     if not problems and mode == "sparse" and selector == "index" and (indexers is None or not cache.has_index):
         problems.append("the index selector (D0) needs indexers and a cache with an index table")
+    if not problems and indexers and (mode == "window" or cache.kv_format == "e4m3"):
+        problems += _head_problems(indexers[0].wq_t_scaled.shape[1] // cache.head_dim, mode, cache.kv_format)
     layers = None
     if sparse_layers is not None:
         layers = frozenset(int(x) for x in sparse_layers)
@@ -702,6 +717,8 @@ def make_state(model, capacity: int, mode: str, *, selector: str = "index", r: i
     """A: mode "full". D0: mode "sparse" with the index selector (index table and indexers). B / C: mode "sparse" with
     selector "recent" / "uniform" (neither an index table nor indexers). A sliding window: mode "window" with window=
     and sinks=. kv_format "e4m3": the same reads over an 8-bit cache."""
+    for problem in _head_problems(geometry_of(model).heads_per_group, mode, kv_format):
+        raise ValueError(problem)
     indexed = mode == "sparse" and selector == "index"
     cache = make_cache(model, capacity, with_index=indexed, index_dim=r, batch=batch, kv_format=kv_format,
                        kv_block=kv_block)

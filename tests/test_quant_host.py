@@ -256,3 +256,35 @@ def test_kept_rows_refused_before_any_launch(native_lib, change, match):
     with pytest.raises(ValueError, match=match):
         _native.call("attnlab_quant_append_kept", *dict(KEPT, **change).values())
     _native.call("attnlab_quant_append_kept", *dict(KEPT, T=0).values())
+
+
+def test_configurations_the_reads_do_not_take_are_refused_before_a_state_is_built():
+    """At construction, and not in the first layer's read, which comes after its rows were written."""
+    pytest.importorskip("transformers")
+    from types import SimpleNamespace
+    from attention_lab.qwen_wrap import LabCache, LabState, make_state, tiny_qwen3
+    size = dict(layers=1, batch=1, groups=2, capacity=64, device="cpu")
+    for kw in (dict(head_dim=128, dtype=torch.float32), dict(head_dim=128, dtype=torch.float16), dict(head_dim=128),
+               dict(head_dim=64, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="bfloat16 rows of head_dim 128"):
+            LabCache(**size, kv_format="e4m3", **{"dtype": torch.float32, **kw})
+    for kw in (dict(head_dim=128, dtype=torch.float32), dict(head_dim=64, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="bfloat16 rows of head_dim 128"):
+            LabState(LabCache(**size, **kw), mode="window", window=8)
+    LabState(LabCache(**size, head_dim=128, dtype=torch.bfloat16), mode="window", window=8)
+
+    def model(h, groups=1):
+        return tiny_qwen3(seed=0, layers=1, hidden=64, heads=h * groups, groups=groups, head_dim=128, intermediate=64,
+                          vocab=32, dtype=torch.bfloat16)
+
+    for h, mode, kw, most in ((9, "sparse", dict(kv_format="e4m3"), 8), (17, "full", dict(kv_format="e4m3"), 16),
+                              (9, "sparse", dict(kv_format="e4m3", selector="recent"), 8), (17, "window", dict(window=4), 16)):
+        with pytest.raises(ValueError, match=f"at most {most} query heads"):
+            make_state(model(h), 64, mode, **kw)
+    make_state(model(16), 64, "window", window=4)
+    make_state(model(17), 64, "full")
+    cache = SimpleNamespace(layers=1, dtype=torch.bfloat16, head_dim=128, kv_format="e4m3", has_index=True)
+    index = SimpleNamespace(wq_t_scaled=torch.zeros(2, 9 * 128, 32))
+    with pytest.raises(ValueError, match="at most 8 query heads"):
+        LabState(cache, [index], mode="sparse")
+    LabState(cache, [index], mode="full")
