@@ -8,8 +8,8 @@ import threading
 import pytest
 import torch
 
-from attention_lab import QuantCache, prepare_request, sparse_decode_step_quant
-from attention_lab import _native, decode, hip_score, hip_select
+from attention_lab import QuantCache, prepare_request, quant_attention, sparse_decode_step_quant
+from attention_lab import _native, decode, hip_range, hip_score, hip_select
 from attention_lab.indexer import GroupedIndexer
 
 pytestmark = pytest.mark.gpu
@@ -170,3 +170,58 @@ def test_a_table_elsewhere_is_refused(gpu):
     step.z = step.z.cpu()
     with pytest.raises(ValueError, match="device"):
         step()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the reads' counters and partials of a stream, to their ends
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("B,G,h,partitions", [
+    (16, 4, 8, 16), (hip_range.COUNTERS // 2, 2, 1, 2), (hip_range.COUNTERS // 4, 4, 2, 1), (16, 4, 8, 15),
+    (hip_range.COUNTERS // 2 + 1, 2, 1, 2), (43, 3, 4, 16)])
+def test_reads_that_fill_the_shared_counters_and_partials(gpu, B, G, h, partitions):
+    """At the last counter, at the partials' last row, and past either: the outputs of reads that are not split, and the same
+    bits call after call."""
+    rows, C = B * G * h * partitions, 300
+    shared = partitions > 1 and B * G <= hip_range.COUNTERS and rows <= hip_range.PARTIALS
+    device, stream = torch.device(gpu), torch.cuda.current_stream().cuda_stream
+    assert (hip_range._split_k(partitions, B * G, h, device, stream, True)[2] is not None) == shared
+    g = torch.Generator(device=gpu).manual_seed(B)
+    codes = lambda: (torch.randint(0, 255, (B, G, C, D), generator=g, device=gpu) % 0x50).to(torch.uint8)  # noqa: E731
+    exps = torch.full((B, G, -(-C // 32)), 122, dtype=torch.uint8, device=gpu)
+    cache = QuantCache(codes().view(torch.float8_e4m3fn), codes().view(torch.float8_e4m3fn), exps, exps, block=32)
+    q = torch.randn(B, G, h, 1, D, generator=g, device=gpu).to(torch.bfloat16)
+    read = lambda P: quant_attention(q, cache, out_dtype=torch.float32, partitions=P)  # noqa: E731
+    whole, first = read(1), read(partitions)
+    # values of one sign, so an output is its own sum of magnitudes; scores below 2^3 in the log2 domain, so either side's
+    # weights are good to 2^-16 + 16 * 2^-20 + 2^-22 and its sums to 2^-17: 2.6 * 2^-16, twice for weights and their sum
+    assert bool(((whole - first).abs() <= 2 * 2 * 2.6 * 2.0 ** -16 * whole.abs()).all())
+    for _ in range(3):
+        assert torch.equal(read(partitions), first)
+    buf = hip_range._MERGES.get((device.index, stream))
+    assert buf is None or not buf[:hip_range.COUNTERS].any()
+
+
+def test_eager_reads_on_two_streams_use_their_own_counters(gpu):
+    """Merges by the last workgroup to arrive, on two streams at once."""
+    B, h, C, P = 1, 4, 6000, 8
+    device, g = torch.device(gpu), torch.Generator(device=gpu).manual_seed(1)
+    codes = (torch.randint(0, 255, (B, G, C, D), generator=g, device=gpu) % 0x50).to(torch.uint8).view(torch.float8_e4m3fn)
+    exps = torch.full((B, G, -(-C // 64)), 122, dtype=torch.uint8, device=gpu)
+    cache = QuantCache(codes, codes, exps, exps)
+    qs = [torch.randn(B, G, h, 1, D, generator=g, device=gpu).to(torch.bfloat16) for _ in range(2)]
+    want = [quant_attention(q, cache, partitions=P) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    counters = set()
+    for s in streams:
+        with torch.cuda.stream(s):
+            counters.add(hip_range._split_k(P, B * G, h, device, s.cuda_stream, True)[2])
+    assert None not in counters and len(counters) == 2
+    for _ in range(5):
+        got = []
+        for s, q in zip(streams, qs):
+            with torch.cuda.stream(s):
+                got.append([quant_attention(q, cache, partitions=P) for _ in range(4)])
+        torch.cuda.synchronize()
+        for g4, w in zip(got, want):
+            assert all(torch.equal(x, w) for x in g4)
