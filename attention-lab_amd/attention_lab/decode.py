@@ -303,7 +303,27 @@ def sparse_decode_step_kernel(q_main, q_pre, k_cache, v_cache, zT, wq_t_scaled, 
 
 # Select state and scratch of sparse_decode_step_quant: the score launch adds into the state and the select launch takes it
 # out again, so both belong to one stream, and no other thread's launches on it may come between them.
-_QUANT_WS: dict = {}      # (device index, stream) -> (Workspace, lock)
+_QUANT_WS: dict = {}      # (device index, stream) -> _StreamScratch
+
+
+def _select_state(buf, B: int, G: int):
+    """The select state of B * G rows in a workspace's bytes."""
+    return buf[:B * G * nat.SELECT_STATE_WORDS * 4].view(torch.int32).view(B, G, nat.SELECT_STATE_WORDS)
+
+
+class _StreamScratch(nat.Workspace):
+    """A stream's workspace, its lock and the views of its state (3 us to build)."""
+
+    def __init__(self):
+        super().__init__()
+        self.lock, self._states = threading.Lock(), {}
+
+    def state(self, device, B: int, G: int):
+        buf = self.bytes(device, B * G * nat.SELECT_STATE_WORDS * 4, "state")
+        held = self._states.get((B, G))
+        if held is None or held[0] is not buf:   # a larger call's buffer has replaced it
+            held = self._states[B, G] = (buf, _select_state(buf, B, G))
+        return held[1]
 
 
 class _GraphScratch:
@@ -322,7 +342,9 @@ def _step_workspace(device, workspace):
         return _GraphScratch, contextlib.nullcontext()
     key = (device.index, nat.stream_of(device))
     held = _QUANT_WS.get(key)
-    return _QUANT_WS.setdefault(key, (nat.Workspace(), threading.Lock())) if held is None else held
+    if held is None:
+        held = _QUANT_WS.setdefault(key, _StreamScratch())
+    return held, held.lock
 
 
 def sparse_decode_step_quant(q_main, q_pre, cache, zT, wq_t_scaled, wk, fixed_rows, off_lo, lo: int, hi: int, k: int,
@@ -334,7 +356,8 @@ def sparse_decode_step_quant(q_main, q_pre, cache, zT, wq_t_scaled, wk, fixed_ro
 
     workspace: None, or a _native.Workspace for the select state and scratch, whose calls must follow one another on one
     stream. By default every stream has its own, threads that share a stream take turns, and a captured call's belongs to
-    its graph, so steps on other streams, in other threads and graphs share nothing.
+    its graph, so steps on other streams, in other threads and graphs share nothing; a replay then zeroes the state of every
+    captured step first (2 us each on MI355X, which a workspace spares).
     """
     B, G, h, T, d = q_main.shape
     if T != 1:
@@ -368,11 +391,11 @@ def sparse_decode_step_quant(q_main, q_pre, cache, zT, wq_t_scaled, wk, fixed_ro
         flat = fixed_rows.reshape(-1)
         pos = positions_from_flat(flat, B, G, S, C, cache.device)
     else:
-        nb = B * G * nat.SELECT_STATE_WORDS * 4
         order = _order(canonical_order or not return_rows)   # the order shows only in rows that leave the call
         wsp, lock = _step_workspace(cache.device, workspace)
         with lock:
-            state = wsp.bytes(cache.device, nb, "state")[:nb].view(torch.int32).view(B, G, -1)
+            state = wsp.state(cache.device, B, G) if type(wsp) is _StreamScratch else \
+                _select_state(wsp.bytes(cache.device, B * G * nat.SELECT_STATE_WORDS * 4, "state"), B, G)
             scratch = hip_select.reserve(cache.device, B * G, hi - lo, k, order, wsp)
             rows = torch.empty(B, G, S, dtype=torch.int32, device=cache.device)
             try:
