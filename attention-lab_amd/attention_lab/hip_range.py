@@ -6,7 +6,8 @@ check their caches; this module checks what the reads share, chooses the split c
 device and torch's current stream of it.
 
 The last workgroup of a (b, g) to arrive merges its split-K partials where a counter tells it that it is: the counters
-and partials of such single launches belong to a stream, whose launches follow one another and leave the counters zero.
+and partials of such single launches belong to a stream (4.3 MB each, held for the process's life), whose launches follow one
+another and leave the counters zero.
 Other calls, a captured one among them, allocate partials of their own and take a second launch for the merge (the same
 sums), so a graph shares nothing with other graphs or calls.
 """

@@ -21,8 +21,9 @@ def window_attention(q, k, v, *, window, sinks: int = FIXED_PREFIX, valid_length
     every legal position. Sums are fp32 under weights of at most 1: n rows of values below 2^128 / n have finite outputs.
     valid_length: an int (default: the capacity), or for one query an int32 [B] device tensor
     with each sequence's length, clamped to [0, C], its query at the last position. A query that reads no position
-    gets zeros. One query takes h <= 8 at every form and out_dtype float32 too; a chunk, and one query with h <= 16 and
-    an int length, gives bfloat16. partitions overrides the split-K count (one query: 1..256, a chunk: 1..16).
+    gets zeros. One query takes h <= 8 at every form and out_dtype float32 too, with weights of 16 bits; a chunk, and one
+    query with h <= 16 and an int length, gives bfloat16, and rounds its weights to bfloat16 before their product with V (2^-8
+    of each at most; their sum is not rounded). partitions overrides the split-K count (one query: 1..256, a chunk: 1..16).
     """
     if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.dtype != torch.bfloat16 or not k.is_contiguous() or not k.is_cuda:
         raise ValueError(f"the cache must be a contiguous bfloat16 [B, G, C, {HEAD_DIM}] tensor on a HIP device")

@@ -15,16 +15,15 @@
 // rounding left, and the two are added at the end, so the weights keep 16 bits without a second product. Softmax is
 // online in the log2 domain; a row's shift m is set 2^8 above its largest score so far and moves, with the sums rescaled,
 // only when a score passes it, so most tiles need no exchange between lanes and no weight is above 1: n rows of values
-// below 2^128 / n have finite sums, as with the exact maximum. Sums and outputs are fp32. The waves of a workgroup merge through LDS, the P
-// workgroups of a (b, g) through partials: the last to arrive merges them in split order, or, without counters, a second
-// small launch does, with the same sums.
+// below 2^128 / n have finite sums, as with the exact maximum. Sums and outputs are fp32. The waves of a workgroup merge
+// through LDS, the P workgroups of a (b, g) through partials: the last to arrive merges them in split order, or, without
+// counters, a second small launch does, with the same sums.
 //
-// What bounds it: the bytes of the rows. A CU streams about 26 GB/s whatever the number of its waves or loads in flight
-// (6.7 TB/s over 256), which 16 requests of 32K (8 groups, h=4) reach: 8-bit 158 us, 6.8 TB/s. Eight 128K caches with a
-// window of 4096 over bf16: 25.6 us, 5.2 TB/s; five of 5K to 20K (h=8): 29.5 us; 1092 listed rows of 16 requests: 14.1 us,
-// 2.6 TB/s of rows apart; one request of 2K: 8 us, the latencies of a launch (5.2 with one tile a wave and nothing to merge)
-// and of the merge. Ranges take three waves a SIMD with one tile each over two with two, and four waves a workgroup over
-// eight or sixteen.
+// What bounds it: the bytes of the rows. A kernel of as many workgroups that only reads a large buffer reaches 7.1 TB/s; 16
+// requests of 32K (8 groups, h=4), 8-bit, take 158 us: 6.8 TB/s. Eight 128K caches with a window of 4096 over bf16: 25.6 us,
+// 5.2 TB/s; five of 5K to 20K (h=8): 29.5 us, 4.4; 1092 listed rows of 16 requests: 14.1 us, 2.6 TB/s of rows apart; one
+// request of 2K: 8 us, the latencies of a launch (5.2 with one tile a wave and nothing to merge) and of the merge. Ranges take
+// three waves a SIMD with one tile each over two with two, and four waves a workgroup over eight or sixteen.
 //
 // Masked rows: their scores are replaced, and their V rows are zeros of scale 1, so whatever they and their scale bytes hold
 // (NaN, infinity) leaves the output alone. A query with no row to read, or whose scores are all -inf, gets zeros.

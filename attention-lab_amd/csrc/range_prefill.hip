@@ -9,14 +9,21 @@
 // block; an 8-bit operand becomes bf16 (exactly, its scale included) as it is read, which costs each wave 128 conversions
 // a block and halves what it reads from LDS.
 //
+// The weights are rounded to bf16, the operand's type, before their product with V; their sum is of the unrounded ones.
+// Outputs are off the 64-bit ones by 0.0023 of them (root mean square), where rounding the output alone costs 0.0016. The
+// one-query kernel's weights of two parts would be half as many products again.
+//
 // What bounds it: the matrix cores are busy 50 % of the time at about 2.1 GHz, the vector units 60 % with the softmax and
 // the conversions; LDS reads wait between (without them the kernel took 320 us where it took 535, without the copies 428).
-// An 8K prompt (8 groups, h=4; 0.55 TFLOP) takes 509 us over bf16 (1.08 PFLOP/s) and 516 over 8 bits, where tiles
+// An 8K prompt (8 groups, h=4; 0.55 TFLOP) takes 509 us over bf16 (1.08 PFLOP/s) and 510 to 520 over 8 bits, where tiles
 // widened on their way into LDS took 562. 1000 queries after 29011 (h=2), 8-bit: 246 us (0.98 PFLOP/s); 1501 queries,
-// window 2047, 8-bit: 75; two 8K prompts (h=4) with a window of 1024 over bf16: 308. A wave with 64 rows halves the reads
-// per product and holds too many registers (632 us and 828); eight waves over 256 rows take 493 us over bf16, 540 over 8 bits
-// and 311 under the window, and are coarser on short prompts; equal runs of all tiles' blocks for each workgroup balance the chip and write twice the partials
-// (86 us for 76 under the window); a wave's priority, half blocks or V read ahead gave nothing.
+// window 2047, 8-bit: 74; two 8K prompts (h=4) with a window of 1024 over bf16: 310. There 4096 workgroups take 80 us apart
+// from their blocks (eight rounds of 10: Q, the first copies with nothing to hide behind, the output) and 14 us for each
+// block: windows of 64, 512, 1024, 2048 and 4096 take 117, 204, 312, 489 and 779 us, none 995. A wave with 64 rows
+// halves the reads per product and holds too many registers (632 us and 828); eight waves over 256 rows take 493 us over
+// bf16, 540 over 8 bits and 311 under the window, and are coarser on short prompts; equal runs of all tiles' blocks for each
+// workgroup balance the chip and write twice the partials (86 us for 76 under the window); a wave's priority, half blocks
+// or V read ahead gave nothing.
 //
 // A masked key has weight zero, but zero times a V row that holds NaN or infinity is NaN. Rows past the visible range are
 // copied as zeros; inside it a key can be masked for one row and visible to the next. So a workgroup with a result that is
