@@ -105,8 +105,8 @@ class _Rollback:
     """What an 8-bit cache needs to take rows back: a block's scale grows for a louder row, and its earlier codes are rounded
     again, so shortening the legal range alone would leave discarded rows' mark on the rows before them. Kept as they came
     (bfloat16, in the cache's store): the last `ring` rows written (position p in slot p % ring), and those of the block
-    that the last forward of more than one token ended in (`pin`), where requests are replayed from. A block's codes and
-    scale follow from its rows and where each write began."""
+    that a prompt's last chunk ended in (`pin`), where requests are replayed from. A block's codes and scale follow from its
+    rows and where each write began."""
 
     def __init__(self, block: int, slots: int):
         self.block = block
@@ -114,6 +114,7 @@ class _Rollback:
         self.lo = 0               # the rows [lo, valid length) are in the ring
         self.starts: list = []    # where the forwards behind the legal rows began
         self.pin = (0, 0)         # the positions [a, b) of the pinned rows
+        self.chunk_end = 0        # the end of a forward of several tokens, or the beginning: one token there may end a prompt
 
     def copy(self) -> "_Rollback":
         new = copy.copy(self)
@@ -124,44 +125,46 @@ class _Rollback:
         """A layer's rows up to `end` went into the ring."""
         self.lo = max(self.lo, end - self.ring)
 
+    @torch.inference_mode()       # the store may be of inference tensors, whichever mode it is written in
     def advance(self, start: int, length: int, store) -> None:
         """A forward of every layer is done."""
-        end = start + length
         if length == 0:
             return
+        end = start + length
         self.starts.append(start)
         a = end - end % self.block
-        if length > 1 and a < end:
+        if (length > 1 or start == self.chunk_end) and a < end:
             self.pin = (a, end)
             for x in "kv":
                 store[x + "_pin"][:, :, :, :end - a].copy_(self.rows(store[x + "_ring"], a, end))
+        self.chunk_end = end if length > 1 else -1
 
     def rows(self, ring, a: int, b: int):
         """The ring's rows [a, b) of one block."""
         at = a % self.ring
         return ring[:, :, :, at:at + b - a]
 
+    @torch.inference_mode()
     def rollback(self, length: int, store) -> None:
         """Bring the block that the legal range will end in to what it was at that length."""
         a = length - length % self.block
-        pinned = self.pin[0] == a and self.pin[1] >= length
-        if a < length and a < self.lo and not pinned:
+        pinned = self.pin[0] == a < length <= self.pin[1]
+        if a < min(length, self.lo) and not pinned:
             raise ValueError(f"rollback to {length}: an 8-bit cache keeps the rows that the block of {self.block} would need "
-                             f"for its last {self.ring} positions and for the last forward of several tokens; roll back "
-                             f"to {a}, a multiple of the block, and write the rows from there again")
-        if a < length and a < self.lo:
-            for x in "kv":
-                self.rows(store[x + "_ring"], a, length).copy_(store[x + "_pin"][:, :, :, :length - a])
-        self.lo = min(self.lo, a)
-        self.starts = [s for s in self.starts if s < length]
-        self.pin = (a, length) if pinned and a < length else self.pin if self.pin[1] <= length else (0, 0)
-        if a == length:
-            return
-        layers = lambda t: t.view(-1, *t.shape[2:])  # noqa: E731 - every layer's block in one launch a write
-        cache = QuantCache(*(layers(store[n]) for n in ("k", "v", "k_exp", "v_exp")), block=self.block)
-        bounds = [a, *(s for s in self.starts if s > a), length]
-        for b, e in zip(bounds, bounds[1:]):
-            quantize_append(cache, *(layers(self.rows(store[x + "_ring"], b, e)) for x in "kv"), b)
+                             f"for its last {self.ring} positions and for the last prompt's end; roll back to {a}, a "
+                             f"multiple of the block, and write the rows from there again")
+        starts = [s for s in self.starts if s < length]
+        if a < length:
+            if a < self.lo:
+                for x in "kv":
+                    self.rows(store[x + "_ring"], a, length).copy_(store[x + "_pin"][:, :, :, :length - a])
+            layers = lambda t: t.view(-1, *t.shape[2:])  # noqa: E731 - every layer's block in one launch a write
+            cache = QuantCache(*(layers(store[n]) for n in ("k", "v", "k_exp", "v_exp")), block=self.block)
+            bounds = [a, *(s for s in starts if s > a), length]
+            for b, e in zip(bounds, bounds[1:]):
+                quantize_append(cache, *(layers(self.rows(store[x + "_ring"], b, e)) for x in "kv"), b)
+        self.pin = (a, length) if pinned else self.pin if self.pin[1] <= length else (0, 0)
+        self.lo, self.starts, self.chunk_end = min(self.lo, a), starts, 0 if length == 0 else -1
 
 
 class LabCache:
@@ -284,7 +287,8 @@ class LabCache:
         An 8-bit cache's last block goes back to the codes and scales it had at that length, as if the discarded rows had
         never been written. For that it keeps rows as they came: it can be rolled back to any length within KEEP_BLOCKS - 1
         blocks of the furthest position written, in the block that the last forward of several tokens ended in (up to its
-        end), and to any multiple of kv_block. Another length raises ValueError and changes nothing.
+        end, or that of a single token right behind it), and to any multiple of kv_block. Another length raises ValueError and
+        changes nothing.
         """
         if not 0 <= int(length) <= self.valid_length:
             raise ValueError(f"rollback to {length} outside [0, {self.valid_length}]")

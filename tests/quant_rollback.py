@@ -75,7 +75,7 @@ def walk(cache, seed, steps, loud=0.1):
             T = min(room, rng.choice([1, 1, 1, 1, 2, 5, rng.randint(1, 40), rng.randint(1, 150)]))
             append(cache, expected, rows(1000 * seed + 2 * n, T, loud), rows(1000 * seed + 2 * n + 1, T, loud))
             near = max(near, valid + T - 3 * cache.kv_block)
-            if T > 1 and (valid + T) % cache.kv_block:
+            if T > 1:
                 pinned = ((valid + T) // cache.kv_block * cache.kv_block, valid + T)
         else:
             to = rng.choice([valid - min(valid, rng.randint(1, 12)), rng.randint(0, valid), pinned[1] if pinned[1] <= valid

@@ -88,6 +88,18 @@ def test_writes_and_rollbacks(gpu, seed, capacity, block):
     assert taken > 5
 
 
+def test_a_cache_made_in_inference_mode_is_written_and_rolled_back_outside(gpu):
+    with torch.inference_mode():
+        c = make(gpu, 100, 16)
+    want = Expected(100, 16)
+    for n, T in enumerate((21, 1, 40)):
+        append(c, want, rows(n, T, 0.1), rows(50 + n, T, 0.1))
+    for to in (21, 19):
+        c.rollback(to)
+        want.rollback(to)
+        want.check(c, "outside inference mode")
+
+
 def test_a_clone_takes_its_own_rows_back(gpu):
     c, want = make(gpu, 120, 32), Expected(120, 32)
     append(c, want, rows(1, 37, 0.2), rows(2, 37, 0.2))

@@ -22,6 +22,7 @@ def host(monkeypatch):
         for codes, exps, x in ((c.k, c.k_exp, k), (c.v, c.v_exp, v)):
             oq.append(codes.view(torch.uint8).numpy(), exps.numpy(), x.double().numpy(), start, c.block)
 
+    @torch.inference_mode()     # the launches write by address, whatever mode the tensors were made in
     def kept(ring, k, v, start):
         quantize(ring.cache, k, v, start)
         R, T = ring.k.shape[2], k.shape[2]
@@ -57,6 +58,38 @@ def test_a_refused_rollback_names_a_length_that_works(host):
     c.rollback(33)
     want.rollback(33)
     want.check(c, "inside the block written again")
+
+
+@pytest.mark.parametrize("chunks", [(64, 64, 1), (64, 37), (1,), (64, 36, 1), (50, 50)])
+def test_a_prompts_end_can_be_returned_to_from_far_away(host, chunks):
+    """Whatever its last chunk's length, one token among them; again and again, and within its block."""
+    c, want = make(420, 32), Expected(420, 32)
+    for n, T in enumerate(chunks):
+        append(c, want, rows(n, T, 0.1), rows(50 + n, T, 0.1))
+    end = c.valid_length
+    for n in range(2):
+        for t in range(40):
+            append(c, want, rows(100 + 50 * n + t, 1, 0.3), rows(300 + 50 * n + t, 1, 0.3))
+        while c.valid_length < end + 200:
+            append(c, want, rows(7, 1, 0.3), rows(8, 1, 0.3))
+        c.rollback(end)
+        want.rollback(end)
+        want.check(c, f"{chunks} {n}")
+    if end % 32 > 1:
+        c.rollback(end - 1)
+        want.rollback(end - 1)
+        want.check(c, "inside the prompt's last block")
+
+
+def test_a_cache_made_in_inference_mode_is_written_and_rolled_back_outside(host):
+    with torch.inference_mode():
+        c = make(100, 16)
+    want = Expected(100, 16)
+    for n, T in enumerate((21, 1, 40)):
+        append(c, want, rows(n, T, 0.1), rows(50 + n, T, 0.1))
+    c.rollback(21)
+    want.rollback(21)
+    want.check(c, "outside inference mode")
 
 
 def test_kept_rows_are_no_part_of_the_cache_that_is_counted(host):
