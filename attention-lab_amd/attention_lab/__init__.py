@@ -19,6 +19,8 @@ from .full import FULL_BACKENDS, full_attention  # noqa: E402
 from .window import window_attention  # noqa: E402
 from .quant import (QuantCache, dequantize_rows, quant_attention, quant_gather_attention,  # noqa: E402
                     quantize_append)
+from .pages import (PagedCache, page_append, page_compact, page_fork, page_reserve,  # noqa: E402
+                    page_truncate)
 from .indexer import GroupedIndexer, candidate_scores, project_keys, project_queries  # noqa: E402
 from .decode import (DecodeRequest, dense_decode_step, gathered_decode_step_kernel, prepare_request,  # noqa: E402
                      select_rows_kernel, select_rows_recent, select_rows_uniform, sparse_decode_step,
@@ -30,6 +32,7 @@ __all__ = [
     "flatten_cache", "gather_attention", "gather_rows", "row_offsets", "subset_attention",
     "FULL_BACKENDS", "full_attention", "window_attention",
     "QuantCache", "dequantize_rows", "quant_attention", "quant_gather_attention", "quantize_append",
+    "PagedCache", "page_append", "page_compact", "page_fork", "page_reserve", "page_truncate",
     "GroupedIndexer", "candidate_scores", "project_keys", "project_queries",
     "DecodeRequest", "dense_decode_step", "gathered_decode_step_kernel", "prepare_request", "select_rows_kernel",
     "select_rows_recent", "select_rows_uniform", "sparse_decode_step", "sparse_decode_step_kernel",

@@ -17,7 +17,7 @@ import torch
 LIB_NAME = "libattnlab.so"
 # ATTNLAB_LIB names another build of the same library (the host-sanitized debug build); unset, the in-tree one
 LIB_PATH = os.environ.get("ATTNLAB_LIB") or os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
-ABI_VERSION = 12
+ABI_VERSION = 13
 # select state per (b, g) row: the first-digit histogram of the top-k (2048 bins, top 11 bits of the order-preserving
 # score key), 64 super-bin counts of 32 bins each, then 64 arrival counters of the step's attend partitions
 # (ATTNLAB_SELECT_STATE_WORDS)
@@ -64,6 +64,12 @@ SIGNATURES = {
     "attnlab_quant_attend": (_i, [_p] * 4 + [_i, _p, _p, _i64] + [_i] * 6 + [_f, _p, _i, _p, _p, _p]),
     "attnlab_range_prefill_part_bytes": (_i64, [_i] * 5),
     "attnlab_range_prefill": (_i, [_p] * 5 + [_i, _p] + [_i] * 9 + [_f, _i, _p, _i64, _p]),
+    "attnlab_page_scratch_bytes": (_i64, [_i] * 2),
+    "attnlab_page_fork": (_i, [_p] * 4 + [_i] * 3 + [_p]),
+    "attnlab_page_truncate": (_i, [_p] * 4 + [_i] * 5 + [_p]),
+    "attnlab_page_reserve": (_i, [_p] * 2 + [_i] * 4 + [_p] * 4 + [_i] * 3 + [_p, _p, _i64, _p]),
+    "attnlab_page_append": (_i, ([_p] + [_i64] * 3) * 2 + [_p] * 2 + [_i] * 3 + [_p] * 3 + [_i] * 3 + [_p]),
+    "attnlab_page_compact": (_i, [_p] * 2 + [_i] * 4 + [_p] * 3 + [_i] * 2 + [_p, _i64, _p]),
     "attnlab_sparse_decode_workspace": (_i64, [_i] * 8),
     "attnlab_sparse_decode_step": (_i, [_p] * 8 + [_i] * 10 + [_f, _i, _i, _p, _p, _i64, _p, _p, _p, _p]),
     "attnlab_sparse_decode_step_f32": (_i, [_p] * 8 + [_i] * 10 + [_f, _i, _i, _p, _p, _i64, _p, _p, _p, _p]),

@@ -1,0 +1,497 @@
+// The pages of a K/V cache that sequences share: branching, making room, writing, shortening and compacting.
+//
+// A cache holds, for every layer, pools K, V [pages, G, page, 128] bf16; for the layers together a table [S, W] of int32 (entry
+// e of slot i: the page of its positions [e page, (e + 1) page), or -1), lengths [S] and refs [pages], refs[p] the number of
+// entries that name page p (0: free). Everything is decided on the device, so that a step can be captured and replayed:
+//
+//   fork      table'[i] = table[parents[i]], lengths'[i] = lengths[parents[i]]; a parent outside [0, S): an empty slot
+//   reserve   lengths'[i] = n + t. If n ends inside a page that others hold too, the slot gets a page of its own with the rows
+//             [0, n % page) copied; where all of its holders are written to, the last of them in slot order keeps it. Then
+//             ceil((n + t) / page) - ceil(n / page) pages more. In the order of slots and entries, lowest free page first
+//   append    a layer's rows of the last t positions, written to their pages
+//   truncate  lengths'[i] = min(n, l), the entries from ceil(l / page) on given back
+//   compact   with u pages in use: the i-th of them at or past u moves to the i-th free one below u
+//
+// Every choice depends on the cache alone, never on the order in which workgroups or atomics run: counts are integer sums,
+// and free pages are dealt out by prefix sums over the pool. Entries and lengths are checked before they address memory.
+//
+// What bounds them: launches and latencies for the bookkeeping, bytes for the copies. The bookkeeping of a reserve is one
+// workgroup's, because its parts depend on each other (who keeps a page, how many are wanted, which are free) and a grid would
+// have to meet three times; the copies that it asks for are a second launch of as many waves as the chip holds.
+#include "common.h"
+
+namespace attnlab {
+namespace {
+
+constexpr int kDim = 128;
+constexpr int kRowWords = kDim * 2 / 16;     // 16-byte words of a row
+constexpr int kMaxSlots = 1024;              // a thread of the reserve's workgroup for each
+constexpr int kColumns = 16;                 // table entries a fork's workgroup exchanges between the slots
+constexpr int kBook = 1024;                  // threads of the reserve's and the compaction's workgroup
+constexpr int kScan = 16;                    // pages a thread looks at in a round
+constexpr int kCopyRows = 16;                // rows of a page that a wave copies at a time: 4 KB, four loads in flight
+constexpr int kAppendRun = 64;               // rows that a workgroup of a long write takes
+constexpr int kCopyGroups = 2048;            // workgroups of a copy: eight per CU, one wave of each SIMD from each
+
+// What a reserve or a compaction leaves to its copies, in the scratch buffer.
+struct Moves {
+    int32_t count, used;                     // entries of `src`, `dst`, `rows`; pages in use (compaction)
+    int32_t pad[2];
+};
+
+struct Book {
+    int32_t* table;                          // [S, W]
+    int32_t* lengths;                        // [S]
+    int32_t* refs;                           // [pages]
+    int S, W, pages, shift;
+};
+
+__device__ __forceinline__ bool names(int32_t page, int pages) { return (uint32_t)page < (uint32_t)pages; }
+
+// The slots' rows exchanged, 16 entries of all of them at a time: no workgroup reads what another writes, so the table is
+// changed in place. One more workgroup does the lengths.
+__global__ __launch_bounds__(256) void page_fork(Book a, const int32_t* parents) {
+    __shared__ int32_t was[kMaxSlots * kColumns];
+    const int tid = threadIdx.x;
+    if (blockIdx.x == gridDim.x - 1) {
+        for (int i = tid; i < a.S; i += 256) was[i] = a.lengths[i];
+        __syncthreads();
+        for (int i = tid; i < a.S; i += 256) {
+            const int p = parents[i];
+            a.lengths[i] = names(p, a.S) ? was[p] : 0;
+        }
+        return;
+    }
+    const int e0 = blockIdx.x * kColumns, col = tid & (kColumns - 1);
+    const bool in = e0 + col < a.W;
+    for (int i = tid / kColumns; i < a.S; i += 256 / kColumns)
+        was[i * kColumns + col] = in ? a.table[(size_t)i * a.W + e0 + col] : -1;
+    __syncthreads();
+    if (!in) return;
+    for (int i = tid / kColumns; i < a.S; i += 256 / kColumns) {
+        const int p = parents[i];
+        const int32_t old = was[i * kColumns + col], now = names(p, a.S) ? was[p * kColumns + col] : -1;
+        if (now == old) continue;
+        if (names(old, a.pages)) atomicSub(a.refs + old, 1);
+        if (names(now, a.pages)) atomicAdd(a.refs + now, 1);
+        a.table[(size_t)i * a.W + e0 + col] = now;
+    }
+}
+
+__global__ __launch_bounds__(256) void page_truncate(Book a, const int32_t* to, int each) {
+    const int i = blockIdx.x, page = 1 << a.shift;
+    const int n = a.lengths[i], l = max(to ? to[i] : each, 0);
+    if (l >= n) return;
+    __syncthreads();
+    if (threadIdx.x == 0) a.lengths[i] = l;
+    const int first = (int)(((int64_t)l + page - 1) >> a.shift);
+    const int end = (int)min((int64_t)a.W, ((int64_t)n + page - 1) >> a.shift);
+    for (int e = first + (int)threadIdx.x; e < end; e += 256) {
+        int32_t* at = a.table + (size_t)i * a.W + e;
+        const int32_t p = *at;
+        if (names(p, a.pages)) atomicSub(a.refs + p, 1);
+        *at = -1;
+    }
+}
+
+// Inclusive prefix sum of x over the workgroup's threads (sh: a word for each of its waves).
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sh, uint32_t& total) {
+    const int wave = threadIdx.x >> 6, waves = kBook / 64;
+    const uint32_t own = wave_incl_scan(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) sh[wave] = own;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < waves; ++w) {
+        before += w < wave ? sh[w] : 0u;
+        total += sh[w];
+    }
+    return before + own;
+}
+
+// Pages base + 1024 u + thread, u < kScan, of which `flag(page)` says whether they count: for each that does, its rank among
+// the pages in ascending order is handed to `take(page, rank)`. `found`: the rank of the first, advanced.
+template <typename Flag, typename Take>
+__device__ __forceinline__ void rank_pages(int base, int pages, uint32_t& found, uint32_t (*sh)[kBook / 64], Flag flag, Take take) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint64_t hit[kScan];
+#pragma unroll
+    for (int u = 0; u < kScan; ++u) hit[u] = __ballot(base + kBook * u + tid < pages && flag(u));
+    __syncthreads();
+    if (lane == 0) {
+#pragma unroll
+        for (int u = 0; u < kScan; ++u) sh[u][wave] = (uint32_t)__popcll(hit[u]);
+    }
+    __syncthreads();
+    for (int u = 0; u < kScan; ++u) {
+        uint32_t before = found;
+        for (int w = 0; w < kBook / 64; ++w) {
+            const uint32_t x = sh[u][w];
+            before += w < wave ? x : 0u;
+            found += x;
+        }
+        if (hit[u] >> lane & 1) take(base + kBook * u + tid, before + (uint32_t)__popcll(hit[u] & ((1ull << lane) - 1)));
+    }
+}
+
+__global__ __launch_bounds__(kBook) void page_reserve(Book a, const int32_t* tokens, int each, int32_t* missing, Moves* moves,
+                                                      int32_t* src, int32_t* dst, int32_t* rows) {
+    __shared__ uint32_t wave_sh[kBook / 64], scan_sh[kScan][kBook / 64];
+    __shared__ int32_t held_sh[kMaxSlots], first_sh[kMaxSlots], part_sh[kMaxSlots];
+    __shared__ uint32_t upto_sh[kMaxSlots], job_sh[kMaxSlots];   // requests up to and with a slot's; its copy's number + 1, or 0
+    const int tid = threadIdx.x, page = 1 << a.shift;
+    const bool slot = tid < a.S;
+    const int n = slot ? max(a.lengths[tid], 0) : 0, t = slot ? max(tokens ? tokens[tid] : each, 0) : 0;
+    const int64_t end = min((int64_t)n + t, (int64_t)INT32_MAX);
+    const int last = n >> a.shift, part = n & (page - 1);
+    int held = t > 0 && part && last < a.W ? a.table[(size_t)tid * a.W + last] : -1;
+    const int refs = names(held, a.pages) ? a.refs[held] : 0;
+    if (refs <= 1) held = -1;                // nobody's, or the slot's alone
+    held_sh[tid] = held;
+    __syncthreads();
+    bool copies = false;
+    if (held >= 0) {
+        int writers = 0, later = 0;
+        for (int j = 0; j < a.S; ++j) {
+            const bool same = held_sh[j] == held;
+            writers += same;
+            later |= same && j > tid;
+        }
+        copies = later || writers < refs;
+    }
+    const int from = (int)(((int64_t)n + page - 1) >> a.shift), upto = (int)((end + page - 1) >> a.shift);
+    const int fresh = max(min(upto, a.W) - from, 0);
+    uint32_t lost = t > 0 ? (uint32_t)max(upto - max(from, a.W), 0) : 0u;   // pages that the table has no entry for
+    uint32_t wanted, jobs;
+    const uint32_t to = block_scan((t > 0 ? (uint32_t)fresh : 0u) + copies, wave_sh, wanted);
+    const uint32_t job = block_scan(copies, wave_sh, jobs);
+    if (slot) {
+        first_sh[tid] = from;
+        part_sh[tid] = part;
+        upto_sh[tid] = to;
+        job_sh[tid] = copies ? job : 0u;
+        if (t > 0) a.lengths[tid] = (int32_t)end;
+    }
+    __syncthreads();
+    // request r -> its slot, and the entry that gets the page (or -1 where there is none left)
+    auto give = [&](uint32_t r, int32_t p) {
+        int lo = 0, hi = a.S - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (upto_sh[mid] > r) hi = mid;
+            else lo = mid + 1;
+        }
+        const uint32_t k = r - (lo ? upto_sh[lo - 1] : 0u), j = job_sh[lo];
+        const bool copy = j && k == 0;
+        const int e = first_sh[lo] + (int)k - (j ? 1 : 0);   // a copy's entry is the one before the first new one
+        a.table[(size_t)lo * a.W + e] = p;
+        if (copy) {
+            src[j - 1] = held_sh[lo];
+            dst[j - 1] = p;
+            rows[j - 1] = p < 0 ? 0 : part_sh[lo];
+        }
+    };
+    uint32_t found = 0;
+    for (int base = 0; base < a.pages && found < wanted; base += kBook * kScan) {
+        int32_t r[kScan];
+#pragma unroll
+        for (int u = 0; u < kScan; ++u) r[u] = a.refs[min(base + kBook * u + tid, a.pages - 1)];
+        rank_pages(base, a.pages, found, scan_sh, [&](int u) { return r[u] <= 0; }, [&](int p, uint32_t rank) {
+            if (rank >= wanted) return;
+            a.refs[p] = 1;
+            give(rank, p);
+        });
+    }
+    for (uint32_t r = found + tid; r < wanted; r += kBook) give(r, -1);
+    if (copies) atomicSub(a.refs + held, 1);
+    const uint32_t out = wanted > found ? wanted - found : 0u;
+    uint32_t over;
+    block_scan(lost, wave_sh, over);
+    if (tid == 0) {
+        moves->count = (int32_t)jobs;
+        if (missing && out + over) missing[0] += (int32_t)(out + over);
+    }
+}
+
+__global__ __launch_bounds__(kBook) void page_compact(Book a, Moves* moves, int32_t* src, int32_t* dst, int32_t* rank_of) {
+    __shared__ uint32_t wave_sh[kBook / 64], scan_sh[kScan][kBook / 64];
+    const int tid = threadIdx.x;
+    uint32_t mine = 0, used;
+    for (int base = 0; base < a.pages; base += kBook * kScan) {
+        int32_t r[kScan];
+#pragma unroll
+        for (int u = 0; u < kScan; ++u) r[u] = a.refs[min(base + kBook * u + tid, a.pages - 1)];
+#pragma unroll
+        for (int u = 0; u < kScan; ++u) mine += base + kBook * u + tid < a.pages && r[u] > 0;
+    }
+    block_scan(mine, wave_sh, used);
+    uint32_t holes = 0, high = 0;
+    for (int base = 0; base < a.pages; base += kBook * kScan) {
+        int32_t r[kScan];
+#pragma unroll
+        for (int u = 0; u < kScan; ++u) r[u] = a.refs[min(base + kBook * u + tid, a.pages - 1)];
+        auto page_of = [&](int u) { return base + kBook * u + tid; };
+        rank_pages(base, a.pages, holes, scan_sh, [&](int u) { return page_of(u) < (int)used && r[u] <= 0; },
+                   [&](int p, uint32_t rank) { dst[rank] = p; });
+        rank_pages(base, a.pages, high, scan_sh, [&](int u) { return page_of(u) >= (int)used && r[u] > 0; },
+                   [&](int p, uint32_t rank) { src[rank] = p; rank_of[p] = (int32_t)rank; });
+#pragma unroll
+        for (int u = 0; u < kScan; ++u)
+            if (page_of(u) >= (int)used && page_of(u) < a.pages && r[u] <= 0) rank_of[page_of(u)] = -1;
+    }
+    __syncthreads();   // as many pages at or past `used` are in use as are free below it
+    for (uint32_t i = tid; i < high; i += kBook) {
+        a.refs[dst[i]] = a.refs[src[i]];
+        a.refs[src[i]] = 0;
+    }
+    if (tid == 0) {
+        moves->count = (int32_t)high;
+        moves->used = (int32_t)used;
+    }
+}
+
+struct CopyArgs {
+    uint16_t* pool[2];                       // K and V of every layer
+    int64_t layer_stride;                    // elements
+    int layers, G, page, pages;
+    const Moves* moves;
+    const int32_t* src;
+    const int32_t* dst;
+    const int32_t* rows;                     // rows of each copy; null: whole pages
+    int32_t* table;                          // compaction: entries at or past moves->used follow their pages
+    int64_t entries;
+    const int32_t* rank_of;
+};
+
+// The pages of `src` copied to `dst` in every layer, K and V. A wave takes up to 16 rows of one (copy, layer, K or V, group) at a
+// time and the grid walks over them; nothing is copied onto a page that another copy reads.
+__global__ __launch_bounds__(256) void page_copy(CopyArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6)), waves = gridDim.x * 4;
+    const int count = a.moves->count;
+    const int chunks = (a.page + kCopyRows - 1) / kCopyRows;
+    const int per = a.layers * 2 * a.G * chunks;
+    const int64_t units = (int64_t)count * per;
+    for (int64_t unit = wave; unit < units; unit += waves) {
+        const int j = (int)(unit / per);
+        int x = (int)(unit - (int64_t)j * per);
+        const int c = x % chunks;
+        x /= chunks;
+        const int g = x % a.G;
+        x /= a.G;
+        const int rows = min((a.rows ? a.rows[j] : a.page) - kCopyRows * c, kCopyRows);
+        const int s = a.src[j], d = a.dst[j];
+        if (rows <= 0 || !names(s, a.pages) || !names(d, a.pages)) continue;
+        uint16_t* base = a.pool[x & 1] + (size_t)(x >> 1) * a.layer_stride + (size_t)kCopyRows * c * kDim;
+        const size_t step = (size_t)a.page * kDim;
+        const u32x4_t* from = reinterpret_cast<const u32x4_t*>(base + ((size_t)s * a.G + g) * step);
+        u32x4_t* to = reinterpret_cast<u32x4_t*>(base + ((size_t)d * a.G + g) * step);
+        const int words = rows * kRowWords;
+        u32x4_t w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (64 * u + lane < words) w[u] = from[64 * u + lane];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (64 * u + lane < words) to[64 * u + lane] = w[u];
+    }
+    if (a.table && count) {
+        const int used = a.moves->used;
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.entries; i += (int64_t)gridDim.x * 256) {
+            const int32_t p = a.table[i];
+            if (p < used || p >= a.pages) continue;
+            const int32_t r = a.rank_of[p];
+            if (r >= 0) a.table[i] = a.dst[r];
+        }
+    }
+}
+
+struct AppendArgs {
+    const uint16_t* x[2];                    // K and V rows: (slot, group, row, dim) at x + i sb + g sg + t st + dim
+    int64_t sb[2], sg[2], st[2];
+    uint16_t* pool[2];                       // the layer's K and V pages
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* tokens;                   // rows of each slot, or null: T
+    int S, W, pages, shift, G, T;
+};
+
+// Where row t of slot i goes: its (page, group, row) in the pool, or -1.
+__device__ __forceinline__ int64_t row_of(const AppendArgs& a, int i, int g, int t, int count, int64_t first) {
+    const int64_t pos = first + t, e = pos >> a.shift;
+    const int p = t < count && pos >= 0 && e < a.W ? a.table[(size_t)i * a.W + e] : -1;
+    return names(p, a.pages) ? (((int64_t)p * a.G + g) << a.shift) + (pos & ((1 << a.shift) - 1)) : -1;
+}
+
+// Sixteen lanes a row, K or V by blockIdx.y. Few tokens (LONG false): rows of all slots and groups in line, sixteen to a
+// workgroup; else 64 consecutive rows of one (slot, group).
+template <bool LONG>
+__global__ __launch_bounds__(256) void page_append(AppendArgs a, int runs) {
+    constexpr int kRows = LONG ? kAppendRun / 16 : 1;
+    const int kv = blockIdx.y, lane16 = threadIdx.x & 15, line = threadIdx.x >> 4;
+    int i, g, t0;
+    if constexpr (LONG) {
+        const int ig = blockIdx.x / runs;
+        t0 = (blockIdx.x - ig * runs) * kAppendRun + line;
+        i = ig / a.G;
+        g = ig - i * a.G;
+    } else {
+        const int64_t x = (int64_t)blockIdx.x * 16 + line;
+        const int64_t ig = x / a.T;
+        t0 = (int)(x - ig * a.T);
+        i = (int)(ig / a.G);
+        g = (int)(ig - (int64_t)i * a.G);
+        if (i >= a.S) return;
+    }
+    const int tokens = a.tokens ? a.tokens[i] : a.T, count = min(tokens, a.T);
+    if (t0 >= count) return;
+    const int64_t first = (int64_t)a.lengths[i] - tokens;
+    const uint16_t* from = a.x[kv] + i * a.sb[kv] + g * a.sg[kv] + 8 * lane16;
+    u32x4_t w[kRows];
+    int64_t at[kRows];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+        at[u] = row_of(a, i, g, t0 + 16 * u, count, first);
+        w[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(from + min(t0 + 16 * u, count - 1) * a.st[kv]));
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u)
+        if (at[u] >= 0) *reinterpret_cast<u32x4_t*>(a.pool[kv] + at[u] * kDim + 8 * lane16) = w[u];
+}
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int check_book(const int32_t* table, const int32_t* lengths, const int32_t* refs, int S, int W, int pages, int page) {
+    ATTNLAB_REQUIRE(1 <= S && S <= kMaxSlots, "slots S=%d outside [1, %d]", S, kMaxSlots);
+    ATTNLAB_REQUIRE(W >= 1 && pages >= 1, "max_pages=%d and num_pages=%d must be positive", W, pages);
+    ATTNLAB_REQUIRE(page >= 1 && page <= (1 << 16) && (page & (page - 1)) == 0,
+                    "page_size=%d must be a power of two in [1, 65536]", page);
+    ATTNLAB_REQUIRE((int64_t)W * page <= INT32_MAX, "max_pages * page_size exceeds 2^31 positions");
+    ATTNLAB_REQUIRE(table && lengths && refs, "table, lengths and refs must be device pointers");
+    return ATTNLAB_OK;
+}
+
+int check_pools(const uint16_t* k, const uint16_t* v, int layers, int pages, int G, int page) {
+    ATTNLAB_REQUIRE(layers >= 1 && G >= 1, "layers=%d and G=%d must be positive", layers, G);
+    ATTNLAB_REQUIRE((int64_t)pages * G * page <= INT32_MAX, "the pool of %d pages x %d groups x %d rows exceeds 2^31 rows", pages,
+                    G, page);
+    ATTNLAB_REQUIRE(k && v && aligned(k, 16) && aligned(v, 16), "k and v must be 16-byte aligned device pointers");
+    return ATTNLAB_OK;
+}
+
+Book book_of(int32_t* table, int32_t* lengths, int32_t* refs, int S, int W, int pages, int page) {
+    return Book{table, lengths, refs, S, W, pages, __builtin_ctz((unsigned)page)};
+}
+
+// Scratch: the header, then src, dst and rows of at most `slots` copies, or src, dst and rank_of of the pages.
+int64_t scratch_words(int S, int pages) { return (int64_t)(sizeof(Moves) / 4) + 3 * (int64_t)(S > pages ? S : pages); }
+
+int launch_copy(const CopyArgs& a, int64_t most, hipStream_t s, const char* what) {
+    const int chunks = (a.page + kCopyRows - 1) / kCopyRows;
+    int64_t groups = (most * a.layers * 2 * a.G * chunks + 3) / 4;
+    if (a.table && groups < (a.entries + 255) / 256) groups = (a.entries + 255) / 256;
+    if (groups > kCopyGroups) groups = kCopyGroups;
+    hipLaunchKernelGGL(page_copy, dim3((unsigned)groups), dim3(256), 0, s, a);
+    return check_launch(what);
+}
+
+}  // namespace
+}  // namespace attnlab
+
+using namespace attnlab;
+
+extern "C" int64_t attnlab_page_scratch_bytes(int S, int num_pages) {
+    return S < 1 || num_pages < 1 ? -1 : 4 * scratch_words(S, num_pages);
+}
+
+extern "C" int attnlab_page_fork(int32_t* table, int32_t* lengths, int32_t* refs, const int32_t* parents, int S, int max_pages,
+                                 int num_pages, void* stream) {
+    const int rc = check_book(table, lengths, refs, S, max_pages, num_pages, 1);
+    if (rc) return rc;
+    ATTNLAB_REQUIRE(parents, "parents must be a device pointer");
+    const int groups = (max_pages + kColumns - 1) / kColumns + 1;
+    hipLaunchKernelGGL(page_fork, dim3((unsigned)groups), dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
+                       book_of(table, lengths, refs, S, max_pages, num_pages, 1), parents);
+    return check_launch("page_fork");
+}
+
+extern "C" int attnlab_page_truncate(int32_t* table, int32_t* lengths, int32_t* refs, const int32_t* to, int length, int S,
+                                     int max_pages, int num_pages, int page_size, void* stream) {
+    const int rc = check_book(table, lengths, refs, S, max_pages, num_pages, page_size);
+    if (rc) return rc;
+    ATTNLAB_REQUIRE(to || length >= 0, "length=%d must not be negative", length);
+    hipLaunchKernelGGL(page_truncate, dim3((unsigned)S), dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
+                       book_of(table, lengths, refs, S, max_pages, num_pages, page_size), to, length);
+    return check_launch("page_truncate");
+}
+
+extern "C" int attnlab_page_reserve(uint16_t* k, uint16_t* v, int layers, int num_pages, int G, int page_size, int32_t* table,
+                                    int32_t* lengths, int32_t* refs, const int32_t* tokens, int each, int S, int max_pages,
+                                    int32_t* missing, void* scratch, int64_t scratch_bytes, void* stream) {
+    int rc = check_book(table, lengths, refs, S, max_pages, num_pages, page_size);
+    if (!rc) rc = check_pools(k, v, layers, num_pages, G, page_size);
+    if (rc) return rc;
+    ATTNLAB_REQUIRE(tokens || each >= 0, "tokens=%d must not be negative", each);
+    ATTNLAB_REQUIRE(scratch && aligned(scratch, 16) && scratch_bytes >= 4 * scratch_words(S, num_pages),
+                    "scratch must be a 16-byte aligned device buffer of %lld bytes", (long long)(4 * scratch_words(S, num_pages)));
+    Moves* moves = static_cast<Moves*>(scratch);
+    int32_t* src = reinterpret_cast<int32_t*>(moves + 1);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(page_reserve, dim3(1), dim3(kBook), 0, s,
+                       book_of(table, lengths, refs, S, max_pages, num_pages, page_size), tokens, each, missing, moves, src,
+                       src + S, src + 2 * S);
+    rc = check_launch("page_reserve");
+    if (rc || S == 1 || page_size == 1) return rc;   // one slot shares with nobody, and one row ends inside no page
+    const CopyArgs c{{k, v}, (int64_t)num_pages * G * page_size * kDim, layers, G, page_size, num_pages, moves, src, src + S,
+                     src + 2 * S, nullptr, 0, nullptr};
+    return launch_copy(c, S, s, "page_reserve (copies)");
+}
+
+extern "C" int attnlab_page_append(const uint16_t* k, int64_t k_b_stride, int64_t k_g_stride, int64_t k_t_stride,
+                                   const uint16_t* v, int64_t v_b_stride, int64_t v_g_stride, int64_t v_t_stride,
+                                   uint16_t* k_pages, uint16_t* v_pages, int num_pages, int G, int page_size,
+                                   const int32_t* table, const int32_t* lengths, const int32_t* tokens, int S, int max_pages,
+                                   int T, void* stream) {
+    ATTNLAB_REQUIRE(T >= 0, "T=%d must not be negative", T);
+    int rc = check_book(table, lengths, table, S, max_pages, num_pages, page_size);
+    if (!rc) rc = check_pools(k_pages, v_pages, 1, num_pages, G, page_size);
+    if (rc || T == 0) return rc;
+    ATTNLAB_REQUIRE(k && v && aligned(k, 16) && aligned(v, 16) &&
+                        ((k_b_stride | k_g_stride | k_t_stride | v_b_stride | v_g_stride | v_t_stride) & 7) == 0,
+                    "k and v must be device pointers with 16-byte aligned rows");
+    const AppendArgs a{{k, v}, {k_b_stride, v_b_stride}, {k_g_stride, v_g_stride}, {k_t_stride, v_t_stride},
+                       {k_pages, v_pages}, table, lengths, tokens, S, max_pages, num_pages,
+                       __builtin_ctz((unsigned)page_size), G, T};
+    const bool lengthy = T > 16;
+    const int64_t runs = ((int64_t)T + kAppendRun - 1) / kAppendRun;
+    const int64_t groups = lengthy ? (int64_t)S * G * runs : ((int64_t)S * G * T + 15) / 16;
+    ATTNLAB_REQUIRE(groups < (int64_t)1 << 31, "grid of %lld workgroups is too large", (long long)groups);
+    const dim3 grid((unsigned)groups, 2), wg(256);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (lengthy) hipLaunchKernelGGL(page_append<true>, grid, wg, 0, s, a, (int)runs);
+    else hipLaunchKernelGGL(page_append<false>, grid, wg, 0, s, a, 0);
+    return check_launch("page_append");
+}
+
+extern "C" int attnlab_page_compact(uint16_t* k, uint16_t* v, int layers, int num_pages, int G, int page_size, int32_t* table,
+                                    int32_t* lengths, int32_t* refs, int S, int max_pages, void* scratch,
+                                    int64_t scratch_bytes, void* stream) {
+    int rc = check_book(table, lengths, refs, S, max_pages, num_pages, page_size);
+    if (!rc) rc = check_pools(k, v, layers, num_pages, G, page_size);
+    if (rc) return rc;
+    ATTNLAB_REQUIRE(scratch && aligned(scratch, 16) && scratch_bytes >= 4 * scratch_words(S, num_pages),
+                    "scratch must be a 16-byte aligned device buffer of %lld bytes", (long long)(4 * scratch_words(S, num_pages)));
+    Moves* moves = static_cast<Moves*>(scratch);
+    int32_t* src = reinterpret_cast<int32_t*>(moves + 1);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(page_compact, dim3(1), dim3(kBook), 0, s,
+                       book_of(table, lengths, refs, S, max_pages, num_pages, page_size), moves, src, src + num_pages,
+                       src + 2 * (int64_t)num_pages);
+    rc = check_launch("page_compact");
+    if (rc) return rc;
+    const CopyArgs c{{k, v}, (int64_t)num_pages * G * page_size * kDim, layers, G, page_size, num_pages, moves, src,
+                     src + num_pages, nullptr, table, (int64_t)S * max_pages, src + 2 * (int64_t)num_pages};
+    return launch_copy(c, num_pages / 2, s, "page_compact (copies)");
+}

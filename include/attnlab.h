@@ -385,6 +385,54 @@ int attnlab_range_prefill(const uint16_t* q, const void* K, const void* V, const
                           int sinks, float scale, int splits, float* part, int64_t part_bytes, void* stream);
 
 /*
+ * A K/V cache in pages that sequences share (no reference counterpart: its caches are branched by copying them,
+ * qwen_wrap.py:117-133; the pools are those of attnlab_attend_paged). k, v: [layers, num_pages, G, page_size, 128] bf16,
+ * 16-byte aligned; page_size a power of two up to 65536; num_pages * G * page_size and max_pages * page_size below 2^31.
+ *   table    int32 [S, max_pages], entry e of slot i the page of its positions [e page_size, (e + 1) page_size), or -1; 1 <= S <=
+ *            1024; -1 past a sequence's pages
+ *   lengths  int32 [S]
+ *   refs     int32 [num_pages], how many entries name each page (0: free)
+ * All are device memory changed in place. The results depend on the cache alone. Calls on one cache must be ordered on one
+ * stream. An entry outside [0, num_pages) is not followed.
+ *
+ * attnlab_page_fork: slot i goes on from slot parents[i] (int32 [S]) as it was before the call: its entries and length; a
+ * parent outside [0, S) leaves the slot empty.
+ *
+ * attnlab_page_truncate: lengths[i] = min(lengths[i], max(to[i], 0)), with `to` null `length`; the entries from
+ * ceil(lengths[i] / page_size) on are given back.
+ *
+ * attnlab_page_reserve: lengths[i] grows by tokens[i] (null: each; less than 1: slot i is left alone). A slot that ended
+ * inside a page with other holders gets a page of its own, the rows up to its length copied in every layer, unless all of the
+ * page's holders grow and it is the last of them. Then an entry is given a page for every page_size positions begun. Pages are the
+ * lowest free ones, in the order of slots and entries; where none is left the entry is -1. missing (int32 [1], nullable) is
+ * raised by the pages not given, those past max_pages among them. scratch: 16-byte aligned, attnlab_page_scratch_bytes(S,
+ * num_pages) bytes, no initialisation.
+ *
+ * attnlab_page_append: one layer's rows, k and v: (slot, group, row t, dim) at k + i k_b_stride + g k_g_stride + t k_t_stride
+ * + dim (bf16 elements; rows 16-byte aligned; strides may be 0), row t < tokens[i] (null: T) of slot i at position
+ * lengths[i] - tokens[i] + t. k_pages, v_pages: the layer's [num_pages, G, page_size, 128]. Positions without a page are
+ * not written.
+ *
+ * attnlab_page_compact: with n pages in use (refs > 0), the i-th of them at or past n moves to the i-th free one below n, in
+ * every layer; table and refs follow. scratch as in attnlab_page_reserve.
+ */
+int64_t attnlab_page_scratch_bytes(int S, int num_pages);
+int attnlab_page_fork(int32_t* table, int32_t* lengths, int32_t* refs, const int32_t* parents, int S, int max_pages,
+                      int num_pages, void* stream);
+int attnlab_page_truncate(int32_t* table, int32_t* lengths, int32_t* refs, const int32_t* to, int length, int S,
+                          int max_pages, int num_pages, int page_size, void* stream);
+int attnlab_page_reserve(uint16_t* k, uint16_t* v, int layers, int num_pages, int G, int page_size, int32_t* table,
+                         int32_t* lengths, int32_t* refs, const int32_t* tokens, int each, int S, int max_pages,
+                         int32_t* missing, void* scratch, int64_t scratch_bytes, void* stream);
+int attnlab_page_append(const uint16_t* k, int64_t k_b_stride, int64_t k_g_stride, int64_t k_t_stride, const uint16_t* v,
+                        int64_t v_b_stride, int64_t v_g_stride, int64_t v_t_stride, uint16_t* k_pages, uint16_t* v_pages,
+                        int num_pages, int G, int page_size, const int32_t* table, const int32_t* lengths,
+                        const int32_t* tokens, int S, int max_pages, int T, void* stream);
+int attnlab_page_compact(uint16_t* k, uint16_t* v, int layers, int num_pages, int G, int page_size, int32_t* table,
+                         int32_t* lengths, int32_t* refs, int S, int max_pages, void* scratch, int64_t scratch_bytes,
+                         void* stream);
+
+/*
  * Workspace (bytes) of attnlab_sparse_decode_step for these sizes: candidate scores, row list, u, tiled-select
  * scratch and split-K partials, each 256-byte aligned, then the key lists of rows of 32769 to 131072 candidates. Its
  * contents need no initialisation. A step of such rows also takes a workspace without that last region (and then selects
