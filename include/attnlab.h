@@ -433,6 +433,22 @@ int attnlab_page_compact(uint16_t* k, uint16_t* v, int layers, int num_pages, in
                          void* stream);
 
 /*
+ * Log probabilities of given tokens, the entropy and the most likely alternatives of N rows of V logits (no reference
+ * counterpart: its scripts take log_softmax on the host). Row r at logits + r stride (elements of `dtype`: ATTNLAB_DT_BF16,
+ * _F16 or _F32, aligned to it; any stride). With lse = log sum_j exp(x_j):
+ *   logprobs[r] = x_token - lse    tokens: int32 [N], or int64 with tokens64; one below 0 gives 0, one of V or more NaN
+ *   entropy[r]  = -sum_j p_j log p_j,  p_j = exp(x_j - lse), 0 log 0 = 0                                  (nullable)
+ *   top_tokens, top_logprobs [N, top]: the largest logits in order, equal ones by the lower token (-0 equals +0, NaN last)
+ * tokens and logprobs are null together. A row with a NaN, an infinity of positive sign or nothing above -inf has no
+ * distribution: its values are NaN (top_tokens stay those of the order). 0 <= top <= min(64, V), V <= 2^20 - 16.
+ * part: 16-byte aligned, attnlab_logprob_part_bytes bytes, no initialisation. Two launches.
+ */
+int64_t attnlab_logprob_part_bytes(int64_t N, int V, int dtype, int top);
+int attnlab_token_logprobs(const void* logits, int dtype, int64_t stride, int64_t N, int V, const void* tokens, int tokens64,
+                           int top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens, void* part,
+                           int64_t part_bytes, void* stream);
+
+/*
  * Workspace (bytes) of attnlab_sparse_decode_step for these sizes: candidate scores, row list, u, tiled-select
  * scratch and split-K partials, each 256-byte aligned, then the key lists of rows of 32769 to 131072 candidates. Its
  * contents need no initialisation. A step of such rows also takes a workspace without that last region (and then selects
