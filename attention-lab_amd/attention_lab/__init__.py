@@ -21,6 +21,7 @@ from .quant import (QuantCache, dequantize_rows, quant_attention, quant_gather_a
                     quantize_append)
 from .pages import (PagedCache, page_append, page_compact, page_fork, page_reserve,  # noqa: E402
                     page_truncate)
+from .shared import shared_prefix_attention  # noqa: E402
 from .logprobs import TokenLogprobs, token_logprobs  # noqa: E402
 from .indexer import GroupedIndexer, candidate_scores, project_keys, project_queries  # noqa: E402
 from .decode import (DecodeRequest, dense_decode_step, gathered_decode_step_kernel, prepare_request,  # noqa: E402
@@ -34,7 +35,7 @@ __all__ = [
     "FULL_BACKENDS", "full_attention", "window_attention",
     "QuantCache", "dequantize_rows", "quant_attention", "quant_gather_attention", "quantize_append",
     "PagedCache", "page_append", "page_compact", "page_fork", "page_reserve", "page_truncate",
-    "TokenLogprobs", "token_logprobs",
+    "shared_prefix_attention", "TokenLogprobs", "token_logprobs",
     "GroupedIndexer", "candidate_scores", "project_keys", "project_queries",
     "DecodeRequest", "dense_decode_step", "gathered_decode_step_kernel", "prepare_request", "select_rows_kernel",
     "select_rows_recent", "select_rows_uniform", "sparse_decode_step", "sparse_decode_step_kernel",

@@ -70,6 +70,9 @@ SIGNATURES = {
     "attnlab_page_reserve": (_i, [_p] * 2 + [_i] * 4 + [_p] * 4 + [_i] * 3 + [_p, _p, _i64, _p]),
     "attnlab_page_append": (_i, ([_p] + [_i64] * 3) * 2 + [_p] * 2 + [_i] * 3 + [_p] * 3 + [_i] * 3 + [_p]),
     "attnlab_page_compact": (_i, [_p] * 2 + [_i] * 4 + [_p] * 3 + [_i] * 2 + [_p, _i64, _p]),
+    "attnlab_shared_part_bytes": (_i64, [_i] * 6),
+    "attnlab_shared_prefix_attend": (_i, [_p] * 3 + [_i] * 2 + [_p, _i64, _i, _p, _i, _p, _i, _p] + [_i] * 5 + [_f] + [_i] * 3 +
+                                     [_p, _p, _i64, _p]),
     "attnlab_logprob_part_bytes": (_i64, [_i64, _i, _i, _i]),
     "attnlab_token_logprobs": (_i, [_p, _i, _i64, _i64, _i, _p, _i, _i] + [_p] * 5 + [_i64, _p]),
     "attnlab_sparse_decode_workspace": (_i64, [_i] * 8),

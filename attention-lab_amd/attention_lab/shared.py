@@ -1,0 +1,109 @@
+"""Attention of sequences that share long prompts, over a paged cache: a prompt's keys and values are read once for all the
+sequences that continue it, where attend_paged reads them once for each.
+
+Beside hip_attend.attend_paged and pages.py, whose forks are what shares pages. The full read's semantics (full.py:17-44) over
+each sequence's own table; no counterpart in the reference, whose caches are contiguous.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _native as nat
+from .hip_attend import HEAD_DIM
+from .hip_range import DEFAULT_SCALE, INT_MAX, MAX_H_CHUNK, aligned_query, check_lengths, check_out
+
+WIDE_ROWS, NARROW_ROWS = 128, 16   # (query, head) rows of a workgroup of either kernel
+MAX_SPLITS = 64
+
+
+def shared_splits(G: int, rows: int, runs: int, keys: int, wide: bool) -> int:
+    """Key splits of the shared part: `rows` (query, head) rows of a group over all sequences, `runs` prompts of `keys` positions."""
+    per = WIDE_ROWS if wide else NARROW_ROWS
+    tiles = G * (rows // per + (runs + 1) // 2)
+    return max(1, min(MAX_SPLITS, (512 if wide else 768) // max(tiles, 1), keys // 256))
+
+
+def own_splits(BG: int, rows: int, keys: int) -> int:
+    """Key splits of the own part: `rows` rows of each of BG (sequence, group) pairs over up to `keys` positions."""
+    wide = rows > MAX_H_CHUNK
+    tiles = BG * -(-rows // (WIDE_ROWS if wide else NARROW_ROWS))
+    return max(1, min(16, (512 if wide else 768) // tiles, keys // 256))
+
+
+def _lengths(x, n: int, device, name: str):
+    """(address or None, int) of a value per sequence or run on the device, or one for all."""
+    if isinstance(x, torch.Tensor):
+        return check_lengths(x, n, device).data_ptr(), 0
+    x = int(x)
+    if not 0 <= x <= INT_MAX:
+        raise ValueError(f"{name}={x} must be in [0, 2^31)")
+    return None, x
+
+
+def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_lengths=0, *, runs=None, scale=None, out=None,
+                            partitions=None):
+    """q [B,G,h,T,128] bfloat16, k_pages and v_pages bfloat16 [num_pages,G,page_size,128] (page_size a power of two),
+    block_table int32 [B,max_pages] -> bfloat16 [B,G,h,T,128].
+
+    Sequence b's T queries sit at the last positions of lengths[b] (an int for all, or int32 [B] on the device; clamped to
+    max_pages * page_size) and read positions j up to their own by its table; positions on an entry outside [0, num_pages) are
+    skipped, and a query that reads nothing gets zeros. h <= 16.
+
+    Sequences runs[r] .. runs[r + 1] - 1 (runs int32 [R + 1] on the device, ascending; None: one run of all) share their first
+    prefix_lengths[r] positions (an int for all, or int32 [R] on the device): below it, rounded down to whole pages, their
+    tables name the same pages, and the first one's are read for all. Sequences in no run, and those not long enough for
+    all of their queries to see the whole prefix, read everything by their own tables. prefix_lengths 0: a read of a paged cache
+    with a length per sequence.
+
+    Nothing is read back to the host, so a captured graph follows the tensors' later values. Weights are rounded to bfloat16
+    before their product with V (2^-8 of each at most; their sum is not rounded), sums are float32. partitions overrides the key
+    split counts (shared part, own part), 1 to 64 each (0 shared: the prefix is ignored)."""
+    if (k_pages.dim() != 4 or k_pages.dtype != torch.bfloat16 or not k_pages.is_contiguous() or k_pages.shape[3] != HEAD_DIM
+            or not k_pages.is_cuda):
+        raise ValueError(f"k_pages must be a contiguous bfloat16 [num_pages, G, page_size, {HEAD_DIM}] pool on a HIP device")
+    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or not v_pages.is_contiguous() \
+            or v_pages.device != k_pages.device:
+        raise ValueError("v_pages must match k_pages")
+    device = k_pages.device
+    pages, G, page, _ = k_pages.shape
+    if q.dim() != 5 or q.shape[1] != G or q.shape[4] != HEAD_DIM or q.dtype != torch.bfloat16 or q.device != device:
+        raise ValueError(f"q must be a bfloat16 [B, {G}, h, T, {HEAD_DIM}] tensor on the pools' device, got {q.dtype} "
+                         f"{tuple(q.shape)}")
+    B, _, h, T, _ = q.shape
+    if not 1 <= h <= MAX_H_CHUNK:
+        raise ValueError(f"h={h} must be in [1, {MAX_H_CHUNK}]")
+    if B < 1 or not pages or not page or page & (page - 1):
+        raise ValueError(f"need at least one sequence and page, and a page_size that is a power of two, got {B}, {pages}, {page}")
+    if (block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] < 1 or block_table.dtype != torch.int32
+            or block_table.stride(1) != 1 and block_table.shape[1] > 1 or block_table.device != device):
+        raise ValueError("block_table must be an int32 [B, max_pages] tensor with unit column stride on the pools' device")
+    W = block_table.shape[1]
+    R = 1
+    if runs is not None:
+        R = runs.numel() - 1
+        if runs.dim() != 1 or R < 1 or runs.dtype != torch.int32 or not runs.is_contiguous() or runs.device != device:
+            raise ValueError("runs must be a contiguous int32 [R + 1] tensor of at least two bounds on the pools' device")
+    lengths_at, length = _lengths(lengths, B, device, "lengths")
+    prefix_at, prefix = _lengths(prefix_lengths, R, device, "prefix_lengths")
+    most = W * page if lengths_at else min(length, W * page)
+    keys = most if prefix_at else min(prefix, most) // page * page
+    rows = B * h * T
+    wide = rows > NARROW_ROWS * R
+    if partitions is None:
+        ns = shared_splits(G, rows, R, keys, wide) if keys else 0
+        no = own_splits(B * G, h * T if T > 1 else 1, most if prefix_at else most - keys)
+    else:
+        ns, no = (int(x) for x in partitions)
+        if not (0 <= ns <= MAX_SPLITS and 1 <= no <= MAX_SPLITS):
+            raise ValueError(f"partitions must be two counts, in [0, {MAX_SPLITS}] and [1, {MAX_SPLITS}]")
+    q, q_at = aligned_query(q)
+    out = check_out(out, q, torch.bfloat16)
+    if T == 0:
+        return out
+    nbytes = nat.lib().attnlab_shared_part_bytes(B, G, h, T, ns, no)
+    part = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+    nat.call_on(device, "attnlab_shared_prefix_attend", q_at, k_pages.data_ptr(), v_pages.data_ptr(), pages, page,
+                block_table.data_ptr(), max(block_table.stride(0), W) if B == 1 else block_table.stride(0), W, lengths_at, length,
+                prefix_at, prefix, nat.ptr(runs), R, B, G, h, T, DEFAULT_SCALE if scale is None else float(scale), wide, ns, no,
+                out.data_ptr(), nat.ptr(part), nbytes, nat.stream_of(device))
+    return out

@@ -433,6 +433,30 @@ int attnlab_page_compact(uint16_t* k, uint16_t* v, int layers, int num_pages, in
                          void* stream);
 
 /*
+ * Attention over a paged cache (attnlab_attend_paged's pools and tables) of sequences that share prompts. Sequence b's T queries
+ * sit at the last positions of its length n (lengths int32 [B] on the device, or null: `length`; clamped to max_pages *
+ * page_size):
+ *   out[b,g,i,t] = sum_j softmax_j(scale q[b,g,i,t] . k_j) v_j    over j <= n - T + t, k_j and v_j by b's table
+ * Positions on an entry outside [0, num_pages) are skipped; a query that reads nothing gets zeros. What a later position of the
+ * sequence holds (NaN, infinity) does not reach an output.
+ * runs (int32 [R + 1] on the device, ascending; null with R = 1: all sequences): the tables of sequences runs[r] .. runs[r + 1]
+ * - 1 name the same pages below prefix_lengths[r] (int32 [R] on the device, or null: prefix_length) rounded down to whole pages;
+ * they are read by the first one's table, once for all. A run begins no earlier than the largest bound before it. A sequence in no
+ * run, or of which some query does not see the whole of that prefix, reads everything by its own table.
+ * q, out: [B, G, h, T, 128] bf16 contiguous, 16-byte aligned, 1 <= h <= 16; block_table [B, bt_stride]. wide: the shared part by
+ * workgroups of 128 (sequence, query, head) rows instead of 16. shared_splits (0: no shared part, every sequence reads by its own
+ * table; up to 64) and own_splits (1..64): workgroups that share the two parts' keys. Unless they are 0 and 1, part (16-byte
+ * aligned, attnlab_shared_part_bytes bytes) holds the partials and a last launch merges them.
+ */
+int64_t attnlab_shared_part_bytes(int B, int G, int h, int T, int shared_splits, int own_splits);
+int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages, int num_pages,
+                                 int page_size, const int32_t* block_table, int64_t bt_stride, int max_pages,
+                                 const int32_t* lengths, int length, const int32_t* prefix_lengths, int prefix_length,
+                                 const int32_t* runs, int R, int B, int G, int h, int T, float scale, int wide,
+                                 int shared_splits, int own_splits, uint16_t* out, float* part, int64_t part_bytes,
+                                 void* stream);
+
+/*
  * Log probabilities of given tokens, the entropy and the most likely alternatives of N rows of V logits (no reference
  * counterpart: its scripts take log_softmax on the host). Row r at logits + r stride (elements of `dtype`: ATTNLAB_DT_BF16,
  * _F16 or _F32, aligned to it; any stride). With lse = log sum_j exp(x_j):
