@@ -16,18 +16,18 @@ WIDE_ROWS, NARROW_ROWS = 128, 16   # (query, head) rows of a workgroup of either
 MAX_SPLITS = 64
 
 
-def shared_splits(G: int, rows: int, runs: int, keys: int, wide: bool) -> int:
-    """Key splits of the shared part: `rows` (query, head) rows of a group over all sequences, `runs` prompts of `keys` positions."""
-    per = WIDE_ROWS if wide else NARROW_ROWS
-    tiles = G * (rows // per + (runs + 1) // 2)
-    return max(1, min(MAX_SPLITS, (512 if wide else 768) // max(tiles, 1), keys // 256))
+def shared_splits(G: int, rows: int, wide: bool) -> int:
+    """Partials of the shared part that a row's room is made for, `rows` (query, head) rows of a group over all sequences: the
+    workgroups that come to a tile of rows if all sequences share, and a piece."""
+    per, workers = (WIDE_ROWS, 512) if wide else (NARROW_ROWS, 768)
+    return min(MAX_SPLITS, workers // (G * -(-rows // per)) + 2)
 
 
 def own_splits(BG: int, rows: int, keys: int) -> int:
     """Key splits of the own part: `rows` rows of each of BG (sequence, group) pairs over up to `keys` positions."""
     wide = rows > MAX_H_CHUNK
     tiles = BG * -(-rows // (WIDE_ROWS if wide else NARROW_ROWS))
-    return max(1, min(16, (512 if wide else 768) // tiles, keys // 256))
+    return max(1, min(16, (512 if wide else 384) // tiles, keys // 256))
 
 
 def _lengths(x, n: int, device, name: str):
@@ -56,8 +56,8 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
     with a length per sequence.
 
     Nothing is read back to the host, so a captured graph follows the tensors' later values. Weights are rounded to bfloat16
-    before their product with V (2^-8 of each at most; their sum is not rounded), sums are float32. partitions overrides the key
-    split counts (shared part, own part), 1 to 64 each (0 shared: the prefix is ignored)."""
+    before their product with V (2^-8 of each at most; their sum is not rounded), sums are float32. partitions overrides how
+    many partials a row may have of the shared part (1 to 64; 0: the prefix is ignored) and of the own one (1 to 64)."""
     if (k_pages.dim() != 4 or k_pages.dtype != torch.bfloat16 or not k_pages.is_contiguous() or k_pages.shape[3] != HEAD_DIM
             or not k_pages.is_cuda):
         raise ValueError(f"k_pages must be a contiguous bfloat16 [num_pages, G, page_size, {HEAD_DIM}] pool on a HIP device")
@@ -87,19 +87,19 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
     prefix_at, prefix = _lengths(prefix_lengths, R, device, "prefix_lengths")
     most = W * page if lengths_at else min(length, W * page)
     keys = most if prefix_at else min(prefix, most) // page * page
+    q, q_at = aligned_query(q)
+    out = check_out(out, q, torch.bfloat16)
+    if T == 0:
+        return out
     rows = B * h * T
-    wide = rows > NARROW_ROWS * R
+    wide = T > 1 or rows > NARROW_ROWS * R
     if partitions is None:
-        ns = shared_splits(G, rows, R, keys, wide) if keys else 0
+        ns = shared_splits(G, rows, wide) if keys else 0
         no = own_splits(B * G, h * T if T > 1 else 1, most if prefix_at else most - keys)
     else:
         ns, no = (int(x) for x in partitions)
         if not (0 <= ns <= MAX_SPLITS and 1 <= no <= MAX_SPLITS):
             raise ValueError(f"partitions must be two counts, in [0, {MAX_SPLITS}] and [1, {MAX_SPLITS}]")
-    q, q_at = aligned_query(q)
-    out = check_out(out, q, torch.bfloat16)
-    if T == 0:
-        return out
     nbytes = nat.lib().attnlab_shared_part_bytes(B, G, h, T, ns, no)
     part = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
     nat.call_on(device, "attnlab_shared_prefix_attend", q_at, k_pages.data_ptr(), v_pages.data_ptr(), pages, page,

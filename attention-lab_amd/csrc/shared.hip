@@ -7,13 +7,19 @@
 // A sequence that ends inside its run's prefix takes no part in the shared read and reads all of its positions in the own part, so
 // the shared one has no masked positions at all.
 //
-// Both parts are split over workgroups by keys; every (row, split) leaves a partial, and a last launch merges a row's.
+// Both parts are split over workgroups by keys; each leaves its rows' partials, and a last launch merges a row's. How a prompt's keys
+// are split is worked out on the device, from runs and prefixes that the host need not know: the blocks of all tiles of rows over the
+// workgroups that the chip holds at once give a share; a tile's whole shares go first, and what is left of the tiles, shorter
+// pieces, fills the gaps. A count beside each row says how many partials it has.
 //
 // Two kernels. `wide`: 128 rows, four waves of 32; blocks of 64 keys, S^T = K Q^T, the softmax on its accumulators, O^T += V^T P^T
 // (v_mfma_f32_32x32x16_bf16), K and V copied into LDS a block ahead without passing through registers. `narrow`: up to 16 rows;
 // each wave walks tiles of 32 keys of its own (v_mfma_f32_16x16x32_bf16), K from memory to the matrix core, V through the wave's
-// LDS. Both look a key's page up a block ahead, one entry a lane, so pages may be of any size and end anywhere in a block; a
-// key without a page is read as zeros and masked.
+// LDS. A part begins at a page's first position, so in pages of 16 positions or more every 16 keys of a block share one: its entry is
+// looked up a block ahead, and the 16 rows are a buffer that ends where they do (or at once, where there is no page), behind which
+// loads give zeros. Smaller pages are looked up key by key. Keys without a row are masked.
+//
+// One launch does both parts, the own part's workgroups behind the shared part's.
 //
 // Weights are rounded to bf16, the operand's type, before their product with V; their sum is of the unrounded ones, sums fp32.
 #include <cfloat>
@@ -31,7 +37,8 @@ constexpr int kTile = 32;                   // keys of a narrow wave's tile
 constexpr int kWaves = 4;
 constexpr float kLazy = 8.0f;               // a row's shift is set 2^8 above its largest score and moves when one passes it
 constexpr int kPart = 132;                  // m, l, two unused words, the 128 unnormalised outputs
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 64;              // partials that a row has of either part, at most
+constexpr int kWideWorkers = 512, kNarrowWorkers = 768;   // shares of the shared part: two workgroups per CU, or three
 
 struct SharedArgs {
     const uint16_t* q;        // [B, G, h, T, 128]
@@ -46,9 +53,10 @@ struct SharedArgs {
     int B, G, h, T, W, R, pages, shift;
     float scale_log2;
     uint16_t* out;            // [B, G, h, T, 128]
-    float* part;              // [B, G, h, T, shared + own, 132]
-    int shared, own;          // key splits of the two parts
-    int tiles;                // row tiles of the shared part, at most
+    float* part;              // [B, G, h, T, shared + own, 132], or null: the own part's one partial is the output
+    int2* counts;             // [B, G, h, T] partials that a row has of the two parts
+    int shared, own;          // partials of the two parts that there is room for (shared 0: no shared part)
+    int own_items, shared_turns, own_turns;   // workgroups of the own part, and an eighth of those of either
 };
 
 // What a masked key's row is read from.
@@ -67,56 +75,49 @@ struct Run {
     int first, count, prefix;   // its sequences; its whole pages' positions (0: nothing shared)
 };
 
-// Calls step(runs of 64 lanes, how many) until it returns true: lane x holds run r0 + x. Runs are [S_r, S_{r+1}) with S_r the
-// largest of runs[0 .. r] within [0, B], so they never overlap.
-template <typename Step>
-__device__ __forceinline__ void walk_runs(const SharedArgs& a, Step step) {
-    const int lane = threadIdx.x & 63;
-    int before = a.runs ? min(max(a.runs[0], 0), a.B) : 0;
-    for (int r0 = 0; r0 < a.R; r0 += 64) {
-        const int r = r0 + lane;
-        int upto = a.runs ? (r < a.R ? min(max(a.runs[r + 1], 0), a.B) : 0) : a.B;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int x = __shfl_up(upto, d, 64);
-            if (lane >= d) upto = max(upto, x);
-        }
-        upto = max(upto, before);
-        int from = __shfl_up(upto, 1, 64);
-        if (lane == 0) from = before;
+// Inclusive running maximum over the wave's lanes, of values of at least 0.
+__device__ __forceinline__ int wave_incl_max(int x) {
+    auto up = [&](uint32_t y) { x = max(x, (int)y); };
+    up(dpp_u32_or_zero<0x111, 0xf>((uint32_t)x));
+    up(dpp_u32_or_zero<0x112, 0xf>((uint32_t)x));
+    up(dpp_u32_or_zero<0x114, 0xf>((uint32_t)x));
+    up(dpp_u32_or_zero<0x118, 0xf>((uint32_t)x));
+    up(dpp_u32_or_zero<0x142, 0xa>((uint32_t)x));
+    up(dpp_u32_or_zero<0x143, 0xc>((uint32_t)x));
+    return x;
+}
+
+// The runs, 64 at a time: lane x holds run 64 i + x. Run r is [S_r, S_{r+1}) with S_r the largest of runs[0 .. r] within [0, B], so
+// they never overlap. Up to 64 stay in registers.
+struct Runs {
+    Run own;       // of the first 64
+    int after;     // where those end
+    __device__ __forceinline__ static Run load(const SharedArgs& a, int r0, int& before) {
+        const int lane = threadIdx.x & 63, r = min(r0 + lane, a.R - 1);   // past the last: that one again, empty
+        int upto = a.runs ? min(max(a.runs[r + 1], 0), a.B) : a.B;
+        const int prefix = prefix_of(a, r);      // loaded with the bound, not behind it
+        upto = max(wave_incl_max(upto), before);
+        const int left = __shfl_up(upto, 1, 64), from = lane == 0 ? before : left;
         before = __builtin_amdgcn_readlane(upto, 63);
-        Run run{from, r < a.R ? upto - from : 0, 0};
-        if (run.count > 0) run.prefix = prefix_of(a, r);
-        if (step(run)) return;
+        return Run{from, upto - from, prefix};
     }
-}
-__device__ __forceinline__ Run lane_run(const Run& run, int at) {
-    return Run{__builtin_amdgcn_readlane(run.first, at), __builtin_amdgcn_readlane(run.count, at),
-               __builtin_amdgcn_readlane(run.prefix, at)};
-}
-// The run of row tile `tile` (of `rows` rows) of the shared part, and the tile's number in it; count 0: none.
-__device__ __forceinline__ Run run_of_tile(const SharedArgs& a, int tile, int rows, int& in_run) {
-    Run found{0, 0, 0};
-    int base = 0;
-    walk_runs(a, [&](const Run& run) {
-        const uint32_t tiles = run.prefix > 0 ? (uint32_t)(((int64_t)run.count * a.T * a.h + rows - 1) / rows) : 0u;
-        const uint32_t upto = wave_incl_scan(tiles) + (uint32_t)base;
-        const uint64_t hit = __ballot((int)upto > tile);
-        if (hit) {
-            const int at = __builtin_ctzll(hit);
-            found = lane_run(run, at);
-            in_run = tile - (__builtin_amdgcn_readlane((int)upto, at) - __builtin_amdgcn_readlane((int)tiles, at));
-            return true;
-        }
-        base = __builtin_amdgcn_readlane((int)upto, 63);
-        return false;
-    });
-    return found;
-}
+    __device__ __forceinline__ explicit Runs(const SharedArgs& a) {
+        after = a.runs ? min(max(a.runs[0], 0), a.B) : 0;
+        own = load(a, 0, after);
+    }
+    // step(64 runs, a lane's one each) until it returns true
+    template <typename Step>
+    __device__ __forceinline__ void walk(const SharedArgs& a, Step step) const {
+        if (step(own)) return;
+        int before = after;
+        for (int r0 = 64; r0 < a.R; r0 += 64)
+            if (step(load(a, r0, before))) return;
+    }
+};
 // The shared positions of sequence b's run (0: none).
 __device__ __forceinline__ int prefix_of_sequence(const SharedArgs& a, int b) {
     int found = 0;
-    walk_runs(a, [&](const Run& run) {
+    Runs(a).walk(a, [&](const Run& run) {
         const uint64_t hit = __ballot(run.count > 0 && run.first <= b && b < run.first + run.count);
         if (hit) found = __builtin_amdgcn_readlane(run.prefix, __builtin_ctzll(hit));
         return hit != 0;
@@ -127,65 +128,125 @@ __device__ __forceinline__ int prefix_of_sequence(const SharedArgs& a, int b) {
 __device__ __forceinline__ bool sees(const SharedArgs& a, int b, int prefix) { return length_of(a, b) - a.T + 1 >= prefix; }
 
 // What a workgroup does: `rows` rows from row r0 of `count` sequences from b0 on, over the blocks [i0, i1) of the keys [base, end)
-// of sequence b0's table, its partials in slot `slot`.
+// of sequence b0's table, its partials in slot `slot`. partials > 0: it says that the rows have so many of this part.
 struct Item {
-    int b0, count, r0, rows, base, end, i0, i1, slot, g;
+    int b0, count, r0, rows, base, end, i0, i1, slot, partials, g;
     bool shared;
 };
+
+constexpr int kLeastBlocks = 4, kLeastTiles = 8;   // a share is of 256 keys at least
+constexpr uint32_t kLongBlocks = 64;
+
+// The shared part's workgroup `turn` of XCD `xcd`: a group, a run, a share of its blocks of kBlock keys, and a tile of kRows of its
+// rows. The tiles that read the same keys lie next to each other, on one XCD. False: there are fewer.
 template <int kRows, int kBlock>
-__device__ __forceinline__ bool item_of(const SharedArgs& a, int lin, Item& w) {
-    const int shared_items = a.G * a.shared * a.tiles;
-    int split, splits;
-    if (lin < shared_items) {   // the tiles that read the same keys lie next to each other, on one XCD
-        const int gs = lin / a.tiles;
-        int tile = 0;
-        const Run run = run_of_tile(a, lin - gs * a.tiles, kRows, tile);
-        if (run.count == 0) return false;
-        w.g = gs / a.shared;
-        split = gs - w.g * a.shared;
-        splits = a.shared;
-        w.b0 = run.first;
-        w.count = run.count;
-        w.r0 = tile * kRows;
-        w.base = 0;
-        w.end = run.prefix;
-        w.slot = split;
-        w.shared = true;
-    } else {
-        lin -= shared_items;
-        const int tiles = (a.T * a.h + kRows - 1) / kRows;
-        split = lin % a.own;
-        lin /= a.own;
-        const int tile = tiles - 1 - lin % tiles;   // later queries read more keys: first
-        lin /= tiles;
-        w.g = lin % a.G;
-        w.b0 = lin / a.G;
-        w.count = 1;
-        w.r0 = tile * kRows;
-        const int prefix = a.shared ? prefix_of_sequence(a, w.b0) : 0, n = length_of(a, w.b0);
-        w.base = sees(a, w.b0, prefix) ? prefix : 0;
-        w.end = max(n - a.T + min(a.T - 1, (w.r0 + kRows - 1) / a.h) + 1, w.base);
-        splits = a.own;
-        w.slot = a.shared + split;
-        w.shared = false;
-        // nobody else writes the shared slots of a sequence that shares nothing
-        if (prefix == 0 && a.shared && split == 0) {
-            const int rows = min(kRows, a.T * a.h - w.r0);
-            for (int x = threadIdx.x; x < rows * a.shared; x += 64 * kWaves) {
-                const int row = w.r0 + x / a.shared, t = row / a.h, head = row - t * a.h;
-                float* pp = a.part + ((((size_t)w.b0 * a.G + w.g) * a.h + head) * a.T + t) * (a.shared + a.own) * kPart +
-                            (size_t)(x % a.shared) * kPart;
-                pp[0] = -INFINITY;
-                pp[1] = 0.0f;
-            }
-        }
+__device__ __forceinline__ bool shared_item(const SharedArgs& a, int xcd, int turn, Item& w) {
+    auto tiles = [&](const Run& r) { return r.prefix > 0 ? (uint32_t)(((int64_t)r.count * a.T * a.h + kRows - 1) / kRows) : 0u; };
+    auto blocks = [&](const Run& r) { return (uint32_t)(r.prefix + kBlock - 1) / kBlock; };
+    auto sum = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_incl_scan(x), 63); };
+    // the blocks of all tiles (sums of 16, 24 and 24 bits of them), and of the longest
+    const Runs runs(a);
+    constexpr uint32_t kWorkers = kRows == kWide ? kWideWorkers : kNarrowWorkers;
+    uint64_t total = 0;
+    uint32_t longest = 1;
+    runs.walk(a, [&](const Run& run) {
+        const uint32_t n = tiles(run), k = blocks(run);
+        const uint64_t own = (uint64_t)n * k;
+        total += sum((uint32_t)own & 0xffffu) + ((uint64_t)sum((uint32_t)(own >> 16) & 0xffffffu) << 16) +
+                 ((uint64_t)sum((uint32_t)(own >> 40)) << 40);
+        longest = max(longest, (uint32_t)__builtin_amdgcn_readlane(wave_incl_max(n ? (int)k : 0), 63));
+        return false;
+    });
+    // a share: even over the workgroups in as many rounds as the tiles would take whole. In several rounds only where a tile is long
+    // enough for a second partial of its rows to pay
+    total *= a.G;
+    uint32_t share = longest;
+    if (total <= (uint64_t)kWorkers * longest) {
+        share = (uint32_t)((total + kWorkers - 1) / kWorkers);
+    } else if (longest >= kLongBlocks && total < (uint64_t)kWorkers * longest * 8) {
+        const uint32_t rounds = (uint32_t)((total + (uint64_t)kWorkers * longest - 1) / ((uint64_t)kWorkers * longest));
+        share = (uint32_t)(total / ((uint64_t)kWorkers * rounds)) + 1;
     }
+    share = min(longest, max(max(share, (longest + a.shared - 1) / a.shared), (uint32_t)(kBlock == kKeys ? kLeastBlocks : kLeastTiles)));
+    // whole shares of a group, and pieces
+    uint32_t whole = 0, pieces = 0;
+    runs.walk(a, [&](const Run& run) {
+        const uint32_t n = tiles(run), k = blocks(run);
+        whole += sum(n * (k / share));
+        pieces += sum(k % share ? n : 0u);
+        return false;
+    });
+    const uint32_t turns = (whole * a.G + 7) / 8, piece_turns = (pieces * a.G + 7) / 8;
+    const bool piece = (uint32_t)turn >= turns;
+    const uint32_t lin = piece ? xcd * piece_turns + turn - turns : xcd * turns + turn, group = piece ? pieces : whole;
+    if (piece && (uint32_t)turn - turns >= piece_turns) return false;
+    if (lin >= group * a.G) return false;
+    w.g = (int)(lin / group);
+    uint32_t rest = lin - w.g * group;
+    runs.walk(a, [&](const Run& run) {
+        const uint32_t n = tiles(run), k = blocks(run), full = k / share, mine = piece ? (k % share ? n : 0u) : n * full;
+        const uint32_t upto = wave_incl_scan(mine);
+        const uint64_t hit = __ballot(upto > rest);
+        if (!hit) {
+            rest -= (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+            return false;
+        }
+        const int x = __builtin_ctzll(hit);
+        auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, x); };
+        const uint32_t at = rest - of(upto - mine), part = piece ? of(full) : at / of(n), tile = piece ? at : at - part * of(n);
+        w.b0 = (int)of(run.first);
+        w.count = (int)of(run.count);
+        w.end = (int)of(run.prefix);
+        w.r0 = (int)tile * kRows;
+        w.slot = (int)part;
+        w.i0 = (int)(part * share);
+        w.i1 = (int)min((uint32_t)w.i0 + share, of(k));
+        w.partials = part == 0 ? (int)((of(k) + share - 1) / share) : 0;
+        return true;
+    });
     w.rows = (int)min((int64_t)w.count * a.T * a.h - w.r0, (int64_t)kRows);
-    const int blocks = (w.end - w.base + kBlock - 1) / kBlock, share = (blocks + splits - 1) / splits;
-    w.i0 = min(split * share, blocks);
-    w.i1 = min(w.i0 + share, blocks);
+    w.base = 0;
+    w.shared = true;
     return true;
 }
+
+// The own part: false where the sequence has no keys for this split.
+template <int kRows, int kBlock>
+__device__ __forceinline__ bool own_item(const SharedArgs& a, int lin, Item& w) {
+    const int tiles = (a.T * a.h + kRows - 1) / kRows;
+    const int split = lin % a.own;
+    lin /= a.own;
+    w.r0 = (tiles - 1 - lin % tiles) * kRows;   // later queries read more keys: first
+    lin /= tiles;
+    w.g = lin % a.G;
+    w.b0 = lin / a.G;
+    w.count = 1;
+    w.rows = min(a.T * a.h - w.r0, kRows);
+    const int n = length_of(a, w.b0), prefix = a.shared ? prefix_of_sequence(a, w.b0) : 0;
+    w.base = n - a.T + 1 >= prefix ? prefix : 0;
+    w.end = max(n - a.T + min(a.T - 1, (w.r0 + kRows - 1) / a.h) + 1, w.base);
+    const int blocks = (w.end - w.base + kBlock - 1) / kBlock;
+    const int share = max((blocks + a.own - 1) / a.own, kBlock == kKeys ? kLeastBlocks : kLeastTiles);
+    w.i0 = split * share;
+    if (split > 0 && w.i0 >= blocks) return false;
+    w.i1 = min(w.i0 + share, blocks);
+    w.slot = a.shared + split;
+    w.partials = split == 0 ? max((blocks + share - 1) / share, 1) : 0;
+    w.shared = false;
+    // nobody else counts the shared partials of a sequence that shares nothing
+    if (a.part && prefix == 0 && split == 0)
+        for (int x = threadIdx.x; x < w.rows; x += 64 * kWaves) {
+            const int t = (w.r0 + x) / a.h, head = w.r0 + x - t * a.h;
+            a.counts[(((size_t)w.b0 * a.G + w.g) * a.h + head) * a.T + t].x = 0;
+        }
+    return true;
+}
+// A row's count of this part's partials: none where the sequence takes no part in the shared read.
+__device__ __forceinline__ void count_partials(const SharedArgs& a, const Item& w, size_t row, bool dead) {
+    if (w.shared) a.counts[row].x = dead ? 0 : w.partials;
+    else a.counts[row].y = w.partials;
+}
+
 struct Row {
     int b, t, head;
     __device__ __forceinline__ Row(const SharedArgs& a, const Item& w, int r) {
@@ -199,17 +260,25 @@ struct Row {
     }
 };
 
-// This lane's key's page (key `key` of sequence b's table), or -1.
-__device__ __forceinline__ int page_of(const SharedArgs& a, const int32_t* row, int key, int end) {
-    if (key >= end) return -1;
-    const int p = row[key >> a.shift];
-    return (uint32_t)p < (uint32_t)a.pages ? p : -1;
-}
-// The address of key `key` in page p, or zeros.
+// The address of key `key`'s row in page p of group g, `chunk` bytes in; zeros where p names none.
 __device__ __forceinline__ const char* key_row(const SharedArgs& a, const uint16_t* pool, int p, int g, int key, int chunk) {
-    const size_t row = (((size_t)(uint32_t)p * a.G + g) << a.shift) + (key & ((1 << a.shift) - 1));
-    return p < 0 ? reinterpret_cast<const char*>(shared_zeros) : reinterpret_cast<const char*>(pool) + row * (2 * kDim) + chunk;
+    const bool ok = (uint32_t)p < (uint32_t)a.pages;
+    const size_t row = (((size_t)(ok ? p : 0) * a.G + g) << a.shift) + (key & ((1 << a.shift) - 1));
+    uint64_t at = reinterpret_cast<uint64_t>(pool) + row * (2 * kDim) + chunk;
+    asm volatile("" : "+v"(at));   // computed by every lane: a select, not a branch
+    return reinterpret_cast<const char*>(ok ? at : reinterpret_cast<uint64_t>(shared_zeros));
 }
+// Sixteen rows of a page from key k16 on, or fewer up to `end`, or none: where they lie and how many bytes.
+struct Sixteen {
+    size_t at;
+    uint32_t rows;
+    __device__ __forceinline__ Sixteen(const SharedArgs& a, int p, int g, int k16, int end) {
+        rows = (uint32_t)p < (uint32_t)a.pages ? (uint32_t)min(max(end - k16, 0), 16) : 0u;
+        at = (size_t)((((uint32_t)p * a.G + g) << a.shift) + (k16 & ((1 << a.shift) - 1))) * kDim;
+    }
+    __device__ __forceinline__ uint32_t bytes() const { return rows * 2 * kDim; }
+    __device__ __forceinline__ uint32_t have() const { return (1u << rows) - 1u; }
+};
 
 // The scale (log2 domain), made positive: a negative one flips the sign of q instead (exact), and zero becomes the smallest normal
 // float, which gives the same weights while a masked key's -inf * scale stays -inf.
@@ -226,13 +295,9 @@ __device__ __forceinline__ uint32_t bf16x2_finite(uint32_t w, uint32_t& flags) {
 // row j at slot c ^ (j & 15) (a read takes 16 rows, one chunk), V's at c ^ (4 (j & 3)) (a transposing read takes 4 chunks of 4
 // consecutive rows). Key 16 z + 8 g + 4 a + b of a 32-key tile is row 16 z + 8 a + 4 g + b of its product, so that a lane's weights
 // are those of eight consecutive keys, the ones whose V its operand holds.
-__global__ __launch_bounds__(256, 2) void shared_wide(SharedArgs a, int first_item) {
+template <bool SMALL>
+__device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* kt0, char* vt0, char* kt1, char* vt1, int& again) {
     constexpr int kRow = 2 * kDim;
-    __shared__ __attribute__((aligned(1024))) char kt0[kKeys * kRow], vt0[kKeys * kRow];
-    __shared__ __attribute__((aligned(1024))) char kt1[kKeys * kRow], vt1[kKeys * kRow];
-    __shared__ int again;
-    Item w;
-    if (!item_of<kWide, kKeys>(a, __builtin_amdgcn_readfirstlane(xcd_contiguous_block()) + first_item, w)) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, g = lane >> 5;
@@ -256,15 +321,35 @@ __global__ __launch_bounds__(256, 2) void shared_wide(SharedArgs a, int first_it
     const int kchunk = 16 * (slot ^ (4 * wave + srow)), vchunk = 16 * (slot ^ (4 * srow));
     const int32_t* pages = a.table + (size_t)w.b0 * a.table_stride;
     auto first_key = [&](int i) { return w.base + kKeys * i; };
-    auto look = [&](int i) { return i < w.i1 ? page_of(a, pages, first_key(i) + lane, w.end) : -1; };
-    auto copy = [&](int kb, int page, char* kt, char* vt) {
+    // the entries of block i's pages, as they stand in the table: lane u of four that of keys 16 u .., or lane j key j's
+    auto look = [&](int i) {
+        const int key = first_key(min(i, w.i1 - 1)) + (SMALL ? lane : 16 * (lane & 3));
+        return pages[min(key, w.end - 1) >> a.shift];
+    };
+    // block i's copies; which of its keys have a row, a bit each
+    auto copy = [&](int kb, int entry, char* kt, char* vt) -> uint64_t {
+        if constexpr (SMALL) {
+            const int page = kb + lane < w.end ? entry : -1;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int j = 16 * u + 4 * wave + srow, p = __shfl(page, j, 64);
-            load_lds16(reinterpret_cast<const uint16_t*>(key_row(a, a.K, p, w.g, kb + j, kchunk)),
-                       reinterpret_cast<uint16_t*>(kt + 4096 * u + 1024 * wave));
-            load_lds16(reinterpret_cast<const uint16_t*>(key_row(a, a.V, p, w.g, kb + j, vchunk)),
-                       reinterpret_cast<uint16_t*>(vt + 4096 * u + 1024 * wave));
+            for (int u = 0; u < 4; ++u) {
+                const int j = 16 * u + 4 * wave + srow, p = __shfl(page, j, 64);
+                load_lds16(reinterpret_cast<const uint16_t*>(key_row(a, a.K, p, w.g, kb + j, kchunk)),
+                           reinterpret_cast<uint16_t*>(kt + 4096 * u + 1024 * wave));
+                load_lds16(reinterpret_cast<const uint16_t*>(key_row(a, a.V, p, w.g, kb + j, vchunk)),
+                           reinterpret_cast<uint16_t*>(vt + 4096 * u + 1024 * wave));
+            }
+            return __ballot((uint32_t)page < (uint32_t)a.pages);
+        } else {
+            uint64_t have = 0;
+            const uint32_t at = kRow * (4 * wave + srow);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const Sixteen r(a, __builtin_amdgcn_readlane(entry, u), w.g, kb + 16 * u, w.end);
+                load_lds16_buf(a.K + r.at, r.bytes(), at + kchunk, reinterpret_cast<uint16_t*>(kt + 4096 * u + 1024 * wave));
+                load_lds16_buf(a.V + r.at, r.bytes(), at + vchunk, reinterpret_cast<uint16_t*>(vt + 4096 * u + 1024 * wave));
+                have |= (uint64_t)r.have() << (16 * u);
+            }
+            return have;
         }
     };
     // operand reads, as byte offsets into a tile. K: this lane's key of a 32-key tile, chunk 2 kk + g. V: rows 16 ks + 8 g + 4 hf +
@@ -434,27 +519,36 @@ __global__ __launch_bounds__(256, 2) void shared_wide(SharedArgs a, int first_it
     // Two tile pairs: the next block's copies are issued when every wave has left the tiles they overwrite, the barrier that also
     // publishes the current block, and land while it is computed; its pages were looked up a block before that.
     uint64_t have = 0;
-    int next = look(w.i0);
+    int next = 0;
     auto issue = [&](int i, char* kt, char* vt) {   // block i's copies; the pages of block i + 1
-        const int page = next;
+        const int entry = next;
         next = look(i + 1);
-        copy(first_key(i), page, kt, vt);
-        return (uint64_t)__ballot(page >= 0);
+        return copy(first_key(i), entry, kt, vt);
     };
-    auto publish = [&]() {
-        __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0): this wave's copies have landed, its reads are done
+    auto publish = [&](bool first_of_two) {
+        // this wave's copies have landed (of the first two blocks, issued at once, the first one's: the second's eight may
+        // still be on their way), its reads are done
+        if (first_of_two) __builtin_amdgcn_s_waitcnt(0x0078);   // vmcnt(8) lgkmcnt(0)
+        else __builtin_amdgcn_s_waitcnt(0x0070);                // vmcnt(0) lgkmcnt(0)
         asm volatile("s_barrier" ::: "memory");
         pin();
     };
     if (tid == 0) again = 0;   // published by the first block's barrier
-    if (w.i0 < w.i1) have = issue(w.i0, kt0, vt0);
+    uint64_t second = 0;
+    if (w.i0 < w.i1) {
+        next = look(w.i0);
+        have = issue(w.i0, kt0, vt0);
+        if (w.i0 + 1 < w.i1) second = issue(w.i0 + 1, kt1, vt1);
+    }
     for (int i = w.i0; i < w.i1; i += 2) {
-        publish();
+        const bool begun = i == w.i0;
+        publish(begun && i + 1 < w.i1);
         uint64_t now = have;
-        if (i + 1 < w.i1) have = issue(i + 1, kt1, vt1);
+        if (begun) have = second;
+        else if (i + 1 < w.i1) have = issue(i + 1, kt1, vt1);
         block(std::false_type{}, first_key(i), now, kt0, vt0);
         if (i + 1 >= w.i1) break;
-        publish();
+        publish(false);
         now = have;
         if (i + 2 < w.i1) have = issue(i + 2, kt0, vt0);
         block(std::false_type{}, first_key(i + 1), now, kt1, vt1);
@@ -477,10 +571,10 @@ __global__ __launch_bounds__(256, 2) void shared_wide(SharedArgs a, int first_it
             for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
-            next = look(w.i0);
+            if (w.i0 < w.i1) next = look(w.i0);
             for (int i = w.i0; i < w.i1; ++i) {
                 have = issue(i, kt0, vt0);
-                publish();
+                publish(false);
                 block(std::true_type{}, first_key(i), have, kt0, vt0);
                 __syncthreads();
             }
@@ -488,12 +582,13 @@ __global__ __launch_bounds__(256, 2) void shared_wide(SharedArgs a, int first_it
     }
     const float l_tot = l_run + shfl_xor_f32(l_run, 32);
     if (R >= w.rows) return;
-    const int slots = a.shared + a.own;
-    if (slots > 1) {
-        float* pp = a.part + (row.at(a, w.g) * slots + w.slot) * kPart;
+    if (a.part) {
+        const size_t at = row.at(a, w.g);
+        float* pp = a.part + (at * (a.shared + a.own) + w.slot) * kPart;
         if (g == 0) {
-            pp[0] = dead ? -INFINITY : m_run;
-            pp[1] = dead ? 0.0f : l_tot;
+            pp[0] = m_run;
+            pp[1] = l_tot;
+            if (w.partials) count_partials(a, w, at, dead);
         }
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
@@ -514,20 +609,19 @@ __global__ __launch_bounds__(256, 2) void shared_wide(SharedArgs a, int first_it
                          pack_bf16x2(o[dt][4 * i4 + 2] * inv, o[dt][4 * i4 + 3] * inv)};
 }
 
-// One tile of a wave: K's rows krow and krow + 4, 16 bytes of every 64; V's rows 4 u + lane / 16.
+// `low`, `high`: 32 KB of LDS in two halves, a wave's V tile in 8 KB of them, then the merge. AHEAD: a tile is on its way while
+// another is computed, where registers allow it anyway.
 struct Tile {
     u32x4_t k[2][4], v[8];
+    uint32_t have;
 };
-
-__global__ __launch_bounds__(64 * kWaves, 3) void shared_narrow(SharedArgs a, int first_item) {
+template <bool SMALL, bool AHEAD>
+__device__ __forceinline__ void narrow(const SharedArgs& a, const Item& w, char* low, char* high, float (*ml_sh)[kNarrow][2]) {
     constexpr int kRow = 2 * kDim;
-    __shared__ __attribute__((aligned(1024))) uint16_t v_sh[kWaves][kTile * kDim];   // a wave's V tile; then the merge
-    __shared__ float ml_sh[kWaves][kNarrow][2];
-    Item w;
-    if (!item_of<kNarrow, kTile>(a, __builtin_amdgcn_readfirstlane(xcd_contiguous_block()) + first_item, w)) return;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, g4 = lane >> 4;
+    auto tile_of = [&](int x) { return (x < 2 ? low : high) + kTile * kRow * (x & 1); };
     // Q^T as the B operand: column n16 is the workgroup's row n16 (past the last: that one again)
     bf16x8_t qb[4];
     const float sc = positive_scale(a.scale_log2);
@@ -540,14 +634,15 @@ __global__ __launch_bounds__(64 * kWaves, 3) void shared_narrow(SharedArgs a, in
             qb[kk] = __builtin_bit_cast(bf16x8_t, x);
         }
     }
-    const int krow = 8 * (n16 >> 2) + (n16 & 3), vrow = lane >> 4;
-    // V in LDS: chunk c of row r at c ^ (4 (r % 4)), so that the rows a transposing read takes together lie in different banks
-    // (lane 4 e + j of 16 reads four elements of row 8 g4 + 4 t + e, and gets 4 rows)
-    char* vt = reinterpret_cast<char*>(v_sh[wave]);
-    const int vst = 256 * vrow + 16 * (n16 ^ (4 * vrow));
+    // Tile t2 of a product holds keys 16 t2 .. + 15, so a lane's weights are of keys 4 g4 .. + 3 and 16 + 4 g4 .. + 3: the rows
+    // whose V it reads. V in LDS: chunk c of row r at c ^ (4 (r % 4)), so that the rows a transposing read takes together lie in
+    // different banks (lane 4 e + j of 16 reads four elements of row 4 g4 + e, and gets 4 rows).
+    const int vrow = lane >> 4;
+    char* vt = tile_of(wave);
+    const int vst = kRow * vrow + 16 * (n16 ^ (4 * vrow));
     int vof[4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) vof[x] = 256 * (8 * g4 + (n16 >> 2)) + 64 * (x ^ (n16 >> 2)) + 8 * (n16 & 3);
+    for (int x = 0; x < 4; ++x) vof[x] = kRow * (4 * g4 + (n16 >> 2)) + 64 * (x ^ (n16 >> 2)) + 8 * (n16 & 3);
 
     float m = -INFINITY, l = 0.0f;
     f32x4_t o[8];
@@ -555,29 +650,56 @@ __global__ __launch_bounds__(64 * kWaves, 3) void shared_narrow(SharedArgs a, in
     for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
     const int32_t* pages = a.table + (size_t)w.b0 * a.table_stride;
-    auto look = [&](int i) { return i < w.i1 ? page_of(a, pages, w.base + kTile * i + (lane & 31), w.end) : -1; };
-    int next = look(w.i0 + wave);
-    for (int i = w.i0 + wave; i < w.i1; i += kWaves) {
-        const int page = next, kb = w.base + kTile * i;
-        Tile f;
-#pragma unroll
-        for (int t2 = 0; t2 < 2; ++t2) {
-            const int j = krow + 4 * t2;
-            const char* r = key_row(a, a.K, __shfl(page, j, 64), w.g, kb + j, 16 * g4);
-            const bool none = r == reinterpret_cast<const char*>(shared_zeros);
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                f.k[t2][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(r + (none ? 0 : 64 * c)));
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const int j = 4 * u + vrow;
-            f.v[u] = __builtin_nontemporal_load(
-                reinterpret_cast<const u32x4_t*>(key_row(a, a.V, __shfl(page, j, 64), w.g, kb + j, 16 * n16)));
-        }
+    auto look = [&](int i) {
+        const int key = w.base + kTile * min(i, w.i1 - 1) + (SMALL ? lane & 31 : 16 * (lane & 1));
+        return pages[min(key, w.end - 1) >> a.shift];
+    };
+    int next = w.i0 < w.i1 ? look(w.i0 + wave) : 0;
+    auto issue = [&](int i, Tile& f) {   // tile i's loads, and the pages of the wave's next one
+        const int entry = next, kb = w.base + kTile * i;
         next = look(i + kWaves);
+        if constexpr (SMALL) {
+            const int page = kb + (lane & 31) < w.end ? entry : -1;
+#pragma unroll
+            for (int t2 = 0; t2 < 2; ++t2) {
+                const int j = 16 * t2 + n16;
+                const char* r = key_row(a, a.K, __shfl(page, j, 64), w.g, kb + j, 16 * g4);
+                const int step = r == reinterpret_cast<const char*>(shared_zeros) ? 0 : 64;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) f.k[t2][c] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(r + step * c));
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int j = 4 * u + vrow;
+                f.v[u] = __builtin_nontemporal_load(
+                    reinterpret_cast<const u32x4_t*>(key_row(a, a.V, __shfl(page, j, 64), w.g, kb + j, 16 * n16)));
+            }
+            f.have = (uint32_t)__ballot((uint32_t)page < (uint32_t)a.pages);
+        } else {
+            constexpr int kNt = 2;   // non-temporal
+            f.have = 0;
+#pragma unroll
+            for (int t2 = 0; t2 < 2; ++t2) {
+                const Sixteen r(a, __builtin_amdgcn_readlane(entry, t2), w.g, kb + 16 * t2, w.end);
+                const __amdgpu_buffer_rsrc_t kr =
+                    __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.K + r.at), 0, (int)r.bytes(), 0x00020000);
+                const __amdgpu_buffer_rsrc_t vr =
+                    __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(a.V + r.at), 0, (int)r.bytes(), 0x00020000);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    f.k[t2][c] = __builtin_bit_cast(
+                        u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(kr, kRow * n16 + 16 * g4 + 64 * c, 0, kNt));
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    f.v[4 * t2 + u] = __builtin_bit_cast(
+                        u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, 16 * lane + 1024 * u, 0, kNt));
+                f.have |= r.have() << (16 * t2);
+            }
+        }
         __builtin_amdgcn_sched_barrier(0);   // every load is on its way before the first result is waited for
-        const uint32_t have = (uint32_t)__ballot(page >= 0);
+    };
+    auto compute = [&](const Tile& f) {
+        const uint32_t have = f.have;
         f32x4_t sv[2];
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
@@ -588,13 +710,13 @@ __global__ __launch_bounds__(64 * kWaves, 3) void shared_narrow(SharedArgs a, in
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) *reinterpret_cast<u32x4_t*>(vt + vst + 1024 * u) = f.v[u];
-        // this lane's scores: column n16, keys 8 g4 + 4 t2 + i
+        // this lane's scores: column n16, keys 16 t2 + 4 g4 + e
         if (~have) {
 #pragma unroll
             for (int t2 = 0; t2 < 2; ++t2)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (!(have >> (8 * g4 + 4 * t2 + e) & 1)) sv[t2][e] = -INFINITY;
+                    if (!(have >> (16 * t2 + 4 * g4 + e) & 1)) sv[t2][e] = -INFINITY;
         }
         float bm = -INFINITY;
 #pragma unroll
@@ -628,31 +750,46 @@ __global__ __launch_bounds__(64 * kWaves, 3) void shared_narrow(SharedArgs a, in
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
             const char* r = vt + vof[dt >> 1] + 32 * (dt & 1);
-            const u32x2v_t w0 = read_tr16(r), w1 = read_tr16(r + 4 * kRow);
+            const u32x2v_t w0 = read_tr16(r), w1 = read_tr16(r + 16 * kRow);
             o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, u32x4_t{w0.x, w0.y, w1.x, w1.y}), pb, o[dt],
                                                            0, 0, 0);
         }
         asm volatile("" ::: "memory");
+    };
+    int i = w.i0 + wave;
+    if constexpr (AHEAD) {
+        Tile f0, f1;
+        if (i < w.i1) issue(i, f0);
+        for (; i < w.i1; i += 2 * kWaves) {
+            if (i + kWaves < w.i1) issue(i + kWaves, f1);
+            compute(f0);
+            if (i + kWaves >= w.i1) break;
+            if (i + 2 * kWaves < w.i1) issue(i + 2 * kWaves, f0);
+            compute(f1);
+        }
+    } else {
+        for (; i < w.i1; i += kWaves) {
+            Tile f;
+            issue(i, f);
+            compute(f);
+        }
     }
     l += shfl_xor_f32(l, 16);
     l += shfl_xor_f32(l, 32);
 
-    // the waves' (m, l, O) through LDS: [wave][row][dim] floats, in the V tiles' memory
+    // the waves' (m, l, O) through LDS: [row][dim] floats in each wave's V tile
+    static_assert(kTile * kRow >= kNarrow * kDim * sizeof(float), "the merge lies in the V tiles");
     __syncthreads();
-    float* red = reinterpret_cast<float*>(&v_sh[0][0]);
-    static_assert(sizeof(v_sh) >= kWaves * kNarrow * kDim * sizeof(float), "the merge lies in the V tiles");
     if (g4 == 0) {
         ml_sh[wave][n16][0] = m;
         ml_sh[wave][n16][1] = l;
     }
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt)
-        *reinterpret_cast<f32x4_t*>(red + (wave * kNarrow + n16) * kDim + 16 * dt + 4 * g4) = o[dt];
+        *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(vt) + n16 * kDim + 16 * dt + 4 * g4) = o[dt];
     __syncthreads();
-    const int slots = a.shared + a.own;
     for (int r = wave; r < w.rows; r += kWaves) {   // wave -> row, lane l -> dims 2 l, 2 l + 1
         const Row row(a, w, r);
-        const bool dead = w.shared && !sees(a, row.b, w.end);
         float ms = -INFINITY;
 #pragma unroll
         for (int x = 0; x < kWaves; ++x) ms = fmaxf(ms, ml_sh[x][r][0]);
@@ -662,16 +799,18 @@ __global__ __launch_bounds__(64 * kWaves, 3) void shared_narrow(SharedArgs a, in
         for (int x = 0; x < kWaves; ++x) {
             const float mx = ml_sh[x][r][0], lx = ml_sh[x][r][1];
             const float y = mx == -INFINITY ? (lx == 0.0f ? 0.0f : 1.0f) : fast_exp2(mx - ms);
-            const float2 v = *reinterpret_cast<const float2*>(red + (x * kNarrow + r) * kDim + 2 * lane);
+            const float2 v = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(tile_of(x)) + r * kDim + 2 * lane);
             ls += y * lx;
             os.x += y * v.x;
             os.y += y * v.y;
         }
-        if (slots > 1) {
-            float* pp = a.part + (row.at(a, w.g) * slots + w.slot) * kPart;
+        if (a.part) {
+            const size_t at = row.at(a, w.g);
+            float* pp = a.part + (at * (a.shared + a.own) + w.slot) * kPart;
             if (lane == 0) {
-                pp[0] = dead ? -INFINITY : ms;
-                pp[1] = dead ? 0.0f : ls;
+                pp[0] = ms;
+                pp[1] = ls;
+                if (w.partials) count_partials(a, w, at, w.shared && !sees(a, row.b, w.end));
             }
             *reinterpret_cast<float2*>(pp + 4 + 2 * lane) = os;
         } else {
@@ -681,32 +820,113 @@ __global__ __launch_bounds__(64 * kWaves, 3) void shared_narrow(SharedArgs a, in
     }
 }
 
-// A row's partials merged in their order: thread -> (row, four dims).
-__global__ __launch_bounds__(256) void shared_combine(const float* part, uint16_t* out, int slots, int64_t rows) {
-    const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (item >= rows * 32) return;
-    const int64_t row = item >> 5;
-    const int d4 = 4 * (int)(item & 31);
+// Both parts, the shared one by tiles of 128 rows (WIDE) or 16, the own one too (OWN_WIDE).
+template <bool WIDE, bool OWN_WIDE, bool SMALL>
+__global__ __launch_bounds__(64 * kWaves, WIDE ? 2 : 3) void shared_read(SharedArgs a) {
+    static_assert(WIDE || !OWN_WIDE, "several queries of a sequence are read wide in both parts");
+    __shared__ __attribute__((aligned(1024))) char t0[kKeys * 2 * kDim], t1[kKeys * 2 * kDim];
+    __shared__ __attribute__((aligned(1024))) char t2[WIDE ? kKeys * 2 * kDim : 1], t3[WIDE ? kKeys * 2 * kDim : 1];
+    __shared__ float ml_sh[kWaves][kNarrow][2];
+    __shared__ int again;
+    // Each XCD an eighth of either part's items, in line. One query a sequence: the two parts evenly mixed, so that the shared part
+    // keeps the matrix cores busy while the own part waits for memory. Several: the shared part, whose items are longer, first.
+    const int xcd = blockIdx.x & 7, turn = blockIdx.x >> 3, turns = gridDim.x >> 3;
+    const int before = OWN_WIDE ? min(turn, a.shared_turns) : (int)((uint64_t)turn * a.shared_turns / turns);
+    const int upto = OWN_WIDE ? min(turn + 1, a.shared_turns) : (int)((uint64_t)(turn + 1) * a.shared_turns / turns);
+    const bool first = upto > before;
+    const int own = __builtin_amdgcn_readfirstlane(xcd * a.own_turns + turn - before);
+    if (!first && own >= a.own_items) return;
+    Item w;
+    if constexpr (WIDE && !OWN_WIDE) {
+        if (first) {
+            if (shared_item<kWide, kKeys>(a, xcd, before, w)) wide<SMALL>(a, w, t0, t1, t2, t3, again);
+        } else {
+            if (own_item<kNarrow, kTile>(a, own, w)) narrow<SMALL, !SMALL>(a, w, t0, t1, ml_sh);
+        }
+    } else {
+        constexpr int kRows = WIDE ? kWide : kNarrow, kBlock = WIDE ? kKeys : kTile;
+        if (!(first ? shared_item<kRows, kBlock>(a, xcd, before, w) : own_item<kRows, kBlock>(a, own, w))) return;
+        if constexpr (WIDE) wide<SMALL>(a, w, t0, t1, t2, t3, again);
+        else narrow<SMALL, false>(a, w, t0, t1, ml_sh);
+    }
+}
+
+// A row's partials merged by GROUPS half waves, each every GROUPS-th of them: lane -> four dims, and the weight of every 32nd.
+template <int GROUPS>
+__global__ __launch_bounds__(256) void shared_combine(const float* part, const int2* counts, uint16_t* out, int shared, int slots,
+                                                      int64_t rows) {
+    constexpr int kHold = 2 * kMaxSplits / 32, kAhead = 4;
+    __shared__ __attribute__((aligned(16))) float sum_sh[8][kDim];
+    const int half = threadIdx.x >> 5, lane = threadIdx.x & 31, group = half % GROUPS;
+    const int64_t row = min((int64_t)blockIdx.x * (8 / GROUPS) + half / GROUPS, rows - 1);   // past the last: that one again
     const float* pp = part + row * slots * kPart;
-    float mx = -INFINITY;
-    for (int s = 0; s < slots; ++s) mx = fmaxf(mx, pp[s * kPart]);
+    const int2 n = counts[row];
+    const int count = min(n.x, shared) + min(n.y, slots - shared);
+    auto slot = [&](int x) { return (size_t)(x < n.x ? x : shared + x - n.x) * kPart; };
+    float wt[kHold], ls[kHold], mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+        wt[i] = -INFINITY;
+        ls[i] = 0.0f;
+        if (32 * i + lane < count) {
+            const float2 ml = *reinterpret_cast<const float2*>(pp + slot(32 * i + lane));
+            wt[i] = ml.x;
+            ls[i] = ml.y;
+        }
+        mx = fmaxf(mx, wt[i]);
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) mx = fmaxf(mx, shfl_xor_f32(mx, d));
     float l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {   // no score above -inf in the split: nothing, unless its scores were NaN
+        wt[i] = wt[i] == -INFINITY ? (ls[i] == 0.0f ? 0.0f : 1.0f) : fast_exp2(wt[i] - mx);
+        l += wt[i] * ls[i];
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) l += shfl_xor_f32(l, d);
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s = 0; s < slots; ++s) {
-        const float m = pp[s * kPart], ls = pp[s * kPart + 1];
-        // no score above -inf in the split: nothing, unless its scores were NaN
-        if (m == -INFINITY && ls == 0.0f) continue;
-        const float w = m == -INFINITY ? 1.0f : fast_exp2(m - mx);
-        const float4 v = *reinterpret_cast<const float4*>(pp + s * kPart + 4 + d4);
-        l += w * ls;
-        o.x += w * v.x;
-        o.y += w * v.y;
-        o.z += w * v.z;
-        o.w += w * v.w;
+    for (int s0 = group; s0 < count; s0 += kAhead * GROUPS) {
+        float4 v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            v[u] = *reinterpret_cast<const float4*>(pp + slot(min(s0 + u * GROUPS, count - 1)) + 4 + 4 * lane);
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int x = s0 + u * GROUPS;
+            const float held = x < 32 ? wt[0] : x < 64 ? wt[1] : x < 96 ? wt[2] : wt[3];
+            const float w = __shfl(held, x & 31, 32);
+            if (x < count) {
+                o.x += w * v[u].x;
+                o.y += w * v[u].y;
+                o.z += w * v[u].z;
+                o.w += w * v[u].w;
+            }
+        }
+    }
+    if constexpr (GROUPS > 1) {
+        *reinterpret_cast<float4*>(&sum_sh[half][4 * lane]) = o;
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (int u = 1; u < GROUPS; ++u) {
+            const float4 v = *reinterpret_cast<const float4*>(&sum_sh[half + u][4 * lane]);
+            o.x += v.x;
+            o.y += v.y;
+            o.z += v.z;
+            o.w += v.w;
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<uint2*>(out + row * kDim + d4) =
+    *reinterpret_cast<uint2*>(out + row * kDim + 4 * lane) =
         make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+}
+
+template <bool WIDE, bool OWN_WIDE>
+void launch_read(const SharedArgs& a, int64_t items, hipStream_t s) {
+    const dim3 grid((unsigned)items), wg(64 * kWaves);
+    if (a.shift < 4) hipLaunchKernelGGL((shared_read<WIDE, OWN_WIDE, true>), grid, wg, 0, s, a);
+    else hipLaunchKernelGGL((shared_read<WIDE, OWN_WIDE, false>), grid, wg, 0, s, a);
 }
 
 }  // namespace
@@ -716,8 +936,8 @@ using namespace attnlab;
 
 extern "C" int64_t attnlab_shared_part_bytes(int B, int G, int h, int T, int shared_splits, int own_splits) {
     if (B < 1 || G < 1 || h < 1 || T < 0 || shared_splits < 0 || own_splits < 1) return -1;
-    const int64_t slots = (int64_t)shared_splits + own_splits;
-    return slots > 1 ? (int64_t)B * G * h * T * slots * kPart * 4 : 0;
+    const int64_t slots = (int64_t)shared_splits + own_splits, rows = (int64_t)B * G * h * T;
+    return slots > 1 ? (rows + 1) / 2 * 16 + rows * slots * kPart * 4 : 0;   // the counts, then the partials
 }
 
 extern "C" int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages, int num_pages,
@@ -768,33 +988,47 @@ extern "C" int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k
     a.shift = __builtin_ctz((unsigned)page_size);
     a.scale_log2 = scale * kLog2e;
     a.out = out;
-    a.part = part;
+    const int64_t rows = (int64_t)B * G * h * T;
+    ATTNLAB_REQUIRE(rows < (int64_t)1 << 31 && R < 1 << 30, "%lld rows of %d runs are too many", (long long)rows, R);
+    if (need) {
+        a.counts = reinterpret_cast<int2*>(part);
+        a.part = part + (rows + 1) / 2 * 4;
+    }
     a.shared = shared_splits;
     a.own = own_splits;
-    const int64_t rows = (int64_t)B * G * h * T, per_group = (int64_t)B * T * h;
-    ATTNLAB_REQUIRE(rows < (int64_t)1 << 31 && per_group + 128 * (int64_t)R < (int64_t)1 << 31, "%lld rows are too many", (long long)rows);
     const bool own_wide = T > 1;
-    const int shared_rows = wide ? kWide : kNarrow, own_rows = own_wide ? kWide : kNarrow;
-    // a run's last tile can be partly empty: at most one such for each run that has a row
-    a.tiles = shared_splits ? (int)(per_group / shared_rows + (R < B ? R : B)) : 0;
-    const int64_t shared_items = (int64_t)G * shared_splits * a.tiles;
-    const int64_t own_items = (int64_t)B * G * ((T * (int64_t)h + own_rows - 1) / own_rows) * own_splits;
-    ATTNLAB_REQUIRE(shared_items + own_items < (int64_t)1 << 31 && rows * 32 / 256 < (int64_t)1 << 31,
-                    "grids of %lld and %lld workgroups are too large", (long long)shared_items, (long long)own_items);
-    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-    const dim3 wg(256);
-    auto launch = [&](bool wide_rows, int64_t items, int first) {
-        if (items == 0) return;
-        if (wide_rows) hipLaunchKernelGGL(shared_wide, dim3((unsigned)items), wg, 0, s, a, first);
-        else hipLaunchKernelGGL(shared_narrow, dim3((unsigned)items), wg, 0, s, a, first);
-    };
-    if ((wide != 0) == own_wide) {
-        launch(own_wide, shared_items + own_items, 0);
-    } else {
-        launch(wide != 0, shared_items, 0);
-        launch(own_wide, own_items, (int)shared_items);
+    if (own_wide) wide = 1;
+    const int own_rows = own_wide ? kWide : kNarrow;
+    const int64_t own = (int64_t)B * G * ((T * (int64_t)h + own_rows - 1) / own_rows) * own_splits;
+    const int workers = shared_splits == 0 ? 0 : wide ? kWideWorkers : kNarrowWorkers;
+    // Workgroups of the shared part: a piece of every tile of rows (a run's last one can be partly empty: one such for each run that
+    // has a row) beside the shares that the chip holds at once, or one of every tile; or all shares of the longest prefixes that
+    // the tables have room for
+    const int64_t tiles = G * ((int64_t)B * T * h / (wide ? kWide : kNarrow) + (R < B ? R : B));
+    const int64_t keys = (int64_t)max_pages * page_size, longest = prefix_lengths || prefix_length > keys ? keys : prefix_length;
+    const int64_t shares = (longest + (wide ? kKeys * kLeastBlocks : kTile * kLeastTiles) - 1) / (wide ? kKeys * kLeastBlocks : kTile * kLeastTiles);
+    int64_t first = 0;
+    if (shared_splits) {
+        first = (tiles > workers ? tiles : workers) + tiles;
+        if (tiles * shares < first) first = tiles * shares;
     }
-    if (need) hipLaunchKernelGGL(shared_combine, dim3((unsigned)((rows * 32 + 255) / 256)), wg, 0, s, part, out,
-                                 shared_splits + own_splits, rows);
+    ATTNLAB_REQUIRE(first + own + 16 < (int64_t)1 << 31 && tiles * kMaxSplits < (int64_t)1 << 31,
+                    "a grid of %lld workgroups is too large", (long long)(first + own));
+    a.own_items = (int)own;
+    a.shared_turns = (int)((first + 7) / 8) + (first ? 1 : 0);   // whole shares and pieces are eighths of their own
+    a.own_turns = (a.own_items + 7) / 8;
+    const int64_t items = 8 * ((int64_t)a.shared_turns + a.own_turns);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    if (own_wide) launch_read<true, true>(a, items, s);
+    else if (wide && shared_splits) launch_read<true, false>(a, items, s);
+    else launch_read<false, false>(a, items, s);
+    if (need) {
+        const int slots = shared_splits + own_splits;
+        const dim3 wg(256);
+        if (slots > 8) hipLaunchKernelGGL(shared_combine<4>, dim3((unsigned)((rows + 1) / 2)), wg, 0, s, a.part, a.counts, out,
+                                          shared_splits, slots, rows);
+        else hipLaunchKernelGGL(shared_combine<1>, dim3((unsigned)((rows + 7) / 8)), wg, 0, s, a.part, a.counts, out, shared_splits,
+                                slots, rows);
+    }
     return check_launch("shared_prefix_attend");
 }

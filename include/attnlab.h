@@ -444,9 +444,10 @@ int attnlab_page_compact(uint16_t* k, uint16_t* v, int layers, int num_pages, in
  * they are read by the first one's table, once for all. A run begins no earlier than the largest bound before it. A sequence in no
  * run, or of which some query does not see the whole of that prefix, reads everything by its own table.
  * q, out: [B, G, h, T, 128] bf16 contiguous, 16-byte aligned, 1 <= h <= 16; block_table [B, bt_stride]. wide: the shared part by
- * workgroups of 128 (sequence, query, head) rows instead of 16. shared_splits (0: no shared part, every sequence reads by its own
- * table; up to 64) and own_splits (1..64): workgroups that share the two parts' keys. Unless they are 0 and 1, part (16-byte
- * aligned, attnlab_shared_part_bytes bytes) holds the partials and a last launch merges them.
+ * workgroups of 128 (sequence, query, head) rows instead of 16 (always so for T > 1). shared_splits (1..64, or 0: no shared part,
+ * every sequence reads by its own table) and own_splits (1..64): partials of the two parts that a row has at most, which limits
+ * how many workgroups share its keys. Unless they are 0 and 1, part (16-byte aligned, attnlab_shared_part_bytes bytes) holds the
+ * partials and a last launch merges them.
  */
 int64_t attnlab_shared_part_bytes(int B, int G, int h, int T, int shared_splits, int own_splits);
 int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages, int num_pages,

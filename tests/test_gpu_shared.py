@@ -168,7 +168,7 @@ def test_cases(gpu, name):
 
 
 @pytest.mark.parametrize("name", ["wide", "ragged_runs", "narrow_runs", "outside", "chunk_17", "chunk_130", "no_runs"])
-@pytest.mark.parametrize("parts", [(0, 1), (1, 1), (3, 2), (64, 64), (0, 5)])
+@pytest.mark.parametrize("parts", [(0, 1), (1, 1), (2, 1), (3, 2), (64, 64), (0, 5)])
 def test_partitions(gpu, name, parts):
     c = make(name, 2)
     c.check(c.call(gpu, partitions=parts))

@@ -32,17 +32,18 @@ def test_nothing_to_do_is_no_launch(native_lib):
 
 def test_part_bytes(native_lib):
     size = native_lib.attnlab_shared_part_bytes
-    assert size(3, 2, 4, 5, 2, 1) == 3 * 2 * 4 * 5 * 3 * 132 * 4 and size(3, 2, 4, 5, 0, 1) == 0
+    assert size(3, 2, 4, 5, 2, 1) == 120 * (8 + 3 * 132 * 4) and size(3, 2, 4, 5, 0, 1) == 0
+    assert size(1, 1, 1, 3, 2, 2) == 32 + 3 * 4 * 132 * 4   # the counts' room is a multiple of 16 bytes
     assert size(0, 2, 4, 5, 1, 1) == size(1, 2, 4, -1, 1, 1) == size(1, 1, 1, 1, -1, 1) == size(1, 1, 1, 1, 1, 0) == -1
 
 
 def test_split_rules():
     for rows in (1, 16, 17, 300, 5000):
-        for runs in (1, 7):
-            for keys in (1, 255, 512, 32768):
-                for wide in (False, True):
-                    assert 1 <= shared.shared_splits(8, rows, runs, keys, wide) <= max(1, keys // 256)
-                assert 1 <= shared.own_splits(8, rows, keys) <= max(1, keys // 256)
+        for G in (1, 8):
+            for wide in (False, True):
+                assert 1 <= shared.shared_splits(G, rows, wide) <= shared.MAX_SPLITS
+        for keys in (1, 255, 512, 32768):
+            assert 1 <= shared.own_splits(8, rows, keys) <= max(1, keys // 256)
 
 
 class OnDevice(torch.Tensor):
