@@ -6,6 +6,7 @@ package, whose scripts take log_softmax of the logits on the host.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -31,10 +32,11 @@ def token_logprobs(logits, tokens=None, *, top: int = 0, entropy: bool = False) 
     64): the most likely tokens, equal logits by the lower token (-0 equals +0, NaN last). A row with a NaN or +inf, or of
     nothing but -inf, has no distribution: its values are NaN. Sums are float32. Rows may have any stride; logits whose last
     dimension has another stride than 1 are copied. There is no gradient: logits that ask for one are refused."""
+    shape = logits.shape
     code = _DTYPES.get(logits.dtype)
-    if code is None or logits.dim() < 1 or not logits.is_cuda:
+    if code is None or not shape or not logits.is_cuda:
         raise ValueError("logits must be a bfloat16, float16 or float32 [..., V] tensor on a HIP device")
-    *lead, V = logits.shape
+    lead, V, device = shape[:-1], shape[-1], logits.device
     if not 1 <= V <= MAX_VOCAB:
         raise ValueError(f"V={V} must be in [1, {MAX_VOCAB}]")
     top = int(top)
@@ -42,25 +44,36 @@ def token_logprobs(logits, tokens=None, *, top: int = 0, entropy: bool = False) 
         raise ValueError(f"top={top} must be in [0, {min(MAX_TOP, V)}]")
     if logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("token_logprobs has no gradient: give it logits that need none (detach them, or use torch.no_grad)")
-    device = logits.device
     if tokens is not None:
-        if tokens.dtype not in (torch.int64, torch.int32) or list(tokens.shape) != lead or tokens.device != device:
-            raise ValueError(f"tokens must be an int64 or int32 {lead} tensor on the logits' device")
+        wide = tokens.dtype is torch.int64
+        if not (wide or tokens.dtype is torch.int32) or tokens.shape != lead or tokens.device != device:
+            raise ValueError(f"tokens must be an int64 or int32 {list(lead)} tensor on the logits' device")
         tokens = tokens.contiguous()
-    if logits.stride(-1) != 1 and V > 1:
+    *strides, last = logits.stride()
+    if last != 1 and V > 1:
         logits = logits.contiguous()
-    rows = logits if len(lead) == 1 else logits.reshape(-1, V)
-    N = rows.shape[0]
-    stride = rows.stride(0) if N > 1 else V
-    made = lambda *n, dtype=torch.float32: torch.empty((*lead, *n), dtype=dtype, device=device)  # noqa: E731
-    found = made() if tokens is not None else None
-    spread = made() if entropy else None
-    best, at = made(top), made(top, dtype=torch.int64)
+        *strides, last = logits.stride()
+    if len(lead) != 1:
+        logits = logits.reshape(-1, V)
+        strides = logits.stride()
+    N = logits.shape[0]
+    # an empty_like is half the time of an empty with its arguments, and the host's part is most of a small call's time
+    like = torch.empty(lead, dtype=torch.float32, device=device)
+    found = like if tokens is not None else None
+    spread = None if not entropy else torch.empty_like(like) if found is like else like
+    best = torch.empty((*lead, top), dtype=torch.float32, device=device)
+    at = torch.empty_like(best, dtype=torch.int64)
     if N == 0:
         return TokenLogprobs(found, spread, best, at)
-    nbytes = nat.lib().attnlab_logprob_part_bytes(N, V, code, top)
+    nbytes = _part_bytes(N, V, code, top)
     part = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    nat.call_on(device, "attnlab_token_logprobs", rows.data_ptr(), code, stride, N, V, nat.ptr(tokens),
-                tokens is not None and tokens.dtype == torch.int64, top, nat.ptr(found), nat.ptr(spread), best.data_ptr(),
+    nat.call_on(device, "attnlab_token_logprobs", logits.data_ptr(), code, strides[0] if N > 1 else V, N, V,
+                None if tokens is None else tokens.data_ptr(), tokens is not None and wide, top,
+                None if found is None else found.data_ptr(), None if spread is None else spread.data_ptr(), best.data_ptr(),
                 at.data_ptr(), part.data_ptr(), nbytes, nat.stream_of(device))
     return TokenLogprobs(found, spread, best, at)
+
+
+@functools.lru_cache(maxsize=256)
+def _part_bytes(N: int, V: int, code: int, top: int) -> int:
+    return nat.lib().attnlab_logprob_part_bytes(N, V, code, top)

@@ -2,17 +2,18 @@
 //   lse = m + log sum_j e^(x_j - m)      logprob = x_token - lse      H = log l - sum_j e^(x_j - m) (x_j - m) / l,  l = e^(lse - m)
 //   top: the k largest x, equal ones by the lower token (NaN last, -0 equal to +0), as logprobs
 //
-// A row is cut into up to 64 segments, a workgroup each. A thread holds up to 64 logits in registers, so each is read once:
-// its own maximum m, l and s = sum p (x - m) come from them, merge over the wave and the workgroup, and leave as a partial
-// (m, l, s). A second launch merges a row's partials. Sums are fp32 in the log2 domain.
+// A row is cut into up to 64 segments, a workgroup each. A thread holds up to 64 logits in registers, as they came, so each is read
+// once: l and s = sum p (x - m) relative to a common m of the wave's merge over the workgroup and leave as a partial (m, l, s). A second
+// launch merges a row's partials. Sums are fp32 in the log2 domain.
 //
-// The top k without a second look at the memory: the k-th largest of a wave's 64 thread maxima is a lower bound of the k-th
+// The top k without a second look at every logit: the k-th largest of a wave's 64 thread maxima is a lower bound of the k-th
 // largest logit, found by a search over the order-preserving key's bits with one ballot a bit; the largest of the four waves'
-// bounds is the workgroup's. What lies above it (k and few more, in any distribution that does not crowd its largest logits into
-// a few threads) goes to LDS, of those that equal it the first k of each wave, and is ranked there by counting. More than LDS
-// takes: k rounds of a maximum over the workgroup, with the same result. The second launch does the same to the segments' lists.
+// bounds is the workgroup's. The few 16-byte words that reach it (k and some more, in any distribution that does not crowd its
+// largest logits into a few threads) go to LDS, and one wave looks them over again and ranks what it finds by counting.
+// More words than that holds: k rounds of a maximum over the workgroup, with the same result. The second launch does the same to
+// the segments' lists.
 //
-// What bounds it: the bytes for float32, for 16-bit logits as much the vector units (9 operations for two bytes, of them an
+// What bounds it: the bytes for float32; for 16-bit logits as much the vector units (9 operations for two bytes, of them an
 // exponential at a quarter of the rate).
 #include <cfloat>
 
@@ -25,7 +26,7 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;
 constexpr int kMaxSegments = 64;
-constexpr int kCandidates = 1024;        // what a segment's workgroup ranks in LDS
+constexpr int kWords = 256;              // words of a segment that are looked over again
 constexpr int kPartWords = 4;            // m, l, s and the largest logit (16 bytes)
 // x log2 e - m cancels what m's rounding left, up to where that is no longer small. A row whose largest logit is past kFar is
 // summed again by differences; a thread whose own is below -2 kFar weighs nothing in any other row (e^-65536 is 0).
@@ -69,15 +70,29 @@ __device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k) {
     return least;
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, shfl_xor_f32(x, d));
-    return x;
+// Over the wave's lanes: a scan along each row of 16, then the rows' ends; the last lane's value, for all.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float x, float none) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(none), __float_as_int(x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float last_lane(float x) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63)); }
+__device__ __forceinline__ float wave_max(float x) {   // NaN where all are
+    x = fmaxf(x, moved<0x111, 0xf>(x, x));
+    x = fmaxf(x, moved<0x112, 0xf>(x, x));
+    x = fmaxf(x, moved<0x114, 0xf>(x, x));
+    x = fmaxf(x, moved<0x118, 0xf>(x, x));
+    x = fmaxf(x, moved<0x142, 0xa>(x, x));
+    x = fmaxf(x, moved<0x143, 0xc>(x, x));
+    return last_lane(x);
 }
 __device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += shfl_xor_f32(x, d);
-    return x;
+    x += moved<0x111, 0xf>(x, 0.0f);
+    x += moved<0x112, 0xf>(x, 0.0f);
+    x += moved<0x114, 0xf>(x, 0.0f);
+    x += moved<0x118, 0xf>(x, 0.0f);
+    x += moved<0x142, 0xa>(x, 0.0f);
+    x += moved<0x143, 0xc>(x, 0.0f);
+    return last_lane(x);
 }
 
 // (m, l, s) against a common maximum mt; m = -inf: nothing but, where they were NaN, its l and s.
@@ -88,27 +103,32 @@ __device__ __forceinline__ void rescale(float m, float mt, float& l, float& s) {
     l *= w;
 }
 
-// One 16-byte word of a row as floats.
+// Element j of a 16-byte word of a row as a float.
 template <int DT>
-__device__ __forceinline__ void unpack(u32x4_t w, float* v) {
+__device__ __forceinline__ float element(const u32x4_t& w, int j) {
+    if constexpr (DT == ATTNLAB_DT_F32) return __uint_as_float(w[j]);
+    else if constexpr (DT == ATTNLAB_DT_BF16) return j & 1 ? bf16_hi(w[j >> 1]) : bf16_lo(w[j >> 1]);
+    else return f16_to_f32((uint16_t)(w[j >> 1] >> (16 * (j & 1))));
+}
+// The word's elements outside [0, V) as -inf; t: the first one's token.
+template <int DT>
+__device__ __forceinline__ void only_logits(u32x4_t& w, int t, int V) {
+    constexpr uint32_t kNone = DT == ATTNLAB_DT_F32 ? 0xff800000u : DT == ATTNLAB_DT_BF16 ? 0xff80u : 0xfc00u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         if constexpr (DT == ATTNLAB_DT_F32) {
-            v[i] = __uint_as_float(w[i]);
-        } else if constexpr (DT == ATTNLAB_DT_BF16) {
-            v[2 * i] = bf16_lo(w[i]);
-            v[2 * i + 1] = bf16_hi(w[i]);
+            if (t + i < 0 || t + i >= V) w[i] = kNone;
         } else {
-            v[2 * i] = f16_to_f32((uint16_t)w[i]);
-            v[2 * i + 1] = f16_to_f32((uint16_t)(w[i] >> 16));
+            if (t + 2 * i < 0 || t + 2 * i >= V) w[i] = (w[i] & 0xffff0000u) | kNone;
+            if (t + 2 * i + 1 < 0 || t + 2 * i + 1 >= V) w[i] = (w[i] & 0xffffu) | kNone << 16;
         }
     }
 }
 
 // `count` keys in `sh` ranked by counting the larger ones; the first `top` of them to `take(rank, key)`.
-template <typename Take>
+template <int THREADS, typename Take>
 __device__ __forceinline__ void rank_keys(const uint64_t* sh, int count, int top, Take take) {
-    for (int i = threadIdx.x; i < count; i += kThreads) {
+    for (int i = threadIdx.x & (THREADS - 1); i < count; i += THREADS) {
         const uint64_t own = sh[i];
         int rank = 0;
         for (int j = 0; j < count; ++j) rank += sh[j] > own;
@@ -119,10 +139,12 @@ __device__ __forceinline__ void rank_keys(const uint64_t* sh, int count, int top
 template <int DT, int U>
 __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     constexpr int kPer = DT == ATTNLAB_DT_F32 ? 4 : 8, kBytes = 16 / kPer;
-    __shared__ uint64_t cand_sh[kCandidates];
+    __shared__ uint64_t cand_sh[kWords * kPer];
+    __shared__ uint16_t word_sh[kWords];
+    __shared__ u32x4_t data_sh[kWords];
     __shared__ float part_sh[kWaves][4];
     __shared__ uint32_t bound_sh[kWaves];
-    __shared__ uint32_t count_sh;
+    __shared__ uint32_t words_sh, count_sh;
     const int seg = blockIdx.x % a.segments;
     const int64_t row = blockIdx.x / a.segments;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -132,72 +154,92 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     const int head = (int)(at & 15) / kBytes;
     const u32x4_t* words = reinterpret_cast<const u32x4_t*>(at & ~(uintptr_t)15);
     const int first = seg * a.words, end = min(first + a.words, (head + a.V + kPer - 1) / kPer);
-    u32x4_t raw[U];
+    // the wave's word u: 64 in line, a segment's end between waves (but for the row's end)
+    auto there = [&](int u) { return first + kThreads * u + 64 * wave < end; };
+    u32x4_t x[U];
+    constexpr uint32_t kNone = DT == ATTNLAB_DT_F32 ? 0xff800000u : DT == ATTNLAB_DT_BF16 ? 0xff80ff80u : 0xfc00fc00u;   // -inf
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int w = first + kThreads * u + tid;
-        if (w < end) raw[u] = __builtin_nontemporal_load(words + w);
+        x[u] = u32x4_t{kNone, kNone, kNone, kNone};
+        if (w < end) x[u] = __builtin_nontemporal_load(words + w);
     }
-    float x[U][kPer];
-    bool whole = true;                   // every element of this thread is a logit
+    if (tid == 0) words_sh = count_sh = 0;
+    // the row's first and last word can hold what is not the row's; `whole`: every element of this thread is a logit
+    bool whole = first + kThreads * (U - 1) + tid < end;
+    if (seg == 0 || seg == a.segments - 1) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int w = first + kThreads * u + tid, t = kPer * w - head;
-        if (w < end) unpack<DT>(raw[u], x[u]);
-        const bool in = w < end && t >= 0 && t + kPer <= a.V;
-        if (!in) {
-            whole = false;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) x[u][j] = w < end && t + j >= 0 && t + j < a.V ? x[u][j] : -INFINITY;
+        for (int u = 0; u < U; ++u) {
+            const int w = first + kThreads * u + tid, t = kPer * w - head;
+            if (w < end && (t < 0 || t + kPer > a.V)) {
+                only_logits<DT>(x[u], t, a.V);
+                whole = false;
+            }
         }
     }
-    float m = x[0][0];
+    auto word_max = [&](const u32x4_t& w) {   // NaN where all are
+        float y = element<DT>(w, 0);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+        for (int j = 1; j < kPer; ++j) y = fmaxf(y, element<DT>(w, j));
+        return y;
+    };
+    // One pass: each word's maximum, and the sums relative to the largest of the wave's first words, near enough to the largest of
+    // all, as soon as a word is there.
+    float m = wave_max(word_max(x[0]));
+    bool near = m > -2.0f * kFar && m < INFINITY;
+    m *= kLog2e;
+    float most[U], l = 0.0f, s = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) m = fmaxf(m, x[u][j]);
-    const float top = m;                 // NaN where all are
-    m = m > -2.0f * kFar ? m * kLog2e : -INFINITY;
-    float l = 0.0f, s = 0.0f;
-    const float nm = m == -INFINITY ? 0.0f : -m;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+        most[u] = -INFINITY;
+        if (!there(u)) continue;
+        most[u] = word_max(x[u]);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            const float d = fmaf(x[u][j], kLog2e, nm), p = fast_exp2(d);
+            const float d = fmaf(element<DT>(x[u], j), kLog2e, -m), p = fast_exp2(d);
             l += p;
             s = fmaf(p, d, s);
         }
-    if (l == l && s != s) {              // some logit is -inf: a weight of zero, and no term
-        s = 0.0f;
+    }
+    float top = most[0];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+    for (int u = 1; u < U; ++u) top = fmaxf(top, most[u]);
+    const float largest = wave_max(top);
+    // Not near enough (a sum past the type's end), or some logit is -inf (a weight of zero, and no term), or none is a number: again, by
+    // the wave's own maximum
+    near = near && l < FLT_MAX && fabsf(s) < FLT_MAX;
+    if (!__all(near)) {
+        m = largest > -2.0f * kFar ? largest * kLog2e : -INFINITY;
+        const float nm = m == -INFINITY ? 0.0f : -m;
+        l = s = 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (!there(u)) continue;
+            asm volatile("" : "+v"(x[u].x), "+v"(x[u].y), "+v"(x[u].z), "+v"(x[u].w));   // unpacked again, not kept
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
-                const float d = fmaxf(fmaf(x[u][j], kLog2e, nm), -1000.0f);
-                s = fmaf(fast_exp2(d), d, s);
+                const float d = fmaf(element<DT>(x[u], j), kLog2e, nm), p = fast_exp2(d);
+                l += p;
+                s = fmaf(p, fmaxf(d, -1000.0f), s);
             }
+        }
     }
-    const float mw = wave_max(m), largest = wave_max(top);
-    rescale(m, mw, l, s);
     l = wave_sum(l);
     s = wave_sum(s);
     if (lane == 0) {
-        part_sh[wave][0] = mw;
+        part_sh[wave][0] = m;
         part_sh[wave][1] = l;
         part_sh[wave][2] = s;
         part_sh[wave][3] = largest;
     }
-    // a thread without logits of its own, or with nothing above -inf among elements that are none: no bound
-    const uint32_t mine = !whole && !(top > -INFINITY) ? 0u : score_key(top);
+    // a thread with nothing above -inf among elements that are no logits: no bound
     uint32_t bound = 0;
     if (a.top) {
-        bound = wave_kth(mine, a.top);
+        bound = wave_kth(!whole && !(top > -INFINITY) ? 0u : score_key(top), a.top);
         if (lane == 0) bound_sh[wave] = bound;
     }
-    if (tid == 0) count_sh = 0;
     __syncthreads();
-    if (tid == 0) {
+    if (tid == kThreads - 1) {
         float ms = part_sh[0][0], ls = 0.0f, ss = 0.0f, xs = part_sh[0][3];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) {
@@ -216,58 +258,49 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     if (!a.top) return;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) bound = max(bound, bound_sh[w]);
-    if (__any(mine >= bound || mine == 0)) {
-        int equal = 0;                   // of this wave so far, in the order of their tokens
+    const float least = logit_of(bound);   // NaN: every word
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int w = first + kThreads * u + tid, t = kPer * w - head;
-            uint32_t own = 0;            // elements that equal the bound
-            bool some = false;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) some |= !(x[u][j] < logit_of(bound));   // NaN too
-            if (!__any(some)) continue;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const uint32_t k = score_key(x[u][j]);
-                const bool in = w < end && t + j >= 0 && t + j < a.V;
-                if (in && k > bound) {
-                    const uint32_t i = atomicAdd(&count_sh, 1u);
-                    if (i < kCandidates) cand_sh[i] = (uint64_t)k << 32 | (uint32_t)~(t + j);
-                }
-                own |= in && k == bound ? 1u << j : 0u;
-            }
-            if (equal < a.top && __any(own != 0)) {
-                const uint32_t mine_here = (uint32_t)__popc(own);
-                const uint32_t upto = wave_incl_scan(mine_here);
-                int at_rank = equal + (int)(upto - mine_here);
-                equal += __builtin_amdgcn_readlane((int)upto, 63);
-#pragma unroll
-                for (int j = 0; j < kPer; ++j)
-                    if (own >> j & 1 && at_rank++ < a.top) {
-                        const uint32_t i = atomicAdd(&count_sh, 1u);
-                        if (i < kCandidates) cand_sh[i] = (uint64_t)bound << 32 | (uint32_t)~(t + j);
-                    }
+    for (int u = 0; u < U; ++u) {
+        const bool reaches = !(most[u] < least) && first + kThreads * u + tid < end;
+        if (reaches) {
+            const uint32_t i = atomicAdd(&words_sh, 1u);
+            if (i < kWords) {
+                word_sh[i] = (uint16_t)(kThreads * u + tid);
+                data_sh[i] = x[u];
             }
         }
     }
     __syncthreads();
-    const uint32_t count = count_sh;
+    const uint32_t listed = words_sh;
     uint64_t* best = a.best + (row * a.segments + seg) * a.top;
-    if (count <= kCandidates) {
-        rank_keys(cand_sh, (int)count, a.top, [&](int r, uint64_t k) { best[r] = k; });
-        for (int r = (int)count + tid; r < a.top; r += kThreads) best[r] = 0;
+    if (listed <= kWords) {
+        if (wave != 0) return;
+        for (uint32_t i = lane; i < listed; i += 64) {
+            const int t = kPer * (first + word_sh[i]) - head;
+            const u32x4_t v = data_sh[i];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const uint32_t k = score_key(element<DT>(v, j));
+                if (k >= bound && t + j >= 0 && t + j < a.V)
+                    cand_sh[atomicAdd(&count_sh, 1u)] = (uint64_t)k << 32 | (uint32_t)~(t + j);
+            }
+        }
+        asm volatile("" ::: "memory");   // a wave's LDS operations take effect in order
+        const int count = (int)count_sh;
+        rank_keys<64>(cand_sh, count, a.top, [&](int r, uint64_t k) { best[r] = k; });
+        for (int r = count + lane; r < a.top; r += 64) best[r] = 0;
         return;
     }
     uint64_t last = ~0ull;               // the largest key below the last one taken, `top` times
     for (int r = 0; r < a.top; ++r) {
         uint64_t k = 0;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int w = first + kThreads * u + tid, t = kPer * w - head;
+        for (int w = first + tid; w < end; w += kThreads) {
+            const int t = kPer * w - head;
+            const u32x4_t v = words[w];
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
-                const uint64_t y = key_of(x[u][j], t + j);
-                if (w < end && t + j >= 0 && t + j < a.V && y < last && y > k) k = y;
+                const uint64_t y = key_of(element<DT>(v, j), t + j);
+                if (t + j >= 0 && t + j < a.V && y < last && y > k) k = y;
             }
         }
 #pragma unroll
@@ -285,16 +318,24 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     }
 }
 
-// A row's partials: lane s of every wave holds segment s.
-template <int DT>
-__global__ __launch_bounds__(kThreads) void logprob_merge(LogprobArgs a) {
-    constexpr int kMost = kMaxSegments * kMaxTop, kHold = kMost / kThreads;
-    __shared__ uint64_t cand_sh[kMost];
+// A row's partials, by THREADS threads: lane s of every wave holds segment s. A wave where the segments' lists hold 256 keys or
+// fewer, four rows to a workgroup; else a workgroup.
+constexpr int kWaveKeys = 256;
+template <int DT, int THREADS>
+__global__ __launch_bounds__(kThreads) void logprob_merge(LogprobArgs a, int64_t N) {
+    constexpr int kMost = THREADS == 64 ? kWaveKeys : kMaxSegments * kMaxTop, kHold = kMost / THREADS, kRows = kThreads / THREADS;
+    __shared__ uint64_t cand_sh[kRows][kMost];
     __shared__ uint32_t bound_sh[kWaves];
     __shared__ float far_sh[kWaves][2];
-    __shared__ uint32_t count_sh;
-    const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ uint32_t count_sh[kRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r = THREADS == 64 ? wave : 0, tid = THREADS == 64 ? lane : (int)threadIdx.x;
+    const int64_t row = (int64_t)blockIdx.x * kRows + r;
+    if (row >= N) return;
+    auto sync = [&]() {   // a wave's LDS operations take effect in order
+        if constexpr (THREADS == 64) asm volatile("" ::: "memory");
+        else __syncthreads();
+    };
     float4 p = make_float4(-INFINITY, 0.0f, 0.0f, -INFINITY);
     if (lane < a.segments) p = *reinterpret_cast<const float4*>(a.part + (row * a.segments + lane) * kPartWords);
     const float m = wave_max(p.x), largest = wave_max(p.w);
@@ -309,28 +350,30 @@ __global__ __launch_bounds__(kThreads) void logprob_merge(LogprobArgs a) {
     const bool far = fabsf(largest) >= kFar && fabsf(largest) < INFINITY;
     if (far) {
         l = s = 0.0f;
-        for (int t = tid; t < a.V; t += kThreads) {
+        for (int t = tid; t < a.V; t += THREADS) {
             const float d = (at(t) - largest) * kLog2e, e = fast_exp2(d);
             l += e;
             s += d < -1000.0f ? 0.0f : e * d;
         }
         l = wave_sum(l);
         s = wave_sum(s);
-        if (lane == 0) {
-            far_sh[wave][0] = l;
-            far_sh[wave][1] = s;
-        }
-        __syncthreads();
-        l = s = 0.0f;
+        if constexpr (THREADS > 64) {
+            if (lane == 0) {
+                far_sh[wave][0] = l;
+                far_sh[wave][1] = s;
+            }
+            __syncthreads();
+            l = s = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            l += far_sh[w][0];
-            s += far_sh[w][1];
+            for (int w = 0; w < kWaves; ++w) {
+                l += far_sh[w][0];
+                s += far_sh[w][1];
+            }
         }
     }
     // no logit above -inf: no distribution
     const float log2l = largest > -INFINITY ? log2f(l) : __builtin_nanf("");
-    // l is relative to m, largest log2 e rounded: what that rounding left goes back
+    // l is relative to m, not the largest logit
     const float lnl = (log2l - (far ? 0.0f : fmaf(largest, kLog2e, -m))) * kLn2;
     auto logprob = [&](float x) { return (x - largest) - lnl; };
     if (tid == 0) {
@@ -339,47 +382,51 @@ __global__ __launch_bounds__(kThreads) void logprob_merge(LogprobArgs a) {
             const int64_t t = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[row] : static_cast<const int32_t*>(a.tokens)[row];
             a.logprob[row] = t < 0 ? 0.0f : t < a.V ? logprob(at(t)) : __builtin_nanf("");
         }
+        count_sh[r] = 0;
     }
     if (!a.top) return;
     const int most = a.segments * a.top;
     const uint64_t* best = a.best + row * most;
-    auto take = [&](int r, uint64_t k) {
-        a.top_logprob[row * a.top + r] = logprob(logit_of((uint32_t)(k >> 32)));
-        a.top_token[row * a.top + r] = (int64_t)(uint32_t)~(uint32_t)k;
-    };
     uint64_t k[kHold];
-    uint32_t mine = 0, bound = 0;
+    uint32_t mine = 0;
 #pragma unroll
     for (int i = 0; i < kHold; ++i) {
-        k[i] = kThreads * i + tid < most ? best[kThreads * i + tid] : 0;
+        k[i] = THREADS * i + tid < most ? best[THREADS * i + tid] : 0;
         mine = max(mine, (uint32_t)(k[i] >> 32));
     }
-    bound = wave_kth(mine, a.top);
-    if (lane == 0) bound_sh[wave] = bound;
-    if (tid == 0) count_sh = 0;
-    __syncthreads();
+    uint32_t bound = wave_kth(mine, a.top);
+    if constexpr (THREADS > 64) {
+        if (lane == 0) bound_sh[wave] = bound;
+    }
+    sync();
+    if constexpr (THREADS > 64) {
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) bound = max(bound, bound_sh[w]);
+        for (int w = 0; w < kWaves; ++w) bound = max(bound, bound_sh[w]);
+    }
 #pragma unroll
     for (int i = 0; i < kHold; ++i)
-        if (k[i] && (uint32_t)(k[i] >> 32) >= bound) cand_sh[atomicAdd(&count_sh, 1u)] = k[i];
-    __syncthreads();
-    rank_keys(cand_sh, (int)count_sh, a.top, take);
+        if (k[i] && (uint32_t)(k[i] >> 32) >= bound) cand_sh[r][atomicAdd(&count_sh[r], 1u)] = k[i];
+    sync();
+    rank_keys<THREADS>(cand_sh[r], (int)count_sh[r], a.top, [&](int i, uint64_t y) {
+        a.top_logprob[row * a.top + i] = logprob(logit_of((uint32_t)(y >> 32)));
+        a.top_token[row * a.top + i] = (int64_t)(uint32_t)~(uint32_t)y;
+    });
 }
 
 int per_word(int dtype) { return dtype == ATTNLAB_DT_F32 ? 4 : 8; }
 
 // Words of a thread (1, 2, 4, 8, 16) and segments of a row: as many segments as give about two workgroups per CU, of 2048 logits
-// or more and at most 64; a thread holds at most 64 logits.
+// or more and at most 64.
 int plan(int64_t N, int V, int dtype, int& segments, int& words) {
     const int per = per_word(dtype), total = (V + 2 * (per - 1)) / per;   // a row that begins inside a word has one more
-    const int most = 64 / per;
+    const int most = dtype == ATTNLAB_DT_F32 ? 16 : 8;   // 64 logits; 16-bit ones of 4, 8 and 16 words: 260, 218, 220 us (4096 rows)
     int u = 1;
     while (u < most && (N * ((total + kThreads * u - 1) / (kThreads * u)) >= 1024 ||
                         (total + kThreads * u - 1) / (kThreads * u) > kMaxSegments || kThreads * u * per < 2048))
         u *= 2;
     segments = (total + kThreads * u - 1) / (kThreads * u);
-    words = (total + segments - 1) / segments;
+    words = ((total + segments - 1) / segments + 63) / 64 * 64;   // whole waves of them
+    segments = (total + words - 1) / words;
     return u;
 }
 
@@ -392,8 +439,9 @@ int launch(const LogprobArgs& a, int u, int64_t N, hipStream_t s) {
     else if (u == 2) hipLaunchKernelGGL((logprob_segment<DT, 2>), grid, wg, 0, s, a);
     else if (u == 4) hipLaunchKernelGGL((logprob_segment<DT, 4>), grid, wg, 0, s, a);
     else if (u == 8) hipLaunchKernelGGL((logprob_segment<DT, 8>), grid, wg, 0, s, a);
-    else if constexpr (DT == ATTNLAB_DT_F32) hipLaunchKernelGGL((logprob_segment<DT, 16>), grid, wg, 0, s, a);
-    hipLaunchKernelGGL(logprob_merge<DT>, dim3((unsigned)N), wg, 0, s, a);
+    else hipLaunchKernelGGL((logprob_segment<DT, 16>), grid, wg, 0, s, a);
+    if (a.segments * a.top <= kWaveKeys) hipLaunchKernelGGL((logprob_merge<DT, 64>), dim3((unsigned)((N + 3) / 4)), wg, 0, s, a, N);
+    else hipLaunchKernelGGL((logprob_merge<DT, kThreads>), dim3((unsigned)N), wg, 0, s, a, N);
     return check_launch("token_logprobs");
 }
 
