@@ -74,7 +74,7 @@ SIGNATURES = {
     "attnlab_shared_prefix_attend": (_i, [_p] * 3 + [_i] * 2 + [_p, _i64, _i, _p, _i, _p, _i, _p] + [_i] * 5 + [_f] + [_i] * 3 +
                                      [_p, _p, _i64, _p]),
     "attnlab_logprob_part_bytes": (_i64, [_i64, _i, _i, _i]),
-    "attnlab_token_logprobs": (_i, [_p, _i, _i64, _i64, _i, _p, _i, _i] + [_p] * 5 + [_i64, _p]),
+    "attnlab_token_logprobs": (_i, [_p, _i, _i64, _i64, _i, _p, _i, _i] + [_p] * 5 + [_i64, _p, _p]),
     "attnlab_sparse_decode_workspace": (_i64, [_i] * 8),
     "attnlab_sparse_decode_step": (_i, [_p] * 8 + [_i] * 10 + [_f, _i, _i, _p, _p, _i64, _p, _p, _p, _p]),
     "attnlab_sparse_decode_step_f32": (_i, [_p] * 8 + [_i] * 10 + [_f, _i, _i, _p, _p, _i64, _p, _p, _p, _p]),

@@ -162,17 +162,21 @@ def _merge_here(h: int, P: int, positions: int, ragged: bool) -> bool:
     return positions <= 1 << 19 if ragged else h * P <= 64 or positions <= 1 << 17
 
 
+def stream_counters(device, stream: int):
+    """(tensor, address) of a stream's counters, which are zero between launches, and partials behind them."""
+    buf = _MERGES.get((device.index, stream))
+    if buf is None:
+        buf = _MERGES[device.index, stream] = torch.zeros(COUNTERS + PARTIALS * PART_WORDS, dtype=torch.int32, device=device)
+    return buf, buf.data_ptr()
+
+
 def _split_k(P: int, BG: int, h: int, device, stream: int, counted: bool):
     """(tensor to hold on to, partials' address, counters' address) of a one-query call split over P workgroups."""
     if P == 1:
         return None, None, None
     rows = BG * P * h
     if counted and P <= MERGE_SLOTS and BG <= COUNTERS and rows <= PARTIALS and not capturing(device):
-        buf = _MERGES.get((device.index, stream))
-        if buf is None:
-            buf = _MERGES[device.index, stream] = torch.zeros(COUNTERS + PARTIALS * PART_WORDS, dtype=torch.int32,
-                                                              device=device)
-        at = buf.data_ptr()
+        buf, at = stream_counters(device, stream)
         return buf, at + 4 * COUNTERS, at
     part = torch.empty(rows * PART_WORDS, dtype=torch.float32, device=device)
     return part, part.data_ptr(), None

@@ -1,7 +1,8 @@
 """Log probabilities of given tokens, with the entropy and the most likely alternatives, on gfx950.
 
 What a program does with a runner's logits: score a prompt token by token, compare a sparse read's distribution with the full
-one's, follow the likeliest continuations. Each logit is read once, whatever is asked for. No counterpart in the reference's
+one's, follow the likeliest continuations. Each logit is read once, whatever is asked for. Few rows take one launch, in which the last
+workgroup of a row merges it, counted by counters of the stream's; a captured call takes two, and shares nothing. No counterpart in the reference's
 package, whose scripts take log_softmax of the logits on the host.
 """
 from __future__ import annotations
@@ -12,9 +13,11 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _native as nat
+from .hip_range import capturing, stream_counters
 
 MAX_TOP = 64
 MAX_VOCAB = (1 << 20) - 16
+MERGED_ROWS = 256     # up to as many rows are merged in the segments' launch
 _DTYPES = {torch.bfloat16: nat.DT_BF16, torch.float16: nat.DT_F16, torch.float32: nat.DT_F32}
 
 
@@ -67,10 +70,12 @@ def token_logprobs(logits, tokens=None, *, top: int = 0, entropy: bool = False) 
         return TokenLogprobs(found, spread, best, at)
     nbytes = _part_bytes(N, V, code, top)
     part = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    stream = nat.stream_of(device)
+    held, arrive = (None, None) if N > MERGED_ROWS or capturing(device) else stream_counters(device, stream)
     nat.call_on(device, "attnlab_token_logprobs", logits.data_ptr(), code, strides[0] if N > 1 else V, N, V,
                 None if tokens is None else tokens.data_ptr(), tokens is not None and wide, top,
                 None if found is None else found.data_ptr(), None if spread is None else spread.data_ptr(), best.data_ptr(),
-                at.data_ptr(), part.data_ptr(), nbytes, nat.stream_of(device))
+                at.data_ptr(), part.data_ptr(), nbytes, arrive, stream)
     return TokenLogprobs(found, spread, best, at)
 
 

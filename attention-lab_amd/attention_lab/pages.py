@@ -33,7 +33,7 @@ INT_MAX = 2 ** 31 - 1
 
 
 def _check_book(t, name: str, shape: tuple, device):
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{name} must be a contiguous int32 {list(shape)} tensor on the cache's device")
     return t
 
@@ -48,7 +48,7 @@ class PagedCache:
     counts the pages that page_reserve could not give."""
 
     __slots__ = ("k", "v", "table", "lengths", "refs", "missing", "layers", "num_pages", "groups", "page_size", "slots",
-                 "max_pages", "device")
+                 "max_pages", "layer_bytes", "device")
 
     def __init__(self, k, v, table, lengths, refs, *, missing=None):
         shape, device = k.shape, k.device
@@ -73,6 +73,7 @@ class PagedCache:
         self.k, self.v, self.device = k, v, device
         self.layers, self.num_pages, self.groups, self.page_size = int(layers), int(pages), int(G), int(page)
         self.slots, self.max_pages = int(S), int(W)
+        self.layer_bytes = 2 * self.num_pages * self.groups * self.page_size * HEAD_DIM   # of K, or of V
 
     @classmethod
     def empty(cls, layers: int, slots: int, groups: int, num_pages: int, page_size: int, max_pages: int, *,
@@ -111,8 +112,8 @@ def _per_slot(cache: PagedCache, x, name: str):
 
 
 def _scratch(cache: PagedCache):
-    """Scratch of one call: from torch's allocator, so that a captured graph has its own."""
-    nbytes = nat.lib().attnlab_page_scratch_bytes(cache.slots, cache.num_pages)
+    """Scratch of one call (attnlab_page_scratch_bytes): from torch's allocator, so that a captured graph has its own."""
+    nbytes = 16 + 12 * max(cache.slots, cache.num_pages)
     return torch.empty(nbytes, dtype=torch.uint8, device=cache.device), nbytes
 
 
@@ -144,23 +145,23 @@ def page_append(cache: PagedCache, layer: int, k, v, tokens=None) -> None:
     """A layer's rows k, v bfloat16 [slots, G, T, 128] (any strides) at the last positions of every slot: row t of slot i at
     lengths[i] - tokens[i] + t for t < tokens[i] (int32 [slots] on the device, what page_reserve was given; None: T for all).
     Rows of a page that another slot holds are its rows too: page_reserve sees to it that there are none."""
-    shape = k.shape
+    shape, device = k.shape, cache.device
     S, G, T, d = shape if len(shape) == 4 else (0, 0, 0, 0)
-    if S != cache.slots or G != cache.groups or d != HEAD_DIM or k.dtype != torch.bfloat16:
+    if S != cache.slots or G != cache.groups or d != HEAD_DIM or k.dtype is not torch.bfloat16:
         raise ValueError(f"k must be a bfloat16 [slots, G, T, {HEAD_DIM}] tensor with slots, G = {cache.slots}, {cache.groups}, got "
                          f"{k.dtype} {tuple(shape)}")
-    if v.shape != shape or v.dtype != k.dtype or k.device != cache.device or v.device != cache.device:
+    if v.shape != shape or v.dtype is not torch.bfloat16 or k.device != device or v.device != device:
         raise ValueError("v must match k, on the cache's device")
     layer = int(layer)
     if not 0 <= layer < cache.layers:
         raise ValueError(f"layer {layer} outside [0, {cache.layers})")
-    at = None if tokens is None else _check_book(tokens, "tokens", (S,), cache.device).data_ptr()
+    at = None if tokens is None else _check_book(tokens, "tokens", (S,), device).data_ptr()
     k, k_at, kb, kg, kt = _rows(k, 8)
     v, v_at, vb, vg, vt = _rows(v, 8)
-    step = 2 * layer * cache.num_pages * G * cache.page_size * HEAD_DIM
-    nat.call_on(cache.device, "attnlab_page_append", k_at, kb, kg, kt, v_at, vb, vg, vt, cache.k.data_ptr() + step,
+    step = layer * cache.layer_bytes
+    nat.call_on(device, "attnlab_page_append", k_at, kb, kg, kt, v_at, vb, vg, vt, cache.k.data_ptr() + step,
                 cache.v.data_ptr() + step, cache.num_pages, G, cache.page_size, cache.table.data_ptr(), cache.lengths.data_ptr(),
-                at, S, cache.max_pages, T, nat.stream_of(cache.device))
+                at, S, cache.max_pages, T, nat.stream_of(device))
 
 
 def page_truncate(cache: PagedCache, lengths=0) -> None:

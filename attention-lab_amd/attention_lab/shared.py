@@ -14,6 +14,7 @@ from .hip_range import DEFAULT_SCALE, INT_MAX, MAX_H_CHUNK, aligned_query, check
 
 WIDE_ROWS, NARROW_ROWS = 128, 16   # (query, head) rows of a workgroup of either kernel
 MAX_SPLITS = 64
+PART_BYTES = 132 * 4               # of a row's partial
 
 
 def shared_splits(G: int, rows: int, wide: bool) -> int:
@@ -58,30 +59,32 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
     Nothing is read back to the host, so a captured graph follows the tensors' later values. Weights are rounded to bfloat16
     before their product with V (2^-8 of each at most; their sum is not rounded), sums are float32. partitions overrides how
     many partials a row may have of the shared part (1 to 64; 0: the prefix is ignored) and of the own one (1 to 64)."""
-    if (k_pages.dim() != 4 or k_pages.dtype != torch.bfloat16 or not k_pages.is_contiguous() or k_pages.shape[3] != HEAD_DIM
+    pool, device = k_pages.shape, k_pages.device
+    if (len(pool) != 4 or pool[3] != HEAD_DIM or k_pages.dtype is not torch.bfloat16 or not k_pages.is_contiguous()
             or not k_pages.is_cuda):
         raise ValueError(f"k_pages must be a contiguous bfloat16 [num_pages, G, page_size, {HEAD_DIM}] pool on a HIP device")
-    if v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype or not v_pages.is_contiguous() \
-            or v_pages.device != k_pages.device:
+    if v_pages.shape != pool or v_pages.dtype is not torch.bfloat16 or not v_pages.is_contiguous() or v_pages.device != device:
         raise ValueError("v_pages must match k_pages")
-    device = k_pages.device
-    pages, G, page, _ = k_pages.shape
-    if q.dim() != 5 or q.shape[1] != G or q.shape[4] != HEAD_DIM or q.dtype != torch.bfloat16 or q.device != device:
+    pages, G, page, _ = pool
+    shape = q.shape
+    if len(shape) != 5 or shape[1] != G or shape[4] != HEAD_DIM or q.dtype is not torch.bfloat16 or q.device != device:
         raise ValueError(f"q must be a bfloat16 [B, {G}, h, T, {HEAD_DIM}] tensor on the pools' device, got {q.dtype} "
-                         f"{tuple(q.shape)}")
-    B, _, h, T, _ = q.shape
+                         f"{tuple(shape)}")
+    B, _, h, T, _ = shape
     if not 1 <= h <= MAX_H_CHUNK:
         raise ValueError(f"h={h} must be in [1, {MAX_H_CHUNK}]")
     if B < 1 or not pages or not page or page & (page - 1):
         raise ValueError(f"need at least one sequence and page, and a page_size that is a power of two, got {B}, {pages}, {page}")
-    if (block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] < 1 or block_table.dtype != torch.int32
-            or block_table.stride(1) != 1 and block_table.shape[1] > 1 or block_table.device != device):
+    rows_b, W = block_table.shape if block_table.dim() == 2 else (0, 0)
+    if rows_b != B or W < 1 or block_table.dtype is not torch.int32 or block_table.device != device:
         raise ValueError("block_table must be an int32 [B, max_pages] tensor with unit column stride on the pools' device")
-    W = block_table.shape[1]
+    step, unit = block_table.stride()
+    if unit != 1 and W > 1:
+        raise ValueError("block_table must be an int32 [B, max_pages] tensor with unit column stride on the pools' device")
     R = 1
     if runs is not None:
         R = runs.numel() - 1
-        if runs.dim() != 1 or R < 1 or runs.dtype != torch.int32 or not runs.is_contiguous() or runs.device != device:
+        if runs.dim() != 1 or R < 1 or runs.dtype is not torch.int32 or not runs.is_contiguous() or runs.device != device:
             raise ValueError("runs must be a contiguous int32 [R + 1] tensor of at least two bounds on the pools' device")
     lengths_at, length = _lengths(lengths, B, device, "lengths")
     prefix_at, prefix = _lengths(prefix_lengths, R, device, "prefix_lengths")
@@ -100,10 +103,11 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
         ns, no = (int(x) for x in partitions)
         if not (0 <= ns <= MAX_SPLITS and 1 <= no <= MAX_SPLITS):
             raise ValueError(f"partitions must be two counts, in [0, {MAX_SPLITS}] and [1, {MAX_SPLITS}]")
-    nbytes = nat.lib().attnlab_shared_part_bytes(B, G, h, T, ns, no)
-    part = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+    rows *= G
+    nbytes = ((rows + 1) // 2 * 16 + rows * (ns + no) * PART_BYTES) if ns + no > 1 else 0   # attnlab_shared_part_bytes
+    part = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     nat.call_on(device, "attnlab_shared_prefix_attend", q_at, k_pages.data_ptr(), v_pages.data_ptr(), pages, page,
-                block_table.data_ptr(), max(block_table.stride(0), W) if B == 1 else block_table.stride(0), W, lengths_at, length,
+                block_table.data_ptr(), max(step, W) if B == 1 else step, W, lengths_at, length,
                 prefix_at, prefix, nat.ptr(runs), R, B, G, h, T, DEFAULT_SCALE if scale is None else float(scale), wide, ns, no,
                 out.data_ptr(), nat.ptr(part), nbytes, nat.stream_of(device))
     return out

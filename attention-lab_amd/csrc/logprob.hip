@@ -4,7 +4,7 @@
 //
 // A row is cut into up to 64 segments, a workgroup each. A thread holds up to 64 logits in registers, as they came, so each is read
 // once: l and s = sum p (x - m) relative to a common m of the wave's merge over the workgroup and leave as a partial (m, l, s). A second
-// launch merges a row's partials. Sums are fp32 in the log2 domain.
+// launch merges a row's partials, or, where there are few rows, the last of its workgroups to arrive. Sums are fp32 in the log2 domain.
 //
 // The top k without a second look at every logit: the k-th largest of a wave's 64 thread maxima is a lower bound of the k-th
 // largest logit, found by a search over the order-preserving key's bits with one ballot a bit; the largest of the four waves'
@@ -45,6 +45,8 @@ struct LogprobArgs {
     float* entropy;                      // [N] or null
     float* top_logprob;                  // [N, top]
     int64_t* top_token;                  // [N, top]
+    uint32_t* arrive;                    // [N] arrival counters, zero on entry and left zero: the last segment's workgroup of a row to
+                                         // arrive merges it (segments * top <= kWaveKeys); null: a second launch does
 };
 
 // Larger logit -> larger key, then lower token -> larger key. Never 0 for a token below 2^31.
@@ -136,7 +138,114 @@ __device__ __forceinline__ void rank_keys(const uint64_t* sh, int count, int top
     }
 }
 
-template <int DT, int U>
+// What threads of a merge exchange.
+struct MergeShared {
+    uint32_t bound[kWaves], count;
+    float far[kWaves][2];
+};
+constexpr int kWaveKeys = 256;
+
+// A row's partials merged by THREADS threads (a wave, or the workgroup): lane s of every wave holds segment s. COHERENT: written by
+// workgroups of this launch, read past the caches of this XCD. cand: room for the segments' keys.
+template <int DT, int THREADS, bool COHERENT>
+__device__ __forceinline__ void merge_row(const LogprobArgs& a, int64_t row, uint64_t* cand, MergeShared& sh) {
+    constexpr int kMost = THREADS == 64 ? kWaveKeys : kMaxSegments * kMaxTop, kHold = kMost / THREADS;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tid = THREADS == 64 ? lane : (int)threadIdx.x;
+    auto sync = [&]() {   // a wave's LDS operations take effect in order
+        if constexpr (THREADS == 64) asm volatile("" ::: "memory");
+        else __syncthreads();
+    };
+    const float* part = a.part + row * a.segments * kPartWords;
+    const int most = a.segments * a.top;
+    const uint64_t* best = a.best + row * most;
+    float4 p = make_float4(-INFINITY, 0.0f, 0.0f, -INFINITY);
+    if (lane < a.segments) {
+        if constexpr (COHERENT) {
+            const float* q = part + lane * kPartWords;
+            p = make_float4(load_coherent(q), load_coherent(q + 1), load_coherent(q + 2), load_coherent(q + 3));
+        } else {
+            p = *reinterpret_cast<const float4*>(part + lane * kPartWords);
+        }
+    }
+    uint64_t k[kHold];
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) {
+        k[i] = 0;
+        if (THREADS * i + tid < most) {
+            const uint64_t* q = best + THREADS * i + tid;
+            k[i] = COHERENT ? __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM) : *q;
+        }
+        mine = max(mine, (uint32_t)(k[i] >> 32));
+    }
+    const float m = wave_max(p.x), largest = wave_max(p.w);
+    rescale(p.x, m, p.y, p.z);
+    float l = wave_sum(p.y), s = wave_sum(p.z);
+    auto at = [&](int64_t t) -> float {
+        if constexpr (DT == ATTNLAB_DT_F32) return static_cast<const float*>(a.x)[row * a.stride + t];
+        const uint16_t w = static_cast<const uint16_t*>(a.x)[row * a.stride + t];
+        return DT == ATTNLAB_DT_BF16 ? bf16_to_f32(w) : f16_to_f32(w);
+    };
+    // a row whose largest logit is far from 0 (one that a mask of the type's lowest value has covered whole)
+    const bool far = fabsf(largest) >= kFar && fabsf(largest) < INFINITY;
+    if (far) {
+        l = s = 0.0f;
+        for (int t = tid; t < a.V; t += THREADS) {
+            const float d = (at(t) - largest) * kLog2e, e = fast_exp2(d);
+            l += e;
+            s += d < -1000.0f ? 0.0f : e * d;
+        }
+        l = wave_sum(l);
+        s = wave_sum(s);
+        if constexpr (THREADS > 64) {
+            if (lane == 0) {
+                sh.far[wave][0] = l;
+                sh.far[wave][1] = s;
+            }
+            __syncthreads();
+            l = s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                l += sh.far[w][0];
+                s += sh.far[w][1];
+            }
+        }
+    }
+    // no logit above -inf: no distribution
+    const float log2l = largest > -INFINITY ? log2f(l) : __builtin_nanf("");
+    // l is relative to m, not the largest logit
+    const float lnl = (log2l - (far ? 0.0f : fmaf(largest, kLog2e, -m))) * kLn2;
+    auto logprob = [&](float x) { return (x - largest) - lnl; };
+    if (tid == 0) {
+        if (a.entropy) a.entropy[row] = (log2l - s / l) * kLn2;
+        if (a.logprob) {
+            const int64_t t = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[row] : static_cast<const int32_t*>(a.tokens)[row];
+            a.logprob[row] = t < 0 ? 0.0f : t < a.V ? logprob(at(t)) : __builtin_nanf("");
+        }
+        sh.count = 0;
+    }
+    if (!a.top) return;
+    uint32_t bound = wave_kth(mine, a.top);
+    if constexpr (THREADS > 64) {
+        if (lane == 0) sh.bound[wave] = bound;
+    }
+    sync();
+    if constexpr (THREADS > 64) {
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) bound = max(bound, sh.bound[w]);
+    }
+#pragma unroll
+    for (int i = 0; i < kHold; ++i)
+        if (k[i] && (uint32_t)(k[i] >> 32) >= bound) cand[atomicAdd(&sh.count, 1u)] = k[i];
+    sync();
+    rank_keys<THREADS>(cand, (int)sh.count, a.top, [&](int i, uint64_t y) {
+        a.top_logprob[row * a.top + i] = logprob(logit_of((uint32_t)(y >> 32)));
+        a.top_token[row * a.top + i] = (int64_t)(uint32_t)~(uint32_t)y;
+    });
+}
+
+template <int DT, int U, bool MERGE>
 __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     constexpr int kPer = DT == ATTNLAB_DT_F32 ? 4 : 8, kBytes = 16 / kPer;
     __shared__ uint64_t cand_sh[kWords * kPer];
@@ -144,7 +253,8 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     __shared__ u32x4_t data_sh[kWords];
     __shared__ float part_sh[kWaves][4];
     __shared__ uint32_t bound_sh[kWaves];
-    __shared__ uint32_t words_sh, count_sh;
+    __shared__ uint32_t words_sh, count_sh, last_sh;
+    __shared__ MergeShared merge_sh;
     const int seg = blockIdx.x % a.segments;
     const int64_t row = blockIdx.x / a.segments;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -253,164 +363,107 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
             ls += lw;
             ss += sw;
         }
-        *reinterpret_cast<float4*>(a.part + (row * a.segments + seg) * kPartWords) = make_float4(ms, ls, ss, xs);
-    }
-    if (!a.top) return;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) bound = max(bound, bound_sh[w]);
-    const float least = logit_of(bound);   // NaN: every word
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const bool reaches = !(most[u] < least) && first + kThreads * u + tid < end;
-        if (reaches) {
-            const uint32_t i = atomicAdd(&words_sh, 1u);
-            if (i < kWords) {
-                word_sh[i] = (uint16_t)(kThreads * u + tid);
-                data_sh[i] = x[u];
-            }
+        float* part = a.part + (row * a.segments + seg) * kPartWords;
+        if constexpr (MERGE) {           // written through to memory, so the merging workgroup reads them on any XCD
+            store_coherent(part, ms);
+            store_coherent(part + 1, ls);
+            store_coherent(part + 2, ss);
+            store_coherent(part + 3, xs);
+        } else {
+            *reinterpret_cast<float4*>(part) = make_float4(ms, ls, ss, xs);
         }
     }
-    __syncthreads();
-    const uint32_t listed = words_sh;
-    uint64_t* best = a.best + (row * a.segments + seg) * a.top;
-    if (listed <= kWords) {
-        if (wave != 0) return;
-        for (uint32_t i = lane; i < listed; i += 64) {
-            const int t = kPer * (first + word_sh[i]) - head;
-            const u32x4_t v = data_sh[i];
+    if (a.top) {
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const uint32_t k = score_key(element<DT>(v, j));
-                if (k >= bound && t + j >= 0 && t + j < a.V)
-                    cand_sh[atomicAdd(&count_sh, 1u)] = (uint64_t)k << 32 | (uint32_t)~(t + j);
+        for (int w = 0; w < kWaves; ++w) bound = max(bound, bound_sh[w]);
+        const float least = logit_of(bound);   // NaN: every word
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool reaches = !(most[u] < least) && first + kThreads * u + tid < end;
+            if (reaches) {
+                const uint32_t i = atomicAdd(&words_sh, 1u);
+                if (i < kWords) {
+                    word_sh[i] = (uint16_t)(kThreads * u + tid);
+                    data_sh[i] = x[u];
+                }
             }
-        }
-        asm volatile("" ::: "memory");   // a wave's LDS operations take effect in order
-        const int count = (int)count_sh;
-        rank_keys<64>(cand_sh, count, a.top, [&](int r, uint64_t k) { best[r] = k; });
-        for (int r = count + lane; r < a.top; r += 64) best[r] = 0;
-        return;
-    }
-    uint64_t last = ~0ull;               // the largest key below the last one taken, `top` times
-    for (int r = 0; r < a.top; ++r) {
-        uint64_t k = 0;
-        for (int w = first + tid; w < end; w += kThreads) {
-            const int t = kPer * w - head;
-            const u32x4_t v = words[w];
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const uint64_t y = key_of(element<DT>(v, j), t + j);
-                if (t + j >= 0 && t + j < a.V && y < last && y > k) k = y;
-            }
-        }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint64_t y = (uint64_t)(uint32_t)__shfl_xor((int)(k >> 32), d, 64) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)k, d, 64);
-            k = y > k ? y : k;
         }
         __syncthreads();
-        if (lane == 0) cand_sh[wave] = k;
-        __syncthreads();
+        const uint32_t listed = words_sh;
+        uint64_t* best = a.best + (row * a.segments + seg) * a.top;
+        auto take = [&](int r, uint64_t k) {
+            if constexpr (MERGE) __hip_atomic_store(best + r, k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            else best[r] = k;
+        };
+        if (listed <= kWords) {
+            if (wave == 0) {
+                for (uint32_t i = lane; i < listed; i += 64) {
+                    const int t = kPer * (first + word_sh[i]) - head;
+                    const u32x4_t v = data_sh[i];
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) k = cand_sh[w] > k ? cand_sh[w] : k;
-        if (tid == 0) best[r] = k;
-        last = k;
+                    for (int j = 0; j < kPer; ++j) {
+                        const uint32_t k = score_key(element<DT>(v, j));
+                        if (k >= bound && t + j >= 0 && t + j < a.V)
+                            cand_sh[atomicAdd(&count_sh, 1u)] = (uint64_t)k << 32 | (uint32_t)~(t + j);
+                    }
+                }
+                asm volatile("" ::: "memory");   // a wave's LDS operations take effect in order
+                const int count = (int)count_sh;
+                rank_keys<64>(cand_sh, count, a.top, take);
+                for (int r = count + lane; r < a.top; r += 64) take(r, 0);
+            }
+        } else {
+            uint64_t last = ~0ull;           // the largest key below the last one taken, `top` times
+            for (int r = 0; r < a.top; ++r) {
+                uint64_t k = 0;
+                for (int w = first + tid; w < end; w += kThreads) {
+                    const int t = kPer * w - head;
+                    const u32x4_t v = words[w];
+#pragma unroll
+                    for (int j = 0; j < kPer; ++j) {
+                        const uint64_t y = key_of(element<DT>(v, j), t + j);
+                        if (t + j >= 0 && t + j < a.V && y < last && y > k) k = y;
+                    }
+                }
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const uint64_t y = (uint64_t)(uint32_t)__shfl_xor((int)(k >> 32), d, 64) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)k, d, 64);
+                    k = y > k ? y : k;
+                }
+                __syncthreads();
+                if (lane == 0) cand_sh[wave] = k;
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) k = cand_sh[w] > k ? cand_sh[w] : k;
+                if (tid == 0) take(r, k);
+                last = k;
+            }
+        }
+    }
+    if constexpr (MERGE) {
+        // Every store of this workgroup has completed before its count (the wait and the barrier), so the one that counts all others
+        // before itself finds every partial in memory. It leaves the counter zero.
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (tid == 0)
+            last_sh = __hip_atomic_fetch_add(a.arrive + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(a.segments - 1);
+        __syncthreads();
+        if (!last_sh || wave != 0) return;
+        static_assert(kWords * kPer >= kWaveKeys, "the merge's keys lie in the segment's");
+        merge_row<DT, 64, true>(a, row, cand_sh, merge_sh);
+        if (lane == 0) __hip_atomic_store(a.arrive + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
-// A row's partials, by THREADS threads: lane s of every wave holds segment s. A wave where the segments' lists hold 256 keys or
-// fewer, four rows to a workgroup; else a workgroup.
-constexpr int kWaveKeys = 256;
+// The rows' partials in a launch of their own: a wave a row where the segments' lists hold kWaveKeys keys or fewer, else a workgroup.
 template <int DT, int THREADS>
 __global__ __launch_bounds__(kThreads) void logprob_merge(LogprobArgs a, int64_t N) {
-    constexpr int kMost = THREADS == 64 ? kWaveKeys : kMaxSegments * kMaxTop, kHold = kMost / THREADS, kRows = kThreads / THREADS;
-    __shared__ uint64_t cand_sh[kRows][kMost];
-    __shared__ uint32_t bound_sh[kWaves];
-    __shared__ float far_sh[kWaves][2];
-    __shared__ uint32_t count_sh[kRows];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r = THREADS == 64 ? wave : 0, tid = THREADS == 64 ? lane : (int)threadIdx.x;
+    constexpr int kRows = kThreads / THREADS;
+    __shared__ uint64_t cand_sh[kRows][THREADS == 64 ? kWaveKeys : kMaxSegments * kMaxTop];
+    __shared__ MergeShared sh[kRows];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = THREADS == 64 ? wave : 0;
     const int64_t row = (int64_t)blockIdx.x * kRows + r;
-    if (row >= N) return;
-    auto sync = [&]() {   // a wave's LDS operations take effect in order
-        if constexpr (THREADS == 64) asm volatile("" ::: "memory");
-        else __syncthreads();
-    };
-    float4 p = make_float4(-INFINITY, 0.0f, 0.0f, -INFINITY);
-    if (lane < a.segments) p = *reinterpret_cast<const float4*>(a.part + (row * a.segments + lane) * kPartWords);
-    const float m = wave_max(p.x), largest = wave_max(p.w);
-    rescale(p.x, m, p.y, p.z);
-    float l = wave_sum(p.y), s = wave_sum(p.z);
-    auto at = [&](int64_t t) -> float {
-        if constexpr (DT == ATTNLAB_DT_F32) return static_cast<const float*>(a.x)[row * a.stride + t];
-        const uint16_t w = static_cast<const uint16_t*>(a.x)[row * a.stride + t];
-        return DT == ATTNLAB_DT_BF16 ? bf16_to_f32(w) : f16_to_f32(w);
-    };
-    // a row whose largest logit is far from 0 (one that a mask of the type's lowest value has covered whole)
-    const bool far = fabsf(largest) >= kFar && fabsf(largest) < INFINITY;
-    if (far) {
-        l = s = 0.0f;
-        for (int t = tid; t < a.V; t += THREADS) {
-            const float d = (at(t) - largest) * kLog2e, e = fast_exp2(d);
-            l += e;
-            s += d < -1000.0f ? 0.0f : e * d;
-        }
-        l = wave_sum(l);
-        s = wave_sum(s);
-        if constexpr (THREADS > 64) {
-            if (lane == 0) {
-                far_sh[wave][0] = l;
-                far_sh[wave][1] = s;
-            }
-            __syncthreads();
-            l = s = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                l += far_sh[w][0];
-                s += far_sh[w][1];
-            }
-        }
-    }
-    // no logit above -inf: no distribution
-    const float log2l = largest > -INFINITY ? log2f(l) : __builtin_nanf("");
-    // l is relative to m, not the largest logit
-    const float lnl = (log2l - (far ? 0.0f : fmaf(largest, kLog2e, -m))) * kLn2;
-    auto logprob = [&](float x) { return (x - largest) - lnl; };
-    if (tid == 0) {
-        if (a.entropy) a.entropy[row] = (log2l - s / l) * kLn2;
-        if (a.logprob) {
-            const int64_t t = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[row] : static_cast<const int32_t*>(a.tokens)[row];
-            a.logprob[row] = t < 0 ? 0.0f : t < a.V ? logprob(at(t)) : __builtin_nanf("");
-        }
-        count_sh[r] = 0;
-    }
-    if (!a.top) return;
-    const int most = a.segments * a.top;
-    const uint64_t* best = a.best + row * most;
-    uint64_t k[kHold];
-    uint32_t mine = 0;
-#pragma unroll
-    for (int i = 0; i < kHold; ++i) {
-        k[i] = THREADS * i + tid < most ? best[THREADS * i + tid] : 0;
-        mine = max(mine, (uint32_t)(k[i] >> 32));
-    }
-    uint32_t bound = wave_kth(mine, a.top);
-    if constexpr (THREADS > 64) {
-        if (lane == 0) bound_sh[wave] = bound;
-    }
-    sync();
-    if constexpr (THREADS > 64) {
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) bound = max(bound, bound_sh[w]);
-    }
-#pragma unroll
-    for (int i = 0; i < kHold; ++i)
-        if (k[i] && (uint32_t)(k[i] >> 32) >= bound) cand_sh[r][atomicAdd(&count_sh[r], 1u)] = k[i];
-    sync();
-    rank_keys<THREADS>(cand_sh[r], (int)count_sh[r], a.top, [&](int i, uint64_t y) {
-        a.top_logprob[row * a.top + i] = logprob(logit_of((uint32_t)(y >> 32)));
-        a.top_token[row * a.top + i] = (int64_t)(uint32_t)~(uint32_t)y;
-    });
+    if (row < N) merge_row<DT, THREADS, false>(a, row, cand_sh[r], sh[r]);
 }
 
 int per_word(int dtype) { return dtype == ATTNLAB_DT_F32 ? 4 : 8; }
@@ -432,16 +485,25 @@ int plan(int64_t N, int V, int dtype, int& segments, int& words) {
 
 constexpr int kMaxVocab = 1 << 20;      // 64 segments of 16384 logits, one word of them lost to a row's alignment
 
+template <int DT, bool MERGE>
+void launch_segments(const LogprobArgs& a, int u, int64_t N, hipStream_t s) {
+    const dim3 grid((unsigned)(N * a.segments)), wg(kThreads);
+    if (u == 1) hipLaunchKernelGGL((logprob_segment<DT, 1, MERGE>), grid, wg, 0, s, a);
+    else if (u == 2) hipLaunchKernelGGL((logprob_segment<DT, 2, MERGE>), grid, wg, 0, s, a);
+    else if (u == 4) hipLaunchKernelGGL((logprob_segment<DT, 4, MERGE>), grid, wg, 0, s, a);
+    else if (u == 8 || DT != ATTNLAB_DT_F32) hipLaunchKernelGGL((logprob_segment<DT, 8, MERGE>), grid, wg, 0, s, a);
+    else if constexpr (DT == ATTNLAB_DT_F32) hipLaunchKernelGGL((logprob_segment<DT, 16, MERGE>), grid, wg, 0, s, a);
+}
+
 template <int DT>
 int launch(const LogprobArgs& a, int u, int64_t N, hipStream_t s) {
-    const dim3 grid((unsigned)(N * a.segments)), wg(kThreads);
-    if (u == 1) hipLaunchKernelGGL((logprob_segment<DT, 1>), grid, wg, 0, s, a);
-    else if (u == 2) hipLaunchKernelGGL((logprob_segment<DT, 2>), grid, wg, 0, s, a);
-    else if (u == 4) hipLaunchKernelGGL((logprob_segment<DT, 4>), grid, wg, 0, s, a);
-    else if (u == 8) hipLaunchKernelGGL((logprob_segment<DT, 8>), grid, wg, 0, s, a);
-    else hipLaunchKernelGGL((logprob_segment<DT, 16>), grid, wg, 0, s, a);
-    if (a.segments * a.top <= kWaveKeys) hipLaunchKernelGGL((logprob_merge<DT, 64>), dim3((unsigned)((N + 3) / 4)), wg, 0, s, a, N);
-    else hipLaunchKernelGGL((logprob_merge<DT, kThreads>), dim3((unsigned)N), wg, 0, s, a, N);
+    if (a.arrive) {
+        launch_segments<DT, true>(a, u, N, s);
+        return check_launch("token_logprobs");
+    }
+    launch_segments<DT, false>(a, u, N, s);
+    if (a.segments * a.top <= kWaveKeys) hipLaunchKernelGGL((logprob_merge<DT, 64>), dim3((unsigned)((N + 3) / 4)), dim3(kThreads), 0, s, a, N);
+    else hipLaunchKernelGGL((logprob_merge<DT, kThreads>), dim3((unsigned)N), dim3(kThreads), 0, s, a, N);
     return check_launch("token_logprobs");
 }
 
@@ -459,7 +521,7 @@ extern "C" int64_t attnlab_logprob_part_bytes(int64_t N, int V, int dtype, int t
 
 extern "C" int attnlab_token_logprobs(const void* logits, int dtype, int64_t stride, int64_t N, int V, const void* tokens,
                                       int tokens64, int top, float* logprobs, float* entropy, float* top_logprobs,
-                                      int64_t* top_tokens, void* part, int64_t part_bytes, void* stream) {
+                                      int64_t* top_tokens, void* part, int64_t part_bytes, uint32_t* arrive, void* stream) {
     ATTNLAB_REQUIRE(dtype == ATTNLAB_DT_BF16 || dtype == ATTNLAB_DT_F16 || dtype == ATTNLAB_DT_F32,
                     "logits must be bf16, fp16 or fp32 (dtype %d)", dtype);
     ATTNLAB_REQUIRE(N >= 0 && 1 <= V && V <= kMaxVocab - 16, "rows N=%lld must not be negative and V=%d be in [1, %d]", (long long)N, V,
@@ -472,13 +534,14 @@ extern "C" int attnlab_token_logprobs(const void* logits, int dtype, int64_t str
     const int bytes = dtype == ATTNLAB_DT_F32 ? 4 : 2;
     ATTNLAB_REQUIRE(reinterpret_cast<uintptr_t>(logits) % bytes == 0, "logits must be aligned to their type");
     LogprobArgs a{logits, stride, V, 0, 0, top, static_cast<float*>(part), nullptr, tokens, tokens64, logprobs, entropy, top_logprobs,
-                  top_tokens};
+                  top_tokens, nullptr};
     const int u = plan(N, V, dtype, a.segments, a.words);
     ATTNLAB_REQUIRE(N * a.segments < (int64_t)1 << 31, "%lld rows of %d segments are too many", (long long)N, a.segments);
     const int64_t need = attnlab_logprob_part_bytes(N, V, dtype, top);
     ATTNLAB_REQUIRE(part && reinterpret_cast<uintptr_t>(part) % 16 == 0 && part_bytes >= need,
                     "part must be a 16-byte aligned device buffer of %lld bytes", (long long)need);
     a.best = reinterpret_cast<uint64_t*>(a.part + N * a.segments * kPartWords);
+    a.arrive = a.segments * top <= kWaveKeys ? arrive : nullptr;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     if (dtype == ATTNLAB_DT_BF16) return launch<ATTNLAB_DT_BF16>(a, u, N, s);
     if (dtype == ATTNLAB_DT_F16) return launch<ATTNLAB_DT_F16>(a, u, N, s);

@@ -30,7 +30,7 @@ constexpr int kColumns = 16;                 // table entries a fork's workgroup
 constexpr int kBook = 1024;                  // threads of the reserve's and the compaction's workgroup
 constexpr int kScan = 16;                    // pages a thread looks at in a round
 constexpr int kCopyRows = 16;                // rows of a page that a wave copies at a time: 4 KB, four loads in flight
-constexpr int kAppendRun = 64;               // rows that a workgroup of a long write takes
+constexpr int kAppendRun = 32;               // rows that a workgroup of a long write takes
 constexpr int kCopyGroups = 2048;            // workgroups of a copy: eight per CU, one wave of each SIMD from each
 
 // What a reserve or a compaction leaves to its copies, in the scratch buffer.
@@ -62,19 +62,35 @@ __global__ __launch_bounds__(256) void page_fork(Book a, const int32_t* parents)
         }
         return;
     }
+    // eight rows of a thread on their way at a time
+    constexpr int kStep = 256 / kColumns, kAhead = 8;
     const int e0 = blockIdx.x * kColumns, col = tid & (kColumns - 1);
     const bool in = e0 + col < a.W;
-    for (int i = tid / kColumns; i < a.S; i += 256 / kColumns)
-        was[i * kColumns + col] = in ? a.table[(size_t)i * a.W + e0 + col] : -1;
+    for (int i0 = tid / kColumns; i0 < a.S; i0 += kStep * kAhead) {
+        int32_t v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            v[u] = in ? a.table[(size_t)min(i0 + kStep * u, a.S - 1) * a.W + e0 + col] : -1;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (i0 + kStep * u < a.S) was[(i0 + kStep * u) * kColumns + col] = v[u];
+    }
     __syncthreads();
     if (!in) return;
-    for (int i = tid / kColumns; i < a.S; i += 256 / kColumns) {
-        const int p = parents[i];
-        const int32_t old = was[i * kColumns + col], now = names(p, a.S) ? was[p * kColumns + col] : -1;
-        if (now == old) continue;
-        if (names(old, a.pages)) atomicSub(a.refs + old, 1);
-        if (names(now, a.pages)) atomicAdd(a.refs + now, 1);
-        a.table[(size_t)i * a.W + e0 + col] = now;
+    for (int i0 = tid / kColumns; i0 < a.S; i0 += kStep * kAhead) {
+        int32_t p[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) p[u] = parents[min(i0 + kStep * u, a.S - 1)];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + kStep * u;
+            if (i >= a.S) break;
+            const int32_t old = was[i * kColumns + col], now = names(p[u], a.S) ? was[p[u] * kColumns + col] : -1;
+            if (now == old) continue;
+            if (names(old, a.pages)) atomicSub(a.refs + old, 1);
+            if (names(now, a.pages)) atomicAdd(a.refs + now, 1);
+            a.table[(size_t)i * a.W + e0 + col] = now;
+        }
     }
 }
 
@@ -94,54 +110,66 @@ __global__ __launch_bounds__(256) void page_truncate(Book a, const int32_t* to, 
     }
 }
 
-// Inclusive prefix sum of x over the workgroup's threads (sh: a word for each of its waves).
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sh, uint32_t& total) {
+// Inclusive prefix sums of x and y over the workgroup's threads (sh: two words for each of its waves), and their totals.
+__device__ __forceinline__ void block_scan(uint32_t& x, uint32_t& y, uint2* sh, uint32_t& all_x, uint32_t& all_y) {
     const int wave = threadIdx.x >> 6, waves = kBook / 64;
-    const uint32_t own = wave_incl_scan(x);
+    x = wave_incl_scan(x);
+    y = wave_incl_scan(y);
+    if ((threadIdx.x & 63) == 63) sh[wave] = make_uint2(x, y);
     __syncthreads();
-    if ((threadIdx.x & 63) == 63) sh[wave] = own;
-    __syncthreads();
-    uint32_t before = 0;
-    total = 0;
+    uint2 before = make_uint2(0, 0);
+    all_x = all_y = 0;
 #pragma unroll
     for (int w = 0; w < waves; ++w) {
-        before += w < wave ? sh[w] : 0u;
-        total += sh[w];
+        const uint2 v = sh[w];
+        before.x += w < wave ? v.x : 0u;
+        before.y += w < wave ? v.y : 0u;
+        all_x += v.x;
+        all_y += v.y;
     }
-    return before + own;
+    x += before.x;
+    y += before.y;
 }
 
 // Pages base + 1024 u + thread, u < kScan, of which `flag(page)` says whether they count: for each that does, its rank among
 // the pages in ascending order is handed to `take(page, rank)`. `found`: the rank of the first, advanced.
 template <typename Flag, typename Take>
-__device__ __forceinline__ void rank_pages(int base, int pages, uint32_t& found, uint32_t (*sh)[kBook / 64], Flag flag, Take take) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+__device__ __forceinline__ void rank_pages(int base, int pages, uint32_t& found, uint4* sh, Flag flag, Take take) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    static_assert(kScan * kBook / 64 == 4 * 64, "a count for each wave and round, four to a lane");
     uint64_t hit[kScan];
 #pragma unroll
     for (int u = 0; u < kScan; ++u) hit[u] = __ballot(base + kBook * u + tid < pages && flag(u));
     __syncthreads();
     if (lane == 0) {
 #pragma unroll
-        for (int u = 0; u < kScan; ++u) sh[u][wave] = (uint32_t)__popcll(hit[u]);
+        for (int u = 0; u < kScan; ++u) reinterpret_cast<uint32_t*>(sh)[kBook / 64 * u + wave] = (uint32_t)__popcll(hit[u]);
     }
     __syncthreads();
+    // every wave sums the counts up for itself: lane l those of round l / 4, waves 4 (l % 4) ..
+    const uint4 c = sh[lane];
+    const uint32_t own = c.x + c.y + c.z + c.w, upto = wave_incl_scan(own);
+    const int part = wave & 3;
+    const uint32_t before = found + upto - own + (part > 0 ? c.x : 0u) + (part > 1 ? c.y : 0u) + (part > 2 ? c.z : 0u);
+    found += (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+#pragma unroll
     for (int u = 0; u < kScan; ++u) {
-        uint32_t before = found;
-        for (int w = 0; w < kBook / 64; ++w) {
-            const uint32_t x = sh[u][w];
-            before += w < wave ? x : 0u;
-            found += x;
-        }
-        if (hit[u] >> lane & 1) take(base + kBook * u + tid, before + (uint32_t)__popcll(hit[u] & ((1ull << lane) - 1)));
+        const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)before, 4 * u + (wave >> 2));
+        if (hit[u] >> lane & 1) take(base + kBook * u + tid, first + (uint32_t)__popcll(hit[u] & ((1ull << lane) - 1)));
     }
 }
 
 __global__ __launch_bounds__(kBook) void page_reserve(Book a, const int32_t* tokens, int each, int32_t* missing, Moves* moves,
                                                       int32_t* src, int32_t* dst, int32_t* rows) {
-    __shared__ uint32_t wave_sh[kBook / 64], scan_sh[kScan][kBook / 64];
-    __shared__ int32_t held_sh[kMaxSlots], first_sh[kMaxSlots], part_sh[kMaxSlots];
+    __shared__ uint2 wave_sh[kBook / 64];
+    __shared__ uint4 scan_sh[64];
+    __shared__ __attribute__((aligned(16))) int32_t held_sh[kMaxSlots];   // -1 past the slots
+    __shared__ int32_t first_sh[kMaxSlots], part_sh[kMaxSlots];
     __shared__ uint32_t upto_sh[kMaxSlots], job_sh[kMaxSlots];   // requests up to and with a slot's; its copy's number + 1, or 0
     const int tid = threadIdx.x, page = 1 << a.shift;
+    int32_t pool[kScan];                     // the first pages' counts, on their way from the start; only free ones change below
+#pragma unroll
+    for (int u = 0; u < kScan; ++u) pool[u] = a.refs[min(kBook * u + tid, a.pages - 1)];
     const bool slot = tid < a.S;
     const int n = slot ? max(a.lengths[tid], 0) : 0, t = slot ? max(tokens ? tokens[tid] : each, 0) : 0;
     const int64_t end = min((int64_t)n + t, (int64_t)INT32_MAX);
@@ -154,19 +182,22 @@ __global__ __launch_bounds__(kBook) void page_reserve(Book a, const int32_t* tok
     bool copies = false;
     if (held >= 0) {
         int writers = 0, later = 0;
-        for (int j = 0; j < a.S; ++j) {
-            const bool same = held_sh[j] == held;
-            writers += same;
-            later |= same && j > tid;
+        for (int j = 0; j < a.S; j += 4) {
+            const int4 v = *reinterpret_cast<const int4*>(held_sh + j);
+            const int same[4] = {v.x == held, v.y == held, v.z == held, v.w == held};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                writers += same[i];
+                later |= same[i] && j + i > tid;
+            }
         }
         copies = later || writers < refs;
     }
     const int from = (int)(((int64_t)n + page - 1) >> a.shift), upto = (int)((end + page - 1) >> a.shift);
     const int fresh = max(min(upto, a.W) - from, 0);
-    uint32_t lost = t > 0 ? (uint32_t)max(upto - max(from, a.W), 0) : 0u;   // pages that the table has no entry for
-    uint32_t wanted, jobs;
-    const uint32_t to = block_scan((t > 0 ? (uint32_t)fresh : 0u) + copies, wave_sh, wanted);
-    const uint32_t job = block_scan(copies, wave_sh, jobs);
+    const int lost = t > 0 ? max(upto - max(from, a.W), 0) : 0;   // pages that the table has no entry for
+    uint32_t wanted, jobs, to = (t > 0 ? (uint32_t)fresh : 0u) + copies, job = copies;
+    block_scan(to, job, wave_sh, wanted, jobs);
     if (slot) {
         first_sh[tid] = from;
         part_sh[tid] = part;
@@ -195,10 +226,11 @@ __global__ __launch_bounds__(kBook) void page_reserve(Book a, const int32_t* tok
     };
     uint32_t found = 0;
     for (int base = 0; base < a.pages && found < wanted; base += kBook * kScan) {
-        int32_t r[kScan];
+        if (base > 0) {
 #pragma unroll
-        for (int u = 0; u < kScan; ++u) r[u] = a.refs[min(base + kBook * u + tid, a.pages - 1)];
-        rank_pages(base, a.pages, found, scan_sh, [&](int u) { return r[u] <= 0; }, [&](int p, uint32_t rank) {
+            for (int u = 0; u < kScan; ++u) pool[u] = a.refs[min(base + kBook * u + tid, a.pages - 1)];
+        }
+        rank_pages(base, a.pages, found, scan_sh, [&](int u) { return pool[u] <= 0; }, [&](int p, uint32_t rank) {
             if (rank >= wanted) return;
             a.refs[p] = 1;
             give(rank, p);
@@ -206,19 +238,18 @@ __global__ __launch_bounds__(kBook) void page_reserve(Book a, const int32_t* tok
     }
     for (uint32_t r = found + tid; r < wanted; r += kBook) give(r, -1);
     if (copies) atomicSub(a.refs + held, 1);
-    const uint32_t out = wanted > found ? wanted - found : 0u;
-    uint32_t over;
-    block_scan(lost, wave_sh, over);
-    if (tid == 0) {
-        moves->count = (int32_t)jobs;
-        if (missing && out + over) missing[0] += (int32_t)(out + over);
+    if (tid == 0) moves->count = (int32_t)jobs;
+    if (missing) {
+        const int out = lost + (tid == 0 && wanted > found ? (int)(wanted - found) : 0);
+        if (out) atomicAdd(missing, out);
     }
 }
 
 __global__ __launch_bounds__(kBook) void page_compact(Book a, Moves* moves, int32_t* src, int32_t* dst, int32_t* rank_of) {
-    __shared__ uint32_t wave_sh[kBook / 64], scan_sh[kScan][kBook / 64];
+    __shared__ uint2 wave_sh[kBook / 64];
+    __shared__ uint4 scan_sh[64];
     const int tid = threadIdx.x;
-    uint32_t mine = 0, used;
+    uint32_t mine = 0, none = 0, used, all;
     for (int base = 0; base < a.pages; base += kBook * kScan) {
         int32_t r[kScan];
 #pragma unroll
@@ -226,7 +257,7 @@ __global__ __launch_bounds__(kBook) void page_compact(Book a, Moves* moves, int3
 #pragma unroll
         for (int u = 0; u < kScan; ++u) mine += base + kBook * u + tid < a.pages && r[u] > 0;
     }
-    block_scan(mine, wave_sh, used);
+    block_scan(mine, none, wave_sh, used, all);
     uint32_t holes = 0, high = 0;
     for (int base = 0; base < a.pages; base += kBook * kScan) {
         int32_t r[kScan];
@@ -326,7 +357,7 @@ __device__ __forceinline__ int64_t row_of(const AppendArgs& a, int i, int g, int
 }
 
 // Sixteen lanes a row, K or V by blockIdx.y. Few tokens (LONG false): rows of all slots and groups in line, sixteen to a
-// workgroup; else 64 consecutive rows of one (slot, group).
+// workgroup; else kAppendRun consecutive rows of one (slot, group).
 template <bool LONG>
 __global__ __launch_bounds__(256) void page_append(AppendArgs a, int runs) {
     constexpr int kRows = LONG ? kAppendRun / 16 : 1;

@@ -466,12 +466,14 @@ int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k_pages, con
  *   top_tokens, top_logprobs [N, top]: the largest logits in order, equal ones by the lower token (-0 equals +0, NaN last)
  * tokens and logprobs are null together. A row with a NaN, an infinity of positive sign or nothing above -inf has no
  * distribution: its values are NaN (top_tokens stay those of the order). 0 <= top <= min(64, V), V <= 2^20 - 16.
- * part: 16-byte aligned, attnlab_logprob_part_bytes bytes, no initialisation. Two launches.
+ * part: 16-byte aligned, attnlab_logprob_part_bytes bytes, no initialisation. Two launches, or one where arrive (uint32 [N],
+ * zero on entry, left zero, not shared with a call that may overlap) is given and a row's segments have at most 256 candidates between
+ * them; the same result.
  */
 int64_t attnlab_logprob_part_bytes(int64_t N, int V, int dtype, int top);
 int attnlab_token_logprobs(const void* logits, int dtype, int64_t stride, int64_t N, int V, const void* tokens, int tokens64,
                            int top, float* logprobs, float* entropy, float* top_logprobs, int64_t* top_tokens, void* part,
-                           int64_t part_bytes, void* stream);
+                           int64_t part_bytes, uint32_t* arrive, void* stream);
 
 /*
  * Workspace (bytes) of attnlab_sparse_decode_step for these sizes: candidate scores, row list, u, tiled-select

@@ -8,7 +8,7 @@ import attention_lab
 from attention_lab import _native, token_logprobs
 
 ARGS = dict(logits=16, dtype=0, stride=1000, N=3, V=1000, tokens=16, tokens64=1, top=5, logprobs=16, entropy=None, top_logprobs=16,
-            top_tokens=16, part=16, part_bytes=1 << 20, stream=None)
+            top_tokens=16, part=16, part_bytes=1 << 20, arrive=None, stream=None)
 
 
 @pytest.mark.parametrize("change,match", [
