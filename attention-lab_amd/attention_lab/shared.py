@@ -17,10 +17,10 @@ MAX_SPLITS = 64
 PART_BYTES = 132 * 4               # of a row's partial
 
 
-def shared_splits(G: int, rows: int, wide: bool) -> int:
+def shared_splits(G: int, rows: int, wide: bool, chunk: bool = False) -> int:
     """Partials of the shared part that a row's room is made for, `rows` (query, head) rows of a group over all sequences: the
-    workgroups that come to a tile of rows if all sequences share, and a piece."""
-    per, workers = (WIDE_ROWS, 512) if wide else (NARROW_ROWS, 768)
+    workgroups that come to a tile of rows if all sequences share, and a piece (chunk: several queries a sequence)."""
+    per, workers = (NARROW_ROWS, 768) if not wide else (WIDE_ROWS, 512 if chunk else 256)
     return min(MAX_SPLITS, workers // (G * -(-rows // per)) + 2)
 
 
@@ -97,7 +97,7 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
     rows = B * h * T
     wide = T > 1 or rows > NARROW_ROWS * R
     if partitions is None:
-        ns = shared_splits(G, rows, wide) if keys else 0
+        ns = shared_splits(G, rows, wide, T > 1) if keys else 0
         no = own_splits(B * G, h * T if T > 1 else 1, most if prefix_at else most - keys)
     else:
         ns, no = (int(x) for x in partitions)

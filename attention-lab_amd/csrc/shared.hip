@@ -38,7 +38,10 @@ constexpr int kWaves = 4;
 constexpr float kLazy = 8.0f;               // a row's shift is set 2^8 above its largest score and moves when one passes it
 constexpr int kPart = 132;                  // m, l, two unused words, the 128 unnormalised outputs
 constexpr int kMaxSplits = 64;              // partials that a row has of either part, at most
-constexpr int kWideWorkers = 512, kNarrowWorkers = 768;   // shares of the shared part: two workgroups per CU, or three
+// Shares that the shared part is cut into: two workgroups per CU where all are wide, three where all are narrow. One where wide ones go
+// with narrow ones of the own part, which take the other half of each CU: 4 prompts of 9K with 13 answers each take 67 us, 79 with two,
+// 69 and 71 with 224 and 320 shares; 48 answers (h=8) of 1500 to 14K 83 and 101; with little to read behind the prompt they are alike.
+constexpr int kWideWorkers = 512, kMixedWorkers = 256, kNarrowWorkers = 768;
 
 struct SharedArgs {
     const uint16_t* q;        // [B, G, h, T, 128]
@@ -139,14 +142,13 @@ constexpr uint32_t kLongBlocks = 64;
 
 // The shared part's workgroup `turn` of XCD `xcd`: a group, a run, a share of its blocks of kBlock keys, and a tile of kRows of its
 // rows. The tiles that read the same keys lie next to each other, on one XCD. False: there are fewer.
-template <int kRows, int kBlock>
+template <int kRows, int kBlock, uint32_t kWorkers>
 __device__ __forceinline__ bool shared_item(const SharedArgs& a, int xcd, int turn, Item& w) {
     auto tiles = [&](const Run& r) { return r.prefix > 0 ? (uint32_t)(((int64_t)r.count * a.T * a.h + kRows - 1) / kRows) : 0u; };
     auto blocks = [&](const Run& r) { return (uint32_t)(r.prefix + kBlock - 1) / kBlock; };
     auto sum = [&](uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_incl_scan(x), 63); };
     // the blocks of all tiles (sums of 16, 24 and 24 bits of them), and of the longest
     const Runs runs(a);
-    constexpr uint32_t kWorkers = kRows == kWide ? kWideWorkers : kNarrowWorkers;
     uint64_t total = 0;
     uint32_t longest = 1;
     runs.walk(a, [&](const Run& run) {
@@ -313,7 +315,8 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
     // keys before `lim` are this lane's row's; the least and the most of the wave's rows
     const int len = w.shared ? 0 : length_of(a, w.b0);
     auto limit = [&](int r) { return w.shared ? INT32_MAX : len - a.T + min(w.r0 + min(r, w.rows - 1), a.T * a.h - 1) / a.h + 1; };
-    const int lim = limit(R), lim_min = limit(32 * wave), lim_max = limit(32 * wave + 31);
+    // (a wave without a row of its own only copies)
+    const int lim = limit(R), lim_min = limit(32 * wave), lim_max = 32 * wave < w.rows ? limit(32 * wave + 31) : 0;
     const bool dead = w.shared && !sees(a, row.b, w.end);
 
     // staging: a load of a wave fills 1 KB of a tile, four rows, lane l slot l % 16 of row l / 16 of them
@@ -828,24 +831,22 @@ __global__ __launch_bounds__(64 * kWaves, WIDE ? 2 : 3) void shared_read(SharedA
     __shared__ __attribute__((aligned(1024))) char t2[WIDE ? kKeys * 2 * kDim : 1], t3[WIDE ? kKeys * 2 * kDim : 1];
     __shared__ float ml_sh[kWaves][kNarrow][2];
     __shared__ int again;
-    // Each XCD an eighth of either part's items, in line. One query a sequence: the two parts evenly mixed, so that the shared part
-    // keeps the matrix cores busy while the own part waits for memory. Several: the shared part, whose items are longer, first.
-    const int xcd = blockIdx.x & 7, turn = blockIdx.x >> 3, turns = gridDim.x >> 3;
-    const int before = OWN_WIDE ? min(turn, a.shared_turns) : (int)((uint64_t)turn * a.shared_turns / turns);
-    const int upto = OWN_WIDE ? min(turn + 1, a.shared_turns) : (int)((uint64_t)(turn + 1) * a.shared_turns / turns);
-    const bool first = upto > before;
-    const int own = __builtin_amdgcn_readfirstlane(xcd * a.own_turns + turn - before);
+    // each XCD an eighth of either part's items, in line, the shared part's, which are longer, first
+    const int xcd = blockIdx.x & 7, turn = blockIdx.x >> 3;
+    const bool first = turn < a.shared_turns;
+    const int own = __builtin_amdgcn_readfirstlane(xcd * a.own_turns + turn - a.shared_turns);
     if (!first && own >= a.own_items) return;
     Item w;
     if constexpr (WIDE && !OWN_WIDE) {
         if (first) {
-            if (shared_item<kWide, kKeys>(a, xcd, before, w)) wide<SMALL>(a, w, t0, t1, t2, t3, again);
+            if (shared_item<kWide, kKeys, kMixedWorkers>(a, xcd, turn, w)) wide<SMALL>(a, w, t0, t1, t2, t3, again);
         } else {
             if (own_item<kNarrow, kTile>(a, own, w)) narrow<SMALL, !SMALL>(a, w, t0, t1, ml_sh);
         }
     } else {
         constexpr int kRows = WIDE ? kWide : kNarrow, kBlock = WIDE ? kKeys : kTile;
-        if (!(first ? shared_item<kRows, kBlock>(a, xcd, before, w) : own_item<kRows, kBlock>(a, own, w))) return;
+        constexpr uint32_t kWorkers = WIDE ? kWideWorkers : kNarrowWorkers;
+        if (!(first ? shared_item<kRows, kBlock, kWorkers>(a, xcd, turn, w) : own_item<kRows, kBlock>(a, own, w))) return;
         if constexpr (WIDE) wide<SMALL>(a, w, t0, t1, t2, t3, again);
         else narrow<SMALL, false>(a, w, t0, t1, ml_sh);
     }
@@ -1000,7 +1001,7 @@ extern "C" int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k
     if (own_wide) wide = 1;
     const int own_rows = own_wide ? kWide : kNarrow;
     const int64_t own = (int64_t)B * G * ((T * (int64_t)h + own_rows - 1) / own_rows) * own_splits;
-    const int workers = shared_splits == 0 ? 0 : wide ? kWideWorkers : kNarrowWorkers;
+    const int workers = !wide ? kNarrowWorkers : own_wide ? kWideWorkers : kMixedWorkers;
     // Workgroups of the shared part: a piece of every tile of rows (a run's last one can be partly empty: one such for each run that
     // has a row) beside the shares that the chip holds at once, or one of every tile; or all shares of the longest prefixes that
     // the tables have room for
