@@ -43,6 +43,7 @@ from .full import full_attention
 from .hip_attend import HEAD_DIM
 from .hip_range import MAX_H, MAX_H_CHUNK, check_window
 from .indexer import GroupedIndexer, project_keys
+from .logprobs import TokenLogprobs, token_logprobs
 from .quant import (BLOCKS, SMALLEST, KeptRows, QuantCache, append_kept, quant_attention, quant_gather_attention,
                     quantize_append)
 from .selection import FIXED_PREFIX, FIXED_RECENT, fixed_budget, selection_layout
@@ -810,6 +811,22 @@ class LabRunner:
         logits = [self.forward(input_ids[:, a:b], phase="prefill", logits_to_keep=0 if keep_logits else 1)
                   for a, b in _chunks(input_ids.shape[1], chunk)]
         return torch.cat(logits, dim=1) if keep_logits else logits[-1]
+
+    def score(self, input_ids: torch.Tensor, chunk: int, *, top: int = 0, entropy: bool = False) -> TokenLogprobs:
+        """prefill of the prompt, with every token's log probability given those before it: token_logprobs of [B, T - 1]
+        positions, position t the distribution behind token t and the logprob of token t + 1. Each chunk's logits are read
+        once and dropped. No counterpart in the reference, whose scripts take log_softmax of kept logits."""
+        B, T = input_ids.shape
+        if T < 2:
+            raise ValueError(f"need at least two tokens to score one, got {T}")
+        parts = []
+        for a, b in _chunks(T, chunk):
+            logits = self.forward(input_ids[:, a:b], phase="prefill", logits_to_keep=0)
+            given = input_ids[:, a + 1:b + 1]
+            if given.shape[1] < b - a:   # the last token has none behind it: padding
+                given = torch.nn.functional.pad(given, (0, 1), value=-1)
+            parts.append(token_logprobs(logits, given, top=top, entropy=entropy))
+        return TokenLogprobs(*(None if field[0] is None else torch.cat(field, dim=1)[:, :T - 1] for field in zip(*parts)))
 
     def step(self, token_ids: torch.Tensor) -> torch.Tensor:
         """One decode step: [B, 1] token ids -> [B, 1, V] next-token logits."""
