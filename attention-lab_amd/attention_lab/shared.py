@@ -51,9 +51,9 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
     skipped, and a query that reads nothing gets zeros. h <= 16.
 
     Sequences runs[r] .. runs[r + 1] - 1 (runs int32 [R + 1] on the device, ascending; None: one run of all) share their first
-    prefix_lengths[r] positions (an int for all, or int32 [R] on the device): below it, rounded down to whole pages, their
-    tables name the same pages, and the first one's are read for all. Sequences in no run, and those not long enough for
-    all of their queries to see the whole prefix, read everything by their own tables. prefix_lengths 0: a read of a paged cache
+    prefix_lengths[r] positions (an int for all, or int32 [R] on the device): below it, rounded down to whole pages, the
+    tables of those that are long enough for all of their queries to see the whole prefix name the same pages, and one's are
+    read for all. The others, and sequences in no run, read everything by their own tables. prefix_lengths 0: a read of a paged cache
     with a length per sequence.
 
     Nothing is read back to the host, so a captured graph follows the tensors' later values. Weights are rounded to bfloat16

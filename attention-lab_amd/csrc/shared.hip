@@ -131,9 +131,9 @@ __device__ __forceinline__ int prefix_of_sequence(const SharedArgs& a, int b) {
 __device__ __forceinline__ bool sees(const SharedArgs& a, int b, int prefix) { return length_of(a, b) - a.T + 1 >= prefix; }
 
 // What a workgroup does: `rows` rows from row r0 of `count` sequences from b0 on, over the blocks [i0, i1) of the keys [base, end)
-// of sequence b0's table, its partials in slot `slot`. partials > 0: it says that the rows have so many of this part.
+// of sequence tb's table, its partials in slot `slot`. partials > 0: it says that the rows have so many of this part.
 struct Item {
-    int b0, count, r0, rows, base, end, i0, i1, slot, partials, g;
+    int b0, tb, count, r0, rows, base, end, i0, i1, slot, partials, g;
     bool shared;
 };
 
@@ -206,6 +206,18 @@ __device__ __forceinline__ bool shared_item(const SharedArgs& a, int xcd, int tu
         w.partials = part == 0 ? (int)((of(k) + share - 1) / share) : 0;
         return true;
     });
+    // The table of the first sequence that sees the whole prefix: one that has ended or been cut back need not name its pages any
+    // more. None: nothing to read, but the rows are to be told so.
+    const int lane = threadIdx.x & 63;
+    w.tb = -1;
+    for (int b = 0; b < w.count && w.tb < 0; b += 64) {
+        const uint64_t hit = __ballot(b + lane < w.count && sees(a, w.b0 + min(b + lane, w.count - 1), w.end));
+        if (hit) w.tb = w.b0 + b + (int)__builtin_ctzll(hit);
+    }
+    if (w.tb < 0) {
+        w.tb = w.b0;
+        w.i1 = w.i0;
+    }
     w.rows = (int)min((int64_t)w.count * a.T * a.h - w.r0, (int64_t)kRows);
     w.base = 0;
     w.shared = true;
@@ -221,7 +233,7 @@ __device__ __forceinline__ bool own_item(const SharedArgs& a, int lin, Item& w) 
     w.r0 = (tiles - 1 - lin % tiles) * kRows;   // later queries read more keys: first
     lin /= tiles;
     w.g = lin % a.G;
-    w.b0 = lin / a.G;
+    w.tb = w.b0 = lin / a.G;
     w.count = 1;
     w.rows = min(a.T * a.h - w.r0, kRows);
     const int n = length_of(a, w.b0), prefix = a.shared ? prefix_of_sequence(a, w.b0) : 0;
@@ -322,7 +334,7 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
     // staging: a load of a wave fills 1 KB of a tile, four rows, lane l slot l % 16 of row l / 16 of them
     const int srow = lane >> 4, slot = lane & 15;
     const int kchunk = 16 * (slot ^ (4 * wave + srow)), vchunk = 16 * (slot ^ (4 * srow));
-    const int32_t* pages = a.table + (size_t)w.b0 * a.table_stride;
+    const int32_t* pages = a.table + (size_t)w.tb * a.table_stride;
     auto first_key = [&](int i) { return w.base + kKeys * i; };
     // the entries of block i's pages, as they stand in the table: lane u of four that of keys 16 u .., or lane j key j's
     auto look = [&](int i) {
@@ -541,6 +553,7 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
     if (w.i0 < w.i1) {
         next = look(w.i0);
         have = issue(w.i0, kt0, vt0);
+        __builtin_amdgcn_sched_barrier(0);   // in this order: the wait for the first block's counts the second's
         if (w.i0 + 1 < w.i1) second = issue(w.i0 + 1, kt1, vt1);
     }
     for (int i = w.i0; i < w.i1; i += 2) {
@@ -652,7 +665,7 @@ __device__ __forceinline__ void narrow(const SharedArgs& a, const Item& w, char*
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt) o[dt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-    const int32_t* pages = a.table + (size_t)w.b0 * a.table_stride;
+    const int32_t* pages = a.table + (size_t)w.tb * a.table_stride;
     auto look = [&](int i) {
         const int key = w.base + kTile * min(i, w.i1 - 1) + (SMALL ? lane & 31 : 16 * (lane & 1));
         return pages[min(key, w.end - 1) >> a.shift];

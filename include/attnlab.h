@@ -439,10 +439,10 @@ int attnlab_page_compact(uint16_t* k, uint16_t* v, int layers, int num_pages, in
  *   out[b,g,i,t] = sum_j softmax_j(scale q[b,g,i,t] . k_j) v_j    over j <= n - T + t, k_j and v_j by b's table
  * Positions on an entry outside [0, num_pages) are skipped; a query that reads nothing gets zeros. What a later position of the
  * sequence holds (NaN, infinity) does not reach an output.
- * runs (int32 [R + 1] on the device, ascending; null with R = 1: all sequences): the tables of sequences runs[r] .. runs[r + 1]
- * - 1 name the same pages below prefix_lengths[r] (int32 [R] on the device, or null: prefix_length) rounded down to whole pages;
- * they are read by the first one's table, once for all. A run begins no earlier than the largest bound before it. A sequence in no
- * run, or of which some query does not see the whole of that prefix, reads everything by its own table.
+ * runs (int32 [R + 1] on the device, ascending; null with R = 1: all sequences): sequences runs[r] .. runs[r + 1] - 1 share the
+ * pages below prefix_lengths[r] (int32 [R] on the device, or null: prefix_length) rounded down to whole pages. The tables of those
+ * of which every query sees all of that prefix name the same pages there, and one's are read for all of them; the others, and
+ * sequences in no run, read everything by their own tables. A run begins no earlier than the largest bound before it.
  * q, out: [B, G, h, T, 128] bf16 contiguous, 16-byte aligned, 1 <= h <= 16; block_table [B, bt_stride]. wide: the shared part by
  * workgroups of 128 (sequence, query, head) rows instead of 16 (always so for T > 1). shared_splits (1..64, or 0: no shared part,
  * every sequence reads by its own table) and own_splits (1..64): partials of the two parts that a row has at most, which limits

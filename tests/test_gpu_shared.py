@@ -189,6 +189,21 @@ def test_short_sequences(gpu, T, sizes):
             c.check(c.call(gpu))
 
 
+@pytest.mark.parametrize("T", [1, 3])
+@pytest.mark.parametrize("n", [4, 70])
+def test_ended_sequences(gpu, T, n):
+    """Slots of a run whose sequences have ended, the first ones among them: empty tables, and the others read on."""
+    lengths = [200 + i % 13 for i in range(n)]
+    for alive in (range(1, n), range(n // 2, n), [n - 1], []):
+        c = Case(12, [n, 3], [160, 64], lengths + [90, 91, 92], 16, 1, 2, T)
+        for i in range(n):
+            if i not in alive:
+                c.table[i] = [-1] * len(c.table[i])
+                c.lengths[i] = 0
+        c.unread()
+        c.check(c.call(gpu))
+
+
 @pytest.mark.parametrize("T", [1, 40])
 def test_missing_pages(gpu, T):
     """Entries that name no page, in the prefix and behind it, at the ends and all of them."""
