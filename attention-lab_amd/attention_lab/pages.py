@@ -44,7 +44,8 @@ class PagedCache:
     k, v bfloat16 [layers, num_pages, G, page_size, 128]; table int32 [slots, max_pages], the page of each slot's positions
     [e page_size, (e + 1) page_size) in its entry e, or -1; lengths int32 [slots]; refs int32 [num_pages], how many entries name
     each page (0: free). All are contiguous tensors on one HIP device, used in place. The operators keep refs in step with the
-    table; a table made elsewhere has to come with its counts and hold -1 past its sequences' pages. missing (int32 [1], optional)
+    table; a table made elsewhere has to come with its counts and hold -1 past its sequences' pages. A page whose count is raised by hand
+    stays in use and is never written in place (a compaction may move it). missing (int32 [1], optional)
     counts the pages that page_reserve could not give."""
 
     __slots__ = ("k", "v", "table", "lengths", "refs", "missing", "layers", "num_pages", "groups", "page_size", "slots",

@@ -474,7 +474,7 @@ extern "C" int attnlab_page_reserve(uint16_t* k, uint16_t* v, int layers, int nu
                        book_of(table, lengths, refs, S, max_pages, num_pages, page_size), tokens, each, missing, moves, src,
                        src + S, src + 2 * S);
     rc = check_launch("page_reserve");
-    if (rc || S == 1 || page_size == 1) return rc;   // one slot shares with nobody, and one row ends inside no page
+    if (rc || page_size == 1) return rc;   // a length ends inside no page of one row
     const CopyArgs c{{k, v}, (int64_t)num_pages * G * page_size * kDim, layers, G, page_size, num_pages, moves, src, src + S,
                      src + 2 * S, nullptr, 0, nullptr};
     return launch_copy(c, S, s, "page_reserve (copies)");

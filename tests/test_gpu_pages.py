@@ -169,6 +169,25 @@ def test_foreign_tables(gpu):
     assert cache.table.tolist() == model.table and cache.refs.tolist() == model.refs
 
 
+def test_pinned_page(gpu):
+    """A count raised by hand keeps a page from being written in place, in a cache of one slot too, and from being given out."""
+    cache, model = fresh(gpu, 6, 2, 1, 2, 8, 16, 4)
+    write(cache, model, gpu, 1, [21])
+    kept = cache.k[:, 1].clone()
+    cache.refs[1] += 1
+    rows = torch.randn(2, 1, 2, 4, 128, generator=gen(7)).to(torch.bfloat16).to(gpu)
+    page_reserve(cache, 4)
+    for layer in range(2):
+        page_append(cache, layer, rows[layer], rows[layer])
+    assert cache.table[0, :2].tolist() == [0, 2] and cache.refs.tolist() == [1, 1, 1, 0, 0, 0, 0, 0]
+    assert torch.equal(cache.k[:, 1], kept) and torch.equal(cache.k[:, 2, :, :5], kept[:, :, :5])
+    assert torch.equal(cache.k[:, 2, :, 5:9], rows[:, 0])
+    page_truncate(cache)
+    assert cache.refs.tolist() == [0, 1, 0, 0, 0, 0, 0, 0]
+    page_compact(cache)
+    assert cache.refs.tolist() == [1, 0, 0, 0, 0, 0, 0, 0] and torch.equal(cache.k[:, 0], kept)
+
+
 def test_step_in_a_graph(gpu):
     """Fork, reserve, append, truncate and compact captured once and replayed with other parents, tokens and rows, with eager
     work between: every replay equals the model."""
