@@ -821,11 +821,11 @@ class LabRunner:
             raise ValueError(f"need at least two tokens to score one, got {T}")
         parts = []
         for a, b in _chunks(T, chunk):
-            logits = self.forward(input_ids[:, a:b], phase="prefill", logits_to_keep=0)
             given = input_ids[:, a + 1:b + 1]
             if given.shape[1] < b - a:   # the last token has none behind it: padding
                 given = torch.nn.functional.pad(given, (0, 1), value=-1)
-            parts.append(token_logprobs(logits, given, top=top, entropy=entropy))
+            parts.append(token_logprobs(self.forward(input_ids[:, a:b], phase="prefill", logits_to_keep=0), given, top=top,
+                                        entropy=entropy))
         return TokenLogprobs(*(None if field[0] is None else torch.cat(field, dim=1)[:, :T - 1] for field in zip(*parts)))
 
     def step(self, token_ids: torch.Tensor) -> torch.Tensor:
