@@ -44,9 +44,9 @@ class PagedCache:
     k, v bfloat16 [layers, num_pages, G, page_size, 128]; table int32 [slots, max_pages], the page of each slot's positions
     [e page_size, (e + 1) page_size) in its entry e, or -1; lengths int32 [slots]; refs int32 [num_pages], how many entries name
     each page (0: free). All are contiguous tensors on one HIP device, used in place. The operators keep refs in step with the
-    table; a table made elsewhere has to come with its counts and hold -1 past its sequences' pages. A page whose count is raised by hand
-    stays in use and is never written in place (a compaction may move it). missing (int32 [1], optional)
-    counts the pages that page_reserve could not give."""
+    table; a table made elsewhere has to come with its counts and hold -1 past its sequences' pages. A page whose count is raised
+    by hand stays in use and is never written in place (a compaction may move it). missing (int32 [1], optional) counts the
+    pages that page_reserve could not give."""
 
     __slots__ = ("k", "v", "table", "lengths", "refs", "missing", "layers", "num_pages", "groups", "page_size", "slots",
                  "max_pages", "layer_bytes", "device")
@@ -64,7 +64,7 @@ class PagedCache:
             raise ValueError(f"table must be [slots, max_pages] with 1 to {MAX_SLOTS} slots and at least one page, got "
                              f"{tuple(table.shape)}")
         S, W = table.shape
-        _check_geometry(pages, G, page, W)
+        _check_geometry(pages, G, page, S, W)
         self.table = _check_book(table, "table", (S, W), device)
         self.lengths = _check_book(lengths, "lengths", (S,), device)
         self.refs = _check_book(refs, "refs", (pages,), device)
@@ -84,7 +84,7 @@ class PagedCache:
                                                                                    max_pages))
         if min(layers, slots, groups, num_pages, page_size, max_pages) < 1 or slots > MAX_SLOTS:
             raise ValueError(f"layers, slots (at most {MAX_SLOTS}), groups, num_pages, page_size and max_pages must be positive")
-        _check_geometry(num_pages, groups, page_size, max_pages)
+        _check_geometry(num_pages, groups, page_size, slots, max_pages)
         k, v = (torch.empty(layers, num_pages, groups, page_size, HEAD_DIM, dtype=torch.bfloat16, device=device) for _ in "kv")
         table = torch.full((slots, max_pages), -1, dtype=torch.int32, device=device)
         lengths, refs, missing = (torch.zeros(n, dtype=torch.int32, device=device) for n in (slots, num_pages, 1))
@@ -94,12 +94,12 @@ class PagedCache:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.table, self.lengths, self.refs))
 
 
-def _check_geometry(pages: int, G: int, page: int, W: int) -> None:
+def _check_geometry(pages: int, G: int, page: int, S: int, W: int) -> None:
     if page & (page - 1) or page > MAX_PAGE:
         raise ValueError(f"page_size must be a power of two up to {MAX_PAGE}, got {page}")
-    if W * page > INT_MAX or pages * G * page > INT_MAX:
-        raise ValueError(f"max_pages * page_size and num_pages * G * page_size must be below 2^31, got {W} * {page} and "
-                         f"{pages} * {G} * {page}")
+    if W * page > INT_MAX or pages * G * page > INT_MAX or S * W > INT_MAX:
+        raise ValueError(f"max_pages * page_size, num_pages * G * page_size and slots * max_pages must be below 2^31, got "
+                         f"{W} * {page}, {pages} * {G} * {page} and {S} * {W}")
 
 
 def _per_slot(cache: PagedCache, x, name: str):
@@ -120,7 +120,7 @@ def _scratch(cache: PagedCache):
 
 def page_fork(cache: PagedCache, parents) -> None:
     """Slot i goes on from what slot parents[i] held before the call (int32 [slots], on the device): it shares its pages and
-    has its length. A parent outside [0, slots) leaves the slot empty. Pages that nobody holds any more are free; no K/V row
+    has its length. parents is a tensor of its own, not one of the cache's. A parent outside [0, slots) leaves the slot empty. Pages that nobody holds any more are free; no K/V row
     is copied before page_reserve."""
     parents = _check_book(parents, "parents", (cache.slots,), cache.device)
     nat.call_on(cache.device, "attnlab_page_fork", cache.table.data_ptr(), cache.lengths.data_ptr(), cache.refs.data_ptr(),

@@ -400,6 +400,7 @@ int check_book(const int32_t* table, const int32_t* lengths, const int32_t* refs
     ATTNLAB_REQUIRE(page >= 1 && page <= (1 << 16) && (page & (page - 1)) == 0,
                     "page_size=%d must be a power of two in [1, 65536]", page);
     ATTNLAB_REQUIRE((int64_t)W * page <= INT32_MAX, "max_pages * page_size exceeds 2^31 positions");
+    ATTNLAB_REQUIRE((int64_t)S * W <= INT32_MAX, "a table of %d slots x %d pages exceeds 2^31 entries", S, W);   // requests are counted
     ATTNLAB_REQUIRE(table && lengths && refs, "table, lengths and refs must be device pointers");
     return ATTNLAB_OK;
 }
@@ -441,7 +442,13 @@ extern "C" int attnlab_page_fork(int32_t* table, int32_t* lengths, int32_t* refs
                                  int num_pages, void* stream) {
     const int rc = check_book(table, lengths, refs, S, max_pages, num_pages, 1);
     if (rc) return rc;
+    auto within = [&](const int32_t* of, int64_t n) {   // read by workgroups that others' writes would overtake
+        const uintptr_t p = reinterpret_cast<uintptr_t>(parents), o = reinterpret_cast<uintptr_t>(of);
+        return p < o + 4 * (uintptr_t)n && o < p + 4 * (uintptr_t)S;
+    };
     ATTNLAB_REQUIRE(parents, "parents must be a device pointer");
+    ATTNLAB_REQUIRE(!within(lengths, S) && !within(refs, num_pages) && !within(table, (int64_t)S * max_pages),
+                    "parents must not lie in the cache's own tensors");
     const int groups = (max_pages + kColumns - 1) / kColumns + 1;
     hipLaunchKernelGGL(page_fork, dim3((unsigned)groups), dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
                        book_of(table, lengths, refs, S, max_pages, num_pages, 1), parents);

@@ -387,7 +387,8 @@ int attnlab_range_prefill(const uint16_t* q, const void* K, const void* V, const
 /*
  * A K/V cache in pages that sequences share (no reference counterpart: its caches are branched by copying them,
  * qwen_wrap.py:117-133; the pools are those of attnlab_attend_paged). k, v: [layers, num_pages, G, page_size, 128] bf16,
- * 16-byte aligned; page_size a power of two up to 65536; num_pages * G * page_size and max_pages * page_size below 2^31.
+ * 16-byte aligned; page_size a power of two up to 65536; num_pages * G * page_size, max_pages * page_size and
+ * S * max_pages below 2^31.
  *   table    int32 [S, max_pages], entry e of slot i the page of its positions [e page_size, (e + 1) page_size), or -1; 1 <= S <=
  *            1024; -1 past a sequence's pages
  *   lengths  int32 [S]
@@ -395,7 +396,7 @@ int attnlab_range_prefill(const uint16_t* q, const void* K, const void* V, const
  * All are device memory changed in place. The results depend on the cache alone. Calls on one cache must be ordered on one
  * stream. An entry outside [0, num_pages) is not followed.
  *
- * attnlab_page_fork: slot i goes on from slot parents[i] (int32 [S]) as it was before the call: its entries and length; a
+ * attnlab_page_fork: slot i goes on from slot parents[i] (int32 [S], none of the cache's own memory) as it was before the call: its entries and length; a
  * parent outside [0, S) leaves the slot empty.
  *
  * attnlab_page_truncate: lengths[i] = min(lengths[i], max(to[i], 0)), with `to` null `length`; the entries from

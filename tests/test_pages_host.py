@@ -54,7 +54,8 @@ def test_exported():
         assert name in attention_lab.__all__ and hasattr(attention_lab, name)
 
 
-FORK = dict(table=16, lengths=16, refs=16, parents=16, S=2, W=4, pages=8, stream=None)
+FORK = dict(table=16, lengths=16, refs=16, parents=1024, S=2, W=4, pages=8, stream=None)
+ALIKE = dict(FORK, lengths=4096, refs=8192, parents=12288)   # table [16, 48), lengths [4096, 4104), refs [8192, 8224)
 TRUNCATE = dict(table=16, lengths=16, refs=16, to=None, length=3, S=2, W=4, pages=8, page=16, stream=None)
 RESERVE = dict(k=16, v=16, layers=2, pages=8, G=2, page=16, table=16, lengths=16, refs=16, tokens=None, each=1, S=2, W=4,
                missing=None, scratch=16, scratch_bytes=4096, stream=None)
@@ -66,7 +67,7 @@ EVERY = (("attnlab_page_fork", FORK), ("attnlab_page_truncate", TRUNCATE), ("att
          ("attnlab_page_append", APPEND), ("attnlab_page_compact", COMPACT))
 REFUSED = [(e, a, c, m) for e, a in EVERY for c, m in (
     (dict(S=0), "slots"), (dict(S=1025), "slots"), (dict(W=0), "positive"), (dict(pages=0), "positive"),
-    (dict(table=None), "pointers"), (dict(lengths=None), "pointers"))]
+    (dict(table=None), "pointers"), (dict(lengths=None), "pointers"), (dict(S=1024, W=1 << 21), "2\\^31 entries"))]
 REFUSED += [(e, a, c, m) for e, a in EVERY[1:] for c, m in (
     (dict(page=48), "power of two"), (dict(page=0), "power of two"), (dict(page=1 << 17), "power of two"),
     (dict(W=1 << 27), "2\\^31"))]
@@ -74,6 +75,7 @@ REFUSED += [(e, a, c, m) for e, a in EVERY[2:] for c, m in (
     (dict(G=0), "positive"), (dict(pages=1 << 26), "2\\^31"), (dict(k=None), "pointers"), (dict(v=24), "pointers"))]
 REFUSED += [
     ("attnlab_page_fork", FORK, dict(parents=None), "parents"), ("attnlab_page_fork", FORK, dict(refs=None), "pointers"),
+    *(("attnlab_page_fork", ALIKE, dict(parents=p), "own tensors") for p in (12, 44, 4096, 4092, 4100, 8188, 8220)),
     ("attnlab_page_truncate", TRUNCATE, dict(length=-1), "negative"),
     ("attnlab_page_reserve", RESERVE, dict(each=-1), "negative"), ("attnlab_page_reserve", RESERVE, dict(layers=0), "positive"),
     ("attnlab_page_reserve", RESERVE, dict(scratch=None), "scratch"), ("attnlab_page_reserve", RESERVE, dict(scratch=8), "scratch"),
@@ -99,6 +101,20 @@ def test_scratch(native_lib):
     size = native_lib.attnlab_page_scratch_bytes
     assert size(3, 100) == 16 + 12 * 100 and size(1024, 5) == 16 + 12 * 1024
     assert size(0, 5) == size(5, 0) == -1
+
+
+def test_python_makes_the_scratch(native_lib, monkeypatch):
+    """The Python side's scratch is what the C side asks for."""
+    seen = []
+    monkeypatch.setattr(_native, "call_on", lambda device, entry, *args: seen.append((entry, args)))
+    monkeypatch.setattr(_native, "stream_of", lambda device: None)
+    for sizes in (dict(), dict(pages=1, S=5), dict(pages=33, S=1)):
+        c = PagedCache(**parts(**sizes))
+        attention_lab.page_reserve(c)
+        attention_lab.page_compact(c)
+        need = native_lib.attnlab_page_scratch_bytes(c.slots, c.num_pages)
+        assert [args[len(_native.SIGNATURES[entry][1]) - 2] for entry, args in seen] == [need, need]
+        seen.clear()
 
 
 class OnDevice(torch.Tensor):
@@ -131,7 +147,7 @@ def test_cache_refuses(change, match):
 
 @pytest.mark.parametrize("sizes,match", [((0, 1, 1, 1, 1, 1), "positive"), ((1, 1025, 1, 1, 1, 1), "positive"),
                                          ((1, 1, 1, 1, 24, 1), "power of two"), ((1, 1, 1, 1, 16, 1 << 28), "2\\^31"),
-                                         ((1, 1, 8, 1 << 24, 16, 1), "2\\^31")])
+                                         ((1, 1, 8, 1 << 24, 16, 1), "2\\^31"), ((1, 1024, 1, 1, 1, 1 << 21), "2\\^31")])
 def test_empty_refuses(sizes, match):
     with pytest.raises(ValueError, match=match):
         PagedCache.empty(*sizes, device="cpu")

@@ -51,6 +51,20 @@ class OnDevice(torch.Tensor):
     is_cuda = True
 
 
+def test_python_makes_the_part_buffer(native_lib, monkeypatch):
+    """The Python side's part buffer is what the C side asks for."""
+    seen = []
+    monkeypatch.setattr(_native, "call_on", lambda device, entry, *args: seen.append(args))
+    monkeypatch.setattr(_native, "stream_of", lambda device: None)
+    pool = torch.zeros(8, 2, 16, 128, dtype=torch.bfloat16).as_subclass(OnDevice)
+    for B, h, T, prefix, partitions in ((3, 4, 1, 32, None), (3, 4, 5, 32, None), (1, 1, 1, 0, None), (5, 7, 1, 16, (64, 64)),
+                                        (1, 1, 3, 16, (0, 2)), (2, 3, 1, 16, (0, 1))):
+        q = torch.zeros(B, 2, h, T, 128, dtype=torch.bfloat16).as_subclass(OnDevice)
+        shared_prefix_attention(q, pool, pool, torch.zeros(B, 4, dtype=torch.int32), 60, prefix, partitions=partitions)
+        args = dict(zip(ARGS, seen.pop()))
+        assert args["part_bytes"] == native_lib.attnlab_shared_part_bytes(B, 2, h, T, args["ns"], args["no"])
+
+
 def test_python_refuses():
     pool = torch.zeros(8, 2, 16, 128, dtype=torch.bfloat16).as_subclass(OnDevice)
     q = torch.zeros(3, 2, 4, 1, 128, dtype=torch.bfloat16)
