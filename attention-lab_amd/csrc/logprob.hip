@@ -3,18 +3,20 @@
 //   top: the k largest x, equal ones by the lower token (NaN last, -0 equal to +0), as logprobs
 //
 // A row is cut into up to 64 segments, a workgroup each. A thread holds up to 64 logits in registers, as they came, so each is read
-// once: l and s = sum p (x - m) relative to a common m of the wave's merge over the workgroup and leave as a partial (m, l, s). A second
-// launch merges a row's partials, or, where there are few rows, the last of its workgroups to arrive. Sums are fp32 in the log2 domain.
+// once: the waves sum l and s = sum p (x - m) relative to an m of their own, and a segment's leave as a partial (m, l, s, largest). The
+// last of a row's workgroups to arrive merges its partials, where there are few rows; else a second launch does. Sums are fp32 in the
+// log2 domain.
 //
 // The top k without a second look at every logit: the k-th largest of a wave's 64 thread maxima is a lower bound of the k-th
-// largest logit, found by a search over the order-preserving key's bits with one ballot a bit; the largest of the four waves'
-// bounds is the workgroup's. The few 16-byte words that reach it (k and some more, in any distribution that does not crowd its
+// largest logit, found by a search over the order-preserving key's bits with one ballot a bit; so are the largest of the four waves'
+// bounds, and, nearer where the waves' logits are alike, the least of the waves' k / 4-th largest. The few 16-byte words that reach it (k and some more, in any distribution that does not crowd its
 // largest logits into a few threads) go to LDS, and one wave looks them over again and ranks what it finds by counting.
-// More words than that holds: k rounds of a maximum over the workgroup, with the same result. The second launch does the same to
-// the segments' lists.
+// More words than that holds: k rounds of a maximum over the workgroup, with the same result. The merge does the same to the
+// segments' lists.
 //
-// What bounds it: the bytes for float32; for 16-bit logits as much the vector units (9 operations for two bytes, of them an
-// exponential at a quarter of the rate).
+// What bounds it, vocabulary of 151936. 4096 bf16 rows, top 5: 207 to 222 us, 1.24 GB at 5.6 to 6.0 TB/s (reads alone go at 7.1); beside
+// the bytes it is the vector units (9 operations for two bytes, of them an exponential at a quarter of the rate). 64 float32 rows, top
+// 20: 16 us, of which the 39 MB take 6 (all workgroups at once), the bounds 1, the lists 2.5, arrivals 1 and the merge 2.5: latencies.
 #include <cfloat>
 
 #include "select.h"
@@ -27,6 +29,9 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;
 constexpr int kMaxSegments = 64;
 constexpr int kWords = 256;              // words of a segment that are looked over again
+// Up to kFew, the k / 4-th largest of the waves are not asked for: few words reach the first bound anyway, and a second search costs
+// more than it saves (4096 rows, top 5: 207 and 217 us; 64 rows, top 20: 18.0 without it and 16.2 with).
+constexpr int kFew = 8;
 constexpr int kPartWords = 4;            // m, l, s and the largest logit (16 bytes)
 // x log2 e - m cancels what m's rounding left, up to where that is no longer small. A row whose largest logit is past kFar is
 // summed again by differences; a thread whose own is below -2 kFar weighs nothing in any other row (e^-65536 is 0).
@@ -57,21 +62,6 @@ __device__ __forceinline__ float logit_of(uint32_t key) {   // of score_key's; N
     return key == 0 ? __builtin_nanf("") : __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
-// The k-th largest of the wave's 64 keys (k <= 64): the largest t with k keys of at least t. The upper half of t by its bits,
-// then the least key from there on.
-__device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k) {
-    uint32_t t = 0;
-#pragma unroll
-    for (int bit = 31; bit >= 16; --bit) {
-        const uint32_t with = t | 1u << bit;
-        if (__popcll(__ballot(key >= with)) >= k) t = with;
-    }
-    uint32_t least = key >= t ? key : 0xffffffffu;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
-    return least;
-}
-
 // Over the wave's lanes: a scan along each row of 16, then the rows' ends; the last lane's value, for all.
 template <int CTRL, int ROWS>
 __device__ __forceinline__ float moved(float x, float none) {
@@ -95,6 +85,34 @@ __device__ __forceinline__ float wave_sum(float x) {
     x += moved<0x142, 0xa>(x, 0.0f);
     x += moved<0x143, 0xc>(x, 0.0f);
     return last_lane(x);
+}
+
+__device__ __forceinline__ uint32_t wave_min(uint32_t x) {
+    auto with = [&](float y) { x = min(x, (uint32_t)__float_as_int(y)); };
+    auto own = [&]() { return __uint_as_float(x); };
+    with(moved<0x111, 0xf>(own(), own()));
+    with(moved<0x112, 0xf>(own(), own()));
+    with(moved<0x114, 0xf>(own(), own()));
+    with(moved<0x118, 0xf>(own(), own()));
+    with(moved<0x142, 0xa>(own(), own()));
+    with(moved<0x143, 0xc>(own(), own()));
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+// This lane's place among those of `hit`.
+__device__ __forceinline__ uint32_t before_me(uint64_t hit) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
+}
+
+// The k-th largest of the wave's 64 keys (k <= 64): the largest t with k keys of at least t. The upper half of t by its bits,
+// then the least key from there on.
+__device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t with = t | 1u << bit;
+        if (__popcll(__ballot(key >= with)) >= k) t = with;
+    }
+    return wave_min(key >= t ? key : 0xffffffffu);
 }
 
 // (m, l, s) against a common maximum mt; m = -inf: nothing but, where they were NaN, its l and s.
@@ -127,13 +145,24 @@ __device__ __forceinline__ void only_logits(u32x4_t& w, int t, int V) {
     }
 }
 
-// `count` keys in `sh` ranked by counting the larger ones; the first `top` of them to `take(rank, key)`.
-template <int THREADS, typename Take>
-__device__ __forceinline__ void rank_keys(const uint64_t* sh, int count, int top, Take take) {
-    for (int i = threadIdx.x & (THREADS - 1); i < count; i += THREADS) {
+// `count` keys in `sh` ranked by counting the larger ones; the first `top` of them to `take(rank, key)`. Eight at a time: zeros, which
+// are larger than none, fill the last ones up (`sync`: they are there for all).
+constexpr int kAtOnce = 8;
+template <int THREADS, typename Sync, typename Take>
+__device__ __forceinline__ void rank_keys(uint64_t* sh, int count, int top, Sync sync, Take take) {
+    const int tid = threadIdx.x & (THREADS - 1), padded = (count + kAtOnce - 1) / kAtOnce * kAtOnce;
+    if (count + tid < padded) sh[count + tid] = 0;
+    sync();
+    for (int i = tid; i < count; i += THREADS) {
         const uint64_t own = sh[i];
         int rank = 0;
-        for (int j = 0; j < count; ++j) rank += sh[j] > own;
+        for (int j = 0; j < padded; j += kAtOnce) {
+            ulonglong2 k[kAtOnce / 2];
+#pragma unroll
+            for (int u = 0; u < kAtOnce / 2; ++u) k[u] = *reinterpret_cast<const ulonglong2*>(sh + j + 2 * u);
+#pragma unroll
+            for (int u = 0; u < kAtOnce / 2; ++u) rank += (k[u].x > own) + (k[u].y > own);
+        }
         if (rank < top) take(rank, own);
     }
 }
@@ -159,6 +188,9 @@ __device__ __forceinline__ void merge_row(const LogprobArgs& a, int64_t row, uin
     const float* part = a.part + row * a.segments * kPartWords;
     const int most = a.segments * a.top;
     const uint64_t* best = a.best + row * most;
+    int64_t token = -1;                      // on its way first, and its logit behind the partials
+    if (tid == 0 && a.logprob)
+        token = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[row] : static_cast<const int32_t*>(a.tokens)[row];
     float4 p = make_float4(-INFINITY, 0.0f, 0.0f, -INFINITY);
     if (lane < a.segments) {
         if constexpr (COHERENT) {
@@ -177,16 +209,16 @@ __device__ __forceinline__ void merge_row(const LogprobArgs& a, int64_t row, uin
             const uint64_t* q = best + THREADS * i + tid;
             k[i] = COHERENT ? __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM) : *q;
         }
-        mine = max(mine, (uint32_t)(k[i] >> 32));
     }
-    const float m = wave_max(p.x), largest = wave_max(p.w);
-    rescale(p.x, m, p.y, p.z);
-    float l = wave_sum(p.y), s = wave_sum(p.z);
     auto at = [&](int64_t t) -> float {
         if constexpr (DT == ATTNLAB_DT_F32) return static_cast<const float*>(a.x)[row * a.stride + t];
         const uint16_t w = static_cast<const uint16_t*>(a.x)[row * a.stride + t];
         return DT == ATTNLAB_DT_BF16 ? bf16_to_f32(w) : f16_to_f32(w);
     };
+    const float given = token >= 0 && token < a.V ? at(token) : __builtin_nanf("");
+    const float m = wave_max(p.x), largest = wave_max(p.w);
+    rescale(p.x, m, p.y, p.z);
+    float l = wave_sum(p.y), s = wave_sum(p.z);
     // a row whose largest logit is far from 0 (one that a mask of the type's lowest value has covered whole)
     const bool far = fabsf(largest) >= kFar && fabsf(largest) < INFINITY;
     if (far) {
@@ -219,13 +251,12 @@ __device__ __forceinline__ void merge_row(const LogprobArgs& a, int64_t row, uin
     auto logprob = [&](float x) { return (x - largest) - lnl; };
     if (tid == 0) {
         if (a.entropy) a.entropy[row] = (log2l - s / l) * kLn2;
-        if (a.logprob) {
-            const int64_t t = a.tokens64 ? static_cast<const int64_t*>(a.tokens)[row] : static_cast<const int32_t*>(a.tokens)[row];
-            a.logprob[row] = t < 0 ? 0.0f : t < a.V ? logprob(at(t)) : __builtin_nanf("");
-        }
+        if (a.logprob) a.logprob[row] = token < 0 ? 0.0f : logprob(given);   // NaN past the last token
         sh.count = 0;
     }
     if (!a.top) return;
+#pragma unroll
+    for (int i = 0; i < kHold; ++i) mine = max(mine, (uint32_t)(k[i] >> 32));
     uint32_t bound = wave_kth(mine, a.top);
     if constexpr (THREADS > 64) {
         if (lane == 0) sh.bound[wave] = bound;
@@ -235,11 +266,26 @@ __device__ __forceinline__ void merge_row(const LogprobArgs& a, int64_t row, uin
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) bound = max(bound, sh.bound[w]);
     }
+    uint32_t count = 0;
 #pragma unroll
-    for (int i = 0; i < kHold; ++i)
-        if (k[i] && (uint32_t)(k[i] >> 32) >= bound) cand[atomicAdd(&sh.count, 1u)] = k[i];
-    sync();
-    rank_keys<THREADS>(cand, (int)sh.count, a.top, [&](int i, uint64_t y) {
+    for (int i = 0; i < kHold; ++i) {
+        const bool in = k[i] && (uint32_t)(k[i] >> 32) >= bound;
+        const uint64_t hit = __ballot(in);
+        if (!hit) continue;
+        uint32_t first = count;
+        if constexpr (THREADS == 64) {
+            count += (uint32_t)__popcll(hit);
+        } else {
+            if (lane == 0) first = atomicAdd(&sh.count, (uint32_t)__popcll(hit));
+            first = (uint32_t)__builtin_amdgcn_readfirstlane((int)first);
+        }
+        if (in) cand[first + before_me(hit)] = k[i];
+    }
+    if constexpr (THREADS > 64) {
+        __syncthreads();
+        count = sh.count;
+    }
+    rank_keys<THREADS>(cand, (int)count, a.top, sync, [&](int i, uint64_t y) {
         a.top_logprob[row * a.top + i] = logprob(logit_of((uint32_t)(y >> 32)));
         a.top_token[row * a.top + i] = (int64_t)(uint32_t)~(uint32_t)y;
     });
@@ -248,12 +294,12 @@ __device__ __forceinline__ void merge_row(const LogprobArgs& a, int64_t row, uin
 template <int DT, int U, bool MERGE>
 __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     constexpr int kPer = DT == ATTNLAB_DT_F32 ? 4 : 8, kBytes = 16 / kPer;
-    __shared__ uint64_t cand_sh[kWords * kPer];
+    __shared__ __attribute__((aligned(16))) uint64_t cand_sh[kWords * kPer];
     __shared__ uint16_t word_sh[kWords];
     __shared__ u32x4_t data_sh[kWords];
     __shared__ float part_sh[kWaves][4];
-    __shared__ uint32_t bound_sh[kWaves];
-    __shared__ uint32_t words_sh, count_sh, last_sh;
+    __shared__ uint2 bound_sh[kWaves];
+    __shared__ uint32_t words_sh, last_sh;
     __shared__ MergeShared merge_sh;
     const int seg = blockIdx.x % a.segments;
     const int64_t row = blockIdx.x / a.segments;
@@ -274,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
         x[u] = u32x4_t{kNone, kNone, kNone, kNone};
         if (w < end) x[u] = __builtin_nontemporal_load(words + w);
     }
-    if (tid == 0) words_sh = count_sh = 0;
+    if (tid == 0) words_sh = 0;
     // the row's first and last word can hold what is not the row's; `whole`: every element of this thread is a logit
     bool whole = first + kThreads * (U - 1) + tid < end;
     if (seg == 0 || seg == a.segments - 1) {
@@ -343,10 +389,10 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
         part_sh[wave][3] = largest;
     }
     // a thread with nothing above -inf among elements that are no logits: no bound
-    uint32_t bound = 0;
     if (a.top) {
-        bound = wave_kth(!whole && !(top > -INFINITY) ? 0u : score_key(top), a.top);
-        if (lane == 0) bound_sh[wave] = bound;
+        const uint32_t key = !whole && !(top > -INFINITY) ? 0u : score_key(top);
+        const uint32_t all = wave_kth(key, a.top), part = a.top > kFew ? wave_kth(key, (a.top + kWaves - 1) / kWaves) : 0u;
+        if (lane == 0) bound_sh[wave] = make_uint2(all, part);
     }
     __syncthreads();
     if (tid == kThreads - 1) {
@@ -374,8 +420,12 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
         }
     }
     if (a.top) {
+        // k of one wave's logits reach its k-th largest maximum, and k / 4 of each wave's the least of the k / 4-th largest
+        uint32_t bound = bound_sh[0].y;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) bound = max(bound, bound_sh[w]);
+        for (int w = 1; w < kWaves; ++w) bound = min(bound, bound_sh[w].y);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) bound = max(bound, bound_sh[w].x);
         const float least = logit_of(bound);   // NaN: every word
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -397,19 +447,22 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
         };
         if (listed <= kWords) {
             if (wave == 0) {
-                for (uint32_t i = lane; i < listed; i += 64) {
-                    const int t = kPer * (first + word_sh[i]) - head;
+                int count = 0;
+                for (uint32_t i0 = 0; i0 < listed; i0 += 64) {
+                    const uint32_t i = min(i0 + lane, listed - 1);
+                    const int t = i0 + lane < listed ? kPer * (first + word_sh[i]) - head : a.V;   // past the last: no logits
                     const u32x4_t v = data_sh[i];
 #pragma unroll
                     for (int j = 0; j < kPer; ++j) {
                         const uint32_t k = score_key(element<DT>(v, j));
-                        if (k >= bound && t + j >= 0 && t + j < a.V)
-                            cand_sh[atomicAdd(&count_sh, 1u)] = (uint64_t)k << 32 | (uint32_t)~(t + j);
+                        const bool in = k >= bound && t + j >= 0 && t + j < a.V;
+                        const uint64_t found = __ballot(in);
+                        if (in) cand_sh[count + before_me(found)] = (uint64_t)k << 32 | (uint32_t)~(t + j);
+                        count += __popcll(found);
                     }
                 }
-                asm volatile("" ::: "memory");   // a wave's LDS operations take effect in order
-                const int count = (int)count_sh;
-                rank_keys<64>(cand_sh, count, a.top, take);
+                // a wave's LDS operations take effect in order
+                rank_keys<64>(cand_sh, count, a.top, [] { asm volatile("" ::: "memory"); }, take);
                 for (int r = count + lane; r < a.top; r += 64) take(r, 0);
             }
         } else {
@@ -459,7 +512,7 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
 template <int DT, int THREADS>
 __global__ __launch_bounds__(kThreads) void logprob_merge(LogprobArgs a, int64_t N) {
     constexpr int kRows = kThreads / THREADS;
-    __shared__ uint64_t cand_sh[kRows][THREADS == 64 ? kWaveKeys : kMaxSegments * kMaxTop];
+    __shared__ __attribute__((aligned(16))) uint64_t cand_sh[kRows][THREADS == 64 ? kWaveKeys : kMaxSegments * kMaxTop];
     __shared__ MergeShared sh[kRows];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = THREADS == 64 ? wave : 0;
     const int64_t row = (int64_t)blockIdx.x * kRows + r;
