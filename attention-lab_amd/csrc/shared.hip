@@ -287,8 +287,11 @@ struct Sixteen {
     size_t at;
     uint32_t rows;
     __device__ __forceinline__ Sixteen(const SharedArgs& a, int p, int g, int k16, int end) {
-        rows = (uint32_t)p < (uint32_t)a.pages ? (uint32_t)min(max(end - k16, 0), 16) : 0u;
-        at = (size_t)((((uint32_t)p * a.G + g) << a.shift) + (k16 & ((1 << a.shift) - 1))) * kDim;
+        // uniform, and in scalar registers: with a descriptor in vector ones every load is a loop over its values (16 questions on 16K:
+        // 503 us, and 459)
+        auto scalar = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+        rows = scalar((uint32_t)p < (uint32_t)a.pages ? (uint32_t)min(max(end - k16, 0), 16) : 0u);
+        at = (size_t)scalar((((uint32_t)p * a.G + g) << a.shift) + (k16 & ((1 << a.shift) - 1))) * kDim;
     }
     __device__ __forceinline__ uint32_t bytes() const { return rows * 2 * kDim; }
     __device__ __forceinline__ uint32_t have() const { return (1u << rows) - 1u; }
