@@ -120,8 +120,8 @@ def _scratch(cache: PagedCache):
 
 def page_fork(cache: PagedCache, parents) -> None:
     """Slot i goes on from what slot parents[i] held before the call (int32 [slots], on the device): it shares its pages and
-    has its length. parents is a tensor of its own, not one of the cache's. A parent outside [0, slots) leaves the slot empty. Pages that nobody holds any more are free; no K/V row
-    is copied before page_reserve."""
+    has its length. parents is a tensor of its own, not one of the cache's. A parent outside [0, slots) leaves the slot empty.
+    Pages that nobody holds any more are free; no K/V row is copied before page_reserve."""
     parents = _check_book(parents, "parents", (cache.slots,), cache.device)
     nat.call_on(cache.device, "attnlab_page_fork", cache.table.data_ptr(), cache.lengths.data_ptr(), cache.refs.data_ptr(),
                 parents.data_ptr(), cache.slots, cache.max_pages, cache.num_pages, nat.stream_of(cache.device))

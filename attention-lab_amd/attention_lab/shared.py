@@ -25,7 +25,8 @@ def shared_splits(G: int, rows: int, wide: bool, chunk: bool = False) -> int:
 
 
 def own_splits(BG: int, rows: int, keys: int) -> int:
-    """Key splits of the own part: `rows` rows of each of BG (sequence, group) pairs over up to `keys` positions."""
+    """Key splits of the own part: `rows` rows of each of BG (sequence, group) pairs over up to `keys` positions. 384 narrow workgroups;
+    with 192 and 768: 2 x 8 answers of 2K behind 2K 42 and 36 us for 33, 16 answers of 300 behind 8K 27 and 32 for 27."""
     wide = rows > MAX_H_CHUNK
     tiles = BG * -(-rows // (WIDE_ROWS if wide else NARROW_ROWS))
     return max(1, min(16, (512 if wide else 384) // tiles, keys // 256))
@@ -95,7 +96,9 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
     if T == 0:
         return out
     rows = B * h * T
-    wide = T > 1 or rows > NARROW_ROWS * R
+    # Tiles of 128 rows from half a narrow one on (us, wide and narrow: 16 runs of 16 rows on 4K 58 and 71, 32 of 8 rows 101 and 92; one
+    # run on 4K of 8 rows 19.0 and 18.3, of 16 rows 19.2 and 19.4, of 64 rows 22 and 26)
+    wide = T > 1 or 2 * rows > NARROW_ROWS * R
     if partitions is None:
         ns = shared_splits(G, rows, wide, T > 1) if keys else 0
         no = own_splits(B * G, h * T if T > 1 else 1, most if prefix_at else most - keys)

@@ -9,8 +9,9 @@
 //
 // The top k without a second look at every logit: the k-th largest of a wave's 64 thread maxima is a lower bound of the k-th
 // largest logit, found by a search over the order-preserving key's bits with one ballot a bit; so are the largest of the four waves'
-// bounds, and, nearer where the waves' logits are alike, the least of the waves' k / 4-th largest. The few 16-byte words that reach it (k and some more, in any distribution that does not crowd its
-// largest logits into a few threads) go to LDS, and one wave looks them over again and ranks what it finds by counting.
+// bounds, and, nearer where the waves' logits are alike, the least of the waves' k / 4-th largest. The few 16-byte words that reach the
+// bound (k and some more, in any distribution that does not crowd its largest logits into a few threads) go to LDS, and one wave
+// looks them over again and ranks what it finds by counting.
 // More words than that holds: k rounds of a maximum over the workgroup, with the same result. The merge does the same to the
 // segments' lists.
 //

@@ -21,6 +21,11 @@
 //
 // One launch does both parts, the own part's workgroups behind the shared part's.
 //
+// What bounds it (8 groups). 16 questions of 211 tokens, h=2, on 16K: 459 to 485 us with the merge's 16, 1.0 PFLOP/s in the shared part;
+// matrix instructions run half of the time and vector ones the other. 4 x 13 answers, h=8, on 9K, up to 1K of their own: 66 us, 4.6 TB/s:
+// one block's copies in flight a workgroup (54 where K and V are in the caches). 16 answers, h=4, on 8K: 22 us, and 4 answers on 512:
+// 15 (the host; 12 on the GPU), chains of latencies: the share 2.3, the first copies 2.7, four blocks 5.8, partials 1, the merge 5.
+//
 // Weights are rounded to bf16, the operand's type, before their product with V; their sum is of the unrounded ones, sums fp32.
 #include <cfloat>
 #include <type_traits>
@@ -137,7 +142,10 @@ struct Item {
     bool shared;
 };
 
-constexpr int kLeastBlocks = 4, kLeastTiles = 8;   // a share is of 256 keys at least
+constexpr int kLeastBlocks = 4, kLeastTiles = 8;   // a share is of 256 keys at least (16 answers on 8K: 28.5 us, with 128 keys 35.8)
+// More tiles than workgroups: tiles of fewer blocks go whole, in as many rounds as it takes, longer ones are shared out evenly. Even
+// and whole, questions of 211 tokens: 20 on 2K 125 and 133 us, on 4K 198 and 224, on 16K 649 and 781; 36 on 2K 221 and 197, on 4K
+// 330 and 307, on 8K 551 and 548, on 16K 1014 and 1034.
 constexpr uint32_t kLongBlocks = 64;
 
 // The shared part's workgroup `turn` of XCD `xcd`: a group, a run, a share of its blocks of kBlock keys, and a tile of kRows of its
@@ -1023,7 +1031,8 @@ extern "C" int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k
     // the tables have room for
     const int64_t tiles = G * ((int64_t)B * T * h / (wide ? kWide : kNarrow) + (R < B ? R : B));
     const int64_t keys = (int64_t)max_pages * page_size, longest = prefix_lengths || prefix_length > keys ? keys : prefix_length;
-    const int64_t shares = (longest + (wide ? kKeys * kLeastBlocks : kTile * kLeastTiles) - 1) / (wide ? kKeys * kLeastBlocks : kTile * kLeastTiles);
+    const int least = wide ? kKeys * kLeastBlocks : kTile * kLeastTiles;
+    const int64_t shares = (longest + least - 1) / least;
     int64_t first = 0;
     if (shared_splits) {
         first = (tiles > workers ? tiles : workers) + tiles;
@@ -1040,6 +1049,8 @@ extern "C" int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k
     else if (wide && shared_splits) launch_read<true, false>(a, items, s);
     else launch_read<false, false>(a, items, s);
     if (need) {
+        // four half waves a row where it can have many partials (16 answers on 8K: 26.8 us, with one 29.0), else one (16 questions:
+        // 461 us, with four 478)
         const int slots = shared_splits + own_splits;
         const dim3 wg(256);
         if (slots > 8) hipLaunchKernelGGL(shared_combine<4>, dim3((unsigned)((rows + 1) / 2)), wg, 0, s, a.part, a.counts, out,

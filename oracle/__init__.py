@@ -15,6 +15,7 @@ Modules (each function cites the reference file:line it restates; paths relative
   ref_path  the reference's torch op sequence on the CPU (matmul -> topk -> cat -> index_select -> SDPA), the timed
             CPU baseline
   weights   GroupedIndexer's seeded weights (indexer.py:38-45)
+  pages     the cache of shared pages as lists on the host (no reference code)
 
 How each function is pinned (no function here is "parity unpinned"):
   rules      the known answers of the reference's tests (test_attention_contracts.py:309-347, 237-239, 262;
@@ -31,4 +32,5 @@ How each function is pinned (no function here is "parity unpinned"):
              tests/test_oracle_pins.py
   weights    golden fixture written by tests/golden/make_golden.py from the reference's own GroupedIndexer -
              tests/test_golden.py
+  pages      known answers of small caches - tests/test_pages_host.py
 """
