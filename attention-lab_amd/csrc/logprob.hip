@@ -310,7 +310,8 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.x) + (uintptr_t)row * a.stride * kBytes;
     const int head = (int)(at & 15) / kBytes;
     const u32x4_t* words = reinterpret_cast<const u32x4_t*>(at & ~(uintptr_t)15);
-    const int first = seg * a.words, end = min(first + a.words, (head + a.V + kPer - 1) / kPer);
+    const int row_words = (head + a.V + kPer - 1) / kPer;   // the last segment can begin behind them
+    const int first = seg * a.words, end = min(first + a.words, row_words);
     // the wave's word u: 64 in line, a segment's end between waves (but for the row's end)
     auto there = [&](int u) { return first + kThreads * u + 64 * wave < end; };
     u32x4_t x[U];
@@ -324,7 +325,7 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     if (tid == 0) words_sh = 0;
     // the row's first and last word can hold what is not the row's; `whole`: every element of this thread is a logit
     bool whole = first + kThreads * (U - 1) + tid < end;
-    if (seg == 0 || seg == a.segments - 1) {
+    if (seg == 0 || first + a.words >= row_words) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int w = first + kThreads * u + tid, t = kPer * w - head;

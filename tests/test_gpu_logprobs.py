@@ -128,6 +128,19 @@ def test_past_the_row_is_not_read(gpu):
             check(x, torch.arange(4), 5, gpu=gpu, dev=dev)
 
 
+@pytest.mark.parametrize("dtype,N,V", [("bf16", 1, 6138), ("f16", 1, 6142), ("bf16", 64, 57342), ("f16", 64, 6140),
+                                       ("f32", 1, 14334), ("f32", 64, 28671)])
+def test_row_that_ends_before_the_last_segment(gpu, dtype, N, V):
+    """A row of which an aligned word that it only partly fills is the last one before the last segment, which is kept for rows that
+    begin inside a word: what is behind the row reaches no output."""
+    x = logits(V, N, V, dtype=dtype)
+    stride = (V + 31) // 16 * 16
+    for bad in (float("nan"), float("inf"), 60000.0):
+        dev = torch.full((N, stride), bad, dtype=x.dtype, device=gpu)[:, :V]
+        dev.copy_(x)
+        check(x, torch.arange(N), 5, gpu=gpu, dev=dev)
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("V", [500, 30011, 151936])
 def test_masked_and_special(gpu, dtype, V):
