@@ -15,9 +15,9 @@
 // More words than that holds: k rounds of a maximum over the workgroup, with the same result. The merge does the same to the
 // segments' lists.
 //
-// What bounds it, vocabulary of 151936. 4096 bf16 rows, top 5: 207 to 222 us, 1.24 GB at 5.6 to 6.0 TB/s (reads alone go at 7.1); beside
-// the bytes it is the vector units (9 operations for two bytes, of them an exponential at a quarter of the rate). 64 float32 rows, top
-// 20: 16 us, of which the 39 MB take 6 (all workgroups at once), the bounds 1, the lists 2.5, arrivals 1 and the merge 2.5: latencies.
+// What bounds it, vocabulary of 151936. 4096 bf16 rows, top 5: 204 to 219 us, 1.24 GB at 5.7 to 6.1 TB/s (reads alone go at 7.1); as much
+// as the bytes it is the vector units (12 operations a logit, half of them in the sums, an exponential among them). 64 float32 rows,
+// top 20: 16 us, of which the 39 MB take 6 (all workgroups at once), the bounds 1, the lists 2.5, arrivals 1 and the merge 2.5: latencies.
 #include <cfloat>
 
 #include "select.h"
@@ -315,21 +315,23 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     // the wave's word u: 64 in line, a segment's end between waves (but for the row's end)
     auto there = [&](int u) { return first + kThreads * u + 64 * wave < end; };
     u32x4_t x[U];
-    constexpr uint32_t kNone = DT == ATTNLAB_DT_F32 ? 0xff800000u : DT == ATTNLAB_DT_BF16 ? 0xff80ff80u : 0xfc00fc00u;   // -inf
+    {   // as a buffer that ends with the segment: zeros behind it
+        constexpr int kNt = 2;   // non-temporal
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<u32x4_t*>(words + first), 0, 16 * max(end - first, 0), 0x00020000);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int w = first + kThreads * u + tid;
-        x[u] = u32x4_t{kNone, kNone, kNone, kNone};
-        if (w < end) x[u] = __builtin_nontemporal_load(words + w);
+        for (int u = 0; u < U; ++u)
+            x[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * tid, 16 * kThreads * u, kNt));
     }
     if (tid == 0) words_sh = 0;
-    // the row's first and last word can hold what is not the row's; `whole`: every element of this thread is a logit
+    // -inf for what is not the row's, in its first and last word and behind it (the waves behind a segment's end between waves skip
+    // their words); `whole`: every element of this thread is a logit
     bool whole = first + kThreads * (U - 1) + tid < end;
     if (seg == 0 || first + a.words >= row_words) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int w = first + kThreads * u + tid, t = kPer * w - head;
-            if (w < end && (t < 0 || t + kPer > a.V)) {
+            const int t = kPer * (first + kThreads * u + tid) - head;
+            if (t < 0 || t + kPer > a.V) {
                 only_logits<DT>(x[u], t, a.V);
                 whole = false;
             }
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     // One pass: each word's maximum, and the sums relative to the largest of the wave's first words, near enough to the largest of
     // all, as soon as a word is there.
     float m = wave_max(word_max(x[0]));
-    bool near = m > -2.0f * kFar && m < INFINITY;
+    bool near = there(0) && m > -2.0f * kFar && m < INFINITY;
     m *= kLog2e;
     float most[U], l = 0.0f, s = 0.0f;
 #pragma unroll
