@@ -37,6 +37,7 @@ constexpr int kPartWords = 4;            // m, l, s and the largest logit (16 by
 // x log2 e - m cancels what m's rounding left, up to where that is no longer small. A row whose largest logit is past kFar is
 // summed again by differences; a thread whose own is below -2 kFar weighs nothing in any other row (e^-65536 is 0).
 constexpr float kFar = 65536.0f;
+constexpr float kNear = 16.0f;           // log2 of what a weight may be above 1: the entropy is off by some 2^-23 of it
 constexpr float kLn2 = 0.69314718055994531f;
 
 struct LogprobArgs {
@@ -365,9 +366,9 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
 #pragma unroll
     for (int u = 1; u < U; ++u) top = fmaxf(top, most[u]);
     const float largest = wave_max(top);
-    // Not near enough (a sum past the type's end), or some logit is -inf (a weight of zero, and no term), or none is a number: again, by
+    // Not near enough (the sum's logarithm and the entropy's quotient would cancel), or some logit is -inf (a weight of zero, and no term), or none is a number: again, by
     // the wave's own maximum
-    near = near && l < FLT_MAX && fabsf(s) < FLT_MAX;
+    near = near && fmaf(top, kLog2e, -m) <= kNear && l < FLT_MAX && fabsf(s) < FLT_MAX;
     if (!__all(near)) {
         m = largest > -2.0f * kFar ? largest * kLog2e : -INFINITY;
         const float nm = m == -INFINITY ? 0.0f : -m;

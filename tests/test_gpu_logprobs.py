@@ -168,6 +168,16 @@ def test_masked_and_special(gpu, dtype, V):
     check(x, tokens, 20, gpu=gpu)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("seed,N,V,scale", [(2269, 130, 4826, 1000.0), (4, 200, 30011, 20.0), (5, 90, 151936, 300.0)])
+def test_peaks_far_above_the_first_logits(gpu, dtype, seed, N, V, scale):
+    """Rows whose few likely logits lie up to 88 above a wave's first ones: entropies near 0 keep their absolute accuracy."""
+    check(logits(seed, N, V, dtype=dtype, scale=scale), torch.arange(N), 7, gpu=gpu)
+    x = logits(seed + 1, N, V, dtype=dtype)
+    x[torch.arange(N), 2048 + 21 * torch.arange(N)] += torch.arange(N).to(x.dtype) % 90
+    check(x, torch.arange(N), 3, gpu=gpu)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_ties(gpu, dtype):
     """Few different values: the order is by token where logits are equal, within a thread, a wave, a segment and across them."""
