@@ -347,15 +347,21 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
     const int kchunk = 16 * (slot ^ (4 * wave + srow)), vchunk = 16 * (slot ^ (4 * srow));
     const int32_t* pages = a.table + (size_t)w.tb * a.table_stride;
     auto first_key = [&](int i) { return w.base + kKeys * i; };
+    const int stop = min(w.end, first_key(w.i1));
     // the entries of block i's pages, as they stand in the table: lane u of four that of keys 16 u .., or lane j key j's
     auto look = [&](int i) {
         const int key = first_key(min(i, w.i1 - 1)) + (SMALL ? lane : 16 * (lane & 3));
         return pages[min(key, w.end - 1) >> a.shift];
     };
-    // block i's copies; which of its keys have a row, a bit each
-    auto copy = [&](int kb, int entry, char* kt, char* vt) -> uint64_t {
+    // block i's copies, and the entries of the next one's pages; which of the block's keys have a row, a bit each
+    // (the entries leave their register before the next ones are loaded into it: moved there later, they would be waited for)
+    int next = 0;
+    auto issue = [&](int i, char* kt, char* vt) -> uint64_t {
+        const int kb = first_key(i);
         if constexpr (SMALL) {
-            const int page = kb + lane < w.end ? entry : -1;
+            const int page = kb + lane < stop ? next : -1;
+            __builtin_amdgcn_sched_barrier(0);
+            next = look(i + 1);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int j = 16 * u + 4 * wave + srow, p = __shfl(page, j, 64);
@@ -368,9 +374,17 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
         } else {
             uint64_t have = 0;
             const uint32_t at = kRow * (4 * wave + srow);
+            int entry[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const Sixteen r(a, __builtin_amdgcn_readlane(entry, u), w.g, kb + 16 * u, w.end);
+                entry[u] = __builtin_amdgcn_readlane(next, u);
+                asm volatile("" : "+s"(entry[u]));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            next = look(i + 1);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const Sixteen r(a, entry[u], w.g, kb + 16 * u, stop);
                 load_lds16_buf(a.K + r.at, r.bytes(), at + kchunk, reinterpret_cast<uint16_t*>(kt + 4096 * u + 1024 * wave));
                 load_lds16_buf(a.V + r.at, r.bytes(), at + vchunk, reinterpret_cast<uint16_t*>(vt + 4096 * u + 1024 * wave));
                 have |= (uint64_t)r.have() << (16 * u);
@@ -543,42 +557,44 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
         }
     };
     // Two tile pairs: the next block's copies are issued when every wave has left the tiles they overwrite, the barrier that also
-    // publishes the current block, and land while it is computed; its pages were looked up a block before that.
+    // publishes the current block, and land while it is computed; its pages were looked up a block before that. Past the last block
+    // there is nothing to copy (no rows, no traffic), and the copies are issued all the same: a wait behind a branch is for the most
+    // that either side may have left, which would be for the copies that are to be on their way (us, with the branch and without: 16
+    // answers, h=8, on 32K 47.3 and 44.5, on 128K 135 and 121; 8 x 4, h=4, on 16K 110 and 100; 16 questions on 16K 467 and 461; the
+    // own part's workgroups beside it lose: 4 x 13 answers, h=8, on 9K 66.2 and 67.7, 2 x 30, h=4, on 16K 52.8 and 55.3).
     uint64_t have = 0;
-    int next = 0;
-    auto issue = [&](int i, char* kt, char* vt) {   // block i's copies; the pages of block i + 1
-        const int entry = next;
-        next = look(i + 1);
-        return copy(first_key(i), entry, kt, vt);
-    };
-    auto publish = [&](bool first_of_two) {
-        // this wave's copies have landed (of the first two blocks, issued at once, the first one's: the second's eight may
-        // still be on their way), its reads are done
-        if (first_of_two) __builtin_amdgcn_s_waitcnt(0x0078);   // vmcnt(8) lgkmcnt(0)
-        else __builtin_amdgcn_s_waitcnt(0x0070);                // vmcnt(0) lgkmcnt(0)
+    auto publish = [&](auto left) {   // this wave's copies have landed but for the last `left` loads, and its reads are done
+        if constexpr (decltype(left)::value == 8) __builtin_amdgcn_s_waitcnt(0x0078);   // vmcnt(8) lgkmcnt(0)
+        else __builtin_amdgcn_s_waitcnt(0x0070);                                        // vmcnt(0) lgkmcnt(0)
         asm volatile("s_barrier" ::: "memory");
         pin();
     };
+    using All = std::integral_constant<int, 0>;
+    using Eight = std::integral_constant<int, 8>;
     if (tid == 0) again = 0;   // published by the first block's barrier
-    uint64_t second = 0;
     if (w.i0 < w.i1) {
         next = look(w.i0);
         have = issue(w.i0, kt0, vt0);
-        __builtin_amdgcn_sched_barrier(0);   // in this order: the wait for the first block's counts the second's
-        if (w.i0 + 1 < w.i1) second = issue(w.i0 + 1, kt1, vt1);
-    }
-    for (int i = w.i0; i < w.i1; i += 2) {
-        const bool begun = i == w.i0;
-        publish(begun && i + 1 < w.i1);
+        // q has landed, with the entries behind it: said here, as a wait for it in the loop would be one for the copies
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) asm volatile("" : "+v"(qb[kk]));
+        __builtin_amdgcn_sched_barrier(0);   // in this order: the wait for the first block's counts the second's eight
         uint64_t now = have;
-        if (begun) have = second;
-        else if (i + 1 < w.i1) have = issue(i + 1, kt1, vt1);
-        block(std::false_type{}, first_key(i), now, kt0, vt0);
-        if (i + 1 >= w.i1) break;
-        publish(false);
-        now = have;
-        if (i + 2 < w.i1) have = issue(i + 2, kt0, vt0);
-        block(std::false_type{}, first_key(i + 1), now, kt1, vt1);
+        have = issue(w.i0 + 1, kt1, vt1);
+        publish(Eight{});
+        block(std::false_type{}, first_key(w.i0), now, kt0, vt0);
+        for (int i = w.i0 + 1; i < w.i1; i += 2) {
+            publish(All{});
+            now = have;
+            have = issue(i + 1, kt0, vt0);
+            block(std::false_type{}, first_key(i), now, kt1, vt1);
+            if (i + 1 >= w.i1) break;
+            publish(All{});
+            now = have;
+            have = issue(i + 2, kt1, vt1);
+            block(std::false_type{}, first_key(i + 1), now, kt0, vt0);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): nothing is written to LDS behind the last block
     }
     // A result that is not finite: a visible key's doing, or zero weights times one that only later queries see. All rows again, with
     // the blocks that have such keys looked over. The shared part has none.
@@ -601,7 +617,7 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
             if (w.i0 < w.i1) next = look(w.i0);
             for (int i = w.i0; i < w.i1; ++i) {
                 have = issue(i, kt0, vt0);
-                publish(false);
+                publish(All{});
                 block(std::true_type{}, first_key(i), have, kt0, vt0);
                 __syncthreads();
             }
