@@ -21,10 +21,11 @@
 //
 // One launch does both parts, the own part's workgroups behind the shared part's.
 //
-// What bounds it (8 groups). 16 questions of 211 tokens, h=2, on 16K: 459 to 485 us with the merge's 16, 1.0 PFLOP/s in the shared part;
-// the matrix cores are busy half of the time, and the softmax lies between a wave's products. 4 x 13 answers, h=8, on 9K, up to 1K of their own: 66 us, 4.6 TB/s:
-// one block's copies in flight a workgroup (54 where K and V are in the caches). 16 answers, h=4, on 8K: 22 us, and 4 answers on 512:
-// 15 (the host; 12 on the GPU), chains of latencies: the share 2.3, the first copies 2.7, four blocks 5.8, partials 1, the merge 5.
+// What bounds it (8 groups). 16 questions of 211 tokens, h=2, on 16K: 455 to 485 us with the merge's 16, 1.0 PFLOP/s in the shared
+// part; the matrix cores are busy half of the time, and the softmax lies between a wave's products. 4 x 13 answers, h=8, on 9K, up to
+// 1K of their own: 66 to 75 us, 4.0 to 4.6 TB/s: one block's copies in flight a workgroup (54 us where K and V are in the caches). 16
+// answers, h=4, on 8K: 22 us, and 4 answers on 512: 15 (the host; 12 on the GPU), chains of latencies: the share 2.3, the first copies
+// 2.7, four blocks 5.8, partials 1, the merge 5.
 //
 // Weights are rounded to bf16, the operand's type, before their product with V; their sum is of the unrounded ones, sums fp32.
 #include <cfloat>
