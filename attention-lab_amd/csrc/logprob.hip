@@ -16,7 +16,7 @@
 // segments' lists.
 //
 // What bounds it, vocabulary of 151936. 4096 bf16 rows, top 5: 204 to 219 us, 1.24 GB at 5.7 to 6.1 TB/s (reads alone go at 7.1); as much
-// as the bytes it is the vector units (12 operations a logit, half of them in the sums, an exponential among them). 64 float32 rows,
+// as the bytes it is the vector units (11 operations a logit, half of them in the sums, an exponential among them). 64 float32 rows,
 // top 20: 16 us, of which the 39 MB take 6 (all workgroups at once), the bounds 1, the lists 2.5, arrivals 1 and the merge 2.5: latencies.
 #include <cfloat>
 
