@@ -316,13 +316,14 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     // the wave's word u: 64 in line, a segment's end between waves (but for the row's end)
     auto there = [&](int u) { return first + kThreads * u + 64 * wave < end; };
     u32x4_t x[U];
-    {   // as a buffer that ends with the segment: zeros behind it
+    {   // as a buffer that ends with the segment: zeros behind it. All of the offset is the vector one: a scalar offset need not count
+        // where it is compared with the end
         constexpr int kNt = 2;   // non-temporal
         const __amdgpu_buffer_rsrc_t r =
             __builtin_amdgcn_make_buffer_rsrc(const_cast<u32x4_t*>(words + first), 0, 16 * max(end - first, 0), 0x00020000);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            x[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * tid, 16 * kThreads * u, kNt));
+            x[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, 16 * tid + 16 * kThreads * u, 0, kNt));
     }
     if (tid == 0) words_sh = 0;
     // -inf for what is not the row's, in its first and last word and behind it (the waves behind a segment's end between waves skip
