@@ -57,8 +57,9 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
     read for all. The others, and sequences in no run, read everything by their own tables. prefix_lengths 0: a read of a paged cache
     with a length per sequence.
 
-    Nothing is read back to the host, so a captured graph follows the tensors' later values. Weights are rounded to bfloat16
-    before their product with V (2^-8 of each at most; their sum is not rounded), sums are float32. partitions overrides how
+    Nothing is read back to the host, so a captured graph follows the tensors' later values. One query's weights keep 16 bits in
+    their product with V; a chunk's (T > 1) are rounded to bfloat16 before it (2^-8 of each at most). Their sum is not rounded, sums
+    are float32. An infinite value that a query sees makes its output NaN or infinite. partitions overrides how
     many partials a row may have of the shared part (1 to 64; 0: the prefix is ignored) and of the own one (1 to 64)."""
     pool, device = k_pages.shape, k_pages.device
     if (len(pool) != 4 or pool[3] != HEAD_DIM or k_pages.dtype is not torch.bfloat16 or not k_pages.is_contiguous()

@@ -27,7 +27,10 @@
 // answers, h=4, on 8K: 22 us, and 4 answers on 512: 15 (the host; 12 on the GPU), chains of latencies: the share 2.3, the first copies
 // 2.7, four blocks 5.8, partials 1, the merge 5.
 //
-// Weights are rounded to bf16, the operand's type, before their product with V; their sum is of the unrounded ones, sums fp32.
+// Weights go to the matrix cores as bf16, the operand's type. Of one query each, what that rounding left is multiplied by V too, so they
+// keep 16 bits, as in the package's other one-query reads (4 x 13 answers on 9K 70.6 us, without the rest 69.9; 16 answers on 8K 22.5 and
+// 22.1); a chunk's are rounded once (2^-8 of each at most), as in its other chunk reads: the second product lies in what bounds the kernel
+// (16 questions on 16K: 642 us with it, 473 without). Their sum is of the unrounded ones, sums fp32.
 #include <cfloat>
 #include <type_traits>
 
@@ -310,6 +313,9 @@ struct Sixteen {
 // float, which gives the same weights while a masked key's -inf * scale stays -inf.
 __device__ __forceinline__ float positive_scale(float x) { return x == 0.0f ? FLT_MIN : fabsf(x); }
 
+// What rounding x and y to the pair `w` left, a bf16 pair too.
+__device__ __forceinline__ uint32_t rest_of(float x, float y, uint32_t w) { return pack_bf16x2(x - bf16_lo(w), y - bf16_hi(w)); }
+
 __device__ __forceinline__ uint32_t bf16x2_finite(uint32_t w, uint32_t& flags) {   // NaN and infinity zeroed, and flagged 1.0
     const uint32_t lo = (w & 0x00007f80u) == 0x00007f80u ? 0x0000ffffu : 0u;
     const uint32_t hi = (w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
@@ -321,7 +327,8 @@ __device__ __forceinline__ uint32_t bf16x2_finite(uint32_t w, uint32_t& flags) {
 // row j at slot c ^ (j & 15) (a read takes 16 rows, one chunk), V's at c ^ (4 (j & 3)) (a transposing read takes 4 chunks of 4
 // consecutive rows). Key 16 z + 8 g + 4 a + b of a 32-key tile is row 16 z + 8 a + 4 g + b of its product, so that a lane's weights
 // are those of eight consecutive keys, the ones whose V its operand holds.
-template <bool SMALL>
+// ONE: one query a sequence, of which only the shared part is read here, and the weights' rest has its product with V.
+template <bool SMALL, bool ONE>
 __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* kt0, char* vt0, char* kt1, char* vt1, int& again) {
     constexpr int kRow = 2 * kDim;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -426,7 +433,7 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
     // `have`: the block's keys that have a row to read, a bit each
     auto block = [&](auto careful, int kb, uint64_t have, const char* ks, const char* vs) __attribute__((always_inline)) {
         if (kb >= lim_max || have == 0) return;
-        const bool ahead = kb + kKeys > lim_min, gaps = ~have != 0;
+        const bool ahead = !ONE && kb + kKeys > lim_min, gaps = ~have != 0;
         auto value = [&](int ks2, int dt) -> bf16x8_t {   // V^T's operand of 16-key step ks2, dims 32 dt ..
             const char* vp = vs + 16 * kRow * ks2 + vof[dt];
             const u32x2v_t lo4 = read_tr16(vp), hi4 = read_tr16(vp + 4 * kRow);
@@ -509,11 +516,11 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
                 for (int i = 0; i < 16; ++i) o[dt][i] *= al;
             m_run = bm;
         }
-        bf16x8_t pb[4];
+        bf16x8_t pb[4], rest[ONE ? 4 : 1];
         const float nm = m_run == -INFINITY ? 0.0f : -m_run;   // no score above -inf yet: weights 0, or NaN for a NaN score
 #pragma unroll
         for (int ks2 = 0; ks2 < 4; ++ks2) {
-            uint32_t w4[4];
+            uint32_t w4[4], r4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float x0 = s[ks2 >> 1][8 * (ks2 & 1) + 2 * e], x1 = s[ks2 >> 1][8 * (ks2 & 1) + 2 * e + 1];
@@ -521,15 +528,20 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
                 const float p1 = fast_exp2(fmaf(x1, sc, nm));
                 l_run += p0 + p1;
                 w4[e] = pack_bf16x2(p0, p1);
+                if constexpr (ONE) r4[e] = rest_of(p0, p1, w4[e]);
             }
             pb[ks2] = __builtin_bit_cast(bf16x8_t, u32x4_t{w4[0], w4[1], w4[2], w4[3]});
+            if constexpr (ONE) rest[ks2] = __builtin_bit_cast(bf16x8_t, u32x4_t{r4[0], r4[1], r4[2], r4[3]});
         }
         if (!careful || !spoilt) {
 #pragma unroll
             for (int ks2 = 0; ks2 < 4; ++ks2)
 #pragma unroll
-                for (int dt = 0; dt < 4; ++dt)
-                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value(ks2, dt), pb[ks2], o[dt], 0, 0, 0);
+                for (int dt = 0; dt < 4; ++dt) {
+                    const bf16x8_t v = value(ks2, dt);
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, pb[ks2], o[dt], 0, 0, 0);
+                    if constexpr (ONE) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, rest[ks2], o[dt], 0, 0, 0);
+                }
         } else {   // the finite values' products, and NaN where a visible key's value is not finite
 #pragma unroll
             for (int dt = 0; dt < 4; ++dt) {
@@ -599,7 +611,7 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
     }
     // A result that is not finite: a visible key's doing, or zero weights times one that only later queries see. All rows again, with
     // the blocks that have such keys looked over. The shared part has none.
-    if (!w.shared) {
+    if (!ONE && !w.shared) {
         float finite = 0.0f * l_run;
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
@@ -684,9 +696,7 @@ __device__ __forceinline__ void narrow(const SharedArgs& a, const Item& w, char*
     const int vrow = lane >> 4;
     char* vt = tile_of(wave);
     const int vst = kRow * vrow + 16 * (n16 ^ (4 * vrow));
-    int vof[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) vof[x] = kRow * (4 * g4 + (n16 >> 2)) + 64 * (x ^ (n16 >> 2)) + 8 * (n16 & 3);
+    int vof = kRow * (4 * g4 + (n16 >> 2)) + 64 * (n16 >> 2) + 8 * (n16 & 3);   // dims 32 x .. at vof ^ 64 x
 
     float m = -INFINITY, l = 0.0f;
     f32x4_t o[8];
@@ -744,6 +754,7 @@ __device__ __forceinline__ void narrow(const SharedArgs& a, const Item& w, char*
     };
     auto compute = [&](const Tile& f) {
         const uint32_t have = f.have;
+        asm volatile("" : "+v"(vof));   // its other forms are made where they are used: registers
         f32x4_t sv[2];
 #pragma unroll
         for (int t2 = 0; t2 < 2; ++t2) {
@@ -787,16 +798,22 @@ __device__ __forceinline__ void narrow(const SharedArgs& a, const Item& w, char*
         l += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
         // a wave's LDS operations take effect in order; these keep the compiler from moving them past each other
         asm volatile("" ::: "memory");
-        uint32_t w4[4];
+        uint32_t w4[4], r4[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w4[e] = pack_bf16x2(pr[2 * e], pr[2 * e + 1]);
+        for (int e = 0; e < 4; ++e) {
+            w4[e] = pack_bf16x2(pr[2 * e], pr[2 * e + 1]);
+            r4[e] = rest_of(pr[2 * e], pr[2 * e + 1], w4[e]);
+        }
         const bf16x8_t pb = __builtin_bit_cast(bf16x8_t, u32x4_t{w4[0], w4[1], w4[2], w4[3]});
+        const bf16x8_t rest = __builtin_bit_cast(bf16x8_t, u32x4_t{r4[0], r4[1], r4[2], r4[3]});
 #pragma unroll
         for (int dt = 0; dt < 8; ++dt) {
-            const char* r = vt + vof[dt >> 1] + 32 * (dt & 1);
+            const char* r = vt + (vof ^ 64 * (dt >> 1)) + 32 * (dt & 1);
             const u32x2v_t w0 = read_tr16(r), w1 = read_tr16(r + 16 * kRow);
-            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, u32x4_t{w0.x, w0.y, w1.x, w1.y}), pb, o[dt],
-                                                           0, 0, 0);
+            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, u32x4_t{w0.x, w0.y, w1.x, w1.y});
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb, o[dt], 0, 0, 0);
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, rest, o[dt], 0, 0, 0);
+            if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);   // an operand at a time: registers
         }
         asm volatile("" ::: "memory");
     };
@@ -880,7 +897,7 @@ __global__ __launch_bounds__(64 * kWaves, WIDE ? 2 : 3) void shared_read(SharedA
     Item w;
     if constexpr (WIDE && !OWN_WIDE) {
         if (first) {
-            if (shared_item<kWide, kKeys, kMixedWorkers>(a, xcd, turn, w)) wide<SMALL>(a, w, t0, t1, t2, t3, again);
+            if (shared_item<kWide, kKeys, kMixedWorkers>(a, xcd, turn, w)) wide<SMALL, true>(a, w, t0, t1, t2, t3, again);
         } else {
             if (own_item<kNarrow, kTile>(a, own, w)) narrow<SMALL, !SMALL>(a, w, t0, t1, ml_sh);
         }
@@ -888,7 +905,7 @@ __global__ __launch_bounds__(64 * kWaves, WIDE ? 2 : 3) void shared_read(SharedA
         constexpr int kRows = WIDE ? kWide : kNarrow, kBlock = WIDE ? kKeys : kTile;
         constexpr uint32_t kWorkers = WIDE ? kWideWorkers : kNarrowWorkers;
         if (!(first ? shared_item<kRows, kBlock, kWorkers>(a, xcd, turn, w) : own_item<kRows, kBlock>(a, own, w))) return;
-        if constexpr (WIDE) wide<SMALL>(a, w, t0, t1, t2, t3, again);
+        if constexpr (WIDE) wide<SMALL, false>(a, w, t0, t1, t2, t3, again);
         else narrow<SMALL, false>(a, w, t0, t1, ml_sh);
     }
 }
