@@ -44,7 +44,8 @@ class PagedCache:
     k, v bfloat16 [layers, num_pages, G, page_size, 128]; table int32 [slots, max_pages], the page of each slot's positions
     [e page_size, (e + 1) page_size) in its entry e, or -1; lengths int32 [slots]; refs int32 [num_pages], how many entries name
     each page (0: free). All are contiguous tensors on one HIP device, used in place. The operators keep refs in step with the
-    table; a table made elsewhere has to come with its counts and hold -1 past its sequences' pages. A page whose count is raised
+    table; a table made elsewhere has to come with its counts and hold -1 past its sequences' pages (entries below -1 are the
+    operators' own, see page_reserve). A page whose count is raised
     by hand stays in use and is never written in place (a compaction may move it). missing (int32 [1], optional) counts the
     pages that page_reserve could not give."""
 
@@ -134,7 +135,10 @@ def page_reserve(cache: PagedCache, tokens=1) -> None:
     A slot that ends inside a page that others hold too gets a page of its own, with the page's rows up to its length copied
     in every layer; if all of a page's holders are written to, the last of them keeps it. New pages are the lowest free ones, in
     the order of slots and positions. Where none is left an entry is -1: its positions are neither written nor read (nor those
-    past max_pages * page_size), and cache.missing counts it."""
+    past max_pages * page_size), and cache.missing counts it. Where none is left for a page of a slot's own, the slot's rows
+    of the shared one stay its own, but neither they nor the new ones are read until page_truncate takes the slot back to
+    them (or before): the entry is below -1 till then. One of the slots that would need a copy, the one with the most rows
+    in the page, writes on in it if every other one is left so or has its copy."""
     at, each = _per_slot(cache, tokens, "tokens")
     scratch, nbytes = _scratch(cache)
     nat.call_on(cache.device, "attnlab_page_reserve", cache.k.data_ptr(), cache.v.data_ptr(), cache.layers, cache.num_pages,

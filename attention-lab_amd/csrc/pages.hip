@@ -7,10 +7,16 @@
 //   fork      table'[i] = table[parents[i]], lengths'[i] = lengths[parents[i]]; a parent outside [0, S): an empty slot
 //   reserve   lengths'[i] = n + t. If n ends inside a page that others hold too, the slot gets a page of its own with the rows
 //             [0, n % page) copied; where all of its holders are written to, the last of them in slot order keeps it. Then
-//             ceil((n + t) / page) - ceil(n / page) pages more. In the order of slots and entries, lowest free page first
+//             ceil((n + t) / page) - ceil(n / page) pages more. In the order of slots and entries, lowest free page first.
+//             A slot for whose copy none is left keeps its rows of the shared page in a claim (below)
 //   append    a layer's rows of the last t positions, written to their pages
 //   truncate  lengths'[i] = min(n, l), the entries from ceil(l / page) on given back
 //   compact   with u pages in use: the i-th of them at or past u moves to the i-th free one below u
+//
+// A claim is an entry of a slot whose length has passed the rows that the entry's page holds for it: the first `rows` of the page are the
+// slot's and stay counted, but it had no page of its own to go on in. It reads as an entry without a page, and a truncation to those
+// rows or fewer makes the page the entry's again. Written as INT32_MIN + rows pages + page: 1 <= rows < the page's, so it lies
+// below -1, and where a page's rows are not known (fork) as in any page, rows < 65536.
 //
 // Every choice depends on the cache alone, never on the order in which workgroups or atomics run: counts are integer sums,
 // and free pages are dealt out by prefix sums over the pool. Entries and lengths are checked before they address memory.
@@ -28,6 +34,7 @@ namespace {
 constexpr int kDim = 128;
 constexpr int kRowWords = kDim * 2 / 16;     // 16-byte words of a row
 constexpr int kMaxSlots = 1024;              // a thread of the reserve's workgroup for each
+constexpr int kMaxPage = 1 << 16;
 constexpr int kColumns = 16;                 // table entries a fork's workgroup exchanges between the slots
 constexpr int kBook = 1024;                  // threads of the reserve's and the compaction's workgroup
 constexpr int kScan = 16;                    // pages a thread looks at in a round
@@ -50,6 +57,25 @@ struct Book {
 };
 
 __device__ __forceinline__ bool names(int32_t page, int pages) { return (uint32_t)page < (uint32_t)pages; }
+
+// A claim's page and rows; -1 and 0 of an entry that is none. `most`: a page's rows.
+struct Claim {
+    int page = -1, rows = 0;
+    __device__ __forceinline__ Claim(int32_t entry, int pages, int most) {
+        if (entry >= -1) return;
+        const uint32_t x = (uint32_t)entry ^ 0x80000000u, n = x / (uint32_t)pages;
+        if (n < 1 || n >= (uint32_t)most) return;
+        page = (int)(x - n * (uint32_t)pages);
+        rows = (int)n;
+    }
+};
+__device__ __forceinline__ int32_t claim_of(int page, int rows, int pages) {
+    return (int32_t)(0x80000000u + (uint32_t)rows * (uint32_t)pages + (uint32_t)page);
+}
+// The page that an entry counts for, or -1.
+__device__ __forceinline__ int counted(int32_t entry, int pages, int most) {
+    return names(entry, pages) ? entry : Claim(entry, pages, most).page;
+}
 
 // The slots' rows exchanged, 16 entries of all of them at a time: no workgroup reads what another writes, so the table is
 // changed in place. One more workgroup does the lengths.
@@ -90,8 +116,9 @@ __global__ __launch_bounds__(256) void page_fork(Book a, const int32_t* parents)
             if (i >= a.S) break;
             const int32_t old = was[i * kColumns + col], now = names(p[u], a.S) ? was[p[u] * kColumns + col] : -1;
             if (now == old) continue;
-            if (names(old, a.pages)) atomicSub(a.refs + old, 1);
-            if (names(now, a.pages)) atomicAdd(a.refs + now, 1);
+            const int from = counted(old, a.pages, kMaxPage), to = counted(now, a.pages, kMaxPage);
+            if (from >= 0) atomicSub(a.refs + from, 1);
+            if (to >= 0) atomicAdd(a.refs + to, 1);
             a.table[(size_t)i * a.W + e0 + col] = now;
         }
     }
@@ -107,9 +134,15 @@ __global__ __launch_bounds__(256) void page_truncate(Book a, const int32_t* to, 
     const int end = (int)min((int64_t)a.W, ((int64_t)n + page - 1) >> a.shift);
     for (int e = first + (int)threadIdx.x; e < end; e += 256) {
         int32_t* at = a.table + (size_t)i * a.W + e;
-        const int32_t p = *at;
-        if (names(p, a.pages)) atomicSub(a.refs + p, 1);
+        const int p = counted(*at, a.pages, page);
+        if (p >= 0) atomicSub(a.refs + p, 1);
         *at = -1;
+    }
+    const int part = l & (page - 1);
+    if (threadIdx.x == 0 && part && (l >> a.shift) < a.W) {   // a claim of all that is left: the page again
+        int32_t* at = a.table + (size_t)i * a.W + (l >> a.shift);
+        const Claim c(*at, a.pages, page);
+        if (part <= c.rows) *at = c.page;
     }
 }
 
@@ -220,7 +253,7 @@ __global__ __launch_bounds__(kBook) void page_reserve(Book a, const int32_t* tok
         const uint32_t k = r - (lo ? upto_sh[lo - 1] : 0u), j = job_sh[lo];
         const bool copy = j && k == 0;
         const int e = first_sh[lo] + (int)k - (j ? 1 : 0);   // a copy's entry is the one before the first new one
-        a.table[(size_t)lo * a.W + e] = p;
+        if (p >= 0 || !copy) a.table[(size_t)lo * a.W + e] = p;
         if (copy) {
             src[j - 1] = held_sh[lo];
             dst[j - 1] = p;
@@ -240,12 +273,34 @@ __global__ __launch_bounds__(kBook) void page_reserve(Book a, const int32_t* tok
         });
     }
     for (uint32_t r = found + tid; r < wanted; r += kBook) give(r, -1);
-    if (copies) atomicSub(a.refs + held, 1);
-    if (tid == 0) moves->count = (int32_t)jobs;
-    if (missing) {
-        const int out = lost + (tid == 0 && wanted > found ? (int)(wanted - found) : 0);
-        if (out) atomicAdd(missing, out);
+    auto granted = [&](int j) { return job_sh[j] && (j ? upto_sh[j - 1] : 0u) < found; };   // a copy is its slot's first request
+    int out = lost + (tid == 0 && wanted > found ? (int)(wanted - found) : 0);
+    if (copies && granted(tid)) {
+        atomicSub(a.refs + held, 1);
+    } else if (held >= 0 && found < wanted) {
+        // No page was left for every copy. Of the writers that are still on this one, the one with the most rows (the last of those)
+        // writes on in place, if its other holders are writers too or claim no more rows than it has; the others claim theirs.
+        int best = -1, best_rows = -1, holders = 0, claimed = 0;
+        for (int j = 0; j < a.S; ++j) {
+            if (held_sh[j] == held) {
+                ++holders;
+                if (!granted(j) && part_sh[j] >= best_rows) {
+                    best = j;
+                    best_rows = part_sh[j];
+                }
+            } else {
+                const Claim c(a.table[(size_t)j * a.W + last], a.pages, page);
+                if (c.page != held) continue;
+                ++holders;
+                claimed = max(claimed, c.rows);
+            }
+        }
+        const bool on = best == tid && holders == refs && claimed <= part;
+        if (!on) a.table[(size_t)tid * a.W + last] = claim_of(held, part, a.pages);
+        out += !on - copies;                 // its copy, if it asked for one, is counted above
     }
+    if (tid == 0) moves->count = (int32_t)jobs;
+    if (missing && out) atomicAdd(missing, out);
 }
 
 __global__ __launch_bounds__(kBook) void page_compact(Book a, Moves* moves, int32_t* src, int32_t* dst, int32_t* rank_of) {
@@ -334,10 +389,12 @@ __global__ __launch_bounds__(256) void page_copy(CopyArgs a) {
     if (a.table && count) {
         const int used = a.moves->used;
         for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.entries; i += (int64_t)gridDim.x * 256) {
-            const int32_t p = a.table[i];
+            const int32_t entry = a.table[i];
+            const Claim c(entry, a.pages, a.page);
+            const int32_t p = c.rows ? c.page : entry;
             if (p < used || p >= a.pages) continue;
             const int32_t r = a.rank_of[p];
-            if (r >= 0) a.table[i] = a.dst[r];
+            if (r >= 0) a.table[i] = c.rows ? claim_of(a.dst[r], c.rows, a.pages) : a.dst[r];
         }
     }
 }

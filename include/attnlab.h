@@ -394,19 +394,23 @@ int attnlab_range_prefill(const uint16_t* q, const void* K, const void* V, const
  *   lengths  int32 [S]
  *   refs     int32 [num_pages], how many entries name each page (0: free)
  * All are device memory changed in place. The results depend on the cache alone. Calls on one cache must be ordered on one
- * stream. An entry outside [0, num_pages) is not followed.
+ * stream. Entries below -1 are these functions' own: INT32_MIN + rows * num_pages + p, with 1 <= rows < page_size, is a claim, an entry that
+ * counts for page p, whose first `rows` rows are the slot's, and that reads as no page (attnlab_page_reserve makes them). Other entries
+ * outside [0, num_pages) are not followed.
  *
  * attnlab_page_fork: slot i goes on from slot parents[i] (int32 [S], none of the cache's own memory) as it was before the call: its entries and length; a
  * parent outside [0, S) leaves the slot empty.
  *
  * attnlab_page_truncate: lengths[i] = min(lengths[i], max(to[i], 0)), with `to` null `length`; the entries from
- * ceil(lengths[i] / page_size) on are given back.
+ * ceil(lengths[i] / page_size) on are given back. A claim that the slot then ends in, at its rows or before, is its page again.
  *
  * attnlab_page_reserve: lengths[i] grows by tokens[i] (null: each; less than 1: slot i is left alone). A slot that ended
  * inside a page with other holders gets a page of its own, the rows up to its length copied in every layer, unless all of the
  * page's holders grow and it is the last of them. Then an entry is given a page for every page_size positions begun. Pages are the
- * lowest free ones, in the order of slots and entries; where none is left the entry is -1. missing (int32 [1], nullable) is
- * raised by the pages not given, those past max_pages among them. scratch: 16-byte aligned, attnlab_page_scratch_bytes(S,
+ * lowest free ones, in the order of slots and entries; where none is left the entry is -1, or, for a copy, a claim of the slot's
+ * rows of the page. One of the holders that are left without a copy, the one with the most rows (the last of those), writes on in
+ * place if all others grow or claim no more rows than it has. missing (int32 [1], nullable) is raised by the pages not given, those
+ * past max_pages among them. scratch: 16-byte aligned, attnlab_page_scratch_bytes(S,
  * num_pages) bytes, no initialisation.
  *
  * attnlab_page_append: one layer's rows, k and v: (slot, group, row t, dim) at k + i k_b_stride + g k_g_stride + t k_t_stride

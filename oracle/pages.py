@@ -15,11 +15,21 @@ class Pages:
         self.pages, self.page = int(k.shape[1]), int(k.shape[3])
         self.missing = missing
 
+    def claim(self, page, rows):
+        """The entry of a slot that has the first `rows` rows of the page, and a length past them."""
+        return -2 ** 31 + rows * self.pages + page
+
+    def claimed(self, entry):
+        """(page, rows) of such an entry; (-1, 0) of others."""
+        rows, page = divmod(entry + 2 ** 31, self.pages)
+        return (page, rows) if entry < -1 and 1 <= rows < self.page else (-1, 0)
+
     @property
     def refs(self):
         n = [0] * self.pages
         for row in self.table:
-            for p in row:
+            for entry in row:
+                p = self.claimed(entry)[0] if entry < 0 else entry
                 if 0 <= p < self.pages:
                     n[p] += 1
         return n
@@ -37,6 +47,10 @@ class Pages:
                 self.lengths[i] = l
                 for e in range(-(-l // self.page), len(self.table[i])):
                     self.table[i][e] = -1
+                if l % self.page and l // self.page < len(self.table[i]):
+                    page, rows = self.claimed(self.table[i][l // self.page])
+                    if l % self.page <= rows:
+                        self.table[i][l // self.page] = page
 
     def reserve(self, tokens):
         page, W = self.page, len(self.table[0])
@@ -49,6 +63,7 @@ class Pages:
         # all of the page's holders grow: the last keeps it
         away = {i for p, who in ends_in.items() for i in (who[:-1] if len(who) == refs[p] else who)}
         free = [p for p in range(self.pages) if refs[p] == 0]
+        was, left = [list(row) for row in self.table], set()
         for i, n, t in grows:
             entries = ([n // page] if i in away else []) + list(range(-(-n // page), -(-(n + t) // page)))
             for e in entries:
@@ -56,12 +71,29 @@ class Pages:
                     self.missing += 1
                     continue
                 p = free.pop(0) if free else -1
+                if p < 0 and e < -(-n // page):
+                    left.add(i)
+                    continue
                 self.missing += p < 0
-                if e < -(-n // page) and p >= 0:
+                if e < -(-n // page):
                     for x in (self.k, self.v):
                         x[:, p, :, :n % page] = x[:, self.table[i][e], :, :n % page]
                 self.table[i][e] = p
             self.lengths[i] = n + t
+        # no page for a copy: the longest writer that is left writes on in place if the others claim no more, and those claim theirs
+        part = {i: n % page for i, n, _ in grows}
+        for p, who in ends_in.items():
+            here = [i for i in who if i in left or i not in away]
+            if not left & set(here):
+                continue
+            e = {i: n // page for i, n, _ in grows}[here[0]]
+            claims = [self.claimed(row[e])[1] for row in was if self.claimed(row[e])[0] == p]
+            best = max(here, key=lambda i: (part[i], i))
+            on = len(who) + len(claims) == refs[p] and max(claims, default=0) <= part[best]
+            for i in here:
+                if not (on and i == best):
+                    self.table[i][e] = self.claim(p, part[i])
+                    self.missing += 1
 
     def append(self, layer, k, v, tokens):
         """k, v [S, G, T, d]."""
@@ -82,7 +114,11 @@ class Pages:
         to = dict(zip([p for p in used if p >= n], holes))
         for src, dst in to.items():
             self.k[:, dst], self.v[:, dst] = self.k[:, src], self.v[:, src]
-        self.table = [[to.get(p, p) for p in row] for row in self.table]
+        def moved(entry):
+            page, rows = self.claimed(entry)
+            return self.claim(to[page], rows) if page in to else to.get(entry, entry)
+
+        self.table = [[moved(entry) for entry in row] for row in self.table]
 
     def rows(self, layer, slot):
         """The slot's rows by position: (k, v) [G, length, d]; only where every position has a page."""
