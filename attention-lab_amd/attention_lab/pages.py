@@ -130,7 +130,7 @@ def page_fork(cache: PagedCache, parents) -> None:
 
 def page_reserve(cache: PagedCache, tokens=1) -> None:
     """Room for `tokens` more positions of every slot (an int, or int32 [slots] on the device; 0 leaves a slot as it is):
-    lengths grow by as many, and page_append may write their rows.
+    lengths grow by as many (to 2^31 - 1 at most, where rows are no longer written), and page_append may write their rows.
 
     A slot that ends inside a page that others hold too gets a page of its own, with the page's rows up to its length copied
     in every layer; if all of a page's holders are written to, the last of them keeps it. New pages are the lowest free ones, in

@@ -438,7 +438,9 @@ __global__ __launch_bounds__(256) void page_append(AppendArgs a, int runs) {
     }
     const int tokens = a.tokens ? a.tokens[i] : a.T, count = min(tokens, a.T);
     if (t0 >= count) return;
-    const int64_t first = (int64_t)a.lengths[i] - tokens;
+    const int length = a.lengths[i];
+    if (length == INT32_MAX) return;         // where a reserve stops counting: which positions the rows have is not known
+    const int64_t first = (int64_t)length - tokens;
     const uint16_t* from = a.x[kv] + i * a.sb[kv] + g * a.sg[kv] + 8 * lane16;
     u32x4_t w[kRows];
     int64_t at[kRows];

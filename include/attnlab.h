@@ -404,7 +404,7 @@ int attnlab_range_prefill(const uint16_t* q, const void* K, const void* V, const
  * attnlab_page_truncate: lengths[i] = min(lengths[i], max(to[i], 0)), with `to` null `length`; the entries from
  * ceil(lengths[i] / page_size) on are given back. A claim that the slot then ends in, at its rows or before, is its page again.
  *
- * attnlab_page_reserve: lengths[i] grows by tokens[i] (null: each; less than 1: slot i is left alone). A slot that ended
+ * attnlab_page_reserve: lengths[i] grows by tokens[i] (null: each; less than 1: slot i is left alone), up to 2^31 - 1. A slot that ended
  * inside a page with other holders gets a page of its own, the rows up to its length copied in every layer, unless all of the
  * page's holders grow and it is the last of them. Then an entry is given a page for every page_size positions begun. Pages are the
  * lowest free ones, in the order of slots and entries; where none is left the entry is -1, or, for a copy, a claim of the slot's
@@ -416,7 +416,7 @@ int attnlab_range_prefill(const uint16_t* q, const void* K, const void* V, const
  * attnlab_page_append: one layer's rows, k and v: (slot, group, row t, dim) at k + i k_b_stride + g k_g_stride + t k_t_stride
  * + dim (bf16 elements; rows 16-byte aligned; strides may be 0), row t < tokens[i] (null: T) of slot i at position
  * lengths[i] - tokens[i] + t. k_pages, v_pages: the layer's [num_pages, G, page_size, 128]. Positions without a page are
- * not written.
+ * not written, nor are the rows of a slot whose length is 2^31 - 1.
  *
  * attnlab_page_compact: with n pages in use (refs > 0), the i-th of them at or past n moves to the i-th free one below n, in
  * every layer; table and refs follow. scratch as in attnlab_page_reserve.

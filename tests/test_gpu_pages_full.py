@@ -151,3 +151,21 @@ def test_in_a_graph(gpu):
         same(cache, model)
         write(cache, model, gpu, 700 + step, [1, 0, 2, 0])       # eager work between replays
         same(cache, model)
+
+
+def test_lengths_past_31_bits(gpu):
+    """A slot that grows past 2^31 - 1 positions: no row of it is written any more, least of all over those it has."""
+    cache, model = fresh(gpu, 9, 1, 2, 2, 8, 8, 4)
+    write(cache, model, gpu, 1, [5, 3])
+    tokens = [2 ** 31 - 1, 2]
+    page_reserve(cache, ints(tokens, gpu))
+    model.reserve([40, 2])                                       # as far as pages go, 40 positions are as many
+    rows = torch.randn(2, 2, 2, 128, generator=gen(4)).to(torch.bfloat16)
+    page_append(cache, 0, rows.to(gpu), rows.to(gpu), ints(tokens, gpu))
+    model.append(0, rows, rows, [0, 2])
+    assert cache.lengths.tolist() == [2 ** 31 - 1, 5] and cache.table.tolist() == model.table
+    assert torch.equal(cache.k.cpu(), model.k) and torch.equal(cache.v.cpu(), model.v)
+    page_truncate(cache, 5)
+    model.truncate([5, 5])
+    cache.missing.fill_(model.missing)
+    same(cache, model)
