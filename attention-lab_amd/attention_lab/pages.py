@@ -170,8 +170,8 @@ def page_append(cache: PagedCache, layer: int, k, v, tokens=None) -> None:
 
 
 def page_truncate(cache: PagedCache, lengths=0) -> None:
-    """Every slot shortened to at most `lengths` positions (an int, or int32 [slots] on the device; a negative one is 0): the
-    pages past them are given back. Rows stay in memory, outside every read."""
+    """Every slot shortened to at most `lengths` positions (an int, or int32 [slots] on the device, a tensor of its own; a
+    negative one is 0): the pages past them are given back. Rows stay in memory, outside every read."""
     at, each = _per_slot(cache, lengths, "lengths")
     nat.call_on(cache.device, "attnlab_page_truncate", cache.table.data_ptr(), cache.lengths.data_ptr(), cache.refs.data_ptr(), at,
                 each, cache.slots, cache.max_pages, cache.num_pages, cache.page_size, nat.stream_of(cache.device))

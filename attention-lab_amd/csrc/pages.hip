@@ -456,6 +456,12 @@ __global__ __launch_bounds__(256) void page_append(AppendArgs a, int runs) {
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// Whether two arrays of na and nb int32 share memory.
+bool meet(const int32_t* a, int64_t na, const int32_t* b, int64_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + 4 * (uintptr_t)nb && y < x + 4 * (uintptr_t)na;
+}
+
 int check_book(const int32_t* table, const int32_t* lengths, const int32_t* refs, int S, int W, int pages, int page) {
     ATTNLAB_REQUIRE(1 <= S && S <= kMaxSlots, "slots S=%d outside [1, %d]", S, kMaxSlots);
     ATTNLAB_REQUIRE(W >= 1 && pages >= 1, "max_pages=%d and num_pages=%d must be positive", W, pages);
@@ -504,12 +510,10 @@ extern "C" int attnlab_page_fork(int32_t* table, int32_t* lengths, int32_t* refs
                                  int num_pages, void* stream) {
     const int rc = check_book(table, lengths, refs, S, max_pages, num_pages, 1);
     if (rc) return rc;
-    auto within = [&](const int32_t* of, int64_t n) {   // read by workgroups that others' writes would overtake
-        const uintptr_t p = reinterpret_cast<uintptr_t>(parents), o = reinterpret_cast<uintptr_t>(of);
-        return p < o + 4 * (uintptr_t)n && o < p + 4 * (uintptr_t)S;
-    };
     ATTNLAB_REQUIRE(parents, "parents must be a device pointer");
-    ATTNLAB_REQUIRE(!within(lengths, S) && !within(refs, num_pages) && !within(table, (int64_t)S * max_pages),
+    // read by workgroups that others' writes would overtake
+    ATTNLAB_REQUIRE(!meet(parents, S, lengths, S) && !meet(parents, S, refs, num_pages) &&
+                        !meet(parents, S, table, (int64_t)S * max_pages),
                     "parents must not lie in the cache's own tensors");
     const int groups = (max_pages + kColumns - 1) / kColumns + 1;
     hipLaunchKernelGGL(page_fork, dim3((unsigned)groups), dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
@@ -522,6 +526,10 @@ extern "C" int attnlab_page_truncate(int32_t* table, int32_t* lengths, int32_t* 
     const int rc = check_book(table, lengths, refs, S, max_pages, num_pages, page_size);
     if (rc) return rc;
     ATTNLAB_REQUIRE(to || length >= 0, "length=%d must not be negative", length);
+    // a slot's workgroup reads to[i] beside others' writes; the lengths themselves change nothing
+    ATTNLAB_REQUIRE(!to || ((to == lengths || !meet(to, S, lengths, S)) && !meet(to, S, refs, num_pages) &&
+                            !meet(to, S, table, (int64_t)S * max_pages)),
+                    "the lengths to truncate to must not lie in the cache's own tensors");
     hipLaunchKernelGGL(page_truncate, dim3((unsigned)S), dim3(256), 0, reinterpret_cast<hipStream_t>(stream),
                        book_of(table, lengths, refs, S, max_pages, num_pages, page_size), to, length);
     return check_launch("page_truncate");

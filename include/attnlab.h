@@ -401,7 +401,7 @@ int attnlab_range_prefill(const uint16_t* q, const void* K, const void* V, const
  * attnlab_page_fork: slot i goes on from slot parents[i] (int32 [S], none of the cache's own memory) as it was before the call: its entries and length; a
  * parent outside [0, S) leaves the slot empty.
  *
- * attnlab_page_truncate: lengths[i] = min(lengths[i], max(to[i], 0)), with `to` null `length`; the entries from
+ * attnlab_page_truncate: lengths[i] = min(lengths[i], max(to[i], 0)), `to` in memory of its own, with `to` null `length`; the entries from
  * ceil(lengths[i] / page_size) on are given back. A claim that the slot then ends in, at its rows or before, is its page again.
  *
  * attnlab_page_reserve: lengths[i] grows by tokens[i] (null: each; less than 1: slot i is left alone), up to 2^31 - 1. A slot that ended
