@@ -815,17 +815,25 @@ class LabRunner:
     def score(self, input_ids: torch.Tensor, chunk: int, *, top: int = 0, entropy: bool = False) -> TokenLogprobs:
         """prefill of the prompt, with every token's log probability given those before it: token_logprobs of [B, T - 1]
         positions, position t the distribution behind token t and the logprob of token t + 1. Each chunk's logits are read
-        once and dropped. No counterpart in the reference, whose scripts take log_softmax of kept logits."""
+        once and dropped. No gradient is recorded. What can be refused is refused before the first chunk. No counterpart in the
+        reference, whose scripts take log_softmax of kept logits."""
         B, T = input_ids.shape
         if T < 2:
             raise ValueError(f"need at least two tokens to score one, got {T}")
+        cache = self.state.cache
+        if cache.valid_length + T > cache.capacity:
+            raise RuntimeError(f"cache capacity {cache.capacity} exceeded: valid {cache.valid_length} + new {T}")
+        head = self.model.lm_head.weight
+        token_logprobs(head.new_empty(0, head.shape[0]), input_ids.new_empty(0), top=top)   # checked, nothing launched
         parts = []
-        for a, b in _chunks(T, chunk):
-            given = input_ids[:, a + 1:b + 1]
-            if given.shape[1] < b - a:   # the last token has none behind it: padding
-                given = torch.nn.functional.pad(given, (0, 1), value=-1)
-            parts.append(token_logprobs(self.forward(input_ids[:, a:b], phase="prefill", logits_to_keep=0), given, top=top,
-                                        entropy=entropy))
+        with torch.no_grad():
+            for a, b in _chunks(T, chunk):
+                given = input_ids[:, a + 1:b + 1]
+                if given.shape[1] < b - a:   # the last token has none behind it: padding
+                    given = torch.nn.functional.pad(given, (0, 1), value=-1)
+                logits = self.forward(input_ids[:, a:b], phase="prefill", logits_to_keep=0)
+                parts.append(token_logprobs(logits, given, top=top, entropy=entropy))
+                del logits   # not held beside the next chunk's
         return TokenLogprobs(*(None if field[0] is None else torch.cat(field, dim=1)[:, :T - 1] for field in zip(*parts)))
 
     def step(self, token_ids: torch.Tensor) -> torch.Tensor:
