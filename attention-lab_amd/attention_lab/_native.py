@@ -13,6 +13,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_NAME = "libattnlab.so"
 # ATTNLAB_LIB names another build of the same library (the host-sanitized debug build); unset, the in-tree one
@@ -164,6 +165,18 @@ def stream_of(device: torch.device) -> int:
 def step_workspace_bytes(B: int, G: int, h: int, lo: int, hi: int, legal: int, k: int, P: int) -> int:
     """attnlab_sparse_decode_workspace, a function of the sizes alone (every layer of a step asks for the same ones)."""
     return lib().attnlab_sparse_decode_workspace(B, G, h, lo, hi, legal, k, P)
+
+
+def refuse_gradients(name: str, *tensors) -> None:
+    """ValueError for tensors that a gradient or a forward-mode tangent would have to pass: the operator has neither, and would
+    drop it without a word."""
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{name} has no gradient: give it tensors that need none (detach them, or use torch.no_grad)")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no forward-mode gradient: give it tensors without a tangent")
 
 
 def ptr(t) -> int | None:

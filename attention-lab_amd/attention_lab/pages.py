@@ -149,7 +149,8 @@ def page_reserve(cache: PagedCache, tokens=1) -> None:
 def page_append(cache: PagedCache, layer: int, k, v, tokens=None) -> None:
     """A layer's rows k, v bfloat16 [slots, G, T, 128] (any strides) at the last positions of every slot: row t of slot i at
     lengths[i] - tokens[i] + t for t < tokens[i] (int32 [slots] on the device, what page_reserve was given; None: T for all).
-    Rows of a page that another slot holds are its rows too: page_reserve sees to it that there are none."""
+    Rows of a page that another slot holds are its rows too: page_reserve sees to it that there are none. k and v lie in memory that
+    the call does not write. There is no gradient: rows that ask for one are refused."""
     shape, device = k.shape, cache.device
     S, G, T, d = shape if len(shape) == 4 else (0, 0, 0, 0)
     if S != cache.slots or G != cache.groups or d != HEAD_DIM or k.dtype is not torch.bfloat16:
@@ -157,6 +158,7 @@ def page_append(cache: PagedCache, layer: int, k, v, tokens=None) -> None:
                          f"{k.dtype} {tuple(shape)}")
     if v.shape != shape or v.dtype is not torch.bfloat16 or k.device != device or v.device != device:
         raise ValueError("v must match k, on the cache's device")
+    nat.refuse_gradients("page_append", k, v)
     layer = int(layer)
     if not 0 <= layer < cache.layers:
         raise ValueError(f"layer {layer} outside [0, {cache.layers})")

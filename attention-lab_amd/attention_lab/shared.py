@@ -59,7 +59,8 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
 
     Nothing is read back to the host, so a captured graph follows the tensors' later values. One query's weights keep 16 bits in
     their product with V; a chunk's (T > 1) are rounded to bfloat16 before it (2^-8 of each at most). Their sum is not rounded, sums
-    are float32. An infinite value that a query sees makes its output NaN or infinite. partitions overrides how
+    are float32. An infinite value that a query sees makes its output NaN or infinite. There is no gradient: tensors that ask for one are
+    refused. partitions overrides how
     many partials a row may have of the shared part (1 to 64; 0: the prefix is ignored) and of the own one (1 to 64)."""
     pool, device = k_pages.shape, k_pages.device
     if (len(pool) != 4 or pool[3] != HEAD_DIM or k_pages.dtype is not torch.bfloat16 or not k_pages.is_contiguous()
@@ -88,6 +89,7 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
         R = runs.numel() - 1
         if runs.dim() != 1 or R < 1 or runs.dtype is not torch.int32 or not runs.is_contiguous() or runs.device != device:
             raise ValueError("runs must be a contiguous int32 [R + 1] tensor of at least two bounds on the pools' device")
+    nat.refuse_gradients("shared_prefix_attention", q, k_pages, v_pages)
     lengths_at, length = _lengths(lengths, B, device, "lengths")
     prefix_at, prefix = _lengths(prefix_lengths, R, device, "prefix_lengths")
     most = W * page if lengths_at else min(length, W * page)
