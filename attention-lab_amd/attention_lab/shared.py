@@ -76,8 +76,9 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
     B, _, h, T, _ = shape
     if not 1 <= h <= MAX_H_CHUNK:
         raise ValueError(f"h={h} must be in [1, {MAX_H_CHUNK}]")
-    if B < 1 or not pages or not page or page & (page - 1):
-        raise ValueError(f"need at least one sequence and page, and a page_size that is a power of two, got {B}, {pages}, {page}")
+    if B < 1 or not pages or not G or not page or page & (page - 1):
+        raise ValueError("need at least one sequence, page and group, and a page_size that is a power of two, got "
+                         f"{B}, {pages}, {G}, {page}")
     rows_b, W = block_table.shape if block_table.dim() == 2 else (0, 0)
     if rows_b != B or W < 1 or block_table.dtype is not torch.int32 or block_table.device != device:
         raise ValueError("block_table must be an int32 [B, max_pages] tensor with unit column stride on the pools' device")
