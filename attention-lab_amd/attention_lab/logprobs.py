@@ -36,7 +36,8 @@ def token_logprobs(logits, tokens=None, *, top: int = 0, entropy: bool = False) 
     logprobs = logits[token] - log sum exp(logits); a token below 0 is padding and gives 0, one of V or more NaN. top (up to
     64): the most likely tokens, equal logits by the lower token (-0 equals +0, NaN last). A row with a NaN or +inf, or of
     nothing but -inf, has no distribution: its values are NaN. Sums are float32. Rows may have any stride; logits whose last
-    dimension has another stride than 1 are copied. There is no gradient: logits that ask for one, or carry a tangent, are refused."""
+    dimension has another stride than 1 are copied. There is no gradient: logits that ask for one, or carry a tangent, are
+    refused."""
     shape = logits.shape
     code = _DTYPES.get(logits.dtype)
     if code is None or not shape or not logits.is_cuda:

@@ -55,7 +55,8 @@ class PagedCache:
     def __init__(self, k, v, table, lengths, refs, *, missing=None):
         shape, device = k.shape, k.device
         if len(shape) != 5 or shape[4] != HEAD_DIM or k.dtype != torch.bfloat16 or not k.is_contiguous() or not k.is_cuda:
-            raise ValueError(f"k must be a contiguous bfloat16 [layers, num_pages, G, page_size, {HEAD_DIM}] tensor on a HIP device")
+            raise ValueError(f"k must be a contiguous bfloat16 [layers, num_pages, G, page_size, {HEAD_DIM}] tensor on a HIP "
+                             "device")
         if v.shape != shape or v.dtype != k.dtype or not v.is_contiguous() or v.device != device:
             raise ValueError("v must match k")
         layers, pages, G, page, _ = shape
@@ -154,8 +155,8 @@ def page_append(cache: PagedCache, layer: int, k, v, tokens=None) -> None:
     shape, device = k.shape, cache.device
     S, G, T, d = shape if len(shape) == 4 else (0, 0, 0, 0)
     if S != cache.slots or G != cache.groups or d != HEAD_DIM or k.dtype is not torch.bfloat16:
-        raise ValueError(f"k must be a bfloat16 [slots, G, T, {HEAD_DIM}] tensor with slots, G = {cache.slots}, {cache.groups}, got "
-                         f"{k.dtype} {tuple(shape)}")
+        raise ValueError(f"k must be a bfloat16 [slots, G, T, {HEAD_DIM}] tensor with slots, G = {cache.slots}, {cache.groups}, "
+                         f"got {k.dtype} {tuple(shape)}")
     if v.shape != shape or v.dtype is not torch.bfloat16 or k.device != device or v.device != device:
         raise ValueError("v must match k, on the cache's device")
     nat.refuse_gradients("page_append", k, v)

@@ -25,8 +25,9 @@ def shared_splits(G: int, rows: int, wide: bool, chunk: bool = False) -> int:
 
 
 def own_splits(BG: int, rows: int, keys: int) -> int:
-    """Key splits of the own part: `rows` rows of each of BG (sequence, group) pairs over up to `keys` positions. 384 narrow workgroups;
-    with 192 and 768: 2 x 8 answers of 2K behind 2K 42 and 36 us for 33, 16 answers of 300 behind 8K 27 and 32 for 27."""
+    """Key splits of the own part: `rows` rows of each of BG (sequence, group) pairs over up to `keys` positions. 384 narrow
+    workgroups; with 192 and 768: 2 x 8 answers of 2K behind 2K 42 and 36 us for 33, 16 answers of 300 behind 8K 27 and 32 for
+    27."""
     wide = rows > MAX_H_CHUNK
     tiles = BG * -(-rows // (WIDE_ROWS if wide else NARROW_ROWS))
     return max(1, min(16, (512 if wide else 384) // tiles, keys // 256))
@@ -54,13 +55,13 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
     Sequences runs[r] .. runs[r + 1] - 1 (runs int32 [R + 1] on the device, ascending; None: one run of all) share their first
     prefix_lengths[r] positions (an int for all, or int32 [R] on the device): below it, rounded down to whole pages, the
     tables of those that are long enough for all of their queries to see the whole prefix name the same pages, and one's are
-    read for all. The others, and sequences in no run, read everything by their own tables. prefix_lengths 0: a read of a paged cache
-    with a length per sequence.
+    read for all. The others, and sequences in no run, read everything by their own tables. prefix_lengths 0: a read of a paged
+    cache with a length per sequence.
 
     Nothing is read back to the host, so a captured graph follows the tensors' later values. One query's weights keep 16 bits in
-    their product with V; a chunk's (T > 1) are rounded to bfloat16 before it (2^-8 of each at most). Their sum is not rounded, sums
-    are float32. An infinite value that a query sees makes its output NaN or infinite. There is no gradient: tensors that ask for one are
-    refused. partitions overrides how
+    their product with V; a chunk's (T > 1) are rounded to bfloat16 before it (2^-8 of each at most). Their sum is not rounded,
+    sums are float32. An infinite value that a query sees makes its output NaN or infinite. There is no gradient: tensors that
+    ask for one are refused. partitions overrides how
     many partials a row may have of the shared part (1 to 64; 0: the prefix is ignored) and of the own one (1 to 64)."""
     pool, device = k_pages.shape, k_pages.device
     if (len(pool) != 4 or pool[3] != HEAD_DIM or k_pages.dtype is not torch.bfloat16 or not k_pages.is_contiguous()
@@ -100,8 +101,8 @@ def shared_prefix_attention(q, k_pages, v_pages, block_table, lengths, prefix_le
     if T == 0:
         return out
     rows = B * h * T
-    # Tiles of 128 rows from half a narrow one on (us, wide and narrow: 16 runs of 16 rows on 4K 58 and 71, 32 of 8 rows 101 and 92; one
-    # run on 4K of 8 rows 19.0 and 18.3, of 16 rows 19.2 and 19.4, of 64 rows 22 and 26)
+    # Tiles of 128 rows from half a narrow one on (us, wide and narrow: 16 runs of 16 rows on 4K 58 and 71, 32 of 8 rows 101 and
+    # 92; one run on 4K of 8 rows 19.0 and 18.3, of 16 rows 19.2 and 19.4, of 64 rows 22 and 26)
     wide = T > 1 or 2 * rows > NARROW_ROWS * R
     if partitions is None:
         ns = shared_splits(G, rows, wide, T > 1) if keys else 0

@@ -3,22 +3,23 @@
 //   top: the k largest x, equal ones by the lower token (NaN last, -0 equal to +0), as logprobs
 //
 // A row is cut into up to 64 segments, a workgroup each. A thread holds up to 64 logits in registers, as they came, so each is read
-// once: the waves sum l and s = sum p (x - m) relative to an m of their own, and a segment's leave as a partial (m, l, s, largest). The
-// last of a row's workgroups to arrive merges its partials, where there are few rows; else a second launch does. Sums are fp32 in the
-// log2 domain.
+// once: the waves sum l and s = sum p (x - m) relative to an m of their own, and a segment's leave as a partial (m, l, s,
+// largest). The last of a row's workgroups to arrive merges its partials, where there are few rows; else a second launch does.
+// Sums are fp32 in the log2 domain.
 //
-// The top k without a second look at every logit: the k-th largest of a wave's 64 thread maxima (or one near it) is a lower bound of the k-th
-// largest logit, found by a search over the order-preserving key's bits with one ballot a bit; so are the largest of the four waves'
-// bounds, and, nearer where the waves' logits are alike, the least of the waves' k / 4-th largest. The few 16-byte words that reach the
-// bound (k and some more, in any distribution that does not crowd its largest logits into a few threads) go to LDS, and one wave
-// looks them over again and ranks what it finds by counting.
-// More words than that holds, which takes logits that are equal in their type: k rounds of a maximum over the workgroup, with the same
-// result (64 bf16 rows of 30000 + N(0, 2.5), which are all the same, top 20: 150 us, of N(0, 2.5) 13). The merge does the same to the
-// segments' lists.
+// The top k without a second look at every logit: the k-th largest of a wave's 64 thread maxima (or one near it) is a lower
+// bound of the k-th largest logit, found by a search over the order-preserving key's bits with one ballot a bit; so are the
+// largest of the four waves' bounds, and, nearer where the waves' logits are alike, the least of the waves' k / 4-th largest.
+// The few 16-byte words that reach the bound (k and some more, in any distribution that does not crowd its largest logits into
+// a few threads) go to LDS, and one wave looks them over again and ranks what it finds by counting. More words than that holds,
+// which takes logits that are equal in their type: k rounds of a maximum over the workgroup, with the same result (64 bf16 rows
+// of 30000 + N(0, 2.5), which are all the same, top 20: 150 us, of N(0, 2.5) 13). The merge does the same to the segments'
+// lists.
 //
-// What bounds it, vocabulary of 151936. 4096 bf16 rows, top 5: 204 to 219 us, 1.24 GB at 5.7 to 6.1 TB/s (reads alone go at 7.1); as much
-// as the bytes it is the vector units (11 operations a logit, half of them in the sums, an exponential among them). 64 float32 rows,
-// top 20: 16 us, of which the 39 MB take 6 (all workgroups at once), the bounds 1, the lists 2.5, arrivals 1 and the merge 2.5: latencies.
+// What bounds it, vocabulary of 151936. 4096 bf16 rows, top 5: 204 to 219 us, 1.24 GB at 5.7 to 6.1 TB/s (reads alone go at
+// 7.1); as much as the bytes it is the vector units (11 operations a logit, half of them in the sums, an exponential among
+// them). 64 float32 rows, top 20: 16 us, of which the 39 MB take 6 (all workgroups at once), the bounds 1, the lists 2.5,
+// arrivals 1 and the merge 2.5: latencies.
 #include <cfloat>
 
 #include "select.h"
@@ -31,8 +32,8 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;
 constexpr int kMaxSegments = 64;
 constexpr int kWords = 256;              // words of a segment that are looked over again
-// Up to kFew, the k / 4-th largest of the waves are not asked for: few words reach the first bound anyway, and a second search costs
-// more than it saves (4096 rows, top 5: 207 and 217 us; 64 rows, top 20: 18.0 without it and 16.2 with).
+// Up to kFew, the k / 4-th largest of the waves are not asked for: few words reach the first bound anyway, and a second search
+// costs more than it saves (4096 rows, top 5: 207 and 217 us; 64 rows, top 20: 18.0 without it and 16.2 with).
 constexpr int kFew = 8;
 constexpr int kPartWords = 4;            // m, l, s and the largest logit (16 bytes)
 // x log2 e - m cancels what m's rounding left, up to where that is no longer small. A row whose largest logit is past kFar is
@@ -53,8 +54,8 @@ struct LogprobArgs {
     float* entropy;                      // [N] or null
     float* top_logprob;                  // [N, top]
     int64_t* top_token;                  // [N, top]
-    uint32_t* arrive;                    // [N] arrival counters, zero on entry and left zero: the last segment's workgroup of a row to
-                                         // arrive merges it (segments * top <= kWaveKeys); null: a second launch does
+    uint32_t* arrive;                    // [N] arrival counters, zero on entry and left zero: the last segment's workgroup of a
+                                         // row to arrive merges it (segments * top <= kWaveKeys); null: a second launch does
 };
 
 // Larger logit -> larger key, then lower token -> larger key. Never 0 for a token below 2^31.
@@ -106,11 +107,11 @@ __device__ __forceinline__ uint32_t before_me(uint64_t hit) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(hit >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit, 0));
 }
 
-// A key that k of the wave's 64 keys reach, and few more (k <= 64): the upper half of the largest such bound by its bits, then the least
-// key from there on. A bf16 logit's key has no more bits, so that is the k-th largest. Another's upper half is a range of 2^-7 of its
-// size, where logits far from 0 (or with a common part, which changes no probability) lie together: the other bits follow where the
-// range holds more than kClose keys too many. 64 float32 rows of 1000 + N(0, 2.5), top 20: 15.5 us, without them 172; of N(0, 2.5) 14.8
-// and 14.7.
+// A key that k of the wave's 64 keys reach, and few more (k <= 64): the upper half of the largest such bound by its bits, then
+// the least key from there on. A bf16 logit's key has no more bits, so that is the k-th largest. Another's upper half is a
+// range of 2^-7 of its size, where logits far from 0 (or with a common part, which changes no probability) lie together: the
+// other bits follow where the range holds more than kClose keys too many. 64 float32 rows of 1000 + N(0, 2.5), top 20: 15.5 us,
+// without them 172; of N(0, 2.5) 14.8 and 14.7.
 constexpr int kClose = 8;
 template <int DT>
 __device__ __forceinline__ uint32_t wave_kth(uint32_t key, int k) {
@@ -162,8 +163,8 @@ __device__ __forceinline__ void only_logits(u32x4_t& w, int t, int V) {
     }
 }
 
-// `count` keys in `sh` ranked by counting the larger ones; the first `top` of them to `take(rank, key)`. Eight at a time: zeros, which
-// are larger than none, fill the last ones up (`sync`: they are there for all).
+// `count` keys in `sh` ranked by counting the larger ones; the first `top` of them to `take(rank, key)`. Eight at a time:
+// zeros, which are larger than none, fill the last ones up (`sync`: they are there for all).
 constexpr int kAtOnce = 8;
 template <int THREADS, typename Sync, typename Take>
 __device__ __forceinline__ void rank_keys(uint64_t* sh, int count, int top, Sync sync, Take take) {
@@ -331,8 +332,8 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     // the wave's word u: 64 in line, a segment's end between waves (but for the row's end)
     auto there = [&](int u) { return first + kThreads * u + 64 * wave < end; };
     u32x4_t x[U];
-    {   // as a buffer that ends with the segment: zeros behind it. All of the offset is the vector one: a scalar offset need not count
-        // where it is compared with the end
+    {   // as a buffer that ends with the segment: zeros behind it. All of the offset is the vector one: a scalar offset need
+        // not count where it is compared with the end
         constexpr int kNt = 2;   // non-temporal
         const __amdgpu_buffer_rsrc_t r =
             __builtin_amdgcn_make_buffer_rsrc(const_cast<u32x4_t*>(words + first), 0, 16 * max(end - first, 0), 0x00020000);
@@ -382,8 +383,8 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
 #pragma unroll
     for (int u = 1; u < U; ++u) top = fmaxf(top, most[u]);
     const float largest = wave_max(top);
-    // Not near enough (the sum's logarithm and the entropy's quotient would cancel), or some logit is -inf (a weight of zero, and no term), or none is a number: again, by
-    // the wave's own maximum
+    // Not near enough (the sum's logarithm and the entropy's quotient would cancel), or some logit is -inf (a weight of zero,
+    // and no term), or none is a number: again, by the wave's own maximum
     near = near && fmaf(top, kLog2e, -m) <= kNear && l < FLT_MAX && fabsf(s) < FLT_MAX;
     if (!__all(near)) {
         m = largest > -2.0f * kFar ? largest * kLog2e : -INFINITY;
@@ -501,7 +502,8 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
                 }
 #pragma unroll
                 for (int d = 1; d < 64; d <<= 1) {
-                    const uint64_t y = (uint64_t)(uint32_t)__shfl_xor((int)(k >> 32), d, 64) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)k, d, 64);
+                    const uint64_t y = (uint64_t)(uint32_t)__shfl_xor((int)(k >> 32), d, 64) << 32 |
+                                       (uint32_t)__shfl_xor((int)(uint32_t)k, d, 64);
                     k = y > k ? y : k;
                 }
                 __syncthreads();
@@ -515,12 +517,13 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
         }
     }
     if constexpr (MERGE) {
-        // Every store of this workgroup has completed before its count (the wait and the barrier), so the one that counts all others
-        // before itself finds every partial in memory. It leaves the counter zero.
+        // Every store of this workgroup has completed before its count (the wait and the barrier), so the one that counts all
+        // others before itself finds every partial in memory. It leaves the counter zero.
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
         if (tid == 0)
-            last_sh = __hip_atomic_fetch_add(a.arrive + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)(a.segments - 1);
+            last_sh = __hip_atomic_fetch_add(a.arrive + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                      (uint32_t)(a.segments - 1);
         __syncthreads();
         if (!last_sh || wave != 0) return;
         static_assert(kWords * kPer >= kWaveKeys, "the merge's keys lie in the segment's");
@@ -529,7 +532,8 @@ __global__ __launch_bounds__(kThreads) void logprob_segment(LogprobArgs a) {
     }
 }
 
-// The rows' partials in a launch of their own: a wave a row where the segments' lists hold kWaveKeys keys or fewer, else a workgroup.
+// The rows' partials in a launch of their own: a wave a row where the segments' lists hold kWaveKeys keys or fewer, else a
+// workgroup.
 template <int DT, int THREADS>
 __global__ __launch_bounds__(kThreads) void logprob_merge(LogprobArgs a, int64_t N) {
     constexpr int kRows = kThreads / THREADS;
@@ -546,7 +550,8 @@ int per_word(int dtype) { return dtype == ATTNLAB_DT_F32 ? 4 : 8; }
 // or more and at most 64.
 int plan(int64_t N, int V, int dtype, int& segments, int& words) {
     const int per = per_word(dtype), total = (V + 2 * (per - 1)) / per;   // a row that begins inside a word has one more
-    const int most = dtype == ATTNLAB_DT_F32 ? 16 : 8;   // 64 logits; 16-bit ones of 4, 8 and 16 words: 260, 218, 220 us (4096 rows)
+    // 64 logits; 16-bit ones of 4, 8 and 16 words: 260, 218, 220 us (4096 rows)
+    const int most = dtype == ATTNLAB_DT_F32 ? 16 : 8;
     int u = 1;
     while (u < most && (N * ((total + kThreads * u - 1) / (kThreads * u)) >= 1024 ||
                         (total + kThreads * u - 1) / (kThreads * u) > kMaxSegments || kThreads * u * per < 2048))
@@ -576,8 +581,9 @@ int launch(const LogprobArgs& a, int u, int64_t N, hipStream_t s) {
         return check_launch("token_logprobs");
     }
     launch_segments<DT, false>(a, u, N, s);
-    if (a.segments * a.top <= kWaveKeys) hipLaunchKernelGGL((logprob_merge<DT, 64>), dim3((unsigned)((N + 3) / 4)), dim3(kThreads), 0, s, a, N);
-    else hipLaunchKernelGGL((logprob_merge<DT, kThreads>), dim3((unsigned)N), dim3(kThreads), 0, s, a, N);
+    const dim3 wg(kThreads);
+    if (a.segments * a.top <= kWaveKeys) hipLaunchKernelGGL((logprob_merge<DT, 64>), dim3((unsigned)((N + 3) / 4)), wg, 0, s, a, N);
+    else hipLaunchKernelGGL((logprob_merge<DT, kThreads>), dim3((unsigned)N), wg, 0, s, a, N);
     return check_launch("token_logprobs");
 }
 
@@ -587,7 +593,8 @@ int launch(const LogprobArgs& a, int u, int64_t N, hipStream_t s) {
 using namespace attnlab;
 
 extern "C" int64_t attnlab_logprob_part_bytes(int64_t N, int V, int dtype, int top) {
-    if (N < 0 || V < 1 || V > kMaxVocab - 16 || dtype < ATTNLAB_DT_BF16 || dtype > ATTNLAB_DT_F32 || top < 0 || top > kMaxTop) return -1;
+    if (N < 0 || V < 1 || V > kMaxVocab - 16 || dtype < ATTNLAB_DT_BF16 || dtype > ATTNLAB_DT_F32 || top < 0 || top > kMaxTop)
+        return -1;
     int segments, words;
     plan(N, V, dtype, segments, words);
     return N * segments * (kPartWords * 4 + 8 * (int64_t)top);
@@ -598,8 +605,8 @@ extern "C" int attnlab_token_logprobs(const void* logits, int dtype, int64_t str
                                       int64_t* top_tokens, void* part, int64_t part_bytes, uint32_t* arrive, void* stream) {
     ATTNLAB_REQUIRE(dtype == ATTNLAB_DT_BF16 || dtype == ATTNLAB_DT_F16 || dtype == ATTNLAB_DT_F32,
                     "logits must be bf16, fp16 or fp32 (dtype %d)", dtype);
-    ATTNLAB_REQUIRE(N >= 0 && 1 <= V && V <= kMaxVocab - 16, "rows N=%lld must not be negative and V=%d be in [1, %d]", (long long)N, V,
-                    kMaxVocab - 16);
+    ATTNLAB_REQUIRE(N >= 0 && 1 <= V && V <= kMaxVocab - 16, "rows N=%lld must not be negative and V=%d be in [1, %d]",
+                    (long long)N, V, kMaxVocab - 16);
     ATTNLAB_REQUIRE(0 <= top && top <= kMaxTop && top <= V, "top=%d outside [0, min(%d, V=%d)]", top, kMaxTop, V);
     ATTNLAB_REQUIRE((tokens == nullptr) == (logprobs == nullptr), "tokens and logprobs go together");
     ATTNLAB_REQUIRE(top == 0 || (top_logprobs && top_tokens), "top=%d needs top_logprobs and top_tokens", top);
@@ -607,8 +614,8 @@ extern "C" int attnlab_token_logprobs(const void* logits, int dtype, int64_t str
     ATTNLAB_REQUIRE(logits, "logits must be a device pointer");
     const int bytes = dtype == ATTNLAB_DT_F32 ? 4 : 2;
     ATTNLAB_REQUIRE(reinterpret_cast<uintptr_t>(logits) % bytes == 0, "logits must be aligned to their type");
-    LogprobArgs a{logits, stride, V, 0, 0, top, static_cast<float*>(part), nullptr, tokens, tokens64, logprobs, entropy, top_logprobs,
-                  top_tokens, nullptr};
+    LogprobArgs a{logits, stride, V, 0, 0, top, static_cast<float*>(part), nullptr, tokens, tokens64, logprobs, entropy,
+                  top_logprobs, top_tokens, nullptr};
     const int u = plan(N, V, dtype, a.segments, a.words);
     ATTNLAB_REQUIRE(N * a.segments < (int64_t)1 << 31, "%lld rows of %d segments are too many", (long long)N, a.segments);
     const int64_t need = attnlab_logprob_part_bytes(N, V, dtype, top);

@@ -13,10 +13,10 @@
 //   truncate  lengths'[i] = min(n, l), the entries from ceil(l / page) on given back
 //   compact   with u pages in use: the i-th of them at or past u moves to the i-th free one below u
 //
-// A claim is an entry of a slot whose length has passed the rows that the entry's page holds for it: the first `rows` of the page are the
-// slot's and stay counted, but it had no page of its own to go on in. It reads as an entry without a page, and a truncation to those
-// rows or fewer makes the page the entry's again. Written as INT32_MIN + rows pages + page: 1 <= rows < the page's, so it lies
-// below -1, and where a page's rows are not known (fork) as in any page, rows < 65536.
+// A claim is an entry of a slot whose length has passed the rows that the entry's page holds for it: the first `rows` of the
+// page are the slot's and stay counted, but it had no page of its own to go on in. It reads as an entry without a page, and a
+// truncation to those rows or fewer makes the page the entry's again. Written as INT32_MIN + rows pages + page: 1 <= rows < the
+// page's, so it lies below -1, and where a page's rows are not known (fork) as in any page, rows < 65536.
 //
 // Every choice depends on the cache alone, never on the order in which workgroups or atomics run: counts are integer sums,
 // and free pages are dealt out by prefix sums over the pool. Entries and lengths are checked before they address memory.
@@ -25,7 +25,8 @@
 // workgroup's, because its parts depend on each other (who keeps a page, how many are wanted, which are free) and a grid would
 // have to meet three times; the copies that it asks for are a second launch of as many waves as the chip holds. 8 prompts x 8
 // answers, 512 pages: fork 3.5 us, reserve 7, its copies (8 layers, up to 64 half pages) 8, a layer's append 3.4; 124 slots of 98
-// entries: fork 4.8, reserve 8.4. Compaction of 2048 pages of 64 rows, half in use: ranking 9 us, copies 212 (537 MB each way, 5.1 TB/s).
+// entries: fork 4.8, reserve 8.4. Compaction of 2048 pages of 64 rows, half in use: ranking 9 us, copies 212 (537 MB each way,
+// 5.1 TB/s).
 #include "common.h"
 
 namespace attnlab {
@@ -39,8 +40,8 @@ constexpr int kColumns = 16;                 // table entries a fork's workgroup
 constexpr int kBook = 1024;                  // threads of the reserve's and the compaction's workgroup
 constexpr int kScan = 16;                    // pages a thread looks at in a round
 constexpr int kCopyRows = 16;                // rows of a page that a wave copies at a time: 4 KB, four loads in flight
-constexpr int kAppendRun = 32;               // rows that a workgroup of a long write takes (four appends of 3 x 1003 rows: 44.5 us with the
-                                             // reserve; 47.2 with 16, 48.2 with 64)
+constexpr int kAppendRun = 32;               // rows that a workgroup of a long write takes (four appends of 3 x 1003 rows: 44.5
+                                             // us with the reserve; 47.2 with 16, 48.2 with 64)
 constexpr int kCopyGroups = 2048;            // workgroups of a copy: eight per CU, one wave of each SIMD from each
 
 // What a reserve or a compaction leaves to its copies, in the scratch buffer.
@@ -278,8 +279,9 @@ __global__ __launch_bounds__(kBook) void page_reserve(Book a, const int32_t* tok
     if (copies && granted(tid)) {
         atomicSub(a.refs + held, 1);
     } else if (held >= 0 && found < wanted) {
-        // No page was left for every copy. Of the writers that are still on this one, the one with the most rows (the last of those)
-        // writes on in place, if its other holders are writers too or claim no more rows than it has; the others claim theirs.
+        // No page was left for every copy. Of the writers that are still on this one, the one with the most rows (the last of
+        // those) writes on in place, if its other holders are writers too or claim no more rows than it has; the others claim
+        // theirs.
         int best = -1, best_rows = -1, holders = 0, claimed = 0;
         for (int j = 0; j < a.S; ++j) {
             if (held_sh[j] == held) {
@@ -468,7 +470,8 @@ int check_book(const int32_t* table, const int32_t* lengths, const int32_t* refs
     ATTNLAB_REQUIRE(page >= 1 && page <= (1 << 16) && (page & (page - 1)) == 0,
                     "page_size=%d must be a power of two in [1, 65536]", page);
     ATTNLAB_REQUIRE((int64_t)W * page <= INT32_MAX, "max_pages * page_size exceeds 2^31 positions");
-    ATTNLAB_REQUIRE((int64_t)S * W <= INT32_MAX, "a table of %d slots x %d pages exceeds 2^31 entries", S, W);   // requests are counted
+    // a reserve counts its requests in 32 bits
+    ATTNLAB_REQUIRE((int64_t)S * W <= INT32_MAX, "a table of %d slots x %d pages exceeds 2^31 entries", S, W);
     ATTNLAB_REQUIRE(table && lengths && refs, "table, lengths and refs must be device pointers");
     return ATTNLAB_OK;
 }

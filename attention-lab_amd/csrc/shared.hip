@@ -7,30 +7,31 @@
 // A sequence that ends inside its run's prefix takes no part in the shared read and reads all of its positions in the own part, so
 // the shared one has no masked positions at all.
 //
-// Both parts are split over workgroups by keys; each leaves its rows' partials, and a last launch merges a row's. How a prompt's keys
-// are split is worked out on the device, from runs and prefixes that the host need not know: the blocks of all tiles of rows over the
-// workgroups that the chip holds at once give a share; a tile's whole shares go first, and what is left of the tiles, shorter
-// pieces, fills the gaps. A count beside each row says how many partials it has.
+// Both parts are split over workgroups by keys; each leaves its rows' partials, and a last launch merges a row's. How a
+// prompt's keys are split is worked out on the device, from runs and prefixes that the host need not know: the blocks of all
+// tiles of rows over the workgroups that the chip holds at once give a share; a tile's whole shares go first, and what is left
+// of the tiles, shorter pieces, fills the gaps. A count beside each row says how many partials it has.
 //
 // Two kernels. `wide`: 128 rows, four waves of 32; blocks of 64 keys, S^T = K Q^T, the softmax on its accumulators, O^T += V^T P^T
 // (v_mfma_f32_32x32x16_bf16), K and V copied into LDS a block ahead without passing through registers. `narrow`: up to 16 rows;
 // each wave walks tiles of 32 keys of its own (v_mfma_f32_16x16x32_bf16), K from memory to the matrix core, V through the wave's
-// LDS. A part begins at a page's first position, so in pages of 16 positions or more every 16 keys of a block share one: its entry is
-// looked up a block ahead, and the 16 rows are a buffer that ends where they do (or at once, where there is no page), behind which
-// loads give zeros. Smaller pages are looked up key by key. Keys without a row are masked.
+// LDS. A part begins at a page's first position, so in pages of 16 positions or more every 16 keys of a block share one: its
+// entry is looked up a block ahead, and the 16 rows are a buffer that ends where they do (or at once, where there is no page),
+// behind which loads give zeros. Smaller pages are looked up key by key. Keys without a row are masked.
 //
 // One launch does both parts, the own part's workgroups behind the shared part's.
 //
 // What bounds it (8 groups). 16 questions of 211 tokens, h=2, on 16K: 455 to 485 us with the merge's 16, 1.0 PFLOP/s in the shared
-// part; the matrix cores are busy half of the time, and the softmax lies between a wave's products. 4 x 13 answers, h=8, on 9K, up to
-// 1K of their own: 66 to 75 us, 4.0 to 4.6 TB/s: one block's copies in flight a workgroup (54 us where K and V are in the caches). 16
-// answers, h=4, on 8K: 22 us, and 4 answers on 512: 15 (the host; 12 on the GPU), chains of latencies: the share 2.3, the first copies
-// 2.7, four blocks 5.8, partials 1, the merge 5.
+// part; the matrix cores are busy half of the time, and the softmax lies between a wave's products. 4 x 13 answers, h=8, on 9K,
+// up to 1K of their own: 66 to 75 us, 4.0 to 4.6 TB/s: one block's copies in flight a workgroup (54 us where K and V are in the
+// caches). 16 answers, h=4, on 8K: 22 us, and 4 answers on 512: 15 (the host; 12 on the GPU), chains of latencies: the share
+// 2.3, the first copies 2.7, four blocks 5.8, partials 1, the merge 5.
 //
-// Weights go to the matrix cores as bf16, the operand's type. Of one query each, what that rounding left is multiplied by V too, so they
-// keep 16 bits, as in the package's other one-query reads (4 x 13 answers on 9K 70.6 us, without the rest 69.9; 16 answers on 8K 22.5 and
-// 22.1); a chunk's are rounded once (2^-8 of each at most), as in its other chunk reads: the second product lies in what bounds the kernel
-// (16 questions on 16K: 642 us with it, 473 without). Their sum is of the unrounded ones, sums fp32.
+// Weights go to the matrix cores as bf16, the operand's type. Of one query each, what that rounding left is multiplied by V
+// too, so they keep 16 bits, as in the package's other one-query reads (4 x 13 answers on 9K 70.6 us, without the rest 69.9; 16
+// answers on 8K 22.5 and 22.1); a chunk's are rounded once (2^-8 of each at most), as in its other chunk reads: the second
+// product lies in what bounds the kernel (16 questions on 16K: 642 us with it, 473 without). Their sum is of the unrounded
+// ones, sums fp32.
 #include <cfloat>
 #include <type_traits>
 
@@ -47,9 +48,10 @@ constexpr int kWaves = 4;
 constexpr float kLazy = 8.0f;               // a row's shift is set 2^8 above its largest score and moves when one passes it
 constexpr int kPart = 132;                  // m, l, two unused words, the 128 unnormalised outputs
 constexpr int kMaxSplits = 64;              // partials that a row has of either part, at most
-// Shares that the shared part is cut into: two workgroups per CU where all are wide, three where all are narrow. One where wide ones go
-// with narrow ones of the own part, which take the other half of each CU: 4 prompts of 9K with 13 answers each take 67 us, 79 with two,
-// 69 and 71 with 224 and 320 shares; 48 answers (h=8) of 1500 to 14K 83 and 101; with little to read behind the prompt they are alike.
+// Shares that the shared part is cut into: two workgroups per CU where all are wide, three where all are narrow. One where wide
+// ones go with narrow ones of the own part, which take the other half of each CU: 4 prompts of 9K with 13 answers each take 67
+// us, 79 with two, 69 and 71 with 224 and 320 shares; 48 answers (h=8) of 1500 to 14K 83 and 101; with little to read behind
+// the prompt they are alike.
 constexpr int kWideWorkers = 512, kMixedWorkers = 256, kNarrowWorkers = 768;
 
 struct SharedArgs {
@@ -146,10 +148,11 @@ struct Item {
     bool shared;
 };
 
-constexpr int kLeastBlocks = 4, kLeastTiles = 8;   // a share is of 256 keys at least (16 answers on 8K: 28.5 us, with 128 keys 35.8)
-// More tiles than workgroups: tiles of fewer blocks go whole, in as many rounds as it takes, longer ones are shared out evenly. Even
-// and whole, questions of 211 tokens: 20 on 2K 125 and 133 us, on 4K 198 and 224, on 16K 649 and 781; 36 on 2K 221 and 197, on 4K
-// 330 and 307, on 8K 551 and 548, on 16K 1014 and 1034.
+// A share is of 256 keys at least (16 answers on 8K: 28.5 us, with 128 keys 35.8)
+constexpr int kLeastBlocks = 4, kLeastTiles = 8;
+// More tiles than workgroups: tiles of fewer blocks go whole, in as many rounds as it takes, longer ones are shared out evenly.
+// Even and whole, questions of 211 tokens: 20 on 2K 125 and 133 us, on 4K 198 and 224, on 16K 649 and 781; 36 on 2K 221 and
+// 197, on 4K 330 and 307, on 8K 551 and 548, on 16K 1014 and 1034.
 constexpr uint32_t kLongBlocks = 64;
 
 // The shared part's workgroup `turn` of XCD `xcd`: a group, a run, a share of its blocks of kBlock keys, and a tile of kRows of its
@@ -171,8 +174,8 @@ __device__ __forceinline__ bool shared_item(const SharedArgs& a, int xcd, int tu
         longest = max(longest, (uint32_t)__builtin_amdgcn_readlane(wave_incl_max(n ? (int)k : 0), 63));
         return false;
     });
-    // a share: even over the workgroups in as many rounds as the tiles would take whole. In several rounds only where a tile is long
-    // enough for a second partial of its rows to pay
+    // a share: even over the workgroups in as many rounds as the tiles would take whole. In several rounds only where a tile is
+    // long enough for a second partial of its rows to pay
     total *= a.G;
     uint32_t share = longest;
     if (total <= (uint64_t)kWorkers * longest) {
@@ -181,7 +184,8 @@ __device__ __forceinline__ bool shared_item(const SharedArgs& a, int xcd, int tu
         const uint32_t rounds = (uint32_t)((total + (uint64_t)kWorkers * longest - 1) / ((uint64_t)kWorkers * longest));
         share = (uint32_t)(total / ((uint64_t)kWorkers * rounds)) + 1;
     }
-    share = min(longest, max(max(share, (longest + a.shared - 1) / a.shared), (uint32_t)(kBlock == kKeys ? kLeastBlocks : kLeastTiles)));
+    const uint32_t least = max((longest + a.shared - 1) / a.shared, (uint32_t)(kBlock == kKeys ? kLeastBlocks : kLeastTiles));
+    share = min(longest, max(share, least));
     // whole shares of a group, and pieces
     uint32_t whole = 0, pieces = 0;
     runs.walk(a, [&](const Run& run) {
@@ -299,8 +303,8 @@ struct Sixteen {
     size_t at;
     uint32_t rows;
     __device__ __forceinline__ Sixteen(const SharedArgs& a, int p, int g, int k16, int end) {
-        // uniform, and in scalar registers: with a descriptor in vector ones every load is a loop over its values (16 questions on 16K:
-        // 503 us, and 459)
+        // uniform, and in scalar registers: with a descriptor in vector ones every load is a loop over its values (16 questions
+        // on 16K: 503 us, and 459)
         auto scalar = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
         rows = scalar((uint32_t)p < (uint32_t)a.pages ? (uint32_t)min(max(end - k16, 0), 16) : 0u);
         at = (size_t)scalar((((uint32_t)p * a.G + g) << a.shift) + (k16 & ((1 << a.shift) - 1))) * kDim;
@@ -571,10 +575,11 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
     };
     // Two tile pairs: the next block's copies are issued when every wave has left the tiles they overwrite, the barrier that also
     // publishes the current block, and land while it is computed; its pages were looked up a block before that. Past the last block
-    // there is nothing to copy (no rows, no traffic), and the copies are issued all the same: a wait behind a branch is for the most
-    // that either side may have left, which would be for the copies that are to be on their way (us, with the branch and without: 16
-    // answers, h=8, on 32K 47.3 and 44.5, on 128K 135 and 121; 8 x 4, h=4, on 16K 110 and 100; 16 questions on 16K 467 and 461; the
-    // own part's workgroups beside it lose: 4 x 13 answers, h=8, on 9K 66.2 and 67.7, 2 x 30, h=4, on 16K 52.8 and 55.3).
+    // there is nothing to copy (no rows, no traffic), and the copies are issued all the same: a wait behind a branch is for the
+    // most that either side may have left, which would be for the copies that are to be on their way (us, with the branch and
+    // without: 16 answers, h=8, on 32K 47.3 and 44.5, on 128K 135 and 121; 8 x 4, h=4, on 16K 110 and 100; 16 questions on 16K
+    // 467 and 461; the own part's workgroups beside it lose: 4 x 13 answers, h=8, on 9K 66.2 and 67.7, 2 x 30, h=4, on 16K 52.8
+    // and 55.3).
     uint64_t have = 0;
     auto publish = [&](auto left) {   // this wave's copies have landed but for the last `left` loads, and its reads are done
         if constexpr (decltype(left)::value == 8) __builtin_amdgcn_s_waitcnt(0x0078);   // vmcnt(8) lgkmcnt(0)
@@ -609,8 +614,8 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
         }
         __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): nothing is written to LDS behind the last block
     }
-    // A result that is not finite: a visible key's doing, or zero weights times one that only later queries see. All rows again, with
-    // the blocks that have such keys looked over. The shared part has none.
+    // A result that is not finite: a visible key's doing, or zero weights times one that only later queries see. All rows
+    // again, with the blocks that have such keys looked over. The shared part has none.
     if (!ONE && !w.shared) {
         float finite = 0.0f * l_run;
 #pragma unroll
@@ -761,7 +766,8 @@ __device__ __forceinline__ void narrow(const SharedArgs& a, const Item& w, char*
             sv[t2] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-                sv[t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f.k[t2][kk]), qb[kk], sv[t2], 0, 0, 0);
+                sv[t2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f.k[t2][kk]), qb[kk], sv[t2], 0, 0,
+                                                                0);
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) *reinterpret_cast<u32x4_t*>(vt + vst + 1024 * u) = f.v[u];
@@ -1025,7 +1031,8 @@ extern "C" int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k
                       reinterpret_cast<uintptr_t>(out)) & 15) == 0, "q, k_pages, v_pages and out must be 16-byte aligned");
     const int64_t need = attnlab_shared_part_bytes(B, G, h, T, shared_splits, own_splits);
     ATTNLAB_REQUIRE(need == 0 || (part && (reinterpret_cast<uintptr_t>(part) & 15) == 0 && part_bytes >= need),
-                    "%d + %d key splits need a 16-byte aligned part buffer of %lld bytes", shared_splits, own_splits, (long long)need);
+                    "%d + %d key splits need a 16-byte aligned part buffer of %lld bytes", shared_splits, own_splits,
+                    (long long)need);
     SharedArgs a{};
     a.q = q;
     a.K = k_pages;
@@ -1060,9 +1067,9 @@ extern "C" int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k
     const int own_rows = own_wide ? kWide : kNarrow;
     const int64_t own = (int64_t)B * G * ((T * (int64_t)h + own_rows - 1) / own_rows) * own_splits;
     const int workers = !wide ? kNarrowWorkers : own_wide ? kWideWorkers : kMixedWorkers;
-    // Workgroups of the shared part: a piece of every tile of rows (a run's last one can be partly empty: one such for each run that
-    // has a row) beside the shares that the chip holds at once, or one of every tile; or all shares of the longest prefixes that
-    // the tables have room for
+    // Workgroups of the shared part: a piece of every tile of rows (a run's last one can be partly empty: one such for each run
+    // that has a row) beside the shares that the chip holds at once, or one of every tile; or all shares of the longest
+    // prefixes that the tables have room for
     const int64_t tiles = G * ((int64_t)B * T * h / (wide ? kWide : kNarrow) + (R < B ? R : B));
     const int64_t keys = (int64_t)max_pages * page_size, longest = prefix_lengths || prefix_length > keys ? keys : prefix_length;
     const int least = wide ? kKeys * kLeastBlocks : kTile * kLeastTiles;

@@ -212,14 +212,14 @@ int attnlab_select_rows(const float* scores, int64_t score_stride, int B, int G,
  * of the selection (and a row whose threshold bin holds more than 8192 keys) is read from `scores`; with scores NULL
  * it is recomputed from the index table zT (z_dtype ATTNLAB_DT_BF16 or ATTNLAB_DT_F32, the score stage's table) and
  * the score stage's u_out, in the score kernel's exact fp32 operation order, so the result is the same; that takes
- * ATTNLAB_ORDER_POSITION (score order reads the picks' scores back). zT and u are ignored when scores are given. attnlab_list_bytes returns 0 where the list select does not apply (hi - lo > 32768, or k large
- * against hi - lo, or `order` ATTNLAB_ORDER_SCORE with k > ATTNLAB_LDS_SORT_K, which the list select does not sort;
- * both functions then fail with ATTNLAB_EINVAL before any launch) and -1 for invalid sizes. `order` is the row order
- * the select stage will be asked for: the score stage refuses a combination the select stage would refuse, because
- * the score stage adds into `state`, which only a completed select stage clears. attnlab_select_lists checks its
- * arguments again; called with other arguments than its score stage (another order, k or shape), it can refuse after
- * the state was filled, and the caller must then zero the state itself. attnlab_sparse_decode_step takes the tiled
- * select itself for score order with k > ATTNLAB_LDS_SORT_K.
+ * ATTNLAB_ORDER_POSITION (score order reads the picks' scores back). zT and u are ignored when scores are given.
+ * attnlab_list_bytes returns 0 where the list select does not apply (hi - lo > 32768, or k large against hi - lo, or `order`
+ * ATTNLAB_ORDER_SCORE with k > ATTNLAB_LDS_SORT_K, which the list select does not sort; both functions then fail with
+ * ATTNLAB_EINVAL before any launch) and -1 for invalid sizes. `order` is the row order the select stage will be asked for: the
+ * score stage refuses a combination the select stage would refuse, because the score stage adds into `state`, which only a
+ * completed select stage clears. attnlab_select_lists checks its arguments again; called with other arguments than its score
+ * stage (another order, k or shape), it can refuse after the state was filled, and the caller must then zero the state itself.
+ * attnlab_sparse_decode_step takes the tiled select itself for score order with k > ATTNLAB_LDS_SORT_K.
  */
 int64_t attnlab_list_bytes(int B, int G, int lo, int hi, int k, int order);
 int attnlab_score_grouped_lists(uint16_t* zT, const uint16_t* k_new, const uint16_t* wk, const uint16_t* q_cat,
@@ -376,8 +376,9 @@ int attnlab_quant_attend(const uint8_t* k_codes, const uint8_t* v_codes, const u
  * The chunk form of attnlab_range_decode, on the matrix cores: T queries at positions q_pos0 + t, query t reading
  * j <= q_pos0 + t, j < legal, and with window > 0: j > q_pos0 + t - window or j < sinks. q, out: [B, G, h, T, 128] bf16
  * contiguous, 1 <= h <= 16; the caches as there. What a masked position holds (NaN, infinity) does not reach an
- * output; a query that sees a value that is not finite gets outputs that are not (infinity may become NaN). splits (1..16): workgroups that share a query tile's key blocks; with more than one, part (16-byte aligned,
- * attnlab_range_prefill_part_bytes bytes) holds their partials and a second launch merges them.
+ * output; a query that sees a value that is not finite gets outputs that are not (infinity may become NaN). splits (1..16):
+ * workgroups that share a query tile's key blocks; with more than one, part (16-byte aligned, attnlab_range_prefill_part_bytes
+ * bytes) holds their partials and a second launch merges them.
  */
 int64_t attnlab_range_prefill_part_bytes(int B, int G, int h, int T, int splits);
 int attnlab_range_prefill(const uint16_t* q, const void* K, const void* V, const uint8_t* k_exp, const uint8_t* v_exp,
@@ -394,24 +395,25 @@ int attnlab_range_prefill(const uint16_t* q, const void* K, const void* V, const
  *   lengths  int32 [S]
  *   refs     int32 [num_pages], how many entries name each page (0: free)
  * All are device memory changed in place. The results depend on the cache alone. Calls on one cache must be ordered on one
- * stream. Entries below -1 are these functions' own: INT32_MIN + rows * num_pages + p, with 1 <= rows < page_size, is a claim, an entry that
- * counts for page p, whose first `rows` rows are the slot's, and that reads as no page (attnlab_page_reserve makes them). Other entries
- * outside [0, num_pages) are not followed.
+ * stream. Entries below -1 are these functions' own: INT32_MIN + rows * num_pages + p, with 1 <= rows < page_size, is a claim,
+ * an entry that counts for page p, whose first `rows` rows are the slot's, and that reads as no page (attnlab_page_reserve
+ * makes them). Other entries outside [0, num_pages) are not followed.
  *
- * attnlab_page_fork: slot i goes on from slot parents[i] (int32 [S], none of the cache's own memory) as it was before the call: its entries and length; a
- * parent outside [0, S) leaves the slot empty.
+ * attnlab_page_fork: slot i goes on from slot parents[i] (int32 [S], none of the cache's own memory) as it was before the call:
+ * its entries and length; a parent outside [0, S) leaves the slot empty.
  *
- * attnlab_page_truncate: lengths[i] = min(lengths[i], max(to[i], 0)), `to` in memory of its own, with `to` null `length`; the entries from
- * ceil(lengths[i] / page_size) on are given back. A claim that the slot then ends in, at its rows or before, is its page again.
+ * attnlab_page_truncate: lengths[i] = min(lengths[i], max(to[i], 0)), `to` in memory of its own, with `to` null `length`; the
+ * entries from ceil(lengths[i] / page_size) on are given back. A claim that the slot then ends in, at its rows or before, is
+ * its page again.
  *
- * attnlab_page_reserve: lengths[i] grows by tokens[i] (null: each; less than 1: slot i is left alone), up to 2^31 - 1. A slot that ended
- * inside a page with other holders gets a page of its own, the rows up to its length copied in every layer, unless all of the
- * page's holders grow and it is the last of them. Then an entry is given a page for every page_size positions begun. Pages are the
- * lowest free ones, in the order of slots and entries; where none is left the entry is -1, or, for a copy, a claim of the slot's
- * rows of the page. One of the holders that are left without a copy, the one with the most rows (the last of those), writes on in
- * place if all others grow or claim no more rows than it has. missing (int32 [1], nullable) is raised by the pages not given, those
- * past max_pages among them. scratch: 16-byte aligned, attnlab_page_scratch_bytes(S,
- * num_pages) bytes, no initialisation.
+ * attnlab_page_reserve: lengths[i] grows by tokens[i] (null: each; less than 1: slot i is left alone), up to 2^31 - 1. A slot
+ * that ended inside a page with other holders gets a page of its own, the rows up to its length copied in every layer, unless
+ * all of the page's holders grow and it is the last of them. Then an entry is given a page for every page_size positions begun.
+ * Pages are the lowest free ones, in the order of slots and entries; where none is left the entry is -1, or, for a copy, a
+ * claim of the slot's rows of the page. One of the holders that are left without a copy, the one with the most rows (the last
+ * of those), writes on in place if all others grow or claim no more rows than it has. missing (int32 [1], nullable) is raised
+ * by the pages not given, those past max_pages among them. scratch: 16-byte aligned, attnlab_page_scratch_bytes(S, num_pages)
+ * bytes, no initialisation.
  *
  * attnlab_page_append: one layer's rows, k and v: (slot, group, row t, dim) at k + i k_b_stride + g k_g_stride + t k_t_stride
  * + dim (bf16 elements; rows 16-byte aligned; strides may be 0), row t < tokens[i] (null: T) of slot i at position
@@ -472,8 +474,8 @@ int attnlab_shared_prefix_attend(const uint16_t* q, const uint16_t* k_pages, con
  * tokens and logprobs are null together. A row with a NaN, an infinity of positive sign or nothing above -inf has no
  * distribution: its values are NaN (top_tokens stay those of the order). 0 <= top <= min(64, V), V <= 2^20 - 16.
  * part: 16-byte aligned, attnlab_logprob_part_bytes bytes, no initialisation. Two launches, or one where arrive (uint32 [N],
- * zero on entry, left zero, not shared with a call that may overlap) is given and a row's segments have at most 256 candidates between
- * them; the same result.
+ * zero on entry, left zero, not shared with a call that may overlap) is given and a row's segments have at most 256 candidates
+ * between them; the same result.
  */
 int64_t attnlab_logprob_part_bytes(int64_t N, int V, int dtype, int top);
 int attnlab_token_logprobs(const void* logits, int dtype, int64_t stride, int64_t N, int V, const void* tokens, int tokens64,
@@ -505,7 +507,8 @@ int64_t attnlab_sparse_decode_workspace(int B, int G, int h, int lo, int hi, int
  * its rows, up to the summation's rounding), and the step runs the position-order select, the faster one.
  * state: select state [B*G, ATTNLAB_SELECT_STATE_WORDS] uint32, zero before the first call; the score kernel fills
  * it and the select kernels (in the one-launch form, the row's last workgroup to read it) clear it, so it stays zero
- * between calls with no memset (the launches stay capturable in a HIP graph). Nullable: the select kernel then runs its own first radix pass on one workgroup per row.
+ * between calls with no memset (the launches stay capturable in a HIP graph). Nullable: the select kernel then runs its own
+ * first radix pass on one workgroup per row.
  */
 int attnlab_sparse_decode_step(const uint16_t* q_main, const uint16_t* q_cat, const uint16_t* K, const uint16_t* V,
                                uint16_t* zT, const uint16_t* wq_t, const uint16_t* wk, const uint16_t* k_new,
@@ -532,8 +535,9 @@ int attnlab_sparse_decode_step_f32(const uint16_t* q_main, const float* q_cat, c
  * loops, harnesses that forbid hipMalloc). The select state and the workspace live in a 32 MiB file-scope device array
  * that each device holds until the process ends; its first 256 * ATTNLAB_SELECT_STATE_WORDS words are the select state
  * (B*G <= 256), the rest the workspace (attnlab_sparse_decode_workspace of these sizes, or that without the long rows'
- * key lists, must fit, or the call returns ATTNLAB_EINVAL). Arguments and outputs as in attnlab_sparse_decode_step (bf16 index table). Every call on a device
- * shares that device's array: calls that overlap on one device race, so order them on one stream.
+ * key lists, must fit, or the call returns ATTNLAB_EINVAL). Arguments and outputs as in attnlab_sparse_decode_step (bf16 index
+ * table). Every call on a device shares that device's array: calls that overlap on one device race, so order them on one
+ * stream.
  */
 int attnlab_sparse_decode_step_noalloc(const uint16_t* q_main, const uint16_t* q_cat, const uint16_t* K,
                                        const uint16_t* V, uint16_t* zT, const uint16_t* wq_t, const uint16_t* wk,
