@@ -25,8 +25,8 @@
 // workgroup's, because its parts depend on each other (who keeps a page, how many are wanted, which are free) and a grid would
 // have to meet three times; the copies that it asks for are a second launch of as many waves as the chip holds. 8 prompts x 8
 // answers, 512 pages: fork 3.5 us, reserve 7, its copies (8 layers, up to 64 half pages) 8, a layer's append 3.4; 124 slots of 98
-// entries: fork 4.8, reserve 8.4. Compaction of 2048 pages of 64 rows, half in use: ranking 9 us, copies 212 (537 MB each way,
-// 5.1 TB/s).
+// entries: fork 4.8, reserve 8.4, truncate 2.2. Compaction of 2048 pages of 64 rows, half in use: ranking 9 us, copies 212 (537
+// MB each way, 5.1 TB/s).
 #include "common.h"
 
 namespace attnlab {

@@ -23,15 +23,16 @@
 //
 // What bounds it (8 groups). 16 questions of 211 tokens, h=2, on 16K: 455 to 485 us with the merge's 16, 1.0 PFLOP/s in the shared
 // part; the matrix cores are busy half of the time, and the softmax lies between a wave's products. 4 x 13 answers, h=8, on 9K,
-// up to 1K of their own: 66 to 75 us, 4.0 to 4.6 TB/s: one block's copies in flight a workgroup (54 us where K and V are in the
-// caches). 16 answers, h=4, on 8K: 22 us, and 4 answers on 512: 15 (the host; 12 on the GPU), chains of latencies: the share
-// 2.3, the first copies 2.7, four blocks 5.8, partials 1, the merge 5.
+// up to 1K of their own: 70 to 75 us, 3.6 to 3.8 TB/s: one block's copies in flight a workgroup, and a block's own chain of
+// products, softmax and products (16 answers, h=8, on 128K: 149 us, 120 where K and V are in the caches). 16 answers, h=4, on 8K:
+// 22.5 us, and 4 answers on 512: 15 (the host; 12 on the GPU), chains of latencies: the share 2.3, the first copies 2.7, four
+// blocks 5.8, partials 1, the merge 5.
 //
 // Weights go to the matrix cores as bf16, the operand's type. Of one query each, what that rounding left is multiplied by V
-// too, so they keep 16 bits, as in the package's other one-query reads (4 x 13 answers on 9K 70.6 us, without the rest 69.9; 16
-// answers on 8K 22.5 and 22.1); a chunk's are rounded once (2^-8 of each at most), as in its other chunk reads: the second
-// product lies in what bounds the kernel (16 questions on 16K: 642 us with it, 473 without). Their sum is of the unrounded
-// ones, sums fp32.
+// too, so they keep 16 bits, as in the package's other one-query reads (us, with the rest and without: 16 answers, h=4, on 8K
+// 24.8 and 24.5; 4 x 13, h=8, on 9K 64.5 and 60.0; 2 x 30, h=4, on 16K 50.1 and 46.6; 16, h=8, on 32K 50.2 and 44.0, on 128K 149
+// and 127; 8 x 4, h=4, on 16K 116 and 116); a chunk's are rounded once (2^-8 of each at most), as in its other chunk reads: the
+// second product lies in what bounds the kernel (16 questions on 16K 642 and 473). Their sum is of the unrounded ones, sums fp32.
 #include <cfloat>
 #include <type_traits>
 
@@ -576,7 +577,7 @@ __device__ __forceinline__ void wide(const SharedArgs& a, const Item& w, char* k
     // Two tile pairs: the next block's copies are issued when every wave has left the tiles they overwrite, the barrier that also
     // publishes the current block, and land while it is computed; its pages were looked up a block before that. Past the last block
     // there is nothing to copy (no rows, no traffic), and the copies are issued all the same: a wait behind a branch is for the
-    // most that either side may have left, which would be for the copies that are to be on their way (us, with the branch and
+    // most that either side may have left, which would be for the copies that are to be on their way (us, of single weights, with the branch and
     // without: 16 answers, h=8, on 32K 47.3 and 44.5, on 128K 135 and 121; 8 x 4, h=4, on 16K 110 and 100; 16 questions on 16K
     // 467 and 461; the own part's workgroups beside it lose: 4 x 13 answers, h=8, on 9K 66.2 and 67.7, 2 x 30, h=4, on 16K 52.8
     // and 55.3).
