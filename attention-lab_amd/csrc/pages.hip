@@ -201,7 +201,8 @@ __global__ __launch_bounds__(kBook) void page_reserve(Book a, const int32_t* tok
     __shared__ uint2 wave_sh[kBook / 64];
     __shared__ uint4 scan_sh[64];
     __shared__ __attribute__((aligned(16))) int32_t held_sh[kMaxSlots];   // -1 past the slots
-    __shared__ int32_t first_sh[kMaxSlots], part_sh[kMaxSlots];
+    __shared__ __attribute__((aligned(16))) int32_t first_sh[kMaxSlots];  // a slot's first new entry; then its rows, where it is left
+    __shared__ int32_t part_sh[kMaxSlots];
     __shared__ uint32_t upto_sh[kMaxSlots], job_sh[kMaxSlots];   // requests up to and with a slot's; its copy's number + 1, or 0
     const int tid = threadIdx.x, page = 1 << a.shift;
     int32_t pool[kScan];                     // the first pages' counts, on their way from the start; only free ones change below
@@ -274,32 +275,53 @@ __global__ __launch_bounds__(kBook) void page_reserve(Book a, const int32_t* tok
         });
     }
     for (uint32_t r = found + tid; r < wanted; r += kBook) give(r, -1);
-    auto granted = [&](int j) { return job_sh[j] && (j ? upto_sh[j - 1] : 0u) < found; };   // a copy is its slot's first request
+    const bool copied = copies && (tid ? upto_sh[tid - 1] : 0u) < found;   // a copy is its slot's first request
+    if (copied) atomicSub(a.refs + held, 1);
     int out = lost + (tid == 0 && wanted > found ? (int)(wanted - found) : 0);
-    if (copies && granted(tid)) {
-        atomicSub(a.refs + held, 1);
-    } else if (held >= 0 && found < wanted) {
-        // No page was left for every copy. Of the writers that are still on this one, the one with the most rows (the last of
-        // those) writes on in place, if its other holders are writers too or claim no more rows than it has; the others claim
-        // theirs.
-        int best = -1, best_rows = -1, holders = 0, claimed = 0;
-        for (int j = 0; j < a.S; ++j) {
-            if (held_sh[j] == held) {
-                ++holders;
-                if (!granted(j) && part_sh[j] >= best_rows) {
-                    best = j;
-                    best_rows = part_sh[j];
-                }
-            } else {
-                const Claim c(a.table[(size_t)j * a.W + last], a.pages, page);
-                if (c.page != held) continue;
-                ++holders;
-                claimed = max(claimed, c.rows);
+    if (found < wanted) {
+        // No page was left for every copy. Of the writers that are still on a page, the one with the most rows (the last of those)
+        // writes on in place, if its other holders are writers too or claim no more rows than it has; the others claim theirs.
+        // (1024 branches of one prompt without a page: 76 us, 65 of them the requests that cannot be met)
+        const bool left = held >= 0 && !copied;
+        __syncthreads();                     // the requests' entries are dealt
+        first_sh[tid] = left ? part << 10 | tid : -1;
+        __syncthreads();
+        int best = -1, holders = 0, claimed = 0;
+        bool on = false;
+        if (left) {
+            for (int j = 0; j < a.S; j += 4) {
+                const int4 h = *reinterpret_cast<const int4*>(held_sh + j), f = *reinterpret_cast<const int4*>(first_sh + j);
+                holders += (h.x == held) + (h.y == held) + (h.z == held) + (h.w == held);
+                best = max(max(max(best, h.x == held ? f.x : -1), max(h.y == held ? f.y : -1, h.z == held ? f.z : -1)),
+                           h.w == held ? f.w : -1);
+            }
+            on = best == (part << 10 | tid);
+        }
+        // claims, at the same entry of their slots, or holders that do not grow: a wave looks for those of its pages, one by one
+        for (uint64_t open = __ballot(on && holders < refs); open; open &= open - 1) {
+            const int x = __builtin_ctzll(open), p = __shfl(held, x, 64), e = __shfl(last, x, 64);
+            int more = 0, rows_of = 0;
+            for (int j = tid & 63; j < a.S; j += 64) {
+                const Claim c(a.table[(size_t)j * a.W + e], a.pages, page);
+                if (c.page != p || held_sh[j] == p) continue;
+                ++more;
+                rows_of = max(rows_of, c.rows);
+            }
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                more += __shfl_xor(more, d, 64);
+                rows_of = max(rows_of, __shfl_xor(rows_of, d, 64));
+            }
+            if ((tid & 63) == x) {
+                holders += more;
+                claimed = rows_of;
             }
         }
-        const bool on = best == tid && holders == refs && claimed <= part;
-        if (!on) a.table[(size_t)tid * a.W + last] = claim_of(held, part, a.pages);
-        out += !on - copies;                 // its copy, if it asked for one, is counted above
+        if (left) {
+            on = on && holders == refs && claimed <= part;
+            if (!on) a.table[(size_t)tid * a.W + last] = claim_of(held, part, a.pages);
+            out += !on - copies;             // its copy, if it asked for one, is counted above
+        }
     }
     if (tid == 0) moves->count = (int32_t)jobs;
     if (missing && out) atomicAdd(missing, out);
