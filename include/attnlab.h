@@ -445,7 +445,9 @@ int attnlab_page_compact(uint16_t* k, uint16_t* v, int layers, int num_pages, in
  * page_size):
  *   out[b,g,i,t] = sum_j softmax_j(scale q[b,g,i,t] . k_j) v_j    over j <= n - T + t, k_j and v_j by b's table
  * Positions on an entry outside [0, num_pages) are skipped; a query that reads nothing gets zeros. What a later position of the
- * sequence holds (NaN, infinity) does not reach an output.
+ * sequence holds (NaN, infinity) does not reach an output; a query that sees a value that is not finite gets outputs that are not
+ * (an infinity may become NaN). A weight of one query (T = 1) keeps 16 bits in its product with V, one of several is rounded to
+ * bf16.
  * runs (int32 [R + 1] on the device, ascending; null with R = 1: all sequences): sequences runs[r] .. runs[r + 1] - 1 share the
  * pages below prefix_lengths[r] (int32 [R] on the device, or null: prefix_length) rounded down to whole pages. The tables of those
  * of which every query sees all of that prefix name the same pages there, and one's are read for all of them; the others, and
